@@ -1294,6 +1294,8 @@ const char* xtq_vit_strerror(int rc) {
         case 11: return "NaN target";
         case 12: return "null or misaligned pointer argument";
         case 13: return "synchronous entry given a stream under graph capture";
+        case 14: return "workspace too small";
+        case 15: return "unsupported element type or activation";
         default: return "unknown status";
     }
 }

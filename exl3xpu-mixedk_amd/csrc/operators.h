@@ -1,0 +1,54 @@
+// operators.h -- internal launch interface of the operators on trellis-coded
+// weights (linear layer, mixture layer, input Gram).  The exported entry points
+// live in operators_capi.hip and are declared in include/exl3_vit.h.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/exl3_vit.h"
+#include "trellis_math.h"
+
+namespace xtq {
+
+// The MI355X's compute units: launches are split to fill them (any number is
+// right).
+constexpr int kCUs = 256;
+
+// A trellis weight as the kernels take it.
+struct Weight {
+    const int16_t* trellis;
+    const uint16_t* suh;
+    const uint16_t* svh;
+    float scale;
+    int k, n, K, code;
+};
+
+// Arguments of a product's epilogue, see finish_unit.
+struct Epilogue {
+    const uint16_t* colscale;   // fp16, per output column
+    float scale;                // for all of them
+    const int32_t* rowexp;      // per row: products are 2^rowexp too small; NULL: 0
+    const void* bias;           // per output column or NULL
+    int bias_f32;               // bias is fp32, else of the activations' type
+    int act;
+    const void* res;            // residual or NULL
+    long long res_stride;
+    void* z;                    // [M][n] values before the activation, or NULL
+    void* y;
+    long long y_stride;
+    int rows, cols;
+};
+
+size_t linear_ws_bytes(int rows, int k, int n, int backward);
+hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
+                         const Epilogue& ep, void* ws, uint32_t* counters, hipStream_t s);
+hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long long dy_stride,
+                             const void* z, int act, int rows, void* dx, long long dx_stride,
+                             void* dbias, int dbias_f32, void* ws, uint32_t* counters,
+                             hipStream_t s);
+
+size_t gram_ws_bytes(int rows, int k);
+hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, int k,
+                       const uint8_t* valid, const float* prev, float* out, void* ws,
+                       hipStream_t s);
+}  // namespace xtq

@@ -1,0 +1,134 @@
+// operators_capi.hip -- C entries of the operators on trellis weights (declared
+// in include/exl3_vit.h): arguments are checked on the host against everything
+// the kernels assume, then the kernels are enqueued.  No state is kept between
+// calls and nothing is locked.
+#include <stdio.h>
+#include <string.h>
+
+#include "operators.h"
+
+namespace {
+
+// Code of a trellis weight's name, or -1: the products take values that fp16
+// holds, which "1mad"'s are not.
+int parse_code(const char* code) {
+    if (!strncmp(code, "exl3_", 5)) code += 5;
+    if (!strcmp(code, "mul1")) return xtq::kCodeMul1;
+    if (!strcmp(code, "3inst")) return xtq::kCode3Inst;
+    if (!strcmp(code, "mcg")) return xtq::kCodeMcg;
+    return -1;
+}
+
+bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+constexpr int kMaxRows = 1048560;       // 65,535 groups of 16 rows (a grid's second dimension)
+
+int check_weight(const xtq_weight* w, xtq::Weight* out) {
+    if (!w || !w->trellis || !w->suh || !w->svh || !w->code) return 12;
+    if (!aligned(w->trellis, 2) || !aligned(w->suh, 2) || !aligned(w->svh, 2)) return 12;
+    if (w->K < 2 || w->K > 7) return 9;
+    const int code = parse_code(w->code);
+    if (code < 0) return 8;
+    if (w->k <= 0 || w->n <= 0 || w->k % 128 || w->n % 128 || w->k > (1 << 22) || w->n > (1 << 22))
+        return 6;
+    *out = xtq::Weight{w->trellis, w->suh, w->svh, w->scale, w->k, w->n, w->K, code};
+    return 0;
+}
+
+// A matrix of 16-bit elements.
+int check_rows(const void* p, int64_t stride, int cols) {
+    if (!p || !aligned(p, 2)) return 12;
+    return stride < cols ? 6 : 0;
+}
+
+int status(hipError_t e, const char* what) {
+    if (e == hipSuccess) return 0;
+    fprintf(stderr, "xtq_vit %s: %s\n", what, hipGetErrorString(e));
+    return 4;
+}
+
+int check_ws(const void* ws, int64_t have, int64_t want) {
+    if (want > 0 && (!ws || !aligned(ws, 16))) return 12;
+    return have < want ? 14 : 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int backward) {
+    if (!w || w->k <= 0 || w->n <= 0 || w->k % 128 || w->n % 128 || rows < 0 || rows > kMaxRows)
+        return -6;
+    return rows ? (int64_t)xtq::linear_ws_bytes(rows, w->k, w->n, backward) : 0;
+}
+
+int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_stride, int rows,
+                   const void* bias, int bias_f32, int act, const void* res, int64_t res_stride,
+                   void* z, void* y, int64_t y_stride, void* ws, int64_t ws_bytes,
+                   uint32_t* counters, void* stream) {
+    xtq::Weight wt;
+    int rc = check_weight(w, &wt);
+    if (rc) return rc;
+    if ((type != XTQ_BF16 && type != XTQ_F16) || act < XTQ_ACT_NONE || act > XTQ_ACT_GELU) return 15;
+    if (rows < 0 || rows > kMaxRows) return 6;
+    if (rows == 0) return 0;
+    if ((rc = check_rows(x, x_stride, wt.k))) return rc;
+    if ((rc = check_rows(y, y_stride, wt.n))) return rc;
+    if (res && (rc = check_rows(res, res_stride, wt.n))) return rc;
+    if (!aligned(z, 2) || !aligned(bias, bias_f32 ? 4 : 2)) return 12;
+    if (!counters || !aligned(counters, 4)) return 12;
+    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, 0)))) return rc;
+    xtq::Epilogue ep{};
+    ep.colscale = wt.svh;
+    ep.scale = wt.scale;
+    ep.bias = bias;
+    ep.bias_f32 = bias_f32;
+    ep.act = act;
+    ep.res = res;
+    ep.res_stride = res_stride;
+    ep.z = z;
+    ep.y = y;
+    ep.y_stride = y_stride;
+    ep.rows = rows;
+    ep.cols = wt.n;
+    return status(xtq::launch_linear(wt, type, x, x_stride, rows, ep, ws, counters,
+                                     (hipStream_t)stream), "linear");
+}
+
+int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy_stride,
+                       const void* z, int act, int rows, void* dx, int64_t dx_stride, void* dbias,
+                       int bias_f32, void* ws, int64_t ws_bytes, uint32_t* counters, void* stream) {
+    xtq::Weight wt;
+    int rc = check_weight(w, &wt);
+    if (rc) return rc;
+    if ((type != XTQ_BF16 && type != XTQ_F16) || act < XTQ_ACT_NONE || act > XTQ_ACT_GELU) return 15;
+    if (rows <= 0 || rows > kMaxRows) return 6;
+    if ((rc = check_rows(dy, dy_stride, wt.n))) return rc;
+    if (!dx && !dbias) return 12;
+    if (dx && (rc = check_rows(dx, dx_stride, wt.k))) return rc;
+    if (act != XTQ_ACT_NONE && (!z || !aligned(z, 2))) return 12;
+    if (!aligned(dbias, bias_f32 ? 4 : 2)) return 12;
+    if (!counters || !aligned(counters, 4)) return 12;
+    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, 1)))) return rc;
+    return status(xtq::launch_linear_bwd(wt, type, dy, dy_stride, z, act, rows, dx, dx_stride, dbias,
+                                         bias_f32, ws, counters, (hipStream_t)stream), "linear_bwd");
+}
+
+int64_t xtq_gram_ws_bytes(int rows, int k) {
+    if (k <= 0 || k % 128 || k > (1 << 22) || rows < 0 || rows > (1 << 30)) return -6;
+    return (int64_t)xtq::gram_ws_bytes(rows, k);
+}
+
+int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, int k, const uint8_t* valid,
+                 const float* prev, float* out, void* ws, int64_t ws_bytes, void* stream) {
+    if (type != XTQ_BF16 && type != XTQ_F16) return 15;
+    if (k <= 0 || k % 128 || k > (1 << 22) || rows < 0 || rows > (1 << 30)) return 6;
+    int rc;
+    if (rows && (rc = check_rows(x, x_stride, k))) return rc;
+    if (!out || !aligned(out, 4) || !aligned(prev, 4)) return 12;
+    if ((rc = check_ws(ws, ws_bytes, xtq::gram_ws_bytes(rows, k)))) return rc;
+    return status(xtq::launch_gram(type, x, x_stride, rows, k, valid, prev, out, ws,
+                                   (hipStream_t)stream), "gram");
+}
+
+}  // extern "C"

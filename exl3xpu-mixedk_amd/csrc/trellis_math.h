@@ -1,0 +1,119 @@
+// trellis_math.h -- device functions shared by the kernels that multiply with
+// trellis-coded weights: codebook values as fp16 pairs, the block-128 transform
+// in registers, activations and their slopes, 16-bit loads and stores.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "viterbi_kernels.h"
+
+namespace xtq {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+// Vectors at the alignment of their 16-bit elements: gfx950 takes global
+// accesses of any width at any address.
+typedef u4 u4_a2 __attribute__((aligned(2)));
+typedef u2 u2_a2 __attribute__((aligned(2)));
+typedef uint32_t u1_a2 __attribute__((aligned(2)));
+typedef f4 f4_a4 __attribute__((aligned(4)));
+
+// Element types of activations (the C-ABI's numbers).
+enum ElemType { kBf16 = 0, kF16 = 1 };
+enum Act { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
+
+// Codebook values of two 16-bit states as a pair of halves; the EXL3 codes'
+// values are fp16 numbers, so nothing is rounded here that the table has not
+// rounded.  mul1: 1024 + byte sum < 2048 is the fp16 number with the bits
+// 0x6400 + byte sum, and one fp16 fused multiply-add rounds once, as the table
+// does.  v_mul_lo_u32 issues at the rate of v_sad_u8 and v_bfe_u32 on gfx950
+// (33-37 T lane-operations/s measured), so a value costs 3.5 instructions.
+template <int CODE>
+__device__ __forceinline__ uint32_t code_pair(uint32_t s0, uint32_t s1) {
+    if constexpr (CODE == kCodeMul1) {
+        uint32_t t = __builtin_amdgcn_sad_u8(s0 * 0x83DCD12Du, 0u, 0x64006400u);
+        t = __builtin_amdgcn_sad_hi_u8(s1 * 0x83DCD12Du, 0u, t);
+        const _Float16 c1 = (_Float16)(1774.0f / 262144.0f), c2 = (_Float16)(-1329.0f / 128.0f);
+        const h2 v = __builtin_elementwise_fma(__builtin_bit_cast(h2, t), (h2){c1, c1},
+                                               (h2){c2, c2});
+        return __builtin_bit_cast(uint32_t, v);
+    } else {
+        uint32_t a = CODE == kCode3Inst ? s0 * 89226354u + 64248484u : s0 * 0xCBAC1FEDu;
+        uint32_t b = CODE == kCode3Inst ? s1 * 89226354u + 64248484u : s1 * 0xCBAC1FEDu;
+        a = (a & 0x8FFF8FFFu) ^ 0x3B603B60u;
+        b = (b & 0x8FFF8FFFu) ^ 0x3B603B60u;
+        const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05040100u);   // low halves
+        const uint32_t hi = __builtin_amdgcn_perm(b, a, 0x07060302u);   // high halves
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, lo) + __builtin_bit_cast(h2, hi));
+    }
+}
+
+// fp32 value of a 16-bit activation.
+template <int T>
+__device__ __forceinline__ float from16(uint32_t bits) {
+    if constexpr (T == kBf16) return __uint_as_float(bits << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+
+// Activation rounded to nearest even to 16 bits (the outputs' only rounding).
+template <int T>
+__device__ __forceinline__ uint32_t to16(float v) {
+    if constexpr (T == kBf16) return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v);
+    else return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+__device__ __forceinline__ float half_bits(uint32_t bits) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+
+// Activations in fp32 (act is uniform).  silu's exp overflows to infinity for
+// z < -88 and the quotient is then -0; gelu is the erf form.
+__device__ __forceinline__ float act_value(float z, int act) {
+    if (act == kActRelu) return z > 0.0f ? z : (z == z ? 0.0f : z);
+    if (act == kActSilu) return z / (1.0f + expf(-z));
+    if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    return z;
+}
+
+// Slope of the activation at z; at infinities the limits (z * exp(-z^2/2)
+// and z * (1 - sigmoid) are products of infinity and zero there).
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == kActRelu) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
+    if (act == kActSilu) {
+        const float s = 1.0f / (1.0f + expf(-z));
+        const float t = fabsf(z) > 100.0f ? 0.0f : z * (1.0f - s);
+        return s * (1.0f + t);
+    }
+    if (act == kActGelu) {
+        const float d = fabsf(z) > 20.0f ? 0.0f : z * expf(-0.5f * z * z);
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + 0.39894228040143268f * d;
+    }
+    return 1.0f;
+}
+
+// Value of the lane whose number differs in bit 4 (M = 16) or 5 (M = 32).
+template <int M>
+__device__ __forceinline__ float lane_xor(float v) {
+    return __shfl_xor(v, M);
+}
+
+// One stage of the block-128 transform over a lane bit: this lane's sum or
+// difference with its partner's.
+template <int M>
+__device__ __forceinline__ float cross_stage(float v, uint32_t lane) {
+    const float o = lane_xor<M>(v);
+    return (lane & M) ? o - v : v + o;
+}
+
+// Exponent s with v * 2^s in [2^top, 2^(top+1)) for finite v > 0; 0 for 0,
+// infinities and NaN (their products then stay what they are).
+__device__ __forceinline__ int shift_to(float v, int top) {
+    if (!(v > 0.0f) || !(v <= 3.4028234663852886e38f)) return 0;
+    return top + 1 - __builtin_amdgcn_frexp_expf(v);
+}
+
+}  // namespace xtq

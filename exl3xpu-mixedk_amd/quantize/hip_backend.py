@@ -36,6 +36,13 @@ class HipViterbiError(RuntimeError):
         self.rc = rc
 
 
+class TrellisWeight(ctypes.Structure):
+    """xtq_weight of include/exl3_vit.h."""
+    _fields_ = [("trellis", ctypes.c_void_p), ("suh", ctypes.c_void_p), ("svh", ctypes.c_void_p),
+                ("scale", ctypes.c_float), ("k", ctypes.c_int32), ("n", ctypes.c_int32),
+                ("K", ctypes.c_int32), ("code", ctypes.c_char_p)]
+
+
 def lib():
     """Load libexl3vit.so once; raises if it has not been built."""
     global _LIB
@@ -68,6 +75,16 @@ def lib():
         L.xtq_had128_left_dev.argtypes = [vp, vp, vp, i32, i32, vp]
         L.xtq_had128_right_dev.argtypes = [vp, vp, vp, i32, i32, vp]
         L.xtq_had128_both_dev.argtypes = [vp, vp, vp, i32, i32, vp, vp, i32, vp]
+        wp, ll = ctypes.POINTER(TrellisWeight), ctypes.c_int64
+        L.xtq_linear_ws_bytes.argtypes = [wp, i32, i32]
+        L.xtq_linear_ws_bytes.restype = ll
+        L.xtq_linear_dev.argtypes = [wp, i32, vp, ll, i32, vp, i32, i32, vp, ll, vp, vp, ll, vp, ll,
+                                     vp, vp]
+        L.xtq_linear_bwd_dev.argtypes = [wp, i32, vp, ll, vp, i32, i32, vp, ll, vp, i32, vp, ll, vp,
+                                         vp]
+        L.xtq_gram_ws_bytes.argtypes = [i32, i32]
+        L.xtq_gram_ws_bytes.restype = ll
+        L.xtq_gram_dev.argtypes = [i32, vp, ll, i32, i32, vp, vp, vp, vp, ll, vp]
         L.xtq_vit_scratch_per_seq.argtypes = [i32]
         L.xtq_vit_scratch_per_seq.restype = i64
         L.xtq_vit_chunk_seqs.argtypes = [i32, i32, ctypes.POINTER(ctypes.c_int)]
@@ -86,7 +103,8 @@ def lib():
                    "xtq_trellis_decode_dev", "xtq_trellis_pack_dev",
                    "xtq_trellis_unpack_dev", "xtq_trellis_pack64_dev",
                    "xtq_trellis_unpack64_dev", "xtq_vit_get_lut", "xtq_had128_left_dev",
-                   "xtq_had128_right_dev", "xtq_had128_both_dev"):
+                   "xtq_had128_right_dev", "xtq_had128_both_dev", "xtq_linear_dev",
+                   "xtq_linear_bwd_dev", "xtq_gram_dev"):
             getattr(L, fn).restype = i32
         _LIB = L
     return _LIB

@@ -1,0 +1,248 @@
+"""trellis_ops.py -- products with weights in the EXL3 trellis format, on the GPU.
+
+What quantize_linear returns is multiplied with as it is: the weight stays in
+its trellis, the kernels decode it on the way to the matrix cores.
+
+    import quantize as xq, trellis_ops as xt
+    r = xq.quantize_linear(W, H, K=4, device="cuda", channel_scales=True)
+    w = xt.TrellisLinear.from_result(r)
+    y = xt.linear(x, w, bias=b, act="silu", residual=res)     # differentiable in x, bias, residual
+    G = xt.input_gram(x)                                      # the H of the next quantize_linear
+
+Activations are bfloat16 or float16 and results have their type; sums are fp32
+and every result is rounded once.  Calls are ordered on the current stream,
+never wait for the GPU, and can be captured in a HIP graph.  There is no
+fallback: tensors that are not on a HIP device raise.
+
+The reference multiplies with its weights in a serving stack of its own
+(serve/patches/0001-exl3-ops-mixed-k.patch); there is no counterpart here to
+cite for these functions.
+"""
+from __future__ import annotations
+
+import ctypes
+import os
+import sys
+
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import hip_backend as _hb  # noqa: E402
+
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_COUNTERS = 4096
+_counters: dict = {}
+
+
+def _counter_words(dev: torch.device, stream: int) -> torch.Tensor:
+    """The zeroed words a call counts its finished parts in: one set per stream,
+    since calls on one stream never overlap (every call leaves them zero).  A
+    captured call gets a set of its own, cleared inside the graph, because the
+    graph may be replayed on any stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(_COUNTERS, dtype=torch.int32, device=dev)
+    key = (dev.index, stream)
+    t = _counters.get(key)
+    if t is None:
+        t = _counters[key] = torch.zeros(_COUNTERS, dtype=torch.int32, device=dev)
+    return t
+
+
+class TrellisLinear:
+    """A trellis weight W [k in, n out] to multiply with: trellis int16
+    [k/16, n/16, 16K], suh [k] and svh [n] fp16 on one HIP device, their K and
+    code, and the weight's scale (quantize_linear's Wscale where the channel
+    scales do not hold it).  Nothing is laid out anew; the tensors are kept."""
+
+    def __init__(self, trellis: torch.Tensor, suh: torch.Tensor, svh: torch.Tensor, K: int,
+                 code: str = "exl3_mul1", scale: float = 1.0):
+        K = int(K)
+        if not 2 <= K <= 7:
+            raise ValueError(f"K must be 2..7, got {K}")
+        if _hb.code_name(code) == "1mad":
+            raise NotImplementedError("the products take the EXL3 codes (mul1, 3inst, mcg): "
+                                      "1mad's values are not fp16 numbers")
+        if trellis.dim() != 3 or trellis.shape[2] != 16 * K:
+            raise ValueError(f"trellis must be [k/16, n/16, {16 * K}], got {tuple(trellis.shape)}")
+        k, n = 16 * trellis.shape[0], 16 * trellis.shape[1]
+        if not k or not n or k % 128 or n % 128:
+            raise ValueError(f"k and n must be multiples of 128, got {k}, {n}")
+        if suh.shape != (k,) or svh.shape != (n,):
+            raise ValueError(f"suh must be [{k}] and svh [{n}], got {tuple(suh.shape)}, "
+                             f"{tuple(svh.shape)}")
+        self.trellis = _hb._dev_tensor(trellis, torch.int16, "trellis")
+        self.suh = _hb._dev_tensor(suh, torch.float16, "suh")
+        self.svh = _hb._dev_tensor(svh, torch.float16, "svh")
+        self.device = self.trellis.device
+        if self.suh.device != self.device or self.svh.device != self.device:
+            raise ValueError("trellis, suh and svh must be on one device")
+        self.k, self.n, self.K, self.code, self.scale = k, n, K, code, float(scale)
+        self._w = _hb.TrellisWeight(self.trellis.data_ptr(), self.suh.data_ptr(),
+                                    self.svh.data_ptr(), self.scale, k, n, K,
+                                    _hb.code_name(code).encode())
+        self._p = ctypes.byref(self._w)
+
+    @classmethod
+    def from_result(cls, r: dict, device="cuda") -> "TrellisLinear":
+        """From a quantize_linear result."""
+        return cls(r["trellis"].to(device), r["suh"].to(device).half(), r["svh"].to(device).half(),
+                   r["K"], code=r["code"], scale=1.0 if r["channel_scales"] else r["Wscale"])
+
+    def __call__(self, x, bias=None, act="none", residual=None):
+        return linear(x, self, bias=bias, act=act, residual=residual)
+
+
+def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """t [.., cols] as rows whose elements are consecutive (a copy if need be)."""
+    t = t.reshape(-1, cols) if t.dim() != 2 else t
+    if t.shape[0] > 1 and (t.stride(1) != 1 or t.stride(0) < cols):
+        return t.contiguous()
+    return t if t.shape[0] != 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def _check_act(act: str) -> int:
+    try:
+        return ACTS[act]
+    except KeyError:
+        raise ValueError(f"act {act!r} not in {tuple(ACTS)}") from None
+
+
+def _like(t: torch.Tensor, x: torch.Tensor, shape, name: str, dtypes) -> None:
+    if t.device != x.device or t.dtype not in dtypes or t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)} of {' or '.join(map(str, dtypes))} on "
+                         f"{x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _forward(x, w, bias, act, residual, keep_z):
+    rows = _rows(x, w.k)
+    m = rows.shape[0]
+    y = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
+    z = torch.empty(m, w.n, dtype=x.dtype, device=x.device) if keep_z else None
+    if m == 0:
+        return y, z
+    res = None if residual is None else _rows(residual, w.n)
+    bias = None if bias is None else bias.contiguous()
+    L = _hb.lib()
+    with torch.cuda.device(x.device):
+        stream = _hb._stream(x.device)
+        need = L.xtq_linear_ws_bytes(w._p, m, 0)
+        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+        rc = L.xtq_linear_dev(
+            w._p, _TYPES[x.dtype], rows.data_ptr(), _stride(rows), m,
+            None if bias is None else bias.data_ptr(), int(bias is not None and
+                                                           bias.dtype == torch.float32), act,
+            None if res is None else res.data_ptr(), 0 if res is None else _stride(res),
+            None if z is None else z.data_ptr(), y.data_ptr(), w.n, ws.data_ptr(), ws.numel(),
+            _counter_words(x.device, stream).data_ptr(), stream)
+    _hb._check("xtq_linear_dev", rc)
+    return y, z
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, residual, w, act):
+        need = ctx.needs_input_grad[0] or (bias is not None and ctx.needs_input_grad[1])
+        y, z = _forward(x, w, bias, act, residual, need and act != 0)
+        ctx.w, ctx.act, ctx.shape = w, act, x.shape
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(z)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        z, = ctx.saved_tensors
+        w = ctx.w
+        want_x, want_b, want_r = ctx.needs_input_grad[:3]
+        dx = dbias = None
+        if want_x or want_b:
+            rows = _rows(dy, w.n)
+            m = rows.shape[0]
+            if want_x:
+                dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device)
+            if want_b:
+                dbias = torch.empty(w.n, dtype=ctx.bias_dtype, device=dy.device)
+            if m == 0:
+                return dx, None if dbias is None else dbias.zero_(), dy if want_r else None, None, None
+            L = _hb.lib()
+            with torch.cuda.device(dy.device):
+                stream = _hb._stream(dy.device)
+                need = L.xtq_linear_ws_bytes(w._p, m, 1)
+                ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dy.device)
+                rc = L.xtq_linear_bwd_dev(
+                    w._p, _TYPES[dy.dtype], rows.data_ptr(), _stride(rows),
+                    None if z is None else z.data_ptr(), ctx.act, m,
+                    None if dx is None else dx.data_ptr(), w.k,
+                    None if dbias is None else dbias.data_ptr(),
+                    int(ctx.bias_dtype == torch.float32), ws.data_ptr(), ws.numel(),
+                    _counter_words(dy.device, stream).data_ptr(), stream)
+            _hb._check("xtq_linear_bwd_dev", rc)
+        return dx, dbias, dy if want_r else None, None, None
+
+
+def linear(x: torch.Tensor, w: TrellisLinear, bias: torch.Tensor | None = None,
+           act: str = "none", residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x W + bias) + residual for x [.., k] (bfloat16 or float16) -> [.., n]
+    in x's type.  act: none, relu, silu or gelu (erf).  bias [n] has x's type or
+    fp32, residual y's shape and x's type.  Differentiable in x, bias and
+    residual (once; the weight is frozen)."""
+    if x.dtype not in _TYPES:
+        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if x.device != w.device:
+        raise ValueError(f"x must be on {w.device}, got {x.device}")
+    if x.dim() < 1 or x.shape[-1] != w.k:
+        raise ValueError(f"x must be [.., {w.k}], got {tuple(x.shape)}")
+    a = _check_act(act)
+    if bias is not None:
+        _like(bias, x, (w.n,), "bias", (x.dtype, torch.float32))
+    if residual is not None:
+        _like(residual, x, (*x.shape[:-1], w.n), "residual", (x.dtype,))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, bias, residual)):
+        return _Linear.apply(x, bias, residual, w, a)
+    return _forward(x, w, bias, a, residual, False)[0]
+
+
+def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
+               prev: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """prev + sum of x_t x_t^T over the tokens t of x [.., k] (bfloat16 or
+    float16) that valid [..] (bool) keeps, as fp32 [k, k]: the input Gram that
+    quantize_linear takes as H_x.  Tokens left out may hold anything.  prev: the
+    Gram so far (None: zero); out: where to write (prev itself accumulates in
+    place)."""
+    if x.dtype not in _TYPES:
+        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"x must be a HIP device tensor, got {x.device}")
+    if x.dim() < 1 or not x.shape[-1] or x.shape[-1] % 128:
+        raise ValueError(f"x must be [.., k] with k a multiple of 128, got {tuple(x.shape)}")
+    k = x.shape[-1]
+    x = x.detach()
+    if valid is not None:
+        _like(valid, x, x.shape[:-1], "valid", (torch.bool,))
+        valid = valid.contiguous()
+    for t, name in ((prev, "prev"), (out, "out")):
+        if t is not None:
+            _like(t, x, (k, k), name, (torch.float32,))
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+    rows = _rows(x, k)
+    m = rows.shape[0]
+    if out is None:
+        out = torch.empty(k, k, dtype=torch.float32, device=x.device)
+    L = _hb.lib()
+    with torch.cuda.device(x.device):
+        need = L.xtq_gram_ws_bytes(m, k)
+        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+        rc = L.xtq_gram_dev(_TYPES[x.dtype], rows.data_ptr() if m else None,
+                            _stride(rows) if m else k, m, k,
+                            None if valid is None else valid.data_ptr(),
+                            None if prev is None else prev.data_ptr(), out.data_ptr(),
+                            ws.data_ptr() if need else None, ws.numel(), _hb._stream(x.device))
+    _hb._check("xtq_gram_dev", rc)
+    return out

@@ -41,6 +41,8 @@
  *  12  null or misaligned pointer argument
  *  13  a synchronous entry was given a stream that is being captured into a
  *      HIP graph (nothing was enqueued; the capture is left intact)
+ *  14  an operator's workspace is too small
+ *  15  an operator's element type or activation is not one of its list
  *
  * Environment (read on every call):
  *   XTQ_VIT_DEVIDX   device index for the host-pointer entries (default: the
@@ -304,6 +306,79 @@ XTQ_API int xtq_had128_right_dev(const float* d_h, const float* d_in, float* d_o
 XTQ_API int xtq_had128_both_dev(const float* d_h, const float* d_in, float* d_out, int rows,
                                 int cols, const float* d_row_scale, const float* d_col_scale,
                                 int divide, void* stream);
+
+/*
+ * Operators on trellis weights (no reference counterpart: the reference
+ * multiplies with its weights in a serving stack of its own).  A weight is what
+ * quantize_linear returns: W [k in][n out] = scale * diag(suh) B Wi B diag(svh),
+ * Wi the decoded trellis, B the block-128 transform of hadamard128
+ * (quantize.py:123-163), scale its Wscale (1 with channel scales).
+ *   - k and n are multiples of 128, K is 2..7, code "mul1", "3inst" or "mcg"
+ *     (fp16 values; else 8).  The structure is read during the call only.
+ *   - type: XTQ_BF16 or XTQ_F16, the type of all activations and results;
+ *     sums are fp32, results rounded once.
+ *   - rows are `stride` elements apart (at least their length), their elements
+ *     consecutive, at any address of their type's alignment.
+ *   - every operator is stream-ordered: it returns once its kernels are enqueued
+ *     on `stream`, allocates nothing, and may be recorded into a HIP graph.
+ *   - ws: device scratch of at least the operator's ws_bytes, 16-byte aligned,
+ *     of any contents, not shared with a call that may run at the same time.
+ *   - counters: XTQ_OP_COUNTERS words, 4-byte aligned, zero before their first
+ *     call; every call leaves them zero.  Not shared with a call that may run at
+ *     the same time.
+ *   - a NaN or an infinity in a row spreads over that row's results (as NaN,
+ *     mostly: the transforms take differences), never to other rows'.
+ *   - zero rows: nothing is enqueued, status 0.
+ */
+typedef struct xtq_weight {
+    const int16_t* trellis;   /* [k/16][n/16][16K] device */
+    const uint16_t* suh;      /* [k] fp16 device */
+    const uint16_t* svh;      /* [n] fp16 device */
+    float scale;
+    int32_t k, n, K;
+    const char* code;
+} xtq_weight;
+
+enum { XTQ_BF16 = 0, XTQ_F16 = 1 };
+enum { XTQ_ACT_NONE = 0, XTQ_ACT_RELU = 1, XTQ_ACT_SILU = 2, XTQ_ACT_GELU = 3 };
+enum { XTQ_OP_COUNTERS = 4096 };
+
+/*
+ * y = act(x W + bias) + res for x [rows][k], y [rows][n].
+ *   bias   [n] fp32 (bias_f32 != 0) or of the activations' type, or NULL
+ *   act    XTQ_ACT_*; gelu is the erf form
+ *   res    [rows][n], or NULL; may be y itself
+ *   z      [rows][n] contiguous (out): x W + bias, for xtq_linear_bwd_dev; or NULL
+ * At most 1,048,560 rows.
+ */
+XTQ_API int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int backward);
+XTQ_API int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_stride,
+                           int rows, const void* bias, int bias_f32, int act, const void* res,
+                           int64_t res_stride, void* z, void* y, int64_t y_stride, void* ws,
+                           int64_t ws_bytes, uint32_t* counters, void* stream);
+
+/*
+ * Gradient of xtq_linear_dev: with dz = dy act'(z), dx = dz W^T [rows][k] and
+ * dbias = the sum of dz's rows.
+ *   z      as the forward call wrote it (unused for XTQ_ACT_NONE)
+ *   dx     or NULL (then only dbias is computed)
+ *   dbias  [n] (out) fp32 or of the activations' type as bias_f32 says, or NULL
+ */
+XTQ_API int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy_stride,
+                               const void* z, int act, int rows, void* dx, int64_t dx_stride,
+                               void* dbias, int bias_f32, void* ws, int64_t ws_bytes,
+                               uint32_t* counters, void* stream);
+
+/*
+ * out = prev + X^T X, [k][k] fp32, over the rows of x [rows][k] whose valid byte
+ * is not zero (all rows for valid NULL; the others are not looked at): the input
+ * Gram that quantize_linear takes (quantize.py:750).  prev NULL: zero; it may be
+ * out itself.  Zero rows give prev or zero.  At most 2^30 rows.
+ */
+XTQ_API int64_t xtq_gram_ws_bytes(int rows, int k);
+XTQ_API int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, int k,
+                         const uint8_t* valid, const float* prev, float* out, void* ws,
+                         int64_t ws_bytes, void* stream);
 
 /*
  * Copies the fp32 decode table of `code` (65536 entries) into host memory
