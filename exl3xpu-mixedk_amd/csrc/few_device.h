@@ -1,0 +1,245 @@
+// few_device.h -- the inner loop of products with trellis weights for few rows.
+//
+// A wave multiplies 16-row groups of activations with "units" of 128 by 128
+// weights (8 by 8 tiles), decoding the trellis in its own registers, straight
+// into the matrix cores' operand layout.  In a tile's symbol order
+// (tensor_core_perm, quantize.py:101-118) the four symbols 32 (c % 8) + 8 q +
+// 4 (c / 8) .. + 3 are column c, rows 2q, 2q + 1, 2q + 8, 2q + 9: lane 16 q + c
+// takes them from one window of 16 + 3 K bits, and two tiles one below the other
+// give the 8 summed elements of its operand of v_mfma_f32_16x16x32_f16.  The
+// activations' fragments follow the same order of the summed dimension, in
+// which the lanes of a row differ in bits 1 and 2 only: of the block-128
+// transform's seven stages, five are inside a lane and two between lanes.
+#pragma once
+#include "operators.h"
+
+#pragma clang fp contract(off)
+
+namespace xtq {
+namespace {
+
+// Where a lane's window lies in every tile: byte offsets of its last words and
+// the shift.  (Words before the first are the stream's last: it is circular.)
+struct Window {
+    uint32_t o[3], sh;
+};
+
+template <int K>
+__device__ __forceinline__ Window lane_window(int lane) {
+    const int c = lane & 15, q = lane >> 4, t0 = 32 * (c & 7) + 8 * q + 4 * (c >> 3);
+    const int e = (t0 + 4) * K - 1, lo = e >> 5;        // the window's last bit
+    Window w;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) w.o[i] = 4u * (uint32_t)((lo - i + 8 * K) % (8 * K));
+    w.sh = 31u - ((uint32_t)e & 31u);
+    return w;
+}
+
+// Words of a window: 16 + 3 K bits ending at a multiple of 4 K.  At K = 7 they
+// can begin one bit before the second last word.
+template <int K>
+constexpr int kWinWords = K == 7 ? 3 : 2;
+
+// Two tile rows by eight tiles on their way from memory: 16 consecutive bytes a
+// lane (a lane loading its own windows' words took 16 cycles of the address
+// unit per load, four times its share of the decoding).  They pass through a
+// buffer of the wave's own in LDS, from which each lane reads its windows.
+template <int K>
+constexpr int kPairBytes = 512 * K;
+
+template <int K>
+struct PairRegs {
+    u4 r[(K + 1) / 2];
+};
+
+template <int K>
+__device__ __forceinline__ void load_pair(PairRegs<K>& t, const uint8_t* tiles, size_t row_bytes, int lane) {
+#pragma unroll
+    for (int i = 0; i < (K + 1) / 2; ++i) {
+        int c = 64 * i + lane;                          // 16-byte piece of the pair
+        if (K & 1) c = c < 32 * K ? c : lane;
+        const bool low = c >= 16 * K;
+        t.r[i] = *(const u4_a2*)(tiles + (low ? row_bytes : 0) + 16 * (low ? c - 16 * K : c));
+    }
+}
+
+template <int K>
+__device__ __forceinline__ void pair_to_lds(const PairRegs<K>& t, uint8_t* buf, int lane) {
+#pragma unroll
+    for (int i = 0; i < (K + 1) / 2; ++i)
+        if (!(K & 1) || i < K / 2 || lane < 32) *(u4*)(buf + 16 * (64 * i + lane)) = t.r[i];
+}
+
+// Orders a wave's own LDS accesses across its lanes (they execute in order; the
+// compiler must keep them so).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Four values of a window, as two pairs of halves.
+template <int K, int CODE>
+__device__ __forceinline__ u2 decode4(const uint32_t* d, uint32_t sh) {
+    const uint32_t w = __builtin_amdgcn_alignbit(d[1], d[0], sh);
+    const uint32_t s3 = w & 0xFFFFu, s2 = __builtin_amdgcn_ubfe(w, K, 16),
+                   s1 = __builtin_amdgcn_ubfe(w, 2 * K, 16);
+    uint32_t s0;
+    if constexpr (3 * K + 16 <= 32) {
+        s0 = __builtin_amdgcn_ubfe(w, 3 * K, 16);
+    } else {
+        const uint32_t hi = K == 7 ? __builtin_amdgcn_alignbit(d[kWinWords<K> - 1], d[1], sh) : d[1] >> sh;
+        s0 = __builtin_amdgcn_alignbit(hi, w, 3 * K) & 0xFFFFu;
+    }
+    return (u2){code_pair<CODE>(s0, s1), code_pair<CODE>(s2, s3)};
+}
+
+__device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b),
+                                                  c, 0, 0, 0);
+}
+
+// acc[g][j] += (tiles j of one pair of tile rows, in LDS) x (fragment g).
+template <int K, int CODE, int G>
+__device__ __forceinline__ void pair_product(f4 (&acc)[G][8], const uint8_t* buf, const Window& win,
+                                             const u4 (&x)[G]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint32_t d[2][kWinWords<K>];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < kWinWords<K>; ++i)
+                d[h][i] = *(const uint32_t*)(buf + win.o[i] + 256 * K * h + 32 * K * j);
+        const u2 a = decode4<K, CODE>(d[0], win.sh), b = decode4<K, CODE>(d[1], win.sh);
+        const u4 m = {a[0], a[1], b[0], b[1]};
+#pragma unroll
+        for (int g = 0; g < G; ++g) acc[g][j] = mfma16(m, x[g], acc[g][j]);
+    }
+}
+
+// A block's values are multiplied with 2^shift, which brings the largest to
+// [2^14, 2^15), before they are rounded to fp16.  A wave's sums go by the
+// smallest shift of its blocks so far: a block of a larger shift is brought down
+// (its fp16 values then lose nothing that counts beside the row's largest), and
+// the sums are when the smallest falls.
+constexpr int kNoShift = 1000;          // a block of zeros
+
+// One row's 128-column block, times its column scales, transformed and rounded,
+// by a wave whose lane l has columns 2 l and 2 l + 1 in x.  Returns the block's
+// shift.  frag: the block's fragments; lo (LO): what the rounding left, so that
+// products with both have 22 bits of the values.
+template <bool LO>
+__device__ __forceinline__ int row_to_frags(float a, float b, int lane, int row, uint32_t* frag, uint32_t* lo) {
+    transform_row(a, b, lane);
+    const float top = wave_max(fmaxf(fabsf(a), fabsf(b)));
+    const int sh = top == 0.0f ? kNoShift : shift_to(top, 14);
+    const int by = sh == kNoShift ? 0 : sh;
+    const float u = ldexpf(a, by), v = ldexpf(b, by);
+    const h2 r = {(_Float16)u, (_Float16)v};
+    // columns 16 i + 2 q + 8 e, + 1: words 2 (i & 1) + e of lane 16 q + row of fragment i / 2
+    const int i = lane >> 3, q = lane & 3, e = (lane >> 2) & 1;
+    const int at = ((i >> 1) * 64 + q * 16 + row) * 4 + 2 * (i & 1) + e;
+    frag[at] = __builtin_bit_cast(uint32_t, r);
+    if constexpr (LO) {
+        const h2 l = {(_Float16)(u - (float)r[0]), (_Float16)(v - (float)r[1])};
+        lo[at] = __builtin_bit_cast(uint32_t, l);
+    }
+    return sh;
+}
+
+// Lane l's two columns of a 128-column block of 16-bit values.
+__device__ __forceinline__ uint32_t load_two(const void* row, int lane) { return ((const u1_a2*)row)[lane]; }
+
+__device__ __forceinline__ void unpack_two(uint32_t w, int type, float& a, float& b) {
+    if (type == kBf16) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xFFFF0000u);
+    } else {
+        a = half_bits(w & 0xFFFFu);
+        b = half_bits(w >> 16);
+    }
+}
+
+// Brings a wave's sums and a block's fragments to one scale; `own`: the block's
+// shift, `shift`: the sums', f: what the fragments are multiplied with.
+__device__ __forceinline__ void meet(f4 (&acc)[8], int& shift, int own, float& f) {
+    const int now = own < shift ? own : shift;
+    if (__any(now < shift && shift != kNoShift)) {
+        const float d = shift == kNoShift ? 1.0f : ldexpf(1.0f, now - shift);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] *= d;
+    }
+    shift = now;
+    f = own == kNoShift ? 1.0f : ldexpf(1.0f, now - own);
+}
+
+__device__ __forceinline__ u4 scaled(u4 x, float f) {
+    const _Float16 h = (_Float16)f;
+    return __builtin_bit_cast(u4, __builtin_bit_cast(h8, x) * (h8){h, h, h, h, h, h, h, h});
+}
+
+// Joining workgroups.  store_shared and load_shared pass what workgroups of other
+// XCDs, whose L2 is another, have to see: agent-scope accesses go through to
+// memory.  arrive is called by all threads once their stores are issued: each
+// wave waits for its own, then one thread counts the workgroup; true for the
+// last of `parts`, which has cleared the count for the next call and may read
+// all parts with load_shared.  (Release and acquire fences would write back and
+// drop whole L2 caches for these few lines.)
+typedef unsigned long long u64;
+__device__ __forceinline__ void store_shared(float* p, f4 v) {
+    const u4 b = __builtin_bit_cast(u4, v);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        __hip_atomic_store((u64*)p + i, (u64)b[2 * i] | (u64)b[2 * i + 1] << 32, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ f4 load_shared(const float* p) {
+    u4 b;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const u64 t = __hip_atomic_load((const u64*)p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        b[2 * i] = (uint32_t)t;
+        b[2 * i + 1] = (uint32_t)(t >> 32);
+    }
+    return __builtin_bit_cast(f4, b);
+}
+
+__device__ __forceinline__ bool arrive(uint32_t* counter, uint32_t parts, int thread) {
+    __shared__ uint32_t before;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (thread == 0) {
+        before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == parts - 1)
+            __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return before == parts - 1;
+}
+
+// Sums over `parts` parts, `stride` floats apart, in order, U of them in flight:
+// what a load waits for here is a trip to memory and back.
+template <int U, int N>
+__device__ __forceinline__ void sum_shared(f4 (&t)[N], const float* p, int step, size_t stride, int parts) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) t[n] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < parts; s += U) {
+        f4 v[U][N];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                v[i][n] = load_shared(p + n * step + (s + i < parts ? s + i : parts - 1) * stride);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (s + i < parts) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) t[n] += v[i][n];
+            }
+    }
+}
+
+}  // namespace
+}  // namespace xtq

@@ -14,6 +14,8 @@
 // one v_mfma_f32_16x16x32.  A fragment moves from memory to LDS and from LDS to
 // registers as 64 consecutive 16-byte pieces: no bank conflict, no address
 // arithmetic.
+#include "epilogue.h"
+#include "few_device.h"
 #include "operators.h"
 
 #pragma clang fp contract(off)
@@ -137,10 +139,11 @@ __global__ __launch_bounds__(256) void transform_kernel(Source s, const int32_t*
             }
     const int sh = row < s.rows ? shift[row] : 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        v[i] = cross_stage<16>(v[i], lane);
-        v[i] = cross_stage<32>(v[i], lane);
+    for (int i = 0; i < 32; i += 2) {
+        cross_pair<16>(v[i], v[i + 1]);
+        cross_pair<32>(v[i], v[i + 1]);
         v[i] = ldexpf(v[i], sh);
+        v[i + 1] = ldexpf(v[i + 1], sh);
     }
     uint16_t* out = frags + ((size_t)grp * nblk + blk) * 2048 + lane * 8;
 #pragma unroll
@@ -205,77 +208,6 @@ __global__ __launch_bounds__(256) void decode_frag_kernel(const int16_t* __restr
         const size_t g = BWD ? i0 + wv : j0 + wv;
         const size_t np = (BWD ? tn : tk) / 2, f = (BWD ? j0 : i0) / 2 + p;
         *(u4*)(frags + (g * np + f) * 512 + lane * 8) = o;
-    }
-}
-
-// ------------------------------------------------------------------ epilogue
-// Results of 128 columns by 16 rows in a wave's registers: v[j][i] of lane
-// 16 q + r is column 16 j + 4 q + i of row r.
-template <int T>
-__device__ void finish_unit(f4* v, const Epilogue& ep, int grp, int blk, int lane) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const f4 a = v[j];
-        const float s0 = a[0] + a[1], d0 = a[0] - a[1], s1 = a[2] + a[3], d1 = a[2] - a[3];
-        v[j] = (f4){s0 + s1, d0 + d1, s0 - s1, d0 - d1};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[j][i] = cross_stage<16>(v[j][i], lane);
-            v[j][i] = cross_stage<32>(v[j][i], lane);
-        }
-    }
-#pragma unroll
-    for (int b = 1; b < 8; b <<= 1)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (!(j & b)) {
-                const f4 a = v[j], c = v[j | b];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[j][i] = a[i] + c[i];
-                    v[j | b][i] = a[i] - c[i];
-                }
-            }
-    const int row = grp * 16 + (lane & 15), q = lane >> 4;
-    if (row >= ep.rows) return;
-    const int e = ep.rowexp ? ep.rowexp[row] : 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int col = blk * 128 + 16 * j + 4 * q;
-        const u2 cs = *(const u2_a2*)(ep.colscale + col);
-        f4 o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            o[i] = ldexpf(v[j][i], e) * (half_bits((cs[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) * ep.scale);
-        if (ep.bias) {
-            if (ep.bias_f32) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] += ((const float*)ep.bias)[col + i];
-            } else {
-                const u2 b = *(const u2_a2*)((const uint16_t*)ep.bias + col);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] += from16<T>((b[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-            }
-        }
-        if (ep.z) {
-            u2 w;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) w[i] = to16<T>(o[2 * i]) | to16<T>(o[2 * i + 1]) << 16;
-            *(u2_a2*)((uint16_t*)ep.z + (size_t)row * ep.cols + col) = w;
-        }
-        if (ep.act != kActNone) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = act_value(o[i], ep.act);
-        }
-        if (ep.res) {
-            const u2 b = *(const u2_a2*)((const uint16_t*)ep.res + (size_t)row * ep.res_stride + col);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] += from16<T>((b[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-        }
-        u2 w;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = to16<T>(o[2 * i]) | to16<T>(o[2 * i + 1]) << 16;
-        *(u2_a2*)((uint16_t*)ep.y + (size_t)row * ep.y_stride + col) = w;
     }
 }
 
@@ -552,15 +484,81 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
     return hipGetLastError();
 }
 
+// Rows to fragments for the products of few rows, a wave for one row's
+// 128-column block.  Rows past the end are zeros.
+__global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __restrict__ x, long long stride,
+                                                            int type, int rows, int k,
+                                                            const uint16_t* __restrict__ suh,
+                                                            u4* __restrict__ frag, int32_t* __restrict__ shift) {
+    const int lane = threadIdx.x & 63, nk = k / 128;
+    const int kb = blockIdx.x * 4 + (threadIdx.x >> 6), row = blockIdx.y;
+    if (kb >= nk) return;
+    float a = 0.0f, b = 0.0f, sa, sb;
+    if (row < rows) unpack_two(load_two(x + (size_t)row * stride + 128 * kb, lane), type, a, b);
+    unpack_two(load_two(suh + 128 * kb, lane), kF16, sa, sb);
+    const size_t at = (size_t)(row >> 4) * nk + kb;
+    const int sh = row_to_frags<false>(a * sa, b * sb, lane, row & 15, (uint32_t*)(frag + at * 256), nullptr);
+    if (lane == 0) shift[at * 16 + (row & 15)] = sh;
+}
+
+// Workgroups per 128 columns of a product of few rows: two for each compute
+// unit, each wave with two 32-row steps at least.
+int few_splits(int k, int n) {
+    const int most = k / 256;
+    int s = 2 * kCUs / (n / 128);
+    if (s > most) s = most;
+    return s < 1 ? 1 : s;
+}
+
+bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_COUNTERS; }
+
+int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+struct FewPlan {
+    int splits;
+    size_t part, frag, shift, total;
+};
+
+FewPlan few_plan(int rows, int k, int n) {
+    FewPlan p;
+    p.splits = few_splits(k, n);
+    const int g = few_groups(rows);
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t a = at; at += align256(bytes); return a; };
+    p.part = take(p.splits > 1 ? (size_t)p.splits * n * g * 64 : 0);
+    const bool apart = rows > kFusedRows;
+    p.frag = take(apart ? (size_t)g * k * 32 : 0);
+    p.shift = take(apart ? (size_t)g * k / 2 : 0);
+    p.total = at;
+    return p;
+}
+
 }  // namespace
 
 size_t linear_ws_bytes(int rows, int k, int n, int backward) {
+    if (!backward && takes_few(rows, n)) return few_plan(rows, k, n).total;
     return backward ? many_plan(rows, n, k, true).total : many_plan(rows, k, n, false).total;
 }
 
 hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
                          const Epilogue& ep, void* ws, uint32_t* counters, hipStream_t s) {
-    (void)counters;
+    if (takes_few(rows, w.n)) {
+        static decltype(&launch_few_k2) const few[] = {launch_few_k2, launch_few_k3, launch_few_k4,
+                                                       launch_few_k5, launch_few_k6, launch_few_k7};
+        const FewPlan p = few_plan(rows, w.k, w.n);
+        uint8_t* base = (uint8_t*)ws;
+        FewArgs a{type, (const uint16_t*)x, x_stride, nullptr, nullptr, p.splits, w.k / 32 / p.splits,
+                  w.k / 32 % p.splits, 65536u / rows + 1, (float*)(base + p.part), counters};
+        if (rows > kFusedRows) {
+            u4* frag = (u4*)(base + p.frag);
+            int32_t* shift = (int32_t*)(base + p.shift);
+            hipLaunchKernelGGL(transform_few_kernel, dim3((w.k / 128 + 3) / 4, 16 * few_groups(rows)),
+                               dim3(256), 0, s, a.x, x_stride, type, rows, w.k, w.suh, frag, shift);
+            a.frag = frag;
+            a.shift = shift;
+        }
+        return few[w.K - 2](w, a, ep, s);
+    }
     const Source src{(const uint16_t*)x, x_stride, nullptr, 0, w.suh, type, rows, w.k};
     return type == kBf16 ? many<kBf16>(w, 0, src, ep, nullptr, 0, ws, s)
                          : many<kF16>(w, 0, src, ep, nullptr, 0, ws, s);

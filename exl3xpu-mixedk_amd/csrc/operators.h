@@ -47,6 +47,29 @@ hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long lon
                              void* dbias, int dbias_f32, void* ws, uint32_t* counters,
                              hipStream_t s);
 
+// Products of up to kFewRows rows (few_kernels.hip), one function per K.  Up to
+// kFusedRows rows the product's kernel transforms x itself; more come
+// transformed (transform_few_kernel): fragments frag [group of 16 rows][k/32][64] and
+// their shifts [group][k/128][16].
+constexpr int kFewRows = 64;
+constexpr int kFusedRows = 16;
+constexpr int kFewWaves = 4;            // waves of a workgroup
+struct FewArgs {
+    int type;
+    const uint16_t* x;
+    long long x_stride;
+    const u4* frag;
+    const int32_t* shift;
+    int splits, steps, more;            // 32-row steps of a split; splits with one more
+    uint32_t rinv;                      // item / rows is item * rinv >> 16
+    float* part;
+    uint32_t* counters;
+};
+#define XTQ_FEW(K) \
+    hipError_t launch_few_k##K(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s);
+XTQ_FEW(2) XTQ_FEW(3) XTQ_FEW(4) XTQ_FEW(5) XTQ_FEW(6) XTQ_FEW(7)
+#undef XTQ_FEW
+
 size_t gram_ws_bytes(int rows, int k);
 hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, int k,
                        const uint8_t* valid, const float* prev, float* out, void* ws,

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "viterbi_kernels.h"
 
 namespace xtq {
@@ -70,13 +72,22 @@ __device__ __forceinline__ float half_bits(uint32_t bits) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
-// Activations in fp32 (act is uniform).  silu's exp overflows to infinity for
-// z < -88 and the quotient is then -0; gelu is the erf form.
-__device__ __forceinline__ float act_value(float z, int act) {
-    if (act == kActRelu) return z > 0.0f ? z : (z == z ? 0.0f : z);
-    if (act == kActSilu) return z / (1.0f + expf(-z));
-    if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    return z;
+// Activations in fp32 (act is uniform); relu keeps NaN.  silu's exp overflows to
+// infinity for z < -88, its reciprocal is 0 and the product -0; v_rcp_f32 and the
+// exponential are within a few units of 2^-24 of a result that is rounded to
+// 16 bits.  gelu is the erf form.
+template <int N>
+__device__ __forceinline__ void activate(float* v, int act) {
+    if (act == kActRelu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+    } else if (act == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= __builtin_amdgcn_rcpf(1.0f + expf(-v[i]));
+    } else if (act == kActGelu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= 0.5f * (1.0f + erff(v[i] * 0.70710678118654752f));
+    }
 }
 
 // Slope of the activation at z; at infinities the limits (z * exp(-z^2/2)
@@ -95,18 +106,79 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     return 1.0f;
 }
 
-// Value of the lane whose number differs in bit 4 (M = 16) or 5 (M = 32).
-template <int M>
-__device__ __forceinline__ float lane_xor(float v) {
-    return __shfl_xor(v, M);
+// Largest value of the lanes that differ in bits 4 and 5.
+__device__ __forceinline__ float rows_max(float v) {
+    const uint32_t a = __float_as_uint(v);
+    auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const uint32_t b = __float_as_uint(v);
+    r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// One stage of the block-128 transform over a lane bit: this lane's sum or
-// difference with its partner's.
+// Value of the lane whose number differs in one bit, M = 1, 2, 4 or 8 (bits
+// inside a row of 16 lanes: data-parallel moves; 4 is the mirror of 8 lanes and
+// the mirror of 4).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    const int b = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, 0xf, 0xf, true));
+}
 template <int M>
-__device__ __forceinline__ float cross_stage(float v, uint32_t lane) {
-    const float o = lane_xor<M>(v);
-    return (lane & M) ? o - v : v + o;
+__device__ __forceinline__ float lane_xor(float v) {
+    if constexpr (M == 1) return dpp<0xB1>(v);
+    else if constexpr (M == 2) return dpp<0x4E>(v);
+    else if constexpr (M == 4) return dpp<0x141>(dpp<0x1B>(v));
+    else return dpp<0x128>(v);
+}
+
+// Largest value of the wave.
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, lane_xor<1>(v));
+    v = fmaxf(v, lane_xor<2>(v));
+    v = fmaxf(v, dpp<0x141>(v));        // the mirror of 8 lanes, of 16: any partner of the other half will do
+    v = fmaxf(v, dpp<0x140>(v));
+    return rows_max(v);
+}
+
+// One stage of the block-128 transform over lane bit 4 (M = 16) or 5 (M = 32),
+// for two values a lane: v_permlane16_swap and v_permlane32_swap exchange one register's upper rows (half) with the other's
+// lower, so one sum and one difference serve both lanes' values, and a second
+// swap brings them home.
+template <int M>
+__device__ __forceinline__ void cross_pair(float& a, float& b) {
+    auto swap = [](float& x, float& y) {
+        const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+        auto r = M == 32 ? __builtin_amdgcn_permlane32_swap(u, v, false, false)
+                         : __builtin_amdgcn_permlane16_swap(u, v, false, false);
+        x = __uint_as_float(r[0]);
+        y = __uint_as_float(r[1]);
+    };
+    swap(a, b);
+    const float s = a + b, d = a - b;
+    a = s;
+    b = d;
+    swap(a, b);
+}
+
+// Block-128 transform (without its 1/sqrt(128)) of one row by a wave: lane l
+// holds elements 2 l and 2 l + 1.
+__device__ __forceinline__ void transform_row(float& a, float& b, int lane) {
+    float s = a + b, d = a - b;
+    auto stage = [&](auto m) {
+        constexpr int M = decltype(m)::value;
+        const float os = lane_xor<M>(s), od = lane_xor<M>(d);
+        s = (lane & M) ? os - s : s + os;
+        d = (lane & M) ? od - d : d + od;
+    };
+    stage(std::integral_constant<int, 1>());
+    stage(std::integral_constant<int, 2>());
+    stage(std::integral_constant<int, 4>());
+    stage(std::integral_constant<int, 8>());
+    cross_pair<16>(s, d);
+    cross_pair<32>(s, d);
+    a = s;
+    b = d;
 }
 
 // Exponent s with v * 2^s in [2^top, 2^(top+1)) for finite v > 0; 0 for 0,
