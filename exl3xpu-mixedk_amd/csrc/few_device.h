@@ -99,10 +99,11 @@ __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
                                                   c, 0, 0, 0);
 }
 
-// acc[g][j] += (tiles j of one pair of tile rows, in LDS) x (fragment g).
-template <int K, int CODE, int G>
+// acc[g][j] += (tiles j of one pair of tile rows, in LDS) x (fragment g, and with
+// LO what its rounding left).
+template <int K, int CODE, int G, bool LO>
 __device__ __forceinline__ void pair_product(f4 (&acc)[G][8], const uint8_t* buf, const Window& win,
-                                             const u4 (&x)[G]) {
+                                             const u4 (&x)[G], const u4 (&lo)[G]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         uint32_t d[2][kWinWords<K>];
@@ -114,7 +115,10 @@ __device__ __forceinline__ void pair_product(f4 (&acc)[G][8], const uint8_t* buf
         const u2 a = decode4<K, CODE>(d[0], win.sh), b = decode4<K, CODE>(d[1], win.sh);
         const u4 m = {a[0], a[1], b[0], b[1]};
 #pragma unroll
-        for (int g = 0; g < G; ++g) acc[g][j] = mfma16(m, x[g], acc[g][j]);
+        for (int g = 0; g < G; ++g) {
+            acc[g][j] = mfma16(m, x[g], acc[g][j]);
+            if constexpr (LO) acc[g][j] = mfma16(m, lo[g], acc[g][j]);
+        }
     }
 }
 
@@ -239,6 +243,174 @@ __device__ __forceinline__ void sum_shared(f4 (&t)[N], const float* p, int step,
                 for (int n = 0; n < N; ++n) t[n] += v[i][n];
             }
     }
+}
+
+// What a workgroup multiplies: 128 columns of a weight, from `tiles` (row_bytes
+// from one tile row to the next), by up to 16 G rows.
+struct FewSource {
+    const uint8_t* tiles;
+    size_t row_bytes;
+    int rows, pairs;                    // pairs: 32-row steps of the weight
+    // FUSED: the rows, transformed here; row i is row list[i] of x (list NULL: i)
+    const uint16_t* x;
+    long long x_stride;
+    const int32_t* list;
+    const uint16_t* suh;
+    int type;
+    uint32_t rinv;                      // item / rows is item * rinv >> 16
+    // else the rows' fragments [g][pair][64] and shifts [g][block][16]
+    const u4 *hi, *lo;
+    const int32_t* shift;
+};
+
+// Blocks transformed at a time (FUSED); 4 KiB of LDS each, 8 with LO.
+template <bool LO>
+constexpr int kSlice = LO ? 4 : 8;
+// 16-byte words of LDS that few_sums takes: the rows' fragments, later the waves'
+// sums.
+constexpr int kFewLds = 2048;
+constexpr int kFewTotals = 8 / kFewWaves;               // tile columns a wave adds
+
+// Sums of steps s0 .. s1 of the summed dimension: total[g][i] of a wave's lane is
+// tile column i kFewWaves + wave of row group g, in the matrix cores' layout.
+template <int K, int CODE, int G, bool FUSED, bool LO>
+__device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4* lds, uint8_t* buf,
+                                         int32_t* shifts, f4 (&total)[G][kFewTotals]) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Window win = lane_window<K>(lane);
+    u4 *const frag = lds, *const frag_lo = lds + kSlice<LO> * 256;
+    f4* const sums = (f4*)lds;
+    f4 acc[G][8];
+    int shift[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        shift[g] = kNoShift;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[g][j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int c0 = s0; c0 < s1;) {
+        const int kb0 = c0 >> 2, cut = (kb0 + kSlice<LO>) << 2, c1 = FUSED && cut < s1 ? cut : s1;
+        const int p0 = c0 + (c1 - c0) * wv / kFewWaves, p1 = c0 + (c1 - c0) * (wv + 1) / kFewWaves;
+        PairRegs<K> r[2];
+        auto load = [&](PairRegs<K>& t, int p) {
+            p = p < p1 ? p : p1 - 1;
+            load_pair<K>(t, a.tiles + (size_t)p * 2 * a.row_bytes, a.row_bytes, lane);
+        };
+        if constexpr (FUSED) {
+            const int nk = ((c1 + 3) >> 2) - kb0, items = a.rows * nk;
+            if (c0 > s0) __syncthreads();
+            for (int t = wv; t < items || t == wv; t += 4 * kFewWaves) {
+                uint32_t xw[4], sw[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int item = t + i * kFewWaves;
+                    if (item >= items) break;
+                    const int kbi = item * a.rinv >> 16, row = item - kbi * a.rows;
+                    const size_t at = a.list ? a.list[row] : row;
+                    xw[i] = load_two(a.x + at * a.x_stride + 128 * (kb0 + kbi), lane);
+                    sw[i] = load_two(a.suh + 128 * (kb0 + kbi), lane);
+                }
+                if (t == wv && p0 < p1) {               // behind the first rows' loads
+                    load(r[0], p0);
+                    load(r[1], p0 + 1);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int item = t + i * kFewWaves;
+                    if (item >= items) break;
+                    const int kbi = item * a.rinv >> 16, row = item - kbi * a.rows;
+                    float u, v, su, sv;
+                    unpack_two(xw[i], a.type, u, v);
+                    unpack_two(sw[i], kF16, su, sv);
+                    const int sh = row_to_frags<LO>(u * su, v * sv, lane, row, (uint32_t*)(frag + kbi * 256),
+                                                    (uint32_t*)(frag_lo + kbi * 256));
+                    if (lane == 0) shifts[kbi * 16 + row] = sh;
+                }
+            }
+            __syncthreads();
+        } else if (p0 < p1) {
+            load(r[0], p0);
+            load(r[1], p0 + 1);
+        }
+        u4 x[G], lo[G], nx[G], nlo[G];
+        float f[G];
+        const u4 zero = {0u, 0u, 0u, 0u};
+        // rows past the end have no fragments: zeros
+        auto fetch = [&](u4 (&t)[G], u4 (&u)[G], int p) {
+            if constexpr (FUSED) {
+                const bool in = (lane & 15) < a.rows;
+                t[0] = in ? frag[(p - 4 * kb0) * 64 + lane] : zero;
+                if constexpr (LO) u[0] = in ? frag_lo[(p - 4 * kb0) * 64 + lane] : zero;
+            } else {
+                p = p < p1 ? p : p1 - 1;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const bool in = 16 * g + (lane & 15) < a.rows;
+                    t[g] = in ? a.hi[((size_t)g * a.pairs + p) * 64 + lane] : zero;
+                    if constexpr (LO) u[g] = in ? a.lo[((size_t)g * a.pairs + p) * 64 + lane] : zero;
+                }
+            }
+        };
+        // pair p lies in its buffer, p + 1 is on its way in r[odd ^ 1], p + 2 in r[odd]
+        auto step = [&](int p, int odd) {
+            pair_to_lds<K>(r[odd ^ 1], buf + (odd ^ 1) * kPairBytes<K>, lane);
+            load(r[odd ^ 1], p + 3);
+            if (p == p0 || (p & 3) == 0) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    int own = kNoShift;
+                    if (16 * g + (lane & 15) < a.rows)
+                        own = FUSED ? shifts[((p >> 2) - kb0) * 16 + (lane & 15)]
+                                    : a.shift[((size_t)g * (a.pairs >> 2) + (p >> 2)) * 16 + (lane & 15)];
+                    meet(acc[g], shift[g], own, f[g]);
+                }
+            }
+            if constexpr (FUSED) {
+                fetch(x, lo, p);
+            } else {
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    x[g] = nx[g];
+                    if constexpr (LO) lo[g] = nlo[g];
+                }
+                fetch(nx, nlo, p + 1);
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                x[g] = scaled(x[g], f[g]);
+                if constexpr (LO) lo[g] = scaled(lo[g], f[g]);
+            }
+            pair_product<K, CODE, G, LO>(acc, buf + odd * kPairBytes<K>, win, x, lo);
+            wave_sync();
+        };
+        if (p0 < p1) {
+            if constexpr (!FUSED) fetch(nx, nlo, p0);
+            pair_to_lds<K>(r[0], buf, lane);
+            load(r[0], p0 + 2);
+            wave_sync();
+            for (int p = p0; p < p1; p += 2) {
+                step(p, 0);
+                if (p + 1 < p1) step(p + 1, 1);
+            }
+        }
+        c0 = c1;
+    }
+    // the waves' sums, in the order of the waves
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const float s = shift[g] == kNoShift ? 0.0f : ldexpf(1.0f, -shift[g] - 7);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[(wv * 8 + j) * 64 + lane] = acc[g][j] * s;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kFewTotals; ++i) {
+            total[g][i] = sums[(i * kFewWaves + wv) * 64 + lane];
+#pragma unroll
+            for (int o = 1; o < kFewWaves; ++o) total[g][i] += sums[(o * 8 + i * kFewWaves + wv) * 64 + lane];
+        }
+    }
+    __syncthreads();
 }
 
 }  // namespace

@@ -1,0 +1,235 @@
+// moe_kernels.hip -- the mixture layer's products with its experts' trellis
+// weights, for a few rows: gate and up, then down.
+//
+// Built once per codebook (XTQ_MOE_CODE); the experts' widths are chosen in the
+// kernels, per workgroup.
+#include "epilogue.h"
+#include "moe_device.h"
+
+#pragma clang fp contract(off)
+
+namespace xtq {
+namespace {
+
+constexpr int kCode = XTQ_MOE_CODE;
+constexpr int kMaxPairBytes = kPairBytes<7>;
+
+// few_sums of an expert's width (one of 2..7: checked when the table was made).
+template <bool FUSED>
+__device__ __forceinline__ void expert_sums(int K, const FewSource& src, int s0, int s1, u4* lds, uint8_t* buf,
+                                            int32_t* shifts, f4 (&total)[1][kFewTotals]) {
+    switch (K) {
+        case 2: return few_sums<2, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
+        case 3: return few_sums<3, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
+        case 4: return few_sums<4, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
+        case 5: return few_sums<5, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
+        case 6: return few_sums<6, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
+        default: return few_sums<7, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
+    }
+}
+
+__device__ __forceinline__ void split_range(int pairs, int splits, int split, int& s0, int& s1) {
+    const int each = pairs / splits, more = pairs - each * splits;
+    s0 = split * each + (split < more ? split : more);
+    s1 = s0 + each + (split < more ? 1 : 0);
+}
+
+// Rows of x for the first product, as fragments and what their rounding left,
+// one wave per chunk, weight (gate, up) and 128-column block.
+__global__ __launch_bounds__(256) void moe_x_kernel(MoeArgs a) {
+    const int lane = threadIdx.x & 63, nk = a.d / 128, role = blockIdx.y, ch = blockIdx.z;
+    const int kb = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (ch >= *a.nchunks || kb >= nk) return;
+    const MoeChunk& c = a.chunks[ch];
+    const xtq_moe_weight w = a.table[3 * c.expert + role];
+    float su, sv;
+    unpack_two(load_two(w.suh + 128 * kb, lane), kF16, su, sv);
+    u4* hi = a.xf + ((size_t)(ch * 2 + role) * 2 * nk + kb) * 256;
+    int32_t* sh = a.xs + ((size_t)(ch * 2 + role) * nk + kb) * 16;
+#pragma unroll 4
+    for (int r = 0; r < c.rows; ++r) {
+        const size_t row = c.slots[r] / a.top;
+        float u, v;
+        unpack_two(load_two(a.x + row * a.x_stride + 128 * kb, lane), a.type, u, v);
+        const int s = row_to_frags<true>(u * su, v * sv, lane, r, (uint32_t*)hi, (uint32_t*)(hi + (size_t)nk * 256));
+        if (lane == 0) sh[r] = s;
+    }
+}
+
+// One weight's (gate's or up's) 128 columns for a chunk over a part of the summed
+// dimension; the last workgroup of the two weights' parts adds them, applies the
+// activation and leaves the product's rows as fragments for the second product.
+template <bool FUSED>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void moe_up_kernel(MoeArgs a) {
+    __shared__ __align__(16) u4 lds[kFewLds];
+    __shared__ __align__(16) uint8_t bufs[kFewWaves][2][kMaxPairBytes];
+    __shared__ int32_t shifts[kSlice<true> * 16];
+    __shared__ int32_t list[16];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nf = a.f / 128, nk = a.d / 128, ch = blockIdx.z, split = blockIdx.y;
+    const int fb = blockIdx.x >> 1, role = blockIdx.x & 1;
+    if (ch >= *a.nchunks) return;
+    const MoeChunk& c = a.chunks[ch];
+    const int rows = c.rows;
+    const xtq_moe_weight w = a.table[3 * c.expert + role];
+    if (FUSED && threadIdx.x < rows) list[threadIdx.x] = c.slots[threadIdx.x] / a.top;
+    if (FUSED) __syncthreads();
+    int s0, s1;
+    split_range(a.d / 32, a.up_splits, split, s0, s1);
+    const u4* hi = FUSED ? nullptr : a.xf + (size_t)(ch * 2 + role) * 2 * nk * 256;
+    const FewSource src{(const uint8_t*)w.trellis + (size_t)fb * 256 * w.K, (size_t)nf * 256 * w.K, rows, a.d / 32,
+                        a.x, a.x_stride, list, w.suh, a.type, 65536u / rows + 1, hi,
+                        FUSED ? nullptr : hi + (size_t)nk * 256,
+                        FUSED ? nullptr : a.xs + (size_t)(ch * 2 + role) * nk * 16};
+    f4 total[1][kFewTotals];
+    expert_sums<FUSED>(w.K, src, s0, s1, lds, bufs[wv][0], shifts, total);
+    // [chunk][fb][role][split]
+    float* part = a.up_part + ((size_t)ch * nf + fb) * 2 * a.up_splits * 2048 + wv * 256 + lane * 4;
+    const bool mine = (lane & 15) < rows;
+    if (mine) {
+#pragma unroll
+        for (int i = 0; i < kFewTotals; ++i)
+            store_shared(part + (size_t)(role * a.up_splits + split) * 2048 + i * kFewWaves * 256, total[0][i]);
+    }
+    if (!arrive(a.counters + kMoeRouterCounters + a.d / 128 + ch * nf + fb, 2 * a.up_splits, threadIdx.x)) return;
+    f4* const sums = (f4*)lds;
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+#pragma unroll
+        for (int i = 0; i < kFewTotals; ++i) total[0][i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+        if (mine) sum_shared<8>(total[0], part + (size_t)o * a.up_splits * 2048, kFewWaves * 256, 2048, a.up_splits);
+#pragma unroll
+        for (int i = 0; i < kFewTotals; ++i) sums[(o * 8 + i * kFewWaves + wv) * 64 + lane] = total[0][i];
+    }
+    const xtq_moe_weight wg = a.table[3 * c.expert], wu = a.table[3 * c.expert + 1], wd = a.table[3 * c.expert + 2];
+    float g0, g1, u0, u1, d0, d1;
+    unpack_two(load_two(wg.svh + 128 * fb, lane), kF16, g0, g1);
+    unpack_two(load_two(wu.svh + 128 * fb, lane), kF16, u0, u1);
+    unpack_two(load_two(wd.suh + 128 * fb, lane), kF16, d0, d1);
+    __syncthreads();
+    u4* out = a.hf + ((size_t)ch * 2 * nf + fb) * 256;
+    for (int r = wv; r < rows; r += kFewWaves) {
+        float v[2], u[2];
+        unit_row(sums, r, lane, v[0], v[1]);
+        unit_row(sums + 512, r, lane, u[0], u[1]);
+        transform_row(v[0], v[1], lane);
+        transform_row(u[0], u[1], lane);
+        v[0] *= g0 * wg.scale;
+        v[1] *= g1 * wg.scale;
+        activate<2>(v, a.act);
+        v[0] *= u[0] * (u0 * wu.scale);
+        v[1] *= u[1] * (u1 * wu.scale);
+        const int sh = row_to_frags<true>(v[0] * d0, v[1] * d1, lane, r, (uint32_t*)out,
+                                          (uint32_t*)(out + (size_t)nf * 256));
+        if (lane == 0) a.hs[((size_t)ch * nf + fb) * 16 + r] = sh;
+    }
+}
+
+// The last step for 128 columns: each row's residual and the weighted results
+// of its slots, four rows in flight by a wave.
+__device__ __forceinline__ void moe_finish(const MoeArgs& a, int db, int first, int step, int lane) {
+    const int col = 128 * db + 2 * lane;
+    const size_t slots = (size_t)a.rows * a.top;
+    for (int r0 = first; r0 < a.rows; r0 += 4 * step) {
+        float o[4][2];
+        bool in[4], any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = r0 + i * step;
+            in[i] = row < a.rows && !(a.valid && !a.valid[row]);
+            any |= in[i];
+            o[i][0] = o[i][1] = 0.0f;
+        }
+        if (any)
+            for (int p = 0; p < a.top * a.down_splits; ++p) {
+                u64 t[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const size_t slot = (size_t)(in[i] ? r0 + i * step : 0) * a.top + p / a.down_splits;
+                    const float* at = a.out + ((size_t)(p % a.down_splits) * slots + slot) * a.d + col;
+                    t[i] = in[i] ? __hip_atomic_load((const u64*)at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i][0] += __uint_as_float((uint32_t)t[i]);
+                    o[i][1] += __uint_as_float((uint32_t)(t[i] >> 32));
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = r0 + i * step;
+            if (row >= a.rows) break;
+            if (a.res) {
+                float u, v;
+                unpack_two(*(const u1_a2*)(a.res + (size_t)row * a.res_stride + col), a.type, u, v);
+                o[i][0] += u;
+                o[i][1] += v;
+            }
+            uint16_t* y = a.y + (size_t)row * a.y_stride + col;
+            if (a.type == kBf16) store16<kBf16, 2>(y, o[i]);
+            else store16<kF16, 2>(y, o[i]);
+        }
+    }
+}
+
+// down's 128 columns for a chunk over a part of the summed dimension, weighted,
+// by slot; the last workgroup of the columns adds each row's slots in order.
+__global__ __launch_bounds__(64 * kFewWaves, 2) void moe_down_kernel(MoeArgs a) {
+    __shared__ __align__(16) u4 lds[kFewLds];
+    __shared__ __align__(16) uint8_t bufs[kFewWaves][2][kMaxPairBytes];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nf = a.f / 128, db = blockIdx.x, split = blockIdx.y, ch = blockIdx.z, nchunks = *a.nchunks;
+    if (ch >= nchunks) {
+        // no row has an expert: residuals and zeros
+        if (nchunks == 0 && ch == 0 && split == 0) moe_finish(a, db, wv, kFewWaves, lane);
+        return;
+    }
+    const MoeChunk& c = a.chunks[ch];
+    const xtq_moe_weight w = a.table[3 * c.expert + 2];
+    int s0, s1;
+    split_range(a.f / 32, a.down_splits, split, s0, s1);
+    const u4* hi = a.hf + (size_t)ch * 2 * nf * 256;
+    const FewSource src{(const uint8_t*)w.trellis + (size_t)db * 256 * w.K, (size_t)(a.d / 128) * 256 * w.K, c.rows,
+                        a.f / 32, nullptr, 0, nullptr, nullptr, 0, 0, hi, hi + (size_t)nf * 256,
+                        a.hs + (size_t)ch * nf * 16};
+    f4 total[1][kFewTotals];
+    expert_sums<false>(w.K, src, s0, s1, lds, bufs[wv][0], nullptr, total);
+    f4* const sums = (f4*)lds;
+#pragma unroll
+    for (int i = 0; i < kFewTotals; ++i) sums[(i * kFewWaves + wv) * 64 + lane] = total[0][i];
+    float v0, v1;
+    unpack_two(load_two(w.svh + 128 * db, lane), kF16, v0, v1);
+    __syncthreads();
+    for (int r = wv; r < c.rows; r += kFewWaves) {
+        float v[2];
+        unit_row(sums, r, lane, v[0], v[1]);
+        transform_row(v[0], v[1], lane);
+        const int slot = c.slots[r];
+        const float by = a.weights[slot] * w.scale;
+        float* at = a.out + ((size_t)split * a.rows * a.top + slot) * a.d + 128 * db + 2 * lane;
+        __hip_atomic_store((u64*)at, (u64)__float_as_uint(v[0] * (v0 * by)) | (u64)__float_as_uint(v[1] * (v1 * by)) << 32,
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!arrive(a.counters + kMoeRouterCounters + db, nchunks * a.down_splits, threadIdx.x)) return;
+    moe_finish(a, db, wv, kFewWaves, lane);
+}
+
+}  // namespace
+
+#define XTQ_CAT2(a, b) a##b
+#define XTQ_CAT(a, b) XTQ_CAT2(a, b)
+
+hipError_t XTQ_CAT(launch_moe_code, XTQ_MOE_CODE)(const MoeArgs& a, hipStream_t s) {
+    const dim3 block(64 * kFewWaves), up(2 * (a.f / 128), a.up_splits, a.max_chunks),
+        down(a.d / 128, a.down_splits, a.max_chunks);
+    if (a.rows <= kMoeFused) {
+        hipLaunchKernelGGL((moe_up_kernel<true>), up, block, 0, s, a);
+    } else {
+        hipLaunchKernelGGL(moe_x_kernel, dim3((a.d / 128 + 3) / 4, 2, a.max_chunks), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((moe_up_kernel<false>), up, block, 0, s, a);
+    }
+    hipLaunchKernelGGL(moe_down_kernel, down, block, 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace xtq

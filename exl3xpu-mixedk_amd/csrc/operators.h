@@ -70,6 +70,11 @@ struct FewArgs {
 XTQ_FEW(2) XTQ_FEW(3) XTQ_FEW(4) XTQ_FEW(5) XTQ_FEW(6) XTQ_FEW(7)
 #undef XTQ_FEW
 
+struct MoeArgs;
+size_t moe_ws_bytes(int rows, int experts, int top, int d, int f);
+size_t moe_counters(int rows, int experts, int top, int d, int f);
+hipError_t launch_moe(MoeArgs a, void* ws, hipStream_t s);
+
 size_t gram_ws_bytes(int rows, int k);
 hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, int k,
                        const uint8_t* valid, const float* prev, float* out, void* ws,

@@ -5,6 +5,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include "moe_device.h"
 #include "operators.h"
 
 namespace {
@@ -50,6 +51,13 @@ int status(hipError_t e, const char* what) {
 int check_ws(const void* ws, int64_t have, int64_t want) {
     if (want > 0 && (!ws || !aligned(ws, 16))) return 12;
     return have < want ? 14 : 0;
+}
+
+bool moe_sizes(int rows, int experts, int top, int d, int f) {
+    return rows >= 0 && rows <= xtq::kMoeRows && experts >= 1 && experts <= xtq::kMoeExperts && top >= 1 &&
+           top <= xtq::kMoeTop && top <= experts && d > 0 && f > 0 && d % 128 == 0 && f % 128 == 0 &&
+           d <= (1 << 20) && f <= (1 << 20) &&
+           (rows == 0 || xtq::moe_counters(rows, experts, top, d, f) <= XTQ_OP_COUNTERS);
 }
 
 }  // namespace
@@ -112,6 +120,73 @@ int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy
     if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, 1)))) return rc;
     return status(xtq::launch_linear_bwd(wt, type, dy, dy_stride, z, act, rows, dx, dx_stride, dbias,
                                          bias_f32, ws, counters, (hipStream_t)stream), "linear_bwd");
+}
+
+int xtq_moe_table(const xtq_weight* weights, int experts, xtq_moe_weight* table) {
+    if (!weights || !table) return 12;
+    if (experts < 1 || experts > xtq::kMoeExperts) return 6;
+    xtq::Weight first{};
+    for (int i = 0; i < 3 * experts; ++i) {
+        xtq::Weight w;
+        const int rc = check_weight(weights + i, &w);
+        if (rc) return rc;
+        if (i == 0) first = w;
+        if (w.code != first.code) return 8;
+        const bool down = i % 3 == 2;
+        if (w.k != (down ? first.n : first.k) || w.n != (down ? first.k : first.n)) return 6;
+        table[i] = xtq_moe_weight{w.trellis, w.suh, w.svh, w.scale, w.K};
+    }
+    return 0;
+}
+
+int64_t xtq_moe_ws_bytes(int rows, int experts, int top, int d, int f) {
+    if (!moe_sizes(rows, experts, top, d, f)) return -6;
+    return rows ? (int64_t)xtq::moe_ws_bytes(rows, experts, top, d, f) : 0;
+}
+
+int xtq_moe_dev(const xtq_moe_weight* table, int experts, int d, int f, const char* code, int type,
+                const void* x, int64_t x_stride, int rows, const void* router, int router_f32, int top,
+                int act, int renorm, const uint8_t* valid, const void* res, int64_t res_stride, void* y,
+                int64_t y_stride, int32_t* ids, float* weights, void* ws, int64_t ws_bytes,
+                uint32_t* counters, void* stream) {
+    if (!table || !aligned(table, 8) || !code) return 12;
+    const int c = parse_code(code);
+    if (c < 0) return 8;
+    if ((type != XTQ_BF16 && type != XTQ_F16) || act < XTQ_ACT_NONE || act > XTQ_ACT_GELU) return 15;
+    if (!moe_sizes(rows, experts, top, d, f)) return 6;
+    if (rows == 0) return 0;
+    int rc;
+    if ((rc = check_rows(x, x_stride, d))) return rc;
+    if ((rc = check_rows(y, y_stride, d))) return rc;
+    if (res && (rc = check_rows(res, res_stride, d))) return rc;
+    if (!router || !aligned(router, router_f32 ? 4 : 2)) return 12;
+    if (!ids || !weights || !aligned(ids, 4) || !aligned(weights, 4)) return 12;
+    if (!counters || !aligned(counters, 4)) return 12;
+    if ((rc = check_ws(ws, ws_bytes, xtq::moe_ws_bytes(rows, experts, top, d, f)))) return rc;
+    xtq::MoeArgs a{};
+    a.table = table;
+    a.experts = experts;
+    a.d = d;
+    a.f = f;
+    a.code = c;
+    a.type = type;
+    a.rows = rows;
+    a.top = top;
+    a.act = act;
+    a.renorm = renorm;
+    a.x = (const uint16_t*)x;
+    a.x_stride = x_stride;
+    a.router = router;
+    a.router_f32 = router_f32;
+    a.valid = valid;
+    a.res = (const uint16_t*)res;
+    a.res_stride = res_stride;
+    a.y = (uint16_t*)y;
+    a.y_stride = y_stride;
+    a.ids = ids;
+    a.weights = weights;
+    a.counters = counters;
+    return status(xtq::launch_moe(a, ws, (hipStream_t)stream), "moe");
 }
 
 int64_t xtq_gram_ws_bytes(int rows, int k) {

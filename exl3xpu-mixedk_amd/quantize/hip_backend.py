@@ -82,6 +82,11 @@ def lib():
                                      vp, vp]
         L.xtq_linear_bwd_dev.argtypes = [wp, i32, vp, ll, vp, i32, i32, vp, ll, vp, i32, vp, ll, vp,
                                          vp]
+        L.xtq_moe_table.argtypes = [wp, i32, vp]
+        L.xtq_moe_ws_bytes.argtypes = [i32] * 5
+        L.xtq_moe_ws_bytes.restype = ll
+        L.xtq_moe_dev.argtypes = [vp, i32, i32, i32, cp, i32, vp, ll, i32, vp, i32, i32, i32, i32, vp,
+                                  vp, ll, vp, ll, vp, vp, vp, ll, vp, vp]
         L.xtq_gram_ws_bytes.argtypes = [i32, i32]
         L.xtq_gram_ws_bytes.restype = ll
         L.xtq_gram_dev.argtypes = [i32, vp, ll, i32, i32, vp, vp, vp, vp, ll, vp]
@@ -104,7 +109,7 @@ def lib():
                    "xtq_trellis_unpack_dev", "xtq_trellis_pack64_dev",
                    "xtq_trellis_unpack64_dev", "xtq_vit_get_lut", "xtq_had128_left_dev",
                    "xtq_had128_right_dev", "xtq_had128_both_dev", "xtq_linear_dev",
-                   "xtq_linear_bwd_dev", "xtq_gram_dev"):
+                   "xtq_linear_bwd_dev", "xtq_gram_dev", "xtq_moe_table", "xtq_moe_dev"):
             getattr(L, fn).restype = i32
         _LIB = L
     return _LIB

@@ -31,7 +31,7 @@ import hip_backend as _hb  # noqa: E402
 
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
-_COUNTERS = 4096
+_COUNTERS = 16384
 _counters: dict = {}
 
 
@@ -206,6 +206,89 @@ def linear(x: torch.Tensor, w: TrellisLinear, bias: torch.Tensor | None = None,
                                        for t in (x, bias, residual)):
         return _Linear.apply(x, bias, residual, w, a)
     return _forward(x, w, bias, a, residual, False)[0]
+
+
+_MOE_ROWS = 64
+
+
+class TrellisExperts:
+    """The experts of a mixture layer: lists of TrellisLinear, gate and up [d, f],
+    down [f, d], one code, each with its own K.  Keeps them and a table of their
+    addresses on the device."""
+
+    def __init__(self, gate, up, down):
+        gate, up, down = list(gate), list(up), list(down)
+        if not gate or len(up) != len(gate) or len(down) != len(gate):
+            raise ValueError(f"one gate, up and down per expert, got {len(gate)}, {len(up)}, {len(down)}")
+        self.weights = [w for ws in zip(gate, up, down) for w in ws]
+        first = gate[0]
+        self.device, self.code, self.d, self.f = first.device, first.code, first.k, first.n
+        for i, w in enumerate(self.weights):
+            want = (self.f, self.d) if i % 3 == 2 else (self.d, self.f)
+            if (w.k, w.n) != want or w.device != self.device or \
+                    _hb.code_name(w.code) != _hb.code_name(self.code):
+                raise ValueError(f"expert {i // 3}'s {('gate', 'up', 'down')[i % 3]} must be "
+                                 f"[{want[0]}, {want[1]}] {self.code} on {self.device}, got "
+                                 f"[{w.k}, {w.n}] {w.code} on {w.device}")
+        n = len(gate)
+        host = (_hb.TrellisWeight * (3 * n))(*[w._w for w in self.weights])
+        words = torch.empty(3 * n, 4, dtype=torch.int64)
+        _hb._check("xtq_moe_table", _hb.lib().xtq_moe_table(host, n, words.data_ptr()))
+        self.n, self.table = n, words.to(self.device)
+        self._code = _hb.code_name(self.code).encode()
+
+
+def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: int,
+        act: str = "silu", renorm: bool = True, residual: torch.Tensor | None = None,
+        valid: torch.Tensor | None = None, return_routing: bool = False):
+    """A mixture-of-experts layer for a few tokens x [.., d]: softmax(x router^T),
+    the top_k experts (ties: the lowest), and residual + sum of their
+    weight * down(act(gate(x)) * up(x)), in x's type.  router [experts, d] has x's
+    type or fp32; renorm divides the weights by their sum.  Tokens that valid [..]
+    (bool) leaves out are not looked at: their result is the residual or 0.
+    return_routing: also the expert numbers int32 [.., top_k] (-1 where left out)
+    and weights fp32.  More than 64 tokens run 64 at a time.  No gradient."""
+    if x.dtype not in _TYPES:
+        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if x.device != experts.device:
+        raise ValueError(f"x must be on {experts.device}, got {x.device}")
+    if x.dim() < 1 or x.shape[-1] != experts.d:
+        raise ValueError(f"x must be [.., {experts.d}], got {tuple(x.shape)}")
+    a, top_k, d = _check_act(act), int(top_k), experts.d
+    if not 1 <= top_k <= min(16, experts.n):
+        raise ValueError(f"top_k must be 1..{min(16, experts.n)}, got {top_k}")
+    _like(router, x, (experts.n, d), "router", (x.dtype, torch.float32))
+    if residual is not None:
+        _like(residual, x, x.shape, "residual", (x.dtype,))
+    if valid is not None:
+        _like(valid, x, x.shape[:-1], "valid", (torch.bool,))
+        valid = valid.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, router, residual)):
+        raise NotImplementedError("moe has no gradient: call it under torch.no_grad()")
+    rows, router = _rows(x, d), router.contiguous()
+    res = None if residual is None else _rows(residual, d)
+    m = rows.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    ids = torch.empty(*x.shape[:-1], top_k, dtype=torch.int32, device=x.device)
+    weights = torch.empty(*x.shape[:-1], top_k, dtype=torch.float32, device=x.device)
+    L = _hb.lib()
+    with torch.cuda.device(x.device):
+        stream = _hb._stream(x.device)
+        for r in range(0, m, _MOE_ROWS):
+            n = min(_MOE_ROWS, m - r)
+            need = L.xtq_moe_ws_bytes(n, experts.n, top_k, d, experts.f)
+            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+            rc = L.xtq_moe_dev(
+                experts.table.data_ptr(), experts.n, d, experts.f, experts._code, _TYPES[x.dtype],
+                rows.data_ptr() + 2 * r * _stride(rows), _stride(rows), n, router.data_ptr(),
+                int(router.dtype == torch.float32), top_k, a, int(bool(renorm)),
+                None if valid is None else valid.data_ptr() + r,
+                None if res is None else res.data_ptr() + 2 * r * _stride(res),
+                0 if res is None else _stride(res), y.data_ptr() + 2 * r * d, d,
+                ids.data_ptr() + 4 * r * top_k, weights.data_ptr() + 4 * r * top_k, ws.data_ptr(),
+                ws.numel(), _counter_words(x.device, stream).data_ptr(), stream)
+            _hb._check("xtq_moe_dev", rc)
+    return (y, ids, weights) if return_routing else y
 
 
 def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,

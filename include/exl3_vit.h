@@ -341,7 +341,7 @@ typedef struct xtq_weight {
 
 enum { XTQ_BF16 = 0, XTQ_F16 = 1 };
 enum { XTQ_ACT_NONE = 0, XTQ_ACT_RELU = 1, XTQ_ACT_SILU = 2, XTQ_ACT_GELU = 3 };
-enum { XTQ_OP_COUNTERS = 4096 };
+enum { XTQ_OP_COUNTERS = 16384 };
 
 /*
  * y = act(x W + bias) + res for x [rows][k], y [rows][n].
@@ -368,6 +368,42 @@ XTQ_API int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, in
                                const void* z, int act, int rows, void* dx, int64_t dx_stride,
                                void* dbias, int bias_f32, void* ws, int64_t ws_bytes,
                                uint32_t* counters, void* stream);
+
+/*
+ * A mixture-of-experts layer for a few rows (at most 64), on trellis experts:
+ *   logits = x router^T, p = softmax(logits), ids = the top largest logits
+ *   (ties: the lowest expert; NaN above all), w = p[ids], divided by their sum
+ *   with renorm,
+ *   y = res + sum_j w_j down_j(act(gate_j(x)) * up_j(x)), added in j's order.
+ * Expert e's gate and up are [d][f], its down [f][d]; every weight has its own K,
+ * all have one code.
+ *   table    [experts][3] (gate, up, down) device: xtq_moe_table's words
+ *   router   [experts][d] contiguous, fp32 (router_f32 != 0) or of x's type
+ *   valid    [rows] bytes or NULL: a row whose byte is 0 is not looked at, its
+ *            ids are -1, its weights 0 and its y the residual or 0
+ *   res      [rows][d] or NULL; may be y itself
+ *   ids      [rows][top] (out), weights [rows][top] fp32 (out)
+ * At most 512 experts, top <= 16 and <= experts; d / 128 and the chosen experts
+ * times f / 128 are bounded by XTQ_OP_COUNTERS (status 6).
+ */
+typedef struct xtq_moe_weight {
+    const int16_t* trellis;
+    const uint16_t* suh;
+    const uint16_t* svh;
+    float scale;
+    int32_t K;
+} xtq_moe_weight;
+
+/* Checks the weights of a layer ([experts][3] host structures) and writes the
+ * table's words (host; the caller copies them to the device). */
+XTQ_API int xtq_moe_table(const xtq_weight* weights, int experts, xtq_moe_weight* table);
+XTQ_API int64_t xtq_moe_ws_bytes(int rows, int experts, int top, int d, int f);
+XTQ_API int xtq_moe_dev(const xtq_moe_weight* table, int experts, int d, int f, const char* code,
+                        int type, const void* x, int64_t x_stride, int rows, const void* router,
+                        int router_f32, int top, int act, int renorm, const uint8_t* valid,
+                        const void* res, int64_t res_stride, void* y, int64_t y_stride,
+                        int32_t* ids, float* weights, void* ws, int64_t ws_bytes,
+                        uint32_t* counters, void* stream);
 
 /*
  * out = prev + X^T X, [k][k] fp32, over the rows of x [rows][k] whose valid byte
