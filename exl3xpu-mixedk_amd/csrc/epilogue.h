@@ -108,17 +108,24 @@ __device__ __forceinline__ void finish_cols(const float* v, const Columns<N>& c,
     store16<T, N>((uint16_t*)ep.y + (size_t)row * ep.y_stride + col, o);
 }
 
+// Columns of a unit's lanes.
+template <int T>
+__device__ __forceinline__ void unit_columns(Columns<4> (&c)[8], const Epilogue& ep, int blk, int lane) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = load_columns<T, 4>(ep, blk * 128 + 16 * j + 4 * (lane >> 4));
+}
+
 // A whole unit.
 template <int T>
-__device__ __forceinline__ void finish_unit(f4* v, const Epilogue& ep, int grp, int blk, int lane) {
+__device__ __forceinline__ void finish_unit(f4* v, const Columns<4> (&c)[8], const Epilogue& ep, int grp, int blk,
+                                            int lane) {
     transform_unit(v);
     const int row = grp * 16 + (lane & 15);
     if (row >= ep.rows) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float t[4] = {v[j][0], v[j][1], v[j][2], v[j][3]};
-        const int col = blk * 128 + 16 * j + 4 * (lane >> 4);
-        finish_cols<T, 4>(t, load_columns<T, 4>(ep, col), ep, row, col);
+        finish_cols<T, 4>(t, c[j], ep, row, blk * 128 + 16 * j + 4 * (lane >> 4));
     }
 }
 

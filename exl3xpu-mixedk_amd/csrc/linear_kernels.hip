@@ -13,7 +13,9 @@
 // 1 KiB, lane 16 q + r holding elements 8 q .. 8 q + 7 of row r, the operand of
 // one v_mfma_f32_16x16x32.  A fragment moves from memory to LDS and from LDS to
 // registers as 64 consecutive 16-byte pieces: no bank conflict, no address
-// arithmetic.
+// arithmetic.  16 fragments of a step lie side by side (frag_at), the rows or
+// columns of a workgroup's tile: it reads two streams of 16 KiB pieces, and not
+// 32 of 1 KiB from as many pages.
 #include "epilogue.h"
 #include "few_device.h"
 #include "operators.h"
@@ -24,6 +26,16 @@ namespace xtq {
 namespace {
 
 constexpr int kFragBytes = 1024;
+
+// Where fragment `step` of group `grp` starts, in elements.  Groups come in
+// sixteens; scratch is sized for whole ones, and what is not written there
+// reaches no result.
+__host__ __device__ __forceinline__ size_t frag_at(size_t grp, size_t step, size_t steps) {
+    return (((grp >> 4) * steps + step) * 16 + (grp & 15)) * 512;
+}
+
+// Bytes of `groups` groups' fragments.
+size_t frag_bytes(size_t groups, size_t steps) { return (groups + 15) / 16 * 16 * steps * kFragBytes; }
 
 __device__ __forceinline__ void unpack8(u4 w, int type, float* v) {
 #pragma unroll
@@ -65,34 +77,6 @@ __device__ __forceinline__ void scale8(const uint16_t* colscale, int col, float*
     unpack8(*(const u4_a2*)(colscale + col), kF16, c);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= c[i];
-}
-
-// Per row, the power of two that brings its transformed values into fp16's
-// range: the largest |x * colscale| goes to [2^7, 2^8), the transform's sums of
-// 128 stay below 2^15.  rowexp[m]: what the product has to be multiplied with
-// (as a power of two), with the two transforms' 1/128.
-__global__ __launch_bounds__(256) void row_exp_kernel(Source s, int32_t* __restrict__ shift,
-                                                      int32_t* __restrict__ rowexp) {
-    __shared__ float part[4];
-    const int row = blockIdx.x;
-    float top = 0.0f;
-    for (int c = threadIdx.x * 8; c < s.cols; c += 2048) {
-        float v[8];
-        load8(s, row, c, v);
-        scale8(s.colscale, c, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-    }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        const int sh = shift_to(top, 7);
-        shift[row] = sh;
-        rowexp[row] = -sh - 7;
-    }
 }
 
 // Rows to fragments: values times column scales, block-128 transform, times
@@ -145,25 +129,67 @@ __global__ __launch_bounds__(256) void transform_kernel(Source s, const int32_t*
         v[i] = ldexpf(v[i], sh);
         v[i + 1] = ldexpf(v[i + 1], sh);
     }
-    uint16_t* out = frags + ((size_t)grp * nblk + blk) * 2048 + lane * 8;
+    uint16_t* out = frags + lane * 8;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         h8 o;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = (_Float16)v[8 * p + i];
-        *(h8*)(out + p * 512) = o;
+        *(h8*)(out + frag_at(grp, 4 * blk + p, 4 * nblk)) = o;
     }
 }
 
-// Column sums' last step: out[c] = sum of part[g][c] over the groups, in order.
-__global__ __launch_bounds__(256) void colsum_kernel(const float* __restrict__ part, int groups,
-                                                     int cols, int type, int f32, void* out) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+// Column sums' last step: out[c] = sum of part[g][c] over the groups, in an
+// order that their number fixes: four threads a column take every fourth group.
+struct ColSum {
+    const float* part;
+    int groups, cols, type, f32;
+    void* out;
+};
+
+__device__ void column_sums(const ColSum& a, int block, float* part) {
+    const int c = block * 64 + (threadIdx.x & 63), wv = threadIdx.x >> 6;
     float t = 0.0f;
-    for (int g = 0; g < groups; ++g) t += part[(size_t)g * cols + c];
-    if (f32) ((float*)out)[c] = t;
-    else ((uint16_t*)out)[c] = (uint16_t)(type == kBf16 ? to16<kBf16>(t) : to16<kF16>(t));
+    if (c < a.cols)
+#pragma unroll 8
+        for (int g = wv; g < a.groups; g += 4) t += a.part[(size_t)g * a.cols + c];
+    part[threadIdx.x] = t;
+    __syncthreads();
+    if (wv || c >= a.cols) return;
+    t = (part[c & 63] + part[64 + (c & 63)]) + (part[128 + (c & 63)] + part[192 + (c & 63)]);
+    if (a.f32) ((float*)a.out)[c] = t;
+    else ((uint16_t*)a.out)[c] = (uint16_t)(a.type == kBf16 ? to16<kBf16>(t) : to16<kF16>(t));
+}
+
+__global__ __launch_bounds__(256) void column_sums_kernel(ColSum a) {
+    __shared__ float part[256];
+    column_sums(a, blockIdx.x, part);
+}
+
+// Per row, the power of two that brings its transformed values into fp16's
+// range: the largest |x * colscale| goes to [2^7, 2^8), the transform's sums of
+// 128 stay below 2^15.  rowexp[m]: what the product has to be multiplied with
+// (as a power of two), with the two transforms' 1/128.
+__device__ void row_exponents(const Source& s, int row, int32_t* __restrict__ shift,
+                              int32_t* __restrict__ rowexp) {
+    __shared__ float part[4];
+    float top = 0.0f;
+    for (int c = threadIdx.x * 8; c < s.cols; c += 2048) {
+        float v[8];
+        load8(s, row, c, v);
+        scale8(s.colscale, c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    }
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        const int sh = shift_to(top, 7);
+        shift[row] = sh;
+        rowexp[row] = -sh - 7;
+    }
 }
 
 // Trellis to fragments of the inner weight.  BWD = 0: fragment (ng, p) holds
@@ -172,15 +198,18 @@ __global__ __launch_bounds__(256) void colsum_kernel(const float* __restrict__ p
 // is symbol 32 (c % 8) + 8 ((r % 8) / 2) + 4 (c / 8) + 2 (r / 8) + r % 2, its state
 // the 16-bit circular window ending with the symbol's K bits.  A workgroup
 // takes 8 by 4 tiles (along the summed dimension by the other), the trellis
-// words staged in LDS.
+// words staged in LDS.  The workgroups past `decoders` find the exponents of the
+// source's rows, which nothing here waits for.
 template <int K, int CODE, int BWD>
-__global__ __launch_bounds__(256) void decode_frag_kernel(const int16_t* __restrict__ trellis,
-                                                          int tk, int tn,
-                                                          uint16_t* __restrict__ frags) {
+__global__ __launch_bounds__(256) void prepare_kernel(const int16_t* __restrict__ trellis, int tk, int tn,
+                                                      uint16_t* __restrict__ frags, int decoders, Source src,
+                                                      int32_t* __restrict__ shift,
+                                                      int32_t* __restrict__ rowexp) {
+    if ((int)blockIdx.x >= decoders) return row_exponents(src, blockIdx.x - decoders, shift, rowexp);
     constexpr int TW = 8 * K;                           // words of a tile
     __shared__ uint32_t words[32 * TW];
-    const int i0 = blockIdx.y * (BWD ? 4 : 8), j0 = blockIdx.x * (BWD ? 8 : 4);   // first tile
     constexpr int NJ = BWD ? 8 : 4;
+    const int nj = tn / NJ, bi = blockIdx.x / nj, i0 = bi * (32 / NJ), j0 = (blockIdx.x - bi * nj) * NJ;   // first tile
     for (int t = threadIdx.x; t < 32 * TW; t += 256) {
         const int tile = t / TW, w = t - tile * TW;
         const int i = i0 + tile / NJ, j = j0 + tile % NJ;
@@ -207,31 +236,45 @@ __global__ __launch_bounds__(256) void decode_frag_kernel(const int16_t* __restr
         for (int j = 0; j < 4; ++j) o[j] = code_pair<CODE>(st[2 * j], st[2 * j + 1]);
         const size_t g = BWD ? i0 + wv : j0 + wv;
         const size_t np = (BWD ? tn : tk) / 2, f = (BWD ? j0 : i0) / 2 + p;
-        *(u4*)(frags + (g * np + f) * 512 + lane * 8) = o;
+        *(u4*)(frags + frag_at(g, f, np) + lane * 8) = o;
     }
 }
 
 // -------------------------------------------------------------------- matrix
 // product of fragments: columns (fragments A) by rows (fragments B).  A
-// workgroup's tile is 256 columns by 256 rows, 8 waves of 128 columns (a whole
-// transform block, so the epilogue's transform stays in registers) by 64 rows.
-constexpr int kTile = 256;              // rows and columns of a workgroup's tile
-constexpr int kStage = 2;               // 32-wide steps of the summed dimension per stage
+// workgroup's tile is 256 columns by 32 NB rows, 4 waves of 128 columns (a whole
+// transform block, so the epilogue's transform stays in registers) by 16 NB
+// rows.  The summed dimension goes by in steps of 32; while the matrix cores
+// work on one step, the next two move from memory into the other two of three
+// LDS buffers.  Two workgroups share a compute unit, so one's epilogue and waits
+// overlap with the other's products.  (One workgroup of 8 waves and 256 by 256,
+// its fragments fetched a step ahead: the epilogue, 17 us a tile, stood alone.)
+constexpr int kTileN = 256;
+
+// Workgroups go round robin over the 8 XCDs, each with an L2 of its own: an XCD
+// gets a run of tiles that lie side by side, in bands of kBand rows of tiles.
+constexpr int kXcds = 8;
+constexpr int kBand = 8;
+
+__device__ __forceinline__ int xcd_order(int id, int all) {
+    const int x = id % kXcds, each = all / kXcds, more = all % kXcds;
+    return x * each + (x < more ? x : more) + id / kXcds;
+}
 
 enum GemmOut { kOutEpilogue, kOutPartial, kOutGram };
 
 struct Gemm {
     const uint16_t *A, *B;
     int ga, gb;                         // 16-wide groups of columns, rows
-    int steps;                          // 32-wide steps of the summed dimension (even)
-    int splits;                         // of the summed dimension
-    float* part;                        // kOutPartial: [splits][blocks of 128][gb][8][64][4]
-    const float* prev;                  // kOutGram
+    int steps;                          // 32-wide steps of the summed dimension
+    int tiles, splits;                  // splits of the summed dimension
+    float* part;                        // partial: [splits][blocks of 128][gb][8][64][4]
+    const float* prev;                  // Gram
     float* out;
     int dim;
 };
 
-template <int T, bool BF>
+template <bool BF>
 __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a),
                                                                     __builtin_bit_cast(b8, b), c, 0, 0, 0);
@@ -242,127 +285,182 @@ __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
 
-template <int T, int OUT, bool BF>
-__global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm g, Epilogue ep) {
-    __shared__ __align__(1024) uint8_t lds[2][2 * 16 * kStage * kFragBytes];
+template <int T, int OUT, bool BF, int NB>
+__global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSum sums) {
+    constexpr int kFrags = 16 + 2 * NB, kOwn = 4 + NB / 2;      // of a step: the workgroup's, a wave's to move
+    // (One LDS object: beside another, the compiler takes every read of this one
+    // for a possible read of what a load to LDS still has to write, and waits.)
+    __shared__ __align__(1024) uint8_t lds[3][kFrags * kFragBytes];
+    // workgroups past the tiles: column sums that the launch before left parts of
+    if ((int)blockIdx.x >= g.tiles) {
+        if (blockIdx.y == 0) column_sums(sums, blockIdx.x - g.tiles, (float*)lds[0]);
+        return;
+    }
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wv & 1, wm = wv >> 1;
+    const int tile = xcd_order(blockIdx.x, g.tiles);
     int tn, tm;
-    if constexpr (OUT == kOutGram) {    // tiles on and below the diagonal, tn <= tm
-        tm = (int)((sqrtf(8.0f * blockIdx.x + 1.0f) - 1.0f) * 0.5f);
-        while ((tm + 1) * (tm + 2) / 2 <= (int)blockIdx.x) ++tm;
-        while (tm * (tm + 1) / 2 > (int)blockIdx.x) --tm;
-        tn = blockIdx.x - tm * (tm + 1) / 2;
-    } else {
-        const int nt = (g.ga + 15) / 16;
-        tn = blockIdx.x % nt;
-        tm = blockIdx.x / nt;
+    if constexpr (OUT == kOutGram) {
+        // tiles that reach the diagonal or lie below: columns tn, rows tm >= R tn
+        constexpr int R = kTileN / (32 * NB);
+        const int mt = (g.gb + 2 * NB - 1) / (2 * NB);
+        int at = tile;
+        for (tn = 0; at >= mt - R * tn; ++tn) at -= mt - R * tn;
+        tm = R * tn + at;
+    } else {                            // bands of kBand tiles of rows
+        const int nt = (g.ga + 15) / 16, mt = (g.gb + 2 * NB - 1) / (2 * NB), band = tile / (nt * kBand);
+        const int high = mt - band * kBand < kBand ? mt - band * kBand : kBand, in = tile - band * nt * kBand;
+        tn = in / high;
+        tm = band * kBand + in - tn * high;
     }
-    const int nst = g.steps / kStage, split = blockIdx.y;
-    const int s0 = (int)((long long)nst * split / g.splits);
-    const int s1 = (int)((long long)nst * (split + 1) / g.splits);
+    const int split = blockIdx.y;
+    const int s0 = (int)((long long)g.steps * split / g.splits);
+    const int s1 = (int)((long long)g.steps * (split + 1) / g.splits);
 
-    // this wave's eight fragments of a stage: 4 groups of A or B by 2 steps
-    const bool isb = wv >= 4;
-    const uint16_t* base = isb ? g.B : g.A;
-    const int lim = (isb ? g.gb : g.ga) - 1, first = (isb ? tm : tn) * 16 + (wv & 3) * 4;
-    auto load = [&](int s, int buf) {
+    // this wave's fragments of a step: a quarter of A's 16 and of B's 2 NB
+    const uint16_t* fa = g.A + (size_t)tn * g.steps * 8192 + wv * 2048 + lane * 8;
+    const int gb0 = tm * 2 * NB;        // first group of rows
+    const uint16_t* fb = g.B + ((size_t)(gb0 >> 4) * g.steps * 16 + (gb0 & 15) + wv * (NB / 2)) * 512 + lane * 8;
+    int to = 0;                         // buffer of the next step to load
+    auto load = [&](int s) {
+        uint8_t* l = lds[to];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            int grp = first + (i >> 1);
-            grp = grp < lim ? grp : lim;
-            const uint16_t* p = base + ((size_t)grp * g.steps + (size_t)s * kStage + (i & 1)) * 512 +
-                                lane * 8;
-            __builtin_amdgcn_global_load_lds((global_void*)p,
-                                             (lds_void*)(lds[buf] + (wv * 8 + i) * kFragBytes), 16, 0, 0);
-        }
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_global_load_lds((global_void*)(fa + (size_t)s * 8192 + i * 512),
+                                             (lds_void*)(l + (wv * 4 + i) * kFragBytes), 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i)
+            __builtin_amdgcn_global_load_lds((global_void*)(fb + (size_t)s * 8192 + i * 512),
+                                             (lds_void*)(l + (16 + wv * (NB / 2) + i) * kFragBytes), 16, 0, 0);
+        to = to == 2 ? 0 : to + 1;
     };
-    f4 acc[8][4];
+    // All waves' pieces of the next step are in LDS, and all waves have read this
+    // one (their reads were waited for before they came here).
+    auto meet_up = [&](bool more) {
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kOwn) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    f4 acc[8][NB];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) acc[j][b] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-    if (s0 < s1) load(s0, 0);
-    for (int s = s0; s < s1; ++s) {
-        const int buf = (s - s0) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        u4 a[2][8], b[2][4];
-        const uint8_t* l = lds[buf] + lane * 16;
+        for (int b = 0; b < NB; ++b) acc[j][b] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    if (s0 < s1) {
+        load(s0);
+        if (s0 + 1 < s1) load(s0 + 1);
+        meet_up(s0 + 1 < s1);
+        int from = 0;
+        for (int s = s0; s < s1; ++s) {
+            if (s + 2 < s1) load(s + 2);
+            u4 a[8], b[NB];
+            const uint8_t* l = lds[from] + lane * 16;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+            for (int i = 0; i < NB; ++i) b[i] = *(const u4*)(l + (16 + wm * NB + i) * kFragBytes);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) a[p][j] = *(const u4*)(l + ((wn * 8 + j) * 2 + p) * kFragBytes);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[p][i] = *(const u4*)(l + (32 + (wm * 4 + i) * 2 + p) * kFragBytes);
-        }
-        if (s + 1 < s1) load(s + 1, buf ^ 1);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
+            for (int j = 0; j < 8; ++j) a[j] = *(const u4*)(l + (wn * 8 + j) * kFragBytes);
+            __builtin_amdgcn_sched_barrier(0);          // all reads under way before the first product
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] = mfma<T, BF>(a[p][j], b[p][i], acc[j][i]);
+                for (int i = 0; i < NB; ++i) acc[j][i] = mfma<BF>(a[j], b[i], acc[j][i]);
+            __builtin_amdgcn_sched_barrier(0);          // none after the others have met
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            meet_up(s + 2 < s1);
+            from = from == 2 ? 0 : from + 1;
+        }
     }
     const int blk = tn * 2 + wn;
     if (blk * 8 >= g.ga) return;
+    Columns<4> cols[8];
+    if constexpr (OUT == kOutEpilogue) unit_columns<T>(cols, ep, blk, lane);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const int grp = tm * 16 + wm * 4 + b;
+    for (int b = 0; b < NB; ++b) {
+        const int grp = gb0 + wm * NB + b;
         if (grp >= g.gb) continue;
+        __builtin_amdgcn_sched_barrier(0);
         f4 v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = acc[j][b];
         if constexpr (OUT == kOutEpilogue) {
-            finish_unit<T>(v, ep, grp, blk, lane);
-        } else if constexpr (OUT == kOutPartial) {
+            finish_unit<T>(v, cols, ep, grp, blk, lane);
+        } else {
             f4* o = (f4*)g.part + (((size_t)split * (g.ga / 8) + blk) * g.gb + grp) * 512 + lane;
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[j * 64] = v[j];
-        } else {
-            const size_t row = (size_t)grp * 16 + (lane & 15);
+        }
+    }
+}
+
+// out = prev + sums, at and below the diagonal and mirrored, for a unit.
+__device__ __forceinline__ void finish_gram(const f4* v, const Gemm& g, int grp, int blk, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    const size_t row = (size_t)grp * 16 + r, col = (size_t)blk * 128 + 4 * q, dim = g.dim;
+    if (blk * 128 + 127 < grp * 16) {   // below the diagonal
+        // mirrored: lane 4 a + b of a row has rows 4 a .. + 3 of column b
+        const size_t mrow = col + (r & 3), mcol = (size_t)grp * 16 + (r & ~3);
+        f4 p[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const size_t col = (size_t)blk * 128 + 16 * j + 4 * (lane >> 4);
-                f4 o = v[j];
-                if (g.prev) {
-                    const f4 p = *(const f4_a4*)(g.prev + row * g.dim + col);
+        for (int j = 0; j < 8; ++j)
+            p[j] = g.prev ? *(const f4_a4*)(g.prev + row * dim + col + 16 * j) : (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = p[i] + v[j][i];
-                }
-                *(f4_a4*)(g.out + row * g.dim + col) = o;
-                if (tn != tm) {
+        for (int j = 0; j < 8; ++j) *(f4_a4*)(g.out + row * dim + col + 16 * j) = p[j] + v[j];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const size_t at = (col + i) * g.dim + row;
-                        g.out[at] = g.prev ? g.prev[at] + v[j][i] : v[j][i];
-                    }
-                }
-            }
+        for (int j = 0; j < 8; ++j)
+            p[j] = g.prev ? *(const f4_a4*)(g.prev + (mrow + 16 * j) * dim + mcol) : (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            *(f4_a4*)(g.out + (mrow + 16 * j) * dim + mcol) = p[j] + transpose4(v[j], lane);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const size_t c = col + 16 * j + i;
+            if (c > row) continue;
+            g.out[row * dim + c] = (g.prev ? g.prev[row * dim + c] : 0.0f) + v[j][i];
+            if (c < row) g.out[c * dim + row] = (g.prev ? g.prev[c * dim + row] : 0.0f) + v[j][i];
         }
     }
 }
 
 // Sums the splits' partial products of a unit (128 columns by 16 rows), in
-// order, and finishes it.
-template <int T>
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits,
-                                                   int blocks, int groups, Epilogue ep) {
+// order, four loads in flight for each of its registers, and finishes it.  (The
+// Gram's sums come this way without splits too: its reads, writes and mirrored
+// writes at the end of the product's own waves took 100 us of 300 for 5120
+// channels.)
+template <int T, bool GRAM>
+__global__ __launch_bounds__(256) void join_kernel(Gemm g, Epilogue ep) {
     const int lane = threadIdx.x & 63, grp = blockIdx.x * 4 + (threadIdx.x >> 6), blk = blockIdx.y;
-    if (grp >= groups) return;
+    if (grp >= g.gb) return;
+    if (GRAM && blk * 128 > grp * 16 + 15) return;      // above the diagonal
     f4 v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < splits; ++s) {
-        const f4* p = (const f4*)part + (((size_t)s * blocks + blk) * groups + grp) * 512 + lane;
+    const f4* p = (const f4*)g.part + ((size_t)blk * g.gb + grp) * 512 + lane;
+    const size_t stride = (size_t)(g.ga / 8) * g.gb * 512;
+    for (int s = 0; s < g.splits; s += 4) {
+        f4 t[4][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const f4 t = p[j * 64];
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[j][i] += t[i];
-        }
+            for (int j = 0; j < 8; ++j) t[i][j] = p[(s + i < g.splits ? s + i : s) * stride + j * 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i < g.splits) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += t[i][j];
+            }
     }
-    finish_unit<T>(v, ep, grp, blk, lane);
+    if constexpr (GRAM) {
+        finish_gram(v, g, grp, blk, lane);
+    } else {
+        Columns<4> cols[8];
+        unit_columns<T>(cols, ep, blk, lane);
+        finish_unit<T>(v, cols, ep, grp, blk, lane);
+    }
 }
 
 // ---------------------------------------------------------------------- Gram
@@ -389,50 +487,62 @@ __global__ __launch_bounds__(256) void transpose_kernel(const uint16_t* __restri
         u4 o;
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = t[8 * q + 2 * i][c] | (uint32_t)t[8 * q + 2 * i + 1][c] << 16;
-        *(u4*)(frags + ((size_t)(c0 / 16 + wv * 2 + g) * steps + p) * 512 + lane * 8) = o;
+        *(u4*)(frags + frag_at(c0 / 16 + wv * 2 + g, p, steps) + lane * 8) = o;
     }
 }
 
+struct Prepare {
+    uint16_t* frags;
+    int decoders;
+    Source src;
+    int32_t *shift, *rowexp;
+};
+
 template <int K, int CODE>
-void decode_kc(const Weight& w, int bwd, uint16_t* frags, hipStream_t s) {
+void prepare_kc(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     const int tk = w.k / 16, tn = w.n / 16;
-    if (bwd) hipLaunchKernelGGL((decode_frag_kernel<K, CODE, 1>), dim3(tn / 8, tk / 4), dim3(256), 0, s,
-                                w.trellis, tk, tn, frags);
-    else hipLaunchKernelGGL((decode_frag_kernel<K, CODE, 0>), dim3(tn / 4, tk / 8), dim3(256), 0, s,
-                            w.trellis, tk, tn, frags);
+    const dim3 grid(p.decoders + p.src.rows);
+    if (bwd) hipLaunchKernelGGL((prepare_kernel<K, CODE, 1>), grid, dim3(256), 0, s, w.trellis, tk, tn, p.frags,
+                                p.decoders, p.src, p.shift, p.rowexp);
+    else hipLaunchKernelGGL((prepare_kernel<K, CODE, 0>), grid, dim3(256), 0, s, w.trellis, tk, tn, p.frags,
+                            p.decoders, p.src, p.shift, p.rowexp);
 }
 
 template <int K>
-void decode_k(const Weight& w, int bwd, uint16_t* frags, hipStream_t s) {
-    if (w.code == kCodeMul1) decode_kc<K, kCodeMul1>(w, bwd, frags, s);
-    else if (w.code == kCodeMcg) decode_kc<K, kCodeMcg>(w, bwd, frags, s);
-    else decode_kc<K, kCode3Inst>(w, bwd, frags, s);
+void prepare_k(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
+    if (w.code == kCodeMul1) prepare_kc<K, kCodeMul1>(w, bwd, p, s);
+    else if (w.code == kCodeMcg) prepare_kc<K, kCodeMcg>(w, bwd, p, s);
+    else prepare_kc<K, kCode3Inst>(w, bwd, p, s);
 }
 
-void decode_frags(const Weight& w, int bwd, uint16_t* frags, hipStream_t s) {
+void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     switch (w.K) {
-        case 2: return decode_k<2>(w, bwd, frags, s);
-        case 3: return decode_k<3>(w, bwd, frags, s);
-        case 4: return decode_k<4>(w, bwd, frags, s);
-        case 5: return decode_k<5>(w, bwd, frags, s);
-        case 6: return decode_k<6>(w, bwd, frags, s);
-        default: return decode_k<7>(w, bwd, frags, s);
+        case 2: return prepare_k<2>(w, bwd, p, s);
+        case 3: return prepare_k<3>(w, bwd, p, s);
+        case 4: return prepare_k<4>(w, bwd, p, s);
+        case 5: return prepare_k<5>(w, bwd, p, s);
+        case 6: return prepare_k<6>(w, bwd, p, s);
+        default: return prepare_k<7>(w, bwd, p, s);
     }
 }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Splits of the summed dimension: as many as fill the compute units, each with
-// at least 8 stages.
+// Parts of the summed dimension, each of 8 steps at least, so that the tiles fill
+// the compute units' two places.
 int gemm_splits(int tiles, int steps) {
-    const int most = steps / kStage / 8;
-    int s = tiles >= kCUs ? 1 : kCUs / tiles;
+    const int most = steps / 8;
+    int s = tiles >= 2 * kCUs ? 1 : 2 * kCUs / tiles;
     if (s > most) s = most;
     return s < 1 ? 1 : s;
 }
 
+// Groups of 16 rows of a wave's tile: 4 (128 rows a workgroup), or 2 while that
+// leaves compute units empty.
+int gemm_nb(int rows, int n) { return (n + kTileN - 1) / kTileN * ((rows + 127) / 128) < kCUs ? 2 : 4; }
+
 struct ManyPlan {
-    int groups, tiles, splits;
+    int groups, nb, tiles, splits;
     size_t shift, rowexp, xf, wf, part, colsum, total;
 };
 
@@ -440,14 +550,15 @@ struct ManyPlan {
 ManyPlan many_plan(int rows, int k, int n, bool colsum) {
     ManyPlan p;
     p.groups = (rows + 15) / 16;
-    p.tiles = ((n + kTile - 1) / kTile) * ((rows + kTile - 1) / kTile);
+    p.nb = gemm_nb(rows, n);
+    p.tiles = (n + kTileN - 1) / kTileN * ((p.groups + 2 * p.nb - 1) / (2 * p.nb));
     p.splits = gemm_splits(p.tiles, k / 32);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t a = at; at += align256(bytes); return a; };
     p.shift = take((size_t)p.groups * 64);
     p.rowexp = take((size_t)p.groups * 64);
-    p.xf = take((size_t)p.groups * 32 * k);
-    p.wf = take((size_t)n * k * 2);
+    p.xf = take(frag_bytes(p.groups, k / 32));
+    p.wf = take(frag_bytes(n / 16, k / 32));
     p.part = take(p.splits > 1 ? (size_t)p.splits * p.groups * 64 * n : 0);
     p.colsum = take(colsum ? (size_t)p.groups * k * 4 : 0);
     p.total = at;
@@ -464,22 +575,26 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
     int32_t *shift = (int32_t*)(base + p.shift), *rowexp = (int32_t*)(base + p.rowexp);
     uint16_t *xf = (uint16_t*)(base + p.xf), *wf = (uint16_t*)(base + p.wf);
     float* colsum = dbias ? (float*)(base + p.colsum) : nullptr;
-    hipLaunchKernelGGL(row_exp_kernel, dim3(rows), dim3(256), 0, s, src, shift, rowexp);
+    const int decoders = ep.y ? (w.k / 16) * (w.n / 16) / 32 : 0;
+    prepare(w, bwd, Prepare{wf, decoders, src, shift, rowexp}, s);
     hipLaunchKernelGGL(transform_kernel, dim3((k / 128 + 3) / 4, p.groups), dim3(256), 0, s, src,
                        (const int32_t*)shift, xf, colsum);
-    if (dbias) hipLaunchKernelGGL(colsum_kernel, dim3((k + 255) / 256), dim3(256), 0, s, colsum, p.groups,
-                                  k, T, dbias_f32, dbias);
-    if (!ep.y) return hipGetLastError();
-    decode_frags(w, bwd, wf, s);
+    const ColSum sums{colsum, p.groups, k, T, dbias_f32, dbias};
+    const int adders = dbias ? (k + 63) / 64 : 0;
+    if (!ep.y) {
+        hipLaunchKernelGGL(column_sums_kernel, dim3(adders), dim3(256), 0, s, sums);
+        return hipGetLastError();
+    }
     ep.rowexp = rowexp;
-    Gemm g{wf, xf, n / 16, p.groups, k / 32, p.splits, (float*)(base + p.part), nullptr, nullptr, 0};
+    const Gemm g{wf, xf, n / 16, p.groups, k / 32, p.tiles, p.splits, (float*)(base + p.part), nullptr, nullptr, 0};
+    const dim3 grid(p.tiles + adders, p.splits), block(256);
     if (p.splits == 1) {
-        hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false>), dim3(p.tiles), dim3(512), 0, s, g, ep);
+        if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 4>), grid, block, 0, s, g, ep, sums);
+        else hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 2>), grid, block, 0, s, g, ep, sums);
     } else {
-        hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false>), dim3(p.tiles, p.splits), dim3(512), 0, s,
-                           g, ep);
-        hipLaunchKernelGGL((join_kernel<T>), dim3((p.groups + 3) / 4, n / 128), dim3(256), 0, s, g.part,
-                           p.splits, n / 128, p.groups, ep);
+        if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 4>), grid, block, 0, s, g, ep, sums);
+        else hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2>), grid, block, 0, s, g, ep, sums);
+        hipLaunchKernelGGL((join_kernel<T, false>), dim3((p.groups + 3) / 4, n / 128), block, 0, s, g, ep);
     }
     return hipGetLastError();
 }
@@ -582,25 +697,48 @@ hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long lon
                          : many<kF16>(w, 1, src, ep, dbias, dbias_f32, ws, s);
 }
 
-size_t gram_ws_bytes(int rows, int k) {
-    const size_t steps = ((size_t)rows + 63) / 64 * 2;
-    return steps * (k / 16) * kFragBytes;
+namespace {
+
+struct GramPlan {
+    int steps, tiles, splits;
+    size_t xf, part, total;
+};
+
+GramPlan gram_plan(int rows, int k) {
+    GramPlan p;
+    p.steps = (int)(((long long)rows + 31) / 32);
+    const int nt = (k + kTileN - 1) / kTileN, mt = (k + 127) / 128;
+    p.tiles = 0;
+    for (int t = 0; t < nt; ++t) p.tiles += mt - 2 * t;
+    p.splits = gemm_splits(p.tiles, p.steps);
+    p.xf = 0;
+    p.part = align256(frag_bytes(k / 16, p.steps));
+    p.total = p.part + (size_t)p.splits * k * k * 4;
+    return p;
 }
+
+template <int T, bool BF>
+hipError_t gram(const GramPlan& p, Gemm g, hipStream_t s) {
+    const Epilogue ep{};
+    const dim3 grid(p.tiles, p.splits), block(256);
+    hipLaunchKernelGGL((gemm_kernel<T, kOutGram, BF, 4>), grid, block, 0, s, g, ep, ColSum{});
+    hipLaunchKernelGGL((join_kernel<T, true>), dim3((g.gb + 3) / 4, g.ga / 8), block, 0, s, g, ep);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t gram_ws_bytes(int rows, int k) { return gram_plan(rows, k).total; }
 
 hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, int k,
                        const uint8_t* valid, const float* prev, float* out, void* ws,
                        hipStream_t s) {
-    const int steps = (rows + 63) / 64 * 2, nt = (k + kTile - 1) / kTile;
+    const GramPlan p = gram_plan(rows, k);
     uint16_t* xf = (uint16_t*)ws;
-    if (steps) hipLaunchKernelGGL(transpose_kernel, dim3(steps, k / 128), dim3(256), 0, s, (const uint16_t*)x, x_stride,
-                       rows, steps, valid, xf);
-    Gemm g{xf, xf, k / 16, k / 16, steps, 1, nullptr, prev, out, k};
-    const Epilogue ep{};
-    if (type == kBf16) hipLaunchKernelGGL((gemm_kernel<kBf16, kOutGram, true>), dim3(nt * (nt + 1) / 2),
-                                          dim3(512), 0, s, g, ep);
-    else hipLaunchKernelGGL((gemm_kernel<kF16, kOutGram, false>), dim3(nt * (nt + 1) / 2), dim3(512), 0, s, g,
-                            ep);
-    return hipGetLastError();
+    if (p.steps) hipLaunchKernelGGL(transpose_kernel, dim3(p.steps, k / 128), dim3(256), 0, s, (const uint16_t*)x,
+                                    x_stride, rows, p.steps, valid, xf);
+    const Gemm g{xf, xf, k / 16, k / 16, p.steps, p.tiles, p.splits, (float*)((uint8_t*)ws + p.part), prev, out, k};
+    return type == kBf16 ? gram<kBf16, true>(p, g, s) : gram<kF16, false>(p, g, s);
 }
 
 }  // namespace xtq

@@ -4,11 +4,13 @@
 
 namespace xtq {
 
-// Work of the experts: up to 16 of an expert's rows, in the order of the experts.
+// Work of the experts: up to 16 of an expert's rows, in the order of the experts,
+// with the expert's weights (gate, up, down), so that a workgroup finds all it
+// needs in one load.
 struct MoeChunk {
-    int32_t expert, rows;
+    xtq_moe_weight w[3];
+    int32_t rows, pad[3];
     int32_t slots[16];                  // token * top + place
-    int32_t pad[14];
 };
 
 // One call's arguments and scratch.  A token's choices are its slots.
@@ -43,7 +45,7 @@ constexpr int kMoeRows = 64;            // rows of a call
 constexpr int kMoeTop = 16;
 constexpr int kMoeExperts = 512;
 constexpr int kMoeFused = 4;            // rows up to which the first product transforms them itself
-constexpr int kMoeRouterCounters = 16;  // one for each 8 rows, one for all
+constexpr int kMoeRouterCounters = 32;  // one for each 4 rows, one for all
 
 #define XTQ_MOE(C) \
     hipError_t launch_moe_code##C(const MoeArgs& a, hipStream_t s);

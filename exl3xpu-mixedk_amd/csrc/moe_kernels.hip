@@ -39,9 +39,9 @@ __device__ __forceinline__ void split_range(int pairs, int splits, int split, in
 __global__ __launch_bounds__(256) void moe_x_kernel(MoeArgs a) {
     const int lane = threadIdx.x & 63, nk = a.d / 128, role = blockIdx.y, ch = blockIdx.z;
     const int kb = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (ch >= *a.nchunks || kb >= nk) return;
     const MoeChunk& c = a.chunks[ch];
-    const xtq_moe_weight w = a.table[3 * c.expert + role];
+    const xtq_moe_weight w = c.w[role];
+    if (ch >= *a.nchunks || kb >= nk) return;
     float su, sv;
     unpack_two(load_two(w.suh + 128 * kb, lane), kF16, su, sv);
     u4* hi = a.xf + ((size_t)(ch * 2 + role) * 2 * nk + kb) * 256;
@@ -68,10 +68,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_up_kernel(MoeArgs a) {
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nf = a.f / 128, nk = a.d / 128, ch = blockIdx.z, split = blockIdx.y;
     const int fb = blockIdx.x >> 1, role = blockIdx.x & 1;
-    if (ch >= *a.nchunks) return;
-    const MoeChunk& c = a.chunks[ch];
+    const MoeChunk& c = a.chunks[ch];   // (read before its number is known to be one)
     const int rows = c.rows;
-    const xtq_moe_weight w = a.table[3 * c.expert + role];
+    const xtq_moe_weight w = c.w[role];
+    if (ch >= *a.nchunks) return;
     if (FUSED && threadIdx.x < rows) list[threadIdx.x] = c.slots[threadIdx.x] / a.top;
     if (FUSED) __syncthreads();
     int s0, s1;
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_up_kernel(MoeArgs a) {
 #pragma unroll
         for (int i = 0; i < kFewTotals; ++i) sums[(o * 8 + i * kFewWaves + wv) * 64 + lane] = total[0][i];
     }
-    const xtq_moe_weight wg = a.table[3 * c.expert], wu = a.table[3 * c.expert + 1], wd = a.table[3 * c.expert + 2];
+    const xtq_moe_weight wg = c.w[0], wu = c.w[1], wd = c.w[2];
     float g0, g1, u0, u1, d0, d1;
     unpack_two(load_two(wg.svh + 128 * fb, lane), kF16, g0, g1);
     unpack_two(load_two(wu.svh + 128 * fb, lane), kF16, u0, u1);
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_up_kernel(MoeArgs a) {
 }
 
 // The last step for 128 columns: each row's residual and the weighted results
-// of its slots, four rows in flight by a wave.
+// of its slots, four rows and eight parts of each in flight by a wave.
 __device__ __forceinline__ void moe_finish(const MoeArgs& a, int db, int first, int step, int lane) {
     const int col = 128 * db + 2 * lane;
     const size_t slots = (size_t)a.rows * a.top;
@@ -140,20 +140,28 @@ __device__ __forceinline__ void moe_finish(const MoeArgs& a, int db, int first, 
             any |= in[i];
             o[i][0] = o[i][1] = 0.0f;
         }
+        const int parts = a.top * a.down_splits;
         if (any)
-            for (int p = 0; p < a.top * a.down_splits; ++p) {
-                u64 t[4];
+            for (int p0 = 0; p0 < parts; p0 += 8) {
+                u64 t[8][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const size_t slot = (size_t)(in[i] ? r0 + i * step : 0) * a.top + p / a.down_splits;
-                    const float* at = a.out + ((size_t)(p % a.down_splits) * slots + slot) * a.d + col;
-                    t[i] = in[i] ? __hip_atomic_load((const u64*)at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+                for (int u = 0; u < 8; ++u) {
+                    const int p = p0 + u < parts ? p0 + u : p0, place = p / a.down_splits;
+                    const float* at = a.out + (size_t)(p - place * a.down_splits) * slots * a.d + col;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        t[u][i] = in[i] ? __hip_atomic_load((const u64*)(at + ((size_t)(r0 + i * step) * a.top + place) * a.d),
+                                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                                        : 0;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[i][0] += __uint_as_float((uint32_t)t[i]);
-                    o[i][1] += __uint_as_float((uint32_t)(t[i] >> 32));
-                }
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (p0 + u < parts) {
+                            o[i][0] += __uint_as_float((uint32_t)t[u][i]);
+                            o[i][1] += __uint_as_float((uint32_t)(t[u][i] >> 32));
+                        }
             }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -179,13 +187,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_down_kernel(MoeArgs a) 
     __shared__ __align__(16) uint8_t bufs[kFewWaves][2][kMaxPairBytes];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nf = a.f / 128, db = blockIdx.x, split = blockIdx.y, ch = blockIdx.z, nchunks = *a.nchunks;
+    const MoeChunk& c = a.chunks[ch];
+    const xtq_moe_weight w = c.w[2];
     if (ch >= nchunks) {
         // no row has an expert: residuals and zeros
         if (nchunks == 0 && ch == 0 && split == 0) moe_finish(a, db, wv, kFewWaves, lane);
         return;
     }
-    const MoeChunk& c = a.chunks[ch];
-    const xtq_moe_weight w = a.table[3 * c.expert + 2];
     int s0, s1;
     split_range(a.f / 32, a.down_splits, split, s0, s1);
     const u4* hi = a.hf + (size_t)ch * 2 * nf * 256;

@@ -7,7 +7,7 @@
 namespace xtq {
 namespace {
 
-constexpr int kGroup = 8;               // rows of a workgroup
+constexpr int kGroup = 4;               // rows of a workgroup
 
 __device__ __forceinline__ float wave_sum(float v) {
     v += lane_xor<1>(v);
@@ -23,12 +23,18 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const uint32_t o = __shfl_xor(v, m);
-        v = o > v ? o : v;
-    }
-    return v;
+    auto most = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+    auto move = [](uint32_t x, auto c) {
+        return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, decltype(c)::value, 0xf, 0xf, true);
+    };
+    v = most(v, move(v, std::integral_constant<int, 0xB1>()));     // pairs, fours, eights, sixteens
+    v = most(v, move(v, std::integral_constant<int, 0x4E>()));
+    v = most(v, move(v, std::integral_constant<int, 0x141>()));
+    v = most(v, move(v, std::integral_constant<int, 0x140>()));
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = most(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return most(r[0], r[1]);
 }
 
 // Order of the logits as unsigned numbers: -0 is 0, NaN is above infinity.
@@ -39,9 +45,10 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 
 // A row's top-k by a wave: the largest logits, ties to the lowest expert, and
-// their softmax weights over all experts (renorm: over the chosen ones).
+// their softmax weights over all experts (renorm: over the chosen ones).  N: 64
+// N experts at most.
+template <int N>
 __device__ void choose(const MoeArgs& a, int row, int lane) {
-    constexpr int N = kMoeExperts / 64;
     if (a.valid && !a.valid[row]) {
         if (lane < a.top) {
             a.ids[row * a.top + lane] = -1;
@@ -108,29 +115,32 @@ __device__ void choose(const MoeArgs& a, int row, int lane) {
 }
 
 // The experts' chunks from all rows' choices, in the order of the experts and of
-// the slots.
+// the rows.  A row chooses an expert once at most, so 64 bits hold an expert's
+// rows, and a slot's place among them is the number of lower bits.
 __device__ void make_chunks(const MoeArgs& a) {
-    __shared__ int32_t count[kMoeExperts], first[kMoeExperts], ids[kMoeRows * kMoeTop];
+    __shared__ unsigned long long mask[kMoeExperts];
+    __shared__ int32_t first[kMoeExperts];
     const int t = threadIdx.x, slots = a.rows * a.top;
-    for (int e = t; e < a.experts; e += blockDim.x) count[e] = 0;
+    for (int e = t; e < a.experts; e += blockDim.x) mask[e] = 0;
     __syncthreads();
-    for (int s = t; s < slots; s += blockDim.x) {
-        // (a masked row's ids are the workgroup's that chose for it, or -1)
-        const int e = a.valid && !a.valid[s / a.top]
-                          ? -1
-                          : __hip_atomic_load(a.ids + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        ids[s] = e;
-        if (e >= 0) atomicAdd(&count[e], 1);
+    int own[kMoeRows * kMoeTop / 256];
+#pragma unroll
+    for (int i = 0; i < kMoeRows * kMoeTop / 256; ++i) {
+        const int s = t + 256 * i, row = s / a.top;
+        own[i] = -1;
+        if (s < slots && !(a.valid && !a.valid[row])) {
+            own[i] = __hip_atomic_load(a.ids + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            atomicOr(&mask[own[i]], 1ull << row);
+        }
     }
     __syncthreads();
     if (t < 64) {                                       // exclusive sums of the experts' chunks
         constexpr int N = kMoeExperts / 64;
-        int own[N], mine = 0;
+        int n[N], mine = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int e = t * N + i;
-            own[i] = e < a.experts ? (count[e] + 15) / 16 : 0;
-            mine += own[i];
+            n[i] = t * N + i < a.experts ? (__popcll(mask[t * N + i]) + 15) / 16 : 0;
+            mine += n[i];
         }
         int upto = mine;
         for (int m = 1; m < 64; m <<= 1) {
@@ -141,71 +151,87 @@ __device__ void make_chunks(const MoeArgs& a) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (t * N + i < a.experts) first[t * N + i] = at;
-            at += own[i];
+            at += n[i];
         }
         if (t == 63) *a.nchunks = upto;
     }
     __syncthreads();
-    for (int e = t; e < a.experts; e += blockDim.x)
-        for (int c = 0; 16 * c < count[e]; ++c) {
-            a.chunks[first[e] + c].expert = e;
-            a.chunks[first[e] + c].rows = count[e] - 16 * c < 16 ? count[e] - 16 * c : 16;
+    for (int e = t; e < a.experts; e += blockDim.x) {
+        const int rows = __popcll(mask[e]);
+        for (int c = 0; 16 * c < rows; ++c) {
+            MoeChunk& k = a.chunks[first[e] + c];
+            for (int i = 0; i < 3; ++i) k.w[i] = a.table[3 * e + i];
+            k.rows = rows - 16 * c < 16 ? rows - 16 * c : 16;
         }
-    // a slot's place among its expert's: the earlier slots of the same expert
-    for (int s = t; s < slots; s += blockDim.x) {
-        const int e = ids[s];
-        if (e < 0) continue;
-        int place = 0;
-        for (int o = 0; o < s; ++o) place += ids[o] == e ? 1 : 0;
-        a.chunks[first[e] + place / 16].slots[place % 16] = s;
+    }
+#pragma unroll
+    for (int i = 0; i < kMoeRows * kMoeTop / 256; ++i) {
+        const int s = t + 256 * i;
+        if (own[i] < 0) continue;
+        const int place = __popcll(mask[own[i]] & ((1ull << (s / a.top)) - 1));
+        a.chunks[first[own[i]] + place / 16].slots[place % 16] = s;
     }
 }
 
-// A wave makes one expert's logits of 8 rows, in fp32.  The workgroup that
-// finishes the last logits of its 8 rows chooses for them, the one that finishes
-// the last rows makes the lists.
+// A workgroup makes one expert's logits of 4 rows, in fp32, its waves a quarter
+// of the products each.  The one that finishes the last logits of its rows
+// chooses for them, the one that finishes the last rows makes the lists.
 __global__ __launch_bounds__(256) void moe_router_kernel(MoeArgs a) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, e = blockIdx.x * 4 + wv, r0 = blockIdx.y * kGroup;
+    __shared__ float sums[4][kGroup];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, e = blockIdx.x, r0 = blockIdx.y * kGroup;
     const int n = a.rows - r0 < kGroup ? a.rows - r0 : kGroup;
-    if (e < a.experts) {
-        float acc[kGroup];
+    float acc[kGroup];
 #pragma unroll
-        for (int i = 0; i < kGroup; ++i) acc[i] = 0.0f;
-        for (int c = 8 * lane; c < a.d; c += 512) {
-            float w[8];
-            if (a.router_f32) {
-                const float* p = (const float*)a.router + (size_t)e * a.d + c;
+    for (int i = 0; i < kGroup; ++i) acc[i] = 0.0f;
+#pragma unroll 2
+    for (int c = 8 * (int)threadIdx.x; c < a.d; c += 2048) {
+        float w[8];
+        if (a.router_f32) {
+            const float* p = (const float*)a.router + (size_t)e * a.d + c;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = p[i];
-            } else {
-                const u4 t = *(const u4_a2*)((const uint16_t*)a.router + (size_t)e * a.d + c);
+            for (int i = 0; i < 8; ++i) w[i] = p[i];
+        } else {
+            const u4 t = *(const u4_a2*)((const uint16_t*)a.router + (size_t)e * a.d + c);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) unpack_two(t[i], a.type, w[2 * i], w[2 * i + 1]);
-            }
-#pragma unroll
-            for (int r = 0; r < kGroup; ++r) {
-                if (r >= n) break;
-                const u4 t = *(const u4_a2*)(a.x + (size_t)(r0 + r) * a.x_stride + c);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float u, v;
-                    unpack_two(t[i], a.type, u, v);
-                    acc[r] = __builtin_fmaf(u, w[2 * i], acc[r]);
-                    acc[r] = __builtin_fmaf(v, w[2 * i + 1], acc[r]);
-                }
-            }
+            for (int i = 0; i < 4; ++i) unpack_two(t[i], a.type, w[2 * i], w[2 * i + 1]);
         }
+        u4 t[kGroup];
 #pragma unroll
-        for (int r = 0; r < kGroup; ++r) {
-            const float s = wave_sum(acc[r]);
-            if (lane == 0 && r < n)
-                __hip_atomic_store(a.logits + (size_t)(r0 + r) * a.experts + e, s, __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_AGENT);
-        }
+        for (int r = 0; r < kGroup; ++r)
+            t[r] = *(const u4_a2*)(a.x + (size_t)(r0 + (r < n ? r : 0)) * a.x_stride + c);
+#pragma unroll
+        for (int r = 0; r < kGroup; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float u, v;
+                unpack_two(t[r][i], a.type, u, v);
+                acc[r] = __builtin_fmaf(u, w[2 * i], acc[r]);
+                acc[r] = __builtin_fmaf(v, w[2 * i + 1], acc[r]);
+            }
+    }
+#pragma unroll
+    for (int r = 0; r < kGroup; ++r) {
+        const float s = wave_sum(acc[r]);
+        if (lane == 0) sums[wv][r] = s;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+        const float s = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+        __hip_atomic_store(a.logits + (size_t)(r0 + threadIdx.x) * a.experts + e, s, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
     }
     if (!arrive(a.counters + blockIdx.y, gridDim.x, threadIdx.x)) return;
-    for (int r = wv; r < n; r += 4) choose(a, r0 + r, lane);
-    if (!arrive(a.counters + kMoeRouterCounters - 1, gridDim.y, threadIdx.x)) return;
+    if (wv < n) {
+        if (a.experts <= 64) choose<1>(a, r0 + wv, lane);
+        else if (a.experts <= 128) choose<2>(a, r0 + wv, lane);
+        else choose<kMoeExperts / 64>(a, r0 + wv, lane);
+    }
+    if (gridDim.y > 1) {
+        if (!arrive(a.counters + kMoeRouterCounters - 1, gridDim.y, threadIdx.x)) return;
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // the choices are read below
+        __syncthreads();
+    }
     make_chunks(a);
 }
 
@@ -217,10 +243,10 @@ int most_chunks(int rows, int experts, int top) {
     return by < slots ? by : slots;
 }
 
-// Parts of a product's summed dimension that fill the compute units twice when
-// the slots fall on different experts; each wave has two 32-row steps at least.
+// Parts of a product's summed dimension that fill the compute units when the
+// slots fall on different experts; each wave has two 32-row steps at least.
 int moe_splits(int dim, int wgs) {
-    int s = 2 * kCUs / wgs;
+    int s = kCUs / wgs;
     if (s > dim / 256) s = dim / 256;
     return s < 1 ? 1 : s;
 }
@@ -276,7 +302,7 @@ hipError_t launch_moe(MoeArgs a, void* ws, hipStream_t s) {
     a.max_chunks = p.chunks;
     a.up_splits = p.up_splits;
     a.down_splits = p.down_splits;
-    hipLaunchKernelGGL(moe_router_kernel, dim3((a.experts + 3) / 4, (a.rows + kGroup - 1) / kGroup), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(moe_router_kernel, dim3(a.experts, (a.rows + kGroup - 1) / kGroup), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.code == kCodeMul1) return launch_moe_code0(a, s);

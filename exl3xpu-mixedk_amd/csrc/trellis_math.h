@@ -72,10 +72,33 @@ __device__ __forceinline__ float half_bits(uint32_t bits) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
-// Activations in fp32 (act is uniform); relu keeps NaN.  silu's exp overflows to
-// infinity for z < -88, its reciprocal is 0 and the product -0; v_rcp_f32 and the
-// exponential are within a few units of 2^-24 of a result that is rounded to
-// 16 bits.  gelu is the erf form.
+// Exponential and reciprocal of the vector unit: a few units of 2^-24, times the
+// argument for the exponential, of results that are rounded to 16 bits.
+__device__ __forceinline__ float fast_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
+__device__ __forceinline__ float fast_rcp(float v) { return __builtin_amdgcn_rcpf(v); }
+
+// Normal distribution function, cdf(z) = erfc(-z / sqrt(2)) / 2, from
+// erfc(x) = t exp(P(t) - x^2), t = 1 / (1 + x / 2), x >= 0: P is a Chebyshev fit of
+// log(erfc(x) exp(x^2) / t) over x <= 20, relative error 3.3e-7 in fp32, so small
+// values keep their digits.
+__device__ __forceinline__ float normal_cdf(float z) {
+    const float x = fabsf(z) * 0.70710678f, t = fast_rcp(__builtin_fmaf(0.5f, x, 1.0f));
+    float p = 0.176894663f;
+    p = __builtin_fmaf(p, t, -0.850723108f);
+    p = __builtin_fmaf(p, t, 1.54551778f);
+    p = __builtin_fmaf(p, t, -1.19725316f);
+    p = __builtin_fmaf(p, t, 0.318832828f);
+    p = __builtin_fmaf(p, t, -0.201707699f);
+    p = __builtin_fmaf(p, t, 0.100208923f);
+    p = __builtin_fmaf(p, t, 0.373702067f);
+    p = __builtin_fmaf(p, t, 1.00003991f);
+    p = __builtin_fmaf(p, t, -1.26551212f);
+    const float h = 0.5f * t * fast_exp(__builtin_fmaf(-x, x, p));
+    return z < 0.0f ? h : 1.0f - h;
+}
+
+// Activations in fp32 (act is uniform); relu keeps NaN.  silu's exponential
+// overflows to infinity for z < -88, its reciprocal is 0 and the product -0.
 template <int N>
 __device__ __forceinline__ void activate(float* v, int act) {
     if (act == kActRelu) {
@@ -83,10 +106,10 @@ __device__ __forceinline__ void activate(float* v, int act) {
         for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
     } else if (act == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= __builtin_amdgcn_rcpf(1.0f + expf(-v[i]));
+        for (int i = 0; i < N; ++i) v[i] *= fast_rcp(1.0f + fast_exp(-v[i]));
     } else if (act == kActGelu) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= 0.5f * (1.0f + erff(v[i] * 0.70710678118654752f));
+        for (int i = 0; i < N; ++i) v[i] *= normal_cdf(v[i]);
     }
 }
 
@@ -95,15 +118,37 @@ __device__ __forceinline__ void activate(float* v, int act) {
 __device__ __forceinline__ float act_slope(float z, int act) {
     if (act == kActRelu) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
     if (act == kActSilu) {
-        const float s = 1.0f / (1.0f + expf(-z));
+        const float s = fast_rcp(1.0f + fast_exp(-z));
         const float t = fabsf(z) > 100.0f ? 0.0f : z * (1.0f - s);
         return s * (1.0f + t);
     }
     if (act == kActGelu) {
-        const float d = fabsf(z) > 20.0f ? 0.0f : z * expf(-0.5f * z * z);
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + 0.39894228040143268f * d;
+        const float d = fabsf(z) > 20.0f ? 0.0f : z * fast_exp(-0.5f * z * z);
+        return __builtin_fmaf(0.39894228f, d, normal_cdf(z));
     }
     return 1.0f;
+}
+
+// Data-parallel move inside a row of 16 lanes (4 of lane_xor is the mirror of 8
+// lanes and the mirror of 4).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    const int b = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, 0xf, 0xf, true));
+}
+
+// 4 by 4 transpose among each four neighbouring lanes: afterwards element i of
+// lane 4 a + b is what element b of lane 4 a + i was.
+__device__ __forceinline__ f4 transpose4(f4 v, int lane) {
+    auto move = [](float x, auto c) { return dpp<decltype(c)::value>(x); };
+    using X1 = std::integral_constant<int, 0xB1>;       // lanes 1 0 3 2
+    using X2 = std::integral_constant<int, 0x4E>;       // lanes 2 3 0 1
+    const bool o1 = lane & 1, o2 = lane & 2;
+    // pairs: lane bit 0 with element bit 0, then lane bit 1 with element bit 1
+    const float a = move(o1 ? v[0] : v[1], X1()), b = move(o1 ? v[2] : v[3], X1());
+    v = o1 ? (f4){a, v[1], b, v[3]} : (f4){v[0], a, v[2], b};
+    const float c = move(o2 ? v[0] : v[2], X2()), d = move(o2 ? v[1] : v[3], X2());
+    return o2 ? (f4){c, d, v[2], v[3]} : (f4){v[0], v[1], c, d};
 }
 
 // Largest value of the lanes that differ in bits 4 and 5.
@@ -116,14 +161,7 @@ __device__ __forceinline__ float rows_max(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Value of the lane whose number differs in one bit, M = 1, 2, 4 or 8 (bits
-// inside a row of 16 lanes: data-parallel moves; 4 is the mirror of 8 lanes and
-// the mirror of 4).
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    const int b = __float_as_int(v);
-    return __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, 0xf, 0xf, true));
-}
+// Value of the lane whose number differs in one bit, M = 1, 2, 4 or 8.
 template <int M>
 __device__ __forceinline__ float lane_xor(float v) {
     if constexpr (M == 1) return dpp<0xB1>(v);
