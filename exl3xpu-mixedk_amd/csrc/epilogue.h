@@ -137,26 +137,21 @@ __device__ __forceinline__ void unit_row(const f4* unit, int row, int lane, floa
     b = p[1];
 }
 
-// Rows first, first + step, .. of units of 128 columns in LDS (`units`: one per
-// 16 rows), four rows at a time by the wave.
-template <int T>
-__device__ __forceinline__ void finish_rows(const f4* units, const Epilogue& ep, int blk, int first, int step,
-                                            int lane) {
+// R rows (row0 + i step, up to ep.rows) of the columns whose sums the wave's
+// lanes hold, 2 l and 2 l + 1 of block blk: transform, scales, bias, activation,
+// residual, store.
+template <int R>
+__device__ __forceinline__ void finish_rows(float (&v)[R][2], const Columns<2>& c, const Epilogue& ep, int type,
+                                            int blk, int row0, int step, int lane) {
     const int col = blk * 128 + 2 * lane;
-    const Columns<2> c = load_columns<T, 2>(ep, col);
-#pragma unroll 1
-    for (int r0 = first; r0 < ep.rows; r0 += 4 * step) {
-        float v[4][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = r0 + i * step < ep.rows ? r0 + i * step : r0;
-            unit_row(units + (row >> 4) * 512, row & 15, lane, v[i][0], v[i][1]);
-        }
+    for (int i = 0; i < R; ++i) transform_row(v[i][0], v[i][1], lane);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) transform_row(v[i][0], v[i][1], lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (r0 + i * step < ep.rows) finish_cols<T, 2>(v[i], c, ep, r0 + i * step, col);
+    for (int i = 0; i < R; ++i) {
+        const int row = row0 + i * step;
+        if (row >= ep.rows) break;
+        if (type == kBf16) finish_cols<kBf16, 2>(v[i], c, ep, row, col);
+        else finish_cols<kF16, 2>(v[i], c, ep, row, col);
     }
 }
 

@@ -199,15 +199,8 @@ __device__ __forceinline__ void store_shared(float* p, f4 v) {
                            __HIP_MEMORY_SCOPE_AGENT);
 }
 
-__device__ __forceinline__ f4 load_shared(const float* p) {
-    u4 b;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const u64 t = __hip_atomic_load((const u64*)p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        b[2 * i] = (uint32_t)t;
-        b[2 * i + 1] = (uint32_t)(t >> 32);
-    }
-    return __builtin_bit_cast(f4, b);
+__device__ __forceinline__ u64 load_shared(const float* p) {
+    return __hip_atomic_load((const u64*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 __device__ __forceinline__ bool arrive(uint32_t* counter, uint32_t parts, int thread) {
@@ -223,24 +216,31 @@ __device__ __forceinline__ bool arrive(uint32_t* counter, uint32_t parts, int th
     return before == parts - 1;
 }
 
-// Sums over `parts` parts, `stride` floats apart, in order, U of them in flight:
-// what a load waits for here is a trip to memory and back.
-template <int U, int N>
-__device__ __forceinline__ void sum_shared(f4 (&t)[N], const float* p, int step, size_t stride, int parts) {
+// Lane l's columns 2 l and 2 l + 1 of R rows (row0 + i step, up to rows), each the
+// sum of `parts` parts `stride` floats apart, in order; R U loads in flight.  A
+// wave's load is one row's 512 bytes: such loads pass no cache, and four lanes'
+// 8 bytes of as many lines took four times as long.
+template <int U, int R>
+__device__ __forceinline__ void sum_rows(float (&v)[R][2], const float* part, int row0, int step, int rows,
+                                         size_t stride, int parts, int lane) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) t[n] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < R; ++i) v[i][0] = v[i][1] = 0.0f;
     for (int s = 0; s < parts; s += U) {
-        f4 v[U][N];
+        u64 t[U][R];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
+        for (int u = 0; u < U; ++u) {
+            const float* p = part + (s + u < parts ? s + u : s) * stride + 2 * lane;
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-                v[i][n] = load_shared(p + n * step + (s + i < parts ? s + i : parts - 1) * stride);
+            for (int i = 0; i < R; ++i) t[u][i] = load_shared(p + (row0 + i * step < rows ? row0 + i * step : row0) * 128);
+        }
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (s + i < parts) {
+        for (int u = 0; u < U; ++u)
+            if (s + u < parts) {
 #pragma unroll
-                for (int n = 0; n < N; ++n) t[n] += v[i][n];
+                for (int i = 0; i < R; ++i) {
+                    v[i][0] += __uint_as_float((uint32_t)t[u][i]);
+                    v[i][1] += __uint_as_float((uint32_t)(t[u][i] >> 32));
+                }
             }
     }
 }
@@ -263,22 +263,30 @@ struct FewSource {
     const int32_t* shift;
 };
 
-// Blocks transformed at a time (FUSED); 4 KiB of LDS each, 8 with LO.
-template <bool LO>
-constexpr int kSlice = LO ? 4 : 8;
-// 16-byte words of LDS that few_sums takes: the rows' fragments, later the waves'
-// sums.
-constexpr int kFewLds = 2048;
-constexpr int kFewTotals = 8 / kFewWaves;               // tile columns a wave adds
+// LDS of a workgroup of W waves: the waves' trellis buffers, and FUSED the rows'
+// fragments (4 KiB a block, 8 with LO), of as many blocks as leave room for a
+// second workgroup on the compute unit; at the end the waves' sums lie there.
+constexpr int few_slice(int K, int W, bool LO) {
+    const int n = (76 * 1024 - W * 2 * 512 * K) / (LO ? 8192 : 4096);
+    return n > 8 ? 8 : n;
+}
+constexpr int few_lds(int K, int W, bool fused, bool LO) {
+    const int need = W * 2 * 512 * K + (fused ? few_slice(K, W, LO) * (LO ? 8192 : 4096) : 0);
+    return need > 32768 ? need : 32768;
+}
+constexpr int kFewMaxSlice = 8;
 
-// Sums of steps s0 .. s1 of the summed dimension: total[g][i] of a wave's lane is
-// tile column i kFewWaves + wave of row group g, in the matrix cores' layout.
-template <int K, int CODE, int G, bool FUSED, bool LO>
-__device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4* lds, uint8_t* buf,
-                                         int32_t* shifts, f4 (&total)[G][kFewTotals]) {
+// Sums of steps s0 .. s1 of the summed dimension by W waves: total[g][i] of a
+// wave's lane is tile column i W + wave of row group g, in the matrix cores'
+// layout.
+template <int K, int CODE, int G, int W, bool FUSED, bool LO>
+__device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4* lds, int32_t* shifts,
+                                         f4 (&total)[G][8 / W]) {
+    constexpr int SL = few_slice(K, W, LO);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Window win = lane_window<K>(lane);
-    u4 *const frag = lds, *const frag_lo = lds + kSlice<LO> * 256;
+    uint8_t* const buf = (uint8_t*)lds + wv * 2 * kPairBytes<K>;
+    u4 *const frag = lds + W * 64 * K, *const frag_lo = frag + SL * 256;
     f4* const sums = (f4*)lds;
     f4 acc[G][8];
     int shift[G];
@@ -289,8 +297,8 @@ __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4*
         for (int j = 0; j < 8; ++j) acc[g][j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
     }
     for (int c0 = s0; c0 < s1;) {
-        const int kb0 = c0 >> 2, cut = (kb0 + kSlice<LO>) << 2, c1 = FUSED && cut < s1 ? cut : s1;
-        const int p0 = c0 + (c1 - c0) * wv / kFewWaves, p1 = c0 + (c1 - c0) * (wv + 1) / kFewWaves;
+        const int kb0 = c0 >> 2, cut = (kb0 + SL) << 2, c1 = FUSED && cut < s1 ? cut : s1;
+        const int p0 = c0 + (c1 - c0) * wv / W, p1 = c0 + (c1 - c0) * (wv + 1) / W;
         PairRegs<K> r[2];
         auto load = [&](PairRegs<K>& t, int p) {
             p = p < p1 ? p : p1 - 1;
@@ -299,11 +307,11 @@ __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4*
         if constexpr (FUSED) {
             const int nk = ((c1 + 3) >> 2) - kb0, items = a.rows * nk;
             if (c0 > s0) __syncthreads();
-            for (int t = wv; t < items || t == wv; t += 4 * kFewWaves) {
+            for (int t = wv; t < items || t == wv; t += 4 * W) {
                 uint32_t xw[4], sw[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int item = t + i * kFewWaves;
+                    const int item = t + i * W;
                     if (item >= items) break;
                     const int kbi = item * a.rinv >> 16, row = item - kbi * a.rows;
                     const size_t at = a.list ? a.list[row] : row;
@@ -316,7 +324,7 @@ __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4*
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int item = t + i * kFewWaves;
+                    const int item = t + i * W;
                     if (item >= items) break;
                     const int kbi = item * a.rinv >> 16, row = item - kbi * a.rows;
                     float u, v, su, sv;
@@ -395,19 +403,28 @@ __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4*
         }
         c0 = c1;
     }
-    // the waves' sums, in the order of the waves
+    // the waves' sums, wave w + 4 added to wave w's first where there are eight
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         const float s = shift[g] == kNoShift ? 0.0f : ldexpf(1.0f, -shift[g] - 7);
+        f4* const mine = sums + (wv & 3) * 512 + lane;
+        __syncthreads();
+        if (W == 8) {
+            if (wv >= 4) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mine[j * 64] = acc[g][j] * s;
+            }
+            __syncthreads();
+        }
+        if (wv < 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mine[j * 64] = W == 8 ? acc[g][j] * s + mine[j * 64] : acc[g][j] * s;
+        }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sums[(wv * 8 + j) * 64 + lane] = acc[g][j] * s;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kFewTotals; ++i) {
-            total[g][i] = sums[(i * kFewWaves + wv) * 64 + lane];
-#pragma unroll
-            for (int o = 1; o < kFewWaves; ++o) total[g][i] += sums[(o * 8 + i * kFewWaves + wv) * 64 + lane];
+        for (int i = 0; i < 8 / W; ++i) {
+            const f4* p = sums + (i * W + wv) * 64 + lane;
+            total[g][i] = (p[0] + p[512]) + (p[1024] + p[1536]);
         }
     }
     __syncthreads();

@@ -16,50 +16,70 @@ namespace {
 // at a time, into LDS.  The waves' sums meet in LDS, the workgroups' in scratch,
 // where the last one to arrive adds them in order and finishes the columns.
 template <int K, int CODE, int G, bool FUSED>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(Weight w, FewArgs a, Epilogue ep) {
-    __shared__ __align__(16) u4 lds[kFewLds];
-    __shared__ __align__(16) uint8_t bufs[kFewWaves][2][kPairBytes<K>];
-    __shared__ int32_t shifts[FUSED ? kSlice<false> * 16 : 1];
+__global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(Weight w, FewArgs a, Epilogue ep) {
+    constexpr int W = few_waves(G), N = 8 / W;
+    __shared__ __align__(16) u4 lds[few_lds(K, W, FUSED, false) / 16];
+    __shared__ int32_t shifts[FUSED ? kFewMaxSlice * 16 : 1];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nb = gridDim.x, blk = blockIdx.x, split = blockIdx.y;
     // this workgroup's 32-row steps
     const int s0 = split * a.steps + (split < a.more ? split : a.more), s1 = s0 + a.steps + (split < a.more ? 1 : 0);
     const FewSource src{(const uint8_t*)w.trellis + (size_t)blk * 256 * K, (size_t)nb * 256 * K, ep.rows, w.k / 32,
                         a.x, a.x_stride, nullptr, w.suh, a.type, a.rinv, a.frag, nullptr, a.shift};
-    f4 total[G][kFewTotals];
-    few_sums<K, CODE, G, FUSED, false>(src, s0, s1, lds, bufs[wv][0], shifts, total);
+    f4 total[G][N];
+    few_sums<K, CODE, G, W, FUSED, false>(src, s0, s1, lds, shifts, total);
+    // (on their way while the workgroups meet)
+    const Columns<2> cols = a.type == kBf16 ? load_columns<kBf16, 2>(ep, blk * 128 + 2 * lane)
+                                            : load_columns<kF16, 2>(ep, blk * 128 + 2 * lane);
     if (a.splits > 1) {
-        float* mine = a.part + ((size_t)split * nb + blk) * G * 2048 + wv * 256 + lane * 4;
+        // [split][blk][row][128]
+        float* mine = a.part + ((size_t)split * nb + blk) * ep.rows * 128 + 4 * (lane >> 4);
 #pragma unroll
-        for (int g = 0; g < G; ++g)
-            if (16 * g + (lane & 15) < ep.rows) {
+        for (int g = 0; g < G; ++g) {
+            const int row = 16 * g + (lane & 15);
+            if (row < ep.rows) {
 #pragma unroll
-                for (int i = 0; i < kFewTotals; ++i)
-                    store_shared(mine + g * 2048 + i * kFewWaves * 256, total[g][i]);
+                for (int i = 0; i < N; ++i) store_shared(mine + row * 128 + 16 * (i * W + wv), total[g][i]);
             }
+        }
         if (!arrive(a.counters + blk, a.splits, threadIdx.x)) return;
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-            if (16 * g + (lane & 15) < ep.rows)
-                sum_shared<16 / G>(total[g], a.part + ((size_t)blk * G + g) * 2048 + wv * 256 + lane * 4,
-                                   kFewWaves * 256, (size_t)nb * G * 2048, a.splits);
+        constexpr int R = G == 1 ? 2 : 4, U = G == 1 ? 16 : 4;
+#pragma unroll 1
+        for (int r0 = wv; r0 < ep.rows; r0 += R * W) {
+            float v[R][2];
+            sum_rows<U, R>(v, a.part + (size_t)blk * ep.rows * 128, r0, W, ep.rows, (size_t)nb * ep.rows * 128,
+                           a.splits, lane);
+            finish_rows<R>(v, cols, ep, a.type, blk, r0, W, lane);
+        }
+        return;
     }
     f4* const sums = (f4*)lds;
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < kFewTotals; ++i) sums[(g * 8 + i * kFewWaves + wv) * 64 + lane] = total[g][i];
+        for (int i = 0; i < N; ++i) sums[(g * 8 + i * W + wv) * 64 + lane] = total[g][i];
     __syncthreads();
-    if (a.type == kBf16) finish_rows<kBf16>(sums, ep, blk, wv, kFewWaves, lane);
-    else finish_rows<kF16>(sums, ep, blk, wv, kFewWaves, lane);
+#pragma unroll 1
+    for (int r0 = wv; r0 < ep.rows; r0 += 4 * W) {
+        float v[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = r0 + i * W < ep.rows ? r0 + i * W : r0;
+            unit_row(sums + (row >> 4) * 512, row & 15, lane, v[i][0], v[i][1]);
+        }
+        finish_rows<4>(v, cols, ep, a.type, blk, r0, W, lane);
+    }
 }
 
 template <int K, int CODE>
 hipError_t few_kc(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s) {
-    const dim3 grid(w.n / 128, a.splits), block(64 * kFewWaves);
-    if (!a.frag) hipLaunchKernelGGL((few_kernel<K, CODE, 1, true>), grid, block, 0, s, w, a, ep);
-    else if (ep.rows <= 32) hipLaunchKernelGGL((few_kernel<K, CODE, 2, false>), grid, block, 0, s, w, a, ep);
-    else hipLaunchKernelGGL((few_kernel<K, CODE, 4, false>), grid, block, 0, s, w, a, ep);
+    const dim3 grid(w.n / 128, a.splits);
+    if (!a.frag)
+        hipLaunchKernelGGL((few_kernel<K, CODE, 1, true>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
+    else if (ep.rows <= 32)
+        hipLaunchKernelGGL((few_kernel<K, CODE, 2, false>), grid, dim3(64 * few_waves(2)), 0, s, w, a, ep);
+    else
+        hipLaunchKernelGGL((few_kernel<K, CODE, 4, false>), grid, dim3(64 * few_waves(4)), 0, s, w, a, ep);
     return hipGetLastError();
 }
 

@@ -617,9 +617,9 @@ __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __re
 }
 
 // Workgroups per 128 columns of a product of few rows: two for each compute
-// unit, each wave with two 32-row steps at least.
-int few_splits(int k, int n) {
-    const int most = k / 256;
+// unit, each wave with a 32-row step at least.
+int few_splits(int k, int n, int waves) {
+    const int most = k / 32 / waves;
     int s = 2 * kCUs / (n / 128);
     if (s > most) s = most;
     return s < 1 ? 1 : s;
@@ -636,11 +636,11 @@ struct FewPlan {
 
 FewPlan few_plan(int rows, int k, int n) {
     FewPlan p;
-    p.splits = few_splits(k, n);
     const int g = few_groups(rows);
+    p.splits = few_splits(k, n, few_waves(g));
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t a = at; at += align256(bytes); return a; };
-    p.part = take(p.splits > 1 ? (size_t)p.splits * n * g * 64 : 0);
+    p.part = take(p.splits > 1 ? (size_t)p.splits * n * rows * 4 : 0);
     const bool apart = rows > kFusedRows;
     p.frag = take(apart ? (size_t)g * k * 32 : 0);
     p.shift = take(apart ? (size_t)g * k / 2 : 0);

@@ -12,19 +12,22 @@ namespace xtq {
 namespace {
 
 constexpr int kCode = XTQ_MOE_CODE;
-constexpr int kMaxPairBytes = kPairBytes<7>;
+constexpr int W = 8;                    // waves of a workgroup
+constexpr int kLds = few_lds(7, W, true, true), kLdsApart = few_lds(7, W, false, true);
+static_assert(kLds >= few_lds(2, W, true, true) && kLds >= few_lds(4, W, true, true) &&
+              kLds >= few_lds(6, W, true, true), "LDS of every width");
 
 // few_sums of an expert's width (one of 2..7: checked when the table was made).
 template <bool FUSED>
-__device__ __forceinline__ void expert_sums(int K, const FewSource& src, int s0, int s1, u4* lds, uint8_t* buf,
-                                            int32_t* shifts, f4 (&total)[1][kFewTotals]) {
+__device__ __forceinline__ void expert_sums(int K, const FewSource& src, int s0, int s1, u4* lds, int32_t* shifts,
+                                            f4 (&total)[1][1]) {
     switch (K) {
-        case 2: return few_sums<2, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
-        case 3: return few_sums<3, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
-        case 4: return few_sums<4, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
-        case 5: return few_sums<5, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
-        case 6: return few_sums<6, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
-        default: return few_sums<7, kCode, 1, FUSED, true>(src, s0, s1, lds, buf, shifts, total);
+        case 2: return few_sums<2, kCode, 1, W, FUSED, true>(src, s0, s1, lds, shifts, total);
+        case 3: return few_sums<3, kCode, 1, W, FUSED, true>(src, s0, s1, lds, shifts, total);
+        case 4: return few_sums<4, kCode, 1, W, FUSED, true>(src, s0, s1, lds, shifts, total);
+        case 5: return few_sums<5, kCode, 1, W, FUSED, true>(src, s0, s1, lds, shifts, total);
+        case 6: return few_sums<6, kCode, 1, W, FUSED, true>(src, s0, s1, lds, shifts, total);
+        default: return few_sums<7, kCode, 1, W, FUSED, true>(src, s0, s1, lds, shifts, total);
     }
 }
 
@@ -60,10 +63,9 @@ __global__ __launch_bounds__(256) void moe_x_kernel(MoeArgs a) {
 // dimension; the last workgroup of the two weights' parts adds them, applies the
 // activation and leaves the product's rows as fragments for the second product.
 template <bool FUSED>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void moe_up_kernel(MoeArgs a) {
-    __shared__ __align__(16) u4 lds[kFewLds];
-    __shared__ __align__(16) uint8_t bufs[kFewWaves][2][kMaxPairBytes];
-    __shared__ int32_t shifts[kSlice<true> * 16];
+__global__ __launch_bounds__(64 * W, 4) void moe_up_kernel(MoeArgs a) {
+    __shared__ __align__(16) u4 lds[(FUSED ? kLds : kLdsApart) / 16];
+    __shared__ int32_t shifts[kFewMaxSlice * 16];
     __shared__ int32_t list[16];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nf = a.f / 128, nk = a.d / 128, ch = blockIdx.z, split = blockIdx.y;
@@ -81,47 +83,40 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_up_kernel(MoeArgs a) {
                         a.x, a.x_stride, list, w.suh, a.type, 65536u / rows + 1, hi,
                         FUSED ? nullptr : hi + (size_t)nk * 256,
                         FUSED ? nullptr : a.xs + (size_t)(ch * 2 + role) * nk * 16};
-    f4 total[1][kFewTotals];
-    expert_sums<FUSED>(w.K, src, s0, s1, lds, bufs[wv][0], shifts, total);
-    // [chunk][fb][role][split]
-    float* part = a.up_part + ((size_t)ch * nf + fb) * 2 * a.up_splits * 2048 + wv * 256 + lane * 4;
-    const bool mine = (lane & 15) < rows;
-    if (mine) {
-#pragma unroll
-        for (int i = 0; i < kFewTotals; ++i)
-            store_shared(part + (size_t)(role * a.up_splits + split) * 2048 + i * kFewWaves * 256, total[0][i]);
-    }
-    if (!arrive(a.counters + kMoeRouterCounters + a.d / 128 + ch * nf + fb, 2 * a.up_splits, threadIdx.x)) return;
-    f4* const sums = (f4*)lds;
-#pragma unroll
-    for (int o = 0; o < 2; ++o) {
-#pragma unroll
-        for (int i = 0; i < kFewTotals; ++i) total[0][i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-        if (mine) sum_shared<8>(total[0], part + (size_t)o * a.up_splits * 2048, kFewWaves * 256, 2048, a.up_splits);
-#pragma unroll
-        for (int i = 0; i < kFewTotals; ++i) sums[(o * 8 + i * kFewWaves + wv) * 64 + lane] = total[0][i];
-    }
+    f4 total[1][1];
+    expert_sums<FUSED>(w.K, src, s0, s1, lds, shifts, total);
+    // [chunk][fb][role][split][row][128]
+    float* part = a.up_part + ((size_t)ch * nf + fb) * 2 * a.up_splits * 2048;
+    if ((lane & 15) < rows)
+        store_shared(part + (size_t)(role * a.up_splits + split) * 2048 + (lane & 15) * 128 + 16 * wv + 4 * (lane >> 4),
+                     total[0][0]);
     const xtq_moe_weight wg = c.w[0], wu = c.w[1], wd = c.w[2];
-    float g0, g1, u0, u1, d0, d1;
+    float g0, g1, u0, u1, d0, d1;       // (on their way while the workgroups meet)
     unpack_two(load_two(wg.svh + 128 * fb, lane), kF16, g0, g1);
     unpack_two(load_two(wu.svh + 128 * fb, lane), kF16, u0, u1);
     unpack_two(load_two(wd.suh + 128 * fb, lane), kF16, d0, d1);
-    __syncthreads();
+    if (!arrive(a.counters + kMoeRouterCounters + a.d / 128 + ch * nf + fb, 2 * a.up_splits, threadIdx.x)) return;
     u4* out = a.hf + ((size_t)ch * 2 * nf + fb) * 256;
-    for (int r = wv; r < rows; r += kFewWaves) {
-        float v[2], u[2];
-        unit_row(sums, r, lane, v[0], v[1]);
-        unit_row(sums + 512, r, lane, u[0], u[1]);
-        transform_row(v[0], v[1], lane);
-        transform_row(u[0], u[1], lane);
-        v[0] *= g0 * wg.scale;
-        v[1] *= g1 * wg.scale;
-        activate<2>(v, a.act);
-        v[0] *= u[0] * (u0 * wu.scale);
-        v[1] *= u[1] * (u1 * wu.scale);
-        const int sh = row_to_frags<true>(v[0] * d0, v[1] * d1, lane, r, (uint32_t*)out,
-                                          (uint32_t*)(out + (size_t)nf * 256));
-        if (lane == 0) a.hs[((size_t)ch * nf + fb) * 16 + r] = sh;
+#pragma unroll 1
+    for (int r0 = wv; r0 < rows; r0 += 2 * W) {
+        float v[2][2], u[2][2];
+        sum_rows<4, 2>(v, part, r0, W, rows, 2048, a.up_splits, lane);
+        sum_rows<4, 2>(u, part + (size_t)a.up_splits * 2048, r0, W, rows, 2048, a.up_splits, lane);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + i * W;
+            if (r >= rows) break;
+            transform_row(v[i][0], v[i][1], lane);
+            transform_row(u[i][0], u[i][1], lane);
+            v[i][0] *= g0 * wg.scale;
+            v[i][1] *= g1 * wg.scale;
+            activate<2>(v[i], a.act);
+            v[i][0] *= u[i][0] * (u0 * wu.scale);
+            v[i][1] *= u[i][1] * (u1 * wu.scale);
+            const int sh = row_to_frags<true>(v[i][0] * d0, v[i][1] * d1, lane, r, (uint32_t*)out,
+                                              (uint32_t*)(out + (size_t)nf * 256));
+            if (lane == 0) a.hs[((size_t)ch * nf + fb) * 16 + r] = sh;
+        }
     }
 }
 
@@ -182,16 +177,15 @@ __device__ __forceinline__ void moe_finish(const MoeArgs& a, int db, int first, 
 
 // down's 128 columns for a chunk over a part of the summed dimension, weighted,
 // by slot; the last workgroup of the columns adds each row's slots in order.
-__global__ __launch_bounds__(64 * kFewWaves, 2) void moe_down_kernel(MoeArgs a) {
-    __shared__ __align__(16) u4 lds[kFewLds];
-    __shared__ __align__(16) uint8_t bufs[kFewWaves][2][kMaxPairBytes];
+__global__ __launch_bounds__(64 * W, 4) void moe_down_kernel(MoeArgs a) {
+    __shared__ __align__(16) u4 lds[kLdsApart / 16];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nf = a.f / 128, db = blockIdx.x, split = blockIdx.y, ch = blockIdx.z, nchunks = *a.nchunks;
     const MoeChunk& c = a.chunks[ch];
     const xtq_moe_weight w = c.w[2];
     if (ch >= nchunks) {
         // no row has an expert: residuals and zeros
-        if (nchunks == 0 && ch == 0 && split == 0) moe_finish(a, db, wv, kFewWaves, lane);
+        if (nchunks == 0 && ch == 0 && split == 0) moe_finish(a, db, wv, W, lane);
         return;
     }
     int s0, s1;
@@ -200,15 +194,14 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_down_kernel(MoeArgs a) 
     const FewSource src{(const uint8_t*)w.trellis + (size_t)db * 256 * w.K, (size_t)(a.d / 128) * 256 * w.K, c.rows,
                         a.f / 32, nullptr, 0, nullptr, nullptr, 0, 0, hi, hi + (size_t)nf * 256,
                         a.hs + (size_t)ch * nf * 16};
-    f4 total[1][kFewTotals];
-    expert_sums<false>(w.K, src, s0, s1, lds, bufs[wv][0], nullptr, total);
+    f4 total[1][1];
+    expert_sums<false>(w.K, src, s0, s1, lds, nullptr, total);
     f4* const sums = (f4*)lds;
-#pragma unroll
-    for (int i = 0; i < kFewTotals; ++i) sums[(i * kFewWaves + wv) * 64 + lane] = total[0][i];
+    sums[wv * 64 + lane] = total[0][0];
     float v0, v1;
     unpack_two(load_two(w.svh + 128 * db, lane), kF16, v0, v1);
     __syncthreads();
-    for (int r = wv; r < c.rows; r += kFewWaves) {
+    for (int r = wv; r < c.rows; r += W) {
         float v[2];
         unit_row(sums, r, lane, v[0], v[1]);
         transform_row(v[0], v[1], lane);
@@ -219,7 +212,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_down_kernel(MoeArgs a) 
                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if (!arrive(a.counters + kMoeRouterCounters + db, nchunks * a.down_splits, threadIdx.x)) return;
-    moe_finish(a, db, wv, kFewWaves, lane);
+    moe_finish(a, db, wv, W, lane);
 }
 
 }  // namespace
@@ -228,7 +221,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void moe_down_kernel(MoeArgs a) 
 #define XTQ_CAT(a, b) XTQ_CAT2(a, b)
 
 hipError_t XTQ_CAT(launch_moe_code, XTQ_MOE_CODE)(const MoeArgs& a, hipStream_t s) {
-    const dim3 block(64 * kFewWaves), up(2 * (a.f / 128), a.up_splits, a.max_chunks),
+    const dim3 block(64 * W), up(2 * (a.f / 128), a.up_splits, a.max_chunks),
         down(a.d / 128, a.down_splits, a.max_chunks);
     if (a.rows <= kMoeFused) {
         hipLaunchKernelGGL((moe_up_kernel<true>), up, block, 0, s, a);

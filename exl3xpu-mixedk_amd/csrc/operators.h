@@ -53,7 +53,9 @@ hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long lon
 // their shifts [group][k/128][16].
 constexpr int kFewRows = 64;
 constexpr int kFusedRows = 16;
-constexpr int kFewWaves = 4;            // waves of a workgroup
+// Waves of a workgroup: 8, which with their registers make four a SIMD, or 4
+// where 16 G rows' sums take the registers of two.
+constexpr int few_waves(int G) { return G == 1 ? 8 : 4; }
 struct FewArgs {
     int type;
     const uint16_t* x;
