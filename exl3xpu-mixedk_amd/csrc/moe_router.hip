@@ -243,10 +243,13 @@ int most_chunks(int rows, int experts, int top) {
     return by < slots ? by : slots;
 }
 
-// Parts of a product's summed dimension that fill the compute units when the
-// slots fall on different experts; each wave has two 32-row steps at least.
-int moe_splits(int dim, int wgs) {
-    int s = kCUs / wgs;
+// Parts of a product's summed dimension that make `most` workgroups when the
+// slots fall on different experts; each wave has a 32-row step at least.  Up's
+// fill the compute units twice; down's once, since the last of its workgroups
+// reads every part of every slot (one token, 8 experts of 2048 by 1024: 15 us,
+// 20 with twice the parts; up 17, 19 with half).
+int moe_splits(int dim, int wgs, int most) {
+    int s = most / wgs;
     if (s > dim / 256) s = dim / 256;
     return s < 1 ? 1 : s;
 }
@@ -260,8 +263,8 @@ MoePlan moe_plan(int rows, int experts, int top, int d, int f) {
     MoePlan p;
     p.chunks = most_chunks(rows, experts, top);
     const int slots = rows * top, likely = slots < experts ? slots : experts;
-    p.up_splits = moe_splits(d, likely * 2 * (f / 128));
-    p.down_splits = moe_splits(f, likely * (d / 128));
+    p.up_splits = moe_splits(d, likely * 2 * (f / 128), 2 * kCUs);
+    p.down_splits = moe_splits(f, likely * (d / 128), kCUs);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t a = at; at += align256(bytes); return a; };
     const size_t n = p.chunks;
