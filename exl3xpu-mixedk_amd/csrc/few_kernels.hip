@@ -15,10 +15,11 @@ namespace {
 // kFusedRows rows): it transforms the rows' part itself, a wave one row's block
 // at a time, into LDS.  The waves' sums meet in LDS, the workgroups' in scratch,
 // where the last one to arrive adds them in order and finishes the columns.
-template <int K, int CODE, int G, bool FUSED>
+// LO: with two terms.
+template <int K, int CODE, int G, bool FUSED, bool LO>
 __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(Weight w, FewArgs a, Epilogue ep) {
     constexpr int W = few_waves(G), N = 8 / W;
-    __shared__ __align__(16) u4 lds[few_lds(K, W, FUSED, false) / 16];
+    __shared__ __align__(16) u4 lds[few_lds(K, W, FUSED, LO) / 16];
     __shared__ int32_t shifts[FUSED ? kFewMaxSlice * 16 : 1];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nb = gridDim.x, blk = blockIdx.x, split = blockIdx.y;
@@ -27,7 +28,7 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(
     const FewSource src{(const uint8_t*)w.trellis + (size_t)blk * 256 * K, (size_t)nb * 256 * K, ep.rows, w.k / 32,
                         a.x, a.x_stride, nullptr, w.suh, a.type, a.rinv, a.frag, nullptr, a.shift};
     f4 total[G][N];
-    few_sums<K, CODE, G, W, FUSED, false>(src, s0, s1, lds, shifts, total);
+    few_sums<K, CODE, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
     // (on their way while the workgroups meet)
     const Columns<2> cols = a.type == kBf16 ? load_columns<kBf16, 2>(ep, blk * 128 + 2 * lane)
                                             : load_columns<kF16, 2>(ep, blk * 128 + 2 * lane);
@@ -74,12 +75,14 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(
 template <int K, int CODE>
 hipError_t few_kc(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s) {
     const dim3 grid(w.n / 128, a.splits);
-    if (!a.frag)
-        hipLaunchKernelGGL((few_kernel<K, CODE, 1, true>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
+    if (a.two)
+        hipLaunchKernelGGL((few_kernel<K, CODE, 1, true, true>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
+    else if (!a.frag)
+        hipLaunchKernelGGL((few_kernel<K, CODE, 1, true, false>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
     else if (ep.rows <= 32)
-        hipLaunchKernelGGL((few_kernel<K, CODE, 2, false>), grid, dim3(64 * few_waves(2)), 0, s, w, a, ep);
+        hipLaunchKernelGGL((few_kernel<K, CODE, 2, false, false>), grid, dim3(64 * few_waves(2)), 0, s, w, a, ep);
     else
-        hipLaunchKernelGGL((few_kernel<K, CODE, 4, false>), grid, dim3(64 * few_waves(4)), 0, s, w, a, ep);
+        hipLaunchKernelGGL((few_kernel<K, CODE, 4, false, false>), grid, dim3(64 * few_waves(4)), 0, s, w, a, ep);
     return hipGetLastError();
 }
 

@@ -84,10 +84,12 @@ __device__ __forceinline__ void scale8(const uint16_t* colscale, int col, float*
 // relative, as fp16 activations have themselves).  A wave takes 16 rows of one
 // 128-column block; lane 16 q + r holds columns 32 p + 8 q + j of row r, so five
 // of the transform's seven stages are between its own registers.  Rows past the
-// end are zeros.  colsum: sums over the 16 rows of the unscaled values, one row
-// of partial sums per 16 rows (for the bias' gradient).
+// end are zeros.  rest: or NULL, the fragments of what the rounding left.
+// colsum: sums over the 16 rows of the unscaled values, one row of partial sums
+// per 16 rows (for the bias' gradient).
 __global__ __launch_bounds__(256) void transform_kernel(Source s, const int32_t* __restrict__ shift,
                                                         uint16_t* __restrict__ frags,
+                                                        uint16_t* __restrict__ rest,
                                                         float* __restrict__ colsum) {
     const int lane = threadIdx.x & 63, nblk = s.cols / 128;
     const int blk = blockIdx.x * 4 + (threadIdx.x >> 6), grp = blockIdx.y;
@@ -136,6 +138,12 @@ __global__ __launch_bounds__(256) void transform_kernel(Source s, const int32_t*
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = (_Float16)v[8 * p + i];
         *(h8*)(out + frag_at(grp, 4 * blk + p, 4 * nblk)) = o;
+        if (rest) {
+            h8 l;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) l[i] = (_Float16)(v[8 * p + i] - (float)o[i]);
+            *(h8*)(rest + lane * 8 + frag_at(grp, 4 * blk + p, 4 * nblk)) = l;
+        }
     }
 }
 
@@ -264,7 +272,7 @@ __device__ __forceinline__ int xcd_order(int id, int all) {
 enum GemmOut { kOutEpilogue, kOutPartial, kOutGram };
 
 struct Gemm {
-    const uint16_t *A, *B;
+    const uint16_t *A, *B, *B2;         // B2: B's second terms (TERMS 2)
     int ga, gb;                         // 16-wide groups of columns, rows
     int steps;                          // 32-wide steps of the summed dimension
     int tiles, splits;                  // splits of the summed dimension
@@ -285,9 +293,10 @@ __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
 
-template <int T, int OUT, bool BF, int NB>
+template <int T, int OUT, bool BF, int NB, int TERMS>
 __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSum sums) {
-    constexpr int kFrags = 16 + 2 * NB, kOwn = 4 + NB / 2;      // of a step: the workgroup's, a wave's to move
+    // of a step: the workgroup's fragments, a wave's to move
+    constexpr int kFrags = 16 + 2 * NB * TERMS, kOwn = 4 + NB / 2 * TERMS;
     // (One LDS object: beside another, the compiler takes every read of this one
     // for a possible read of what a load to LDS still has to write, and waits.)
     __shared__ __align__(1024) uint8_t lds[3][kFrags * kFragBytes];
@@ -320,7 +329,8 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSu
     // this wave's fragments of a step: a quarter of A's 16 and of B's 2 NB
     const uint16_t* fa = g.A + (size_t)tn * g.steps * 8192 + wv * 2048 + lane * 8;
     const int gb0 = tm * 2 * NB;        // first group of rows
-    const uint16_t* fb = g.B + ((size_t)(gb0 >> 4) * g.steps * 16 + (gb0 & 15) + wv * (NB / 2)) * 512 + lane * 8;
+    const size_t at_b = ((size_t)(gb0 >> 4) * g.steps * 16 + (gb0 & 15) + wv * (NB / 2)) * 512 + lane * 8;
+    const uint16_t *fb = g.B + at_b, *fb2 = TERMS == 2 ? g.B2 + at_b : nullptr;
     int to = 0;                         // buffer of the next step to load
     auto load = [&](int s) {
         uint8_t* l = lds[to];
@@ -332,6 +342,12 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSu
         for (int i = 0; i < NB / 2; ++i)
             __builtin_amdgcn_global_load_lds((global_void*)(fb + (size_t)s * 8192 + i * 512),
                                              (lds_void*)(l + (16 + wv * (NB / 2) + i) * kFragBytes), 16, 0, 0);
+        if constexpr (TERMS == 2) {
+#pragma unroll
+            for (int i = 0; i < NB / 2; ++i)
+                __builtin_amdgcn_global_load_lds((global_void*)(fb2 + (size_t)s * 8192 + i * 512),
+                                                 (lds_void*)(l + (16 + 2 * NB + wv * (NB / 2) + i) * kFragBytes), 16, 0, 0);
+        }
         to = to == 2 ? 0 : to + 1;
     };
     // All waves' pieces of the next step are in LDS, and all waves have read this
@@ -354,17 +370,21 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSu
         int from = 0;
         for (int s = s0; s < s1; ++s) {
             if (s + 2 < s1) load(s + 2);
-            u4 a[8], b[NB];
+            u4 a[8], b[TERMS][NB];
             const uint8_t* l = lds[from] + lane * 16;
 #pragma unroll
-            for (int i = 0; i < NB; ++i) b[i] = *(const u4*)(l + (16 + wm * NB + i) * kFragBytes);
+            for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+                for (int i = 0; i < NB; ++i) b[t][i] = *(const u4*)(l + (16 + 2 * NB * t + wm * NB + i) * kFragBytes);
 #pragma unroll
             for (int j = 0; j < 8; ++j) a[j] = *(const u4*)(l + (wn * 8 + j) * kFragBytes);
             __builtin_amdgcn_sched_barrier(0);          // all reads under way before the first product
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int i = 0; i < NB; ++i) acc[j][i] = mfma<BF>(a[j], b[i], acc[j][i]);
+                for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) acc[j][i] = mfma<BF>(a[j], b[t][i], acc[j][i]);
             __builtin_amdgcn_sched_barrier(0);          // none after the others have met
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             meet_up(s + 2 < s1);
@@ -543,14 +563,14 @@ int gemm_nb(int rows, int n) { return (n + kTileN - 1) / kTileN * ((rows + 127) 
 
 struct ManyPlan {
     int groups, nb, tiles, splits;
-    size_t shift, rowexp, xf, wf, part, colsum, total;
+    size_t shift, rowexp, xf, x2, wf, part, colsum, total;
 };
 
 // Scratch of a product of `rows` rows: summed dimension k, columns n.
-ManyPlan many_plan(int rows, int k, int n, bool colsum) {
+ManyPlan many_plan(int rows, int k, int n, bool colsum, bool two) {
     ManyPlan p;
     p.groups = (rows + 15) / 16;
-    p.nb = gemm_nb(rows, n);
+    p.nb = two ? 2 : gemm_nb(rows, n);     // (two terms: the LDS of two workgroups)
     p.tiles = (n + kTileN - 1) / kTileN * ((p.groups + 2 * p.nb - 1) / (2 * p.nb));
     p.splits = gemm_splits(p.tiles, k / 32);
     size_t at = 0;
@@ -558,6 +578,7 @@ ManyPlan many_plan(int rows, int k, int n, bool colsum) {
     p.shift = take((size_t)p.groups * 64);
     p.rowexp = take((size_t)p.groups * 64);
     p.xf = take(frag_bytes(p.groups, k / 32));
+    p.x2 = take(two ? frag_bytes(p.groups, k / 32) : 0);
     p.wf = take(frag_bytes(n / 16, k / 32));
     p.part = take(p.splits > 1 ? (size_t)p.splits * p.groups * 64 * n : 0);
     p.colsum = take(colsum ? (size_t)p.groups * k * 4 : 0);
@@ -568,17 +589,17 @@ ManyPlan many_plan(int rows, int k, int n, bool colsum) {
 // The product of a source's rows with a weight (bwd: its transpose).
 template <int T>
 hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* dbias, int dbias_f32,
-                void* ws, hipStream_t s) {
+                bool two, void* ws, hipStream_t s) {
     const int k = src.cols, n = ep.cols, rows = src.rows;
-    const ManyPlan p = many_plan(rows, k, n, dbias != nullptr);
+    const ManyPlan p = many_plan(rows, k, n, dbias != nullptr, two);
     uint8_t* base = (uint8_t*)ws;
     int32_t *shift = (int32_t*)(base + p.shift), *rowexp = (int32_t*)(base + p.rowexp);
-    uint16_t *xf = (uint16_t*)(base + p.xf), *wf = (uint16_t*)(base + p.wf);
+    uint16_t *xf = (uint16_t*)(base + p.xf), *x2 = two ? (uint16_t*)(base + p.x2) : nullptr, *wf = (uint16_t*)(base + p.wf);
     float* colsum = dbias ? (float*)(base + p.colsum) : nullptr;
     const int decoders = ep.y ? (w.k / 16) * (w.n / 16) / 32 : 0;
     prepare(w, bwd, Prepare{wf, decoders, src, shift, rowexp}, s);
     hipLaunchKernelGGL(transform_kernel, dim3((k / 128 + 3) / 4, p.groups), dim3(256), 0, s, src,
-                       (const int32_t*)shift, xf, colsum);
+                       (const int32_t*)shift, xf, x2, colsum);
     const ColSum sums{colsum, p.groups, k, T, dbias_f32, dbias};
     const int adders = dbias ? (k + 63) / 64 : 0;
     if (!ep.y) {
@@ -586,14 +607,16 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
         return hipGetLastError();
     }
     ep.rowexp = rowexp;
-    const Gemm g{wf, xf, n / 16, p.groups, k / 32, p.tiles, p.splits, (float*)(base + p.part), nullptr, nullptr, 0};
+    const Gemm g{wf, xf, x2, n / 16, p.groups, k / 32, p.tiles, p.splits, (float*)(base + p.part), nullptr, nullptr, 0};
     const dim3 grid(p.tiles + adders, p.splits), block(256);
     if (p.splits == 1) {
-        if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 4>), grid, block, 0, s, g, ep, sums);
-        else hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 2>), grid, block, 0, s, g, ep, sums);
+        if (two) hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 2, 2>), grid, block, 0, s, g, ep, sums);
+        else if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 4, 1>), grid, block, 0, s, g, ep, sums);
+        else hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 2, 1>), grid, block, 0, s, g, ep, sums);
     } else {
-        if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 4>), grid, block, 0, s, g, ep, sums);
-        else hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2>), grid, block, 0, s, g, ep, sums);
+        if (two) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 2>), grid, block, 0, s, g, ep, sums);
+        else if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 4, 1>), grid, block, 0, s, g, ep, sums);
+        else hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 1>), grid, block, 0, s, g, ep, sums);
         hipLaunchKernelGGL((join_kernel<T, false>), dim3((p.groups + 3) / 4, n / 128), block, 0, s, g, ep);
     }
     return hipGetLastError();
@@ -625,7 +648,9 @@ int few_splits(int k, int n, int waves) {
     return s < 1 ? 1 : s;
 }
 
-bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_COUNTERS; }
+bool takes_few(int rows, int n, bool two) {
+    return rows <= (two ? kFusedRows : kFewRows) && n / 128 <= XTQ_OP_COUNTERS;
+}
 
 int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
@@ -651,18 +676,25 @@ FewPlan few_plan(int rows, int k, int n) {
 }  // namespace
 
 size_t linear_ws_bytes(int rows, int k, int n, int backward) {
-    if (!backward && takes_few(rows, n)) return few_plan(rows, k, n).total;
-    return backward ? many_plan(rows, n, k, true).total : many_plan(rows, k, n, false).total;
+    if (backward == 1) return many_plan(rows, n, k, true, false).total;
+    auto forward = [&](bool two) {
+        return takes_few(rows, n, two) ? few_plan(rows, k, n).total : many_plan(rows, k, n, false, two).total;
+    };
+    const size_t one = forward(false);
+    if (backward == 0) return one;
+    const size_t two = forward(true);   // (the activation decides which it is)
+    return one > two ? one : two;
 }
 
 hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
                          const Epilogue& ep, void* ws, uint32_t* counters, hipStream_t s) {
-    if (takes_few(rows, w.n)) {
+    const bool two = two_terms(type, ep.act, ep.z != nullptr);
+    if (takes_few(rows, w.n, two)) {
         static decltype(&launch_few_k2) const few[] = {launch_few_k2, launch_few_k3, launch_few_k4,
                                                        launch_few_k5, launch_few_k6, launch_few_k7};
         const FewPlan p = few_plan(rows, w.k, w.n);
         uint8_t* base = (uint8_t*)ws;
-        FewArgs a{type, (const uint16_t*)x, x_stride, nullptr, nullptr, p.splits, w.k / 32 / p.splits,
+        FewArgs a{type, two, (const uint16_t*)x, x_stride, nullptr, nullptr, p.splits, w.k / 32 / p.splits,
                   w.k / 32 % p.splits, 65536u / rows + 1, (float*)(base + p.part), counters};
         if (rows > kFusedRows) {
             u4* frag = (u4*)(base + p.frag);
@@ -675,8 +707,8 @@ hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_s
         return few[w.K - 2](w, a, ep, s);
     }
     const Source src{(const uint16_t*)x, x_stride, nullptr, 0, w.suh, type, rows, w.k};
-    return type == kBf16 ? many<kBf16>(w, 0, src, ep, nullptr, 0, ws, s)
-                         : many<kF16>(w, 0, src, ep, nullptr, 0, ws, s);
+    return type == kBf16 ? many<kBf16>(w, 0, src, ep, nullptr, 0, two, ws, s)
+                         : many<kF16>(w, 0, src, ep, nullptr, 0, two, ws, s);
 }
 
 hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long long dy_stride,
@@ -693,8 +725,8 @@ hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long lon
     ep.y_stride = dx_stride;
     ep.rows = rows;
     ep.cols = w.k;
-    return type == kBf16 ? many<kBf16>(w, 1, src, ep, dbias, dbias_f32, ws, s)
-                         : many<kF16>(w, 1, src, ep, dbias, dbias_f32, ws, s);
+    return type == kBf16 ? many<kBf16>(w, 1, src, ep, dbias, dbias_f32, false, ws, s)
+                         : many<kF16>(w, 1, src, ep, dbias, dbias_f32, false, ws, s);
 }
 
 namespace {
@@ -721,7 +753,7 @@ template <int T, bool BF>
 hipError_t gram(const GramPlan& p, Gemm g, hipStream_t s) {
     const Epilogue ep{};
     const dim3 grid(p.tiles, p.splits), block(256);
-    hipLaunchKernelGGL((gemm_kernel<T, kOutGram, BF, 4>), grid, block, 0, s, g, ep, ColSum{});
+    hipLaunchKernelGGL((gemm_kernel<T, kOutGram, BF, 4, 1>), grid, block, 0, s, g, ep, ColSum{});
     hipLaunchKernelGGL((join_kernel<T, true>), dim3((g.gb + 3) / 4, g.ga / 8), block, 0, s, g, ep);
     return hipGetLastError();
 }
@@ -737,7 +769,7 @@ hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, in
     uint16_t* xf = (uint16_t*)ws;
     if (p.steps) hipLaunchKernelGGL(transpose_kernel, dim3(p.steps, k / 128), dim3(256), 0, s, (const uint16_t*)x,
                                     x_stride, rows, p.steps, valid, xf);
-    const Gemm g{xf, xf, k / 16, k / 16, p.steps, p.tiles, p.splits, (float*)((uint8_t*)ws + p.part), prev, out, k};
+    const Gemm g{xf, xf, nullptr, k / 16, k / 16, p.steps, p.tiles, p.splits, (float*)((uint8_t*)ws + p.part), prev, out, k};
     return type == kBf16 ? gram<kBf16, true>(p, g, s) : gram<kF16, false>(p, g, s);
 }
 

@@ -39,6 +39,17 @@ struct Epilogue {
     int rows, cols;
 };
 
+// Whether a product's rows enter with 22 bits, as two fp16 terms: where a slope
+// will be taken at its results and an error of 2^-12 of a row's norm is not
+// below the gradient's own roundoff.  relu's slope jumps at zero: results that
+// near to it take the wrong side, e of them for an error e, and the gradient is
+// off by the root of that.  The other slopes move by about e, which bf16's 2^-9
+// hides and fp16's 2^-12 does not.
+inline bool two_terms(int type, int act, bool keeps_z) {
+    return keeps_z && (act == kActRelu || (type == kF16 && act != kActNone));
+}
+
+// backward: 0 forward, 1 gradient, 2 forward with two terms.
 size_t linear_ws_bytes(int rows, int k, int n, int backward);
 hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
                          const Epilogue& ep, void* ws, uint32_t* counters, hipStream_t s);
@@ -58,6 +69,7 @@ constexpr int kFusedRows = 16;
 constexpr int few_waves(int G) { return G == 1 ? 8 : 4; }
 struct FewArgs {
     int type;
+    int two;                            // two terms (up to kFusedRows rows)
     const uint16_t* x;
     long long x_stride;
     const u4* frag;

@@ -64,10 +64,11 @@ bool moe_sizes(int rows, int experts, int top, int d, int f) {
 
 extern "C" {
 
-int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int backward) {
+int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int what) {
+    if (what < XTQ_LINEAR_FORWARD || what > XTQ_LINEAR_TRAIN) return -15;
     if (!w || w->k <= 0 || w->n <= 0 || w->k % 128 || w->n % 128 || rows < 0 || rows > kMaxRows)
         return -6;
-    return rows ? (int64_t)xtq::linear_ws_bytes(rows, w->k, w->n, backward) : 0;
+    return rows ? (int64_t)xtq::linear_ws_bytes(rows, w->k, w->n, what) : 0;
 }
 
 int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_stride, int rows,
@@ -85,7 +86,8 @@ int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_strid
     if (res && (rc = check_rows(res, res_stride, wt.n))) return rc;
     if (!aligned(z, 2) || !aligned(bias, bias_f32 ? 4 : 2)) return 12;
     if (!counters || !aligned(counters, 4)) return 12;
-    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, 0)))) return rc;
+    const int what = xtq::two_terms(type, act, z != nullptr) ? XTQ_LINEAR_TRAIN : XTQ_LINEAR_FORWARD;
+    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, what)))) return rc;
     xtq::Epilogue ep{};
     ep.colscale = wt.svh;
     ep.scale = wt.scale;
@@ -117,7 +119,7 @@ int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy
     if (act != XTQ_ACT_NONE && (!z || !aligned(z, 2))) return 12;
     if (!aligned(dbias, bias_f32 ? 4 : 2)) return 12;
     if (!counters || !aligned(counters, 4)) return 12;
-    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, 1)))) return rc;
+    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, XTQ_LINEAR_GRADIENT)))) return rc;
     return status(xtq::launch_linear_bwd(wt, type, dy, dy_stride, z, act, rows, dx, dx_stride, dbias,
                                          bias_f32, ws, counters, (hipStream_t)stream), "linear_bwd");
 }

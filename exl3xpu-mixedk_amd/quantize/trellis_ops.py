@@ -130,7 +130,7 @@ def _forward(x, w, bias, act, residual, keep_z):
     L = _hb.lib()
     with torch.cuda.device(x.device):
         stream = _hb._stream(x.device)
-        need = L.xtq_linear_ws_bytes(w._p, m, 0)
+        need = L.xtq_linear_ws_bytes(w._p, m, 2 if keep_z else 0)
         ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
         rc = L.xtq_linear_dev(
             w._p, _TYPES[x.dtype], rows.data_ptr(), _stride(rows), m,

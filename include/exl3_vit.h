@@ -342,16 +342,21 @@ typedef struct xtq_weight {
 enum { XTQ_BF16 = 0, XTQ_F16 = 1 };
 enum { XTQ_ACT_NONE = 0, XTQ_ACT_RELU = 1, XTQ_ACT_SILU = 2, XTQ_ACT_GELU = 3 };
 enum { XTQ_OP_COUNTERS = 16384 };
+enum { XTQ_LINEAR_FORWARD = 0, XTQ_LINEAR_GRADIENT = 1, XTQ_LINEAR_TRAIN = 2 };
 
 /*
  * y = act(x W + bias) + res for x [rows][k], y [rows][n].
  *   bias   [n] fp32 (bias_f32 != 0) or of the activations' type, or NULL
  *   act    XTQ_ACT_*; gelu is the erf form
  *   res    [rows][n], or NULL; may be y itself
- *   z      [rows][n] contiguous (out): x W + bias, for xtq_linear_bwd_dev; or NULL
- * At most 1,048,560 rows.
+ *   z      [rows][n] contiguous (out): x W + bias, for xtq_linear_bwd_dev; or NULL.
+ *          With z, and act relu or (for XTQ_F16) silu or gelu, x enters the
+ *          product with 22 bits instead of 11, since slopes will be taken at z.
+ * At most 1,048,560 rows.  xtq_linear_ws_bytes: the scratch of xtq_linear_dev
+ * without z (XTQ_LINEAR_FORWARD) or with it (XTQ_LINEAR_TRAIN, never less), or of
+ * xtq_linear_bwd_dev (XTQ_LINEAR_GRADIENT).
  */
-XTQ_API int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int backward);
+XTQ_API int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int what);
 XTQ_API int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_stride,
                            int rows, const void* bias, int bias_f32, int act, const void* res,
                            int64_t res_stride, void* z, void* y, int64_t y_stride, void* ws,

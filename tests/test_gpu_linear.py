@@ -6,7 +6,8 @@ weight's incoherent columns carry that into a result's row as the same share of 
 128 columns), a result once to its type; sums are fp32 (2^-24 sqrt(k) and less).  A row's error is held to
 2 (u + 2 * 2^-11) of its norm, u the result's roundoff: the factor 2 is for activations, whose slopes go up to
 1.13 while they make the row smaller.  A saved pre-activation is rounded to the activations' type, which moves
-a gradient by less than u / 2 of its norm.  Gram sums are fp32 sums of exact products: 2^-24 times the steps'
+a gradient by less than u / 2 of its norm; where slopes are taken at it, it comes from activations of 22 bits
+(relu, and fp16), or its error is below bf16's roundoff.  Gram sums are fp32 sums of exact products: 2^-24 times the steps'
 chain of at most rows / 16 additions is their worst case, 1e-6 of the norm covers its square root."""
 import pytest
 import torch
@@ -102,13 +103,7 @@ def test_linear_gradient(xt, oracle_mod, act, dtype, bias_dtype, m):
     assert dx.dtype == dtype and db.dtype == bias_dtype and torch.equal(dr, dy)
     xd, bd, dyd = x.detach().cpu().double(), bias.detach().cpu().double(), dy.cpu().double()
     z = xd @ W + bd
-    # The slope is the one at the call's own z.  z's error is a share of its row's norm, and where a row's values
-    # are hundreds, that is not small beside the unit width over which silu, gelu and relu bend: the few values
-    # near zero have another slope at the exact z.  The call's z is itself held to the forward tolerance.
-    zc = xt.linear(x.detach(), xt.TrellisLinear(*w, K), bias=bias.detach())
-    assert float(R.row_errors(zc, z).max()) <= _tol(dtype)
-    zs = zc.cpu().double()
-    dz = dyd * R.slope(zs, act)
+    dz = dyd * R.slope(z, act)
     tol = _tol(dtype) + R.roundoff(dtype) / 2
     assert float(R.row_errors(dx, dz @ W.t()).max()) <= tol
     assert float(R.row_errors(db[None], dz.sum(0)[None]).max()) <= tol
@@ -126,6 +121,27 @@ def test_linear_gradient(xt, oracle_mod, act, dtype, bias_dtype, m):
     dif = (f(xd, bd + h * u) - f(xd, bd - h * u)) / (2 * h)
     got = float((db.cpu().double() * u).sum())
     assert abs(got - dif) <= tol * float(dz.sum(0).norm() * 4) + 1e-5
+
+
+@pytest.mark.parametrize("act,dtype", [("relu", torch.bfloat16), ("relu", torch.float16), ("silu", torch.float16),
+                                       ("gelu", torch.float16)])
+@pytest.mark.parametrize("m", (12, 40, 300))
+def test_linear_gradient_takes_exact_slopes(xt, oracle_mod, act, dtype, m):
+    """The slopes are those at the exact z: with an error e of z's norm, relu would take the wrong side of zero for
+    e / pi of all values and be off by sqrt(2 e / pi) (0.011 for activations of 11 bits).  Tolerance of the whole
+    dx: 3/4 of the result's roundoff and of 2^-11 (their root mean squares are below), and for e = 4e-7 (22 bits,
+    fp32 sums) 5e-4."""
+    k, n, K = 512, 512, 4
+    w = R.random_weight(k, n, K, 71)
+    W = R.dense(oracle_mod, *w, K, "exl3_mul1")
+    x = _x(m, k, dtype, m, spread=0.3).requires_grad_()
+    dy = _x(m, n, dtype, 7, spread=0.3)
+    y = xt.linear(x, xt.TrellisLinear(*w, K), act=act)
+    dx, = torch.autograd.grad(y, x, dy)
+    z = x.detach().cpu().double() @ W
+    want = (dy.cpu().double() * R.slope(z, act)) @ W.t()
+    tol = 0.75 * (R.roundoff(dtype) + 2.0 ** -11) + 5e-4
+    assert float(R.row_errors(dx.reshape(1, -1), want.reshape(1, -1)).max()) <= tol
 
 
 @pytest.mark.parametrize("m", (3, 70))
