@@ -293,6 +293,70 @@ __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
 
+// out = prev + sums of 32 rows by 128 columns of the Gram, at and below the
+// diagonal and mirrored.  They go through t, 32 lines in LDS that only this wave
+// uses, and come out as whole lines of memory: 512 bytes of a row, 128 of a
+// mirrored one.
+constexpr int kGramLine = 132;
+
+__device__ __forceinline__ void finish_gram(const f4 (&v)[2][8], float* t, const Gemm& g, int grp, int blk,
+                                            int lane) {
+    const int row0 = grp * 16, col0 = blk * 128, r = lane & 15, q = lane >> 4;
+    const size_t dim = g.dim;
+    const bool below = col0 + 127 < row0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *(f4*)(t + (16 * h + r) * kGramLine + 16 * j + 4 * q) = v[h][j];
+    wave_sync();
+    auto put = [&](const f4* s, const size_t* at, auto keep) {
+        f4 p[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            p[n] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+            if (g.prev && below) p[n] = *(const f4_a4*)(g.prev + at[n]);
+            else if (g.prev)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (keep(n, i)) p[n][i] = g.prev[at[n] + i];
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            if (below) *(f4_a4*)(g.out + at[n]) = p[n] + s[n];
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (keep(n, i)) g.out[at[n] + i] = p[n][i] + s[n][i];
+        }
+    };
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        f4 s[8];
+        size_t at[8];
+        const int row = 16 * half + (lane >> 5), col = 4 * (lane & 31);     // row + 2 n
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            s[n] = *(const f4*)(t + (row + 2 * n) * kGramLine + col);
+            at[n] = (size_t)(row0 + row + 2 * n) * dim + col0 + col;
+        }
+        put(s, at, [&](int n, int i) { return col0 + col + i <= row0 + row + 2 * n; });
+    }
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        f4 s[8];
+        size_t at[8];
+        const int row = 4 * (lane & 7), col = 64 * half + (lane >> 3);      // col + 8 n
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = t[(row + i) * kGramLine + col + 8 * n];
+            at[n] = (size_t)(col0 + col + 8 * n) * dim + row0 + row;
+        }
+        put(s, at, [&](int n, int i) { return col0 + col + 8 * n < row0 + row + i; });
+    }
+    wave_sync();
+}
+
 template <int T, int OUT, bool BF, int NB, int TERMS>
 __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSum sums) {
     // of a step: the workgroup's fragments, a wave's to move
@@ -393,6 +457,23 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSu
     }
     const int blk = tn * 2 + wn;
     if (blk * 8 >= g.ga) return;
+    if constexpr (OUT == kOutGram) {
+        if (g.splits == 1) {
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                const int grp = gb0 + wm * NB + b;
+                if (grp >= g.gb || blk * 128 > grp * 16 + 31) continue;     // (above the diagonal)
+                f4 v[2][8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[0][j] = acc[j][b];
+                    v[1][j] = acc[j][b + 1];
+                }
+                finish_gram(v, (float*)lds + wv * 32 * kGramLine, g, grp, blk, lane);
+            }
+            return;
+        }
+    }
     Columns<4> cols[8];
     if constexpr (OUT == kOutEpilogue) unit_columns<T>(cols, ep, blk, lane);
 #pragma unroll
@@ -413,74 +494,50 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSu
     }
 }
 
-// out = prev + sums, at and below the diagonal and mirrored, for a unit.
-__device__ __forceinline__ void finish_gram(const f4* v, const Gemm& g, int grp, int blk, int lane) {
-    const int r = lane & 15, q = lane >> 4;
-    const size_t row = (size_t)grp * 16 + r, col = (size_t)blk * 128 + 4 * q, dim = g.dim;
-    if (blk * 128 + 127 < grp * 16) {   // below the diagonal
-        // mirrored: lane 4 a + b of a row has rows 4 a .. + 3 of column b
-        const size_t mrow = col + (r & 3), mcol = (size_t)grp * 16 + (r & ~3);
-        f4 p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            p[j] = g.prev ? *(const f4_a4*)(g.prev + row * dim + col + 16 * j) : (f4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) *(f4_a4*)(g.out + row * dim + col + 16 * j) = p[j] + v[j];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            p[j] = g.prev ? *(const f4_a4*)(g.prev + (mrow + 16 * j) * dim + mcol) : (f4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            *(f4_a4*)(g.out + (mrow + 16 * j) * dim + mcol) = p[j] + transpose4(v[j], lane);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const size_t c = col + 16 * j + i;
-            if (c > row) continue;
-            g.out[row * dim + c] = (g.prev ? g.prev[row * dim + c] : 0.0f) + v[j][i];
-            if (c < row) g.out[c * dim + row] = (g.prev ? g.prev[c * dim + row] : 0.0f) + v[j][i];
-        }
-    }
-}
-
-// Sums the splits' partial products of a unit (128 columns by 16 rows), in
-// order, four loads in flight for each of its registers, and finishes it.  (The
-// Gram's sums come this way without splits too: its reads, writes and mirrored
-// writes at the end of the product's own waves took 100 us of 300 for 5120
-// channels.)
-template <int T, bool GRAM>
-__global__ __launch_bounds__(256) void join_kernel(Gemm g, Epilogue ep) {
-    const int lane = threadIdx.x & 63, grp = blockIdx.x * 4 + (threadIdx.x >> 6), blk = blockIdx.y;
-    if (grp >= g.gb) return;
-    if (GRAM && blk * 128 > grp * 16 + 15) return;      // above the diagonal
-    f4 v[8];
+// The sum over the splits of a unit (128 columns by 16 rows), in order, U of
+// them in flight for each register.
+template <int U>
+__device__ __forceinline__ void sum_splits(f4 (&v)[8], const Gemm& g, int grp, int blk, int lane) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
     const f4* p = (const f4*)g.part + ((size_t)blk * g.gb + grp) * 512 + lane;
     const size_t stride = (size_t)(g.ga / 8) * g.gb * 512;
-    for (int s = 0; s < g.splits; s += 4) {
-        f4 t[4][8];
+    for (int s = 0; s < g.splits; s += U) {
+        f4 t[U][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < U; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[i][j] = p[(s + i < g.splits ? s + i : s) * stride + j * 64];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < U; ++i)
             if (s + i < g.splits) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += t[i][j];
             }
     }
-    if constexpr (GRAM) {
-        finish_gram(v, g, grp, blk, lane);
-    } else {
-        Columns<4> cols[8];
-        unit_columns<T>(cols, ep, blk, lane);
-        finish_unit<T>(v, cols, ep, grp, blk, lane);
-    }
+}
+
+// Joins the splits' partial products and finishes them, a wave one unit.
+template <int T>
+__global__ __launch_bounds__(256) void join_kernel(Gemm g, Epilogue ep) {
+    const int lane = threadIdx.x & 63, grp = blockIdx.x * 4 + (threadIdx.x >> 6), blk = blockIdx.y;
+    if (grp >= g.gb) return;
+    f4 v[8];
+    sum_splits<4>(v, g, grp, blk, lane);
+    Columns<4> cols[8];
+    unit_columns<T>(cols, ep, blk, lane);
+    finish_unit<T>(v, cols, ep, grp, blk, lane);
+}
+
+// The same for the Gram, a wave two units.
+__global__ __launch_bounds__(256) void join_gram_kernel(Gemm g) {
+    __shared__ __align__(16) float t[4][32 * kGramLine];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, grp = (blockIdx.x * 4 + wv) * 2, blk = blockIdx.y;
+    if (grp >= g.gb || blk * 128 > grp * 16 + 31) return;       // (above the diagonal)
+    f4 v[2][8];
+    sum_splits<2>(v[0], g, grp, blk, lane);
+    sum_splits<2>(v[1], g, grp + 1, blk, lane);
+    finish_gram(v, t[wv], g, grp, blk, lane);
 }
 
 // ---------------------------------------------------------------------- Gram
@@ -508,6 +565,107 @@ __global__ __launch_bounds__(256) void transpose_kernel(const uint16_t* __restri
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = t[8 * q + 2 * i][c] | (uint32_t)t[8 * q + 2 * i + 1][c] << 16;
         *(u4*)(frags + frag_at(c0 / 16 + wv * 2 + g, p, steps) + lane * 8) = o;
+    }
+}
+
+// The Gram of few rows in one launch.  A workgroup makes 64 by 64 of it (at or
+// below the diagonal) from x as it lies: lane 16 q + r loads four channels,
+// 4 r .. + 3, of the eight rows 8 q .. 8 q + 7 of a 32-row step, and what it then
+// holds of channel 4 r + j is its part of an MFMA operand whose index r stands
+// for that channel: the transpose is 16 byte permutes between a lane's own
+// registers.  Its eight waves take a step each in turn and meet in LDS, in an
+// order that the number of rows fixes.
+constexpr int kGramTile = 64, kGramWaves = 8;
+
+template <bool BF>
+__global__ __launch_bounds__(64 * kGramWaves, 2) void gram_few_kernel(const uint16_t* __restrict__ x, long long stride,
+                                                                      int rows, int dim,
+                                                                      const uint8_t* __restrict__ valid,
+                                                                      const float* prev, float* out) {
+    __shared__ __align__(16) f4 lds[kGramWaves / 2][16][64];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int tm = 0, tn = xcd_order(blockIdx.x, gridDim.x);
+    // rows of tiles of 1, 2, 3 .. tiles
+    tm = (int)((sqrtf(8.0f * tn + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > tn) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= tn) ++tm;
+    tn -= tm * (tm + 1) / 2;
+    const uint16_t *xa = x + tn * kGramTile + 4 * r, *xb = x + tm * kGramTile + 4 * r;
+    const int steps = (int)(((long long)rows + 31) / 32);
+    u2 a[8], b[8];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int row = s * 32 + 8 * q + e;
+            a[e] = b[e] = (u2){0u, 0u};
+            if (row < rows && (!valid || valid[row])) {
+                a[e] = *(const u2_a2*)(xa + row * (size_t)stride);
+                b[e] = *(const u2_a2*)(xb + row * (size_t)stride);
+            }
+        }
+    };
+    f4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i >> 2][i & 3] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = wv; s < steps; s += kGramWaves) {
+        load(s);
+        u4 fa[4], fb[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+                fa[j][i] = __builtin_amdgcn_perm(a[2 * i + 1][j >> 1], a[2 * i][j >> 1], sel);
+                fb[j][i] = __builtin_amdgcn_perm(b[2 * i + 1][j >> 1], b[2 * i][j >> 1], sel);
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = mfma<BF>(fa[j], fb[i], acc[j][i]);
+    }
+    // waves 4 .. 7 to 0 .. 3, these to all
+    if (wv >= kGramWaves / 2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lds[wv - kGramWaves / 2][i][lane] = acc[i >> 2][i & 3];
+    __syncthreads();
+    if (wv < kGramWaves / 2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lds[wv][i][lane] = acc[i >> 2][i & 3] + lds[wv][i][lane];
+    __syncthreads();
+    f4 sum[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        sum[i] = lds[0][2 * wv + i][lane];
+#pragma unroll
+        for (int w = 1; w < kGramWaves / 2; ++w) sum[i] += lds[w][2 * wv + i][lane];
+    }
+    __syncthreads();
+    // operand indices 4 q + i and r of products (j, i2) are channels
+    // 16 q + 4 i + j and 4 r + i2
+    constexpr int kRow = kGramTile + 4;
+    float* const t = (float*)lds;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = 2 * wv + n, col = 16 * q + 4 * i + (at >> 2), row = 4 * r + (at & 3);
+            if (tm != tn || col <= row) t[row * kRow + col] = sum[n][i];
+            if (tm == tn && col < row) t[col * kRow + row] = sum[n][i];
+        }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int line = 8 * wv + 4 * n + q;
+        const size_t at = (size_t)(tm * kGramTile + line) * dim + tn * kGramTile + 4 * r;
+        const f4 v = *(const f4*)(t + line * kRow + 4 * r);
+        *(f4_a4*)(out + at) = prev ? *(const f4_a4*)(prev + at) + v : v;
+        if (tm == tn) continue;
+        const size_t to = (size_t)(tn * kGramTile + line) * dim + tm * kGramTile + 4 * r;
+        f4 m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = t[(4 * r + i) * kRow + line];
+        *(f4_a4*)(out + to) = prev ? *(const f4_a4*)(prev + to) + m : m;
     }
 }
 
@@ -617,7 +775,7 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
         if (two) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 2>), grid, block, 0, s, g, ep, sums);
         else if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 4, 1>), grid, block, 0, s, g, ep, sums);
         else hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 1>), grid, block, 0, s, g, ep, sums);
-        hipLaunchKernelGGL((join_kernel<T, false>), dim3((p.groups + 3) / 4, n / 128), block, 0, s, g, ep);
+        hipLaunchKernelGGL((join_kernel<T>), dim3((p.groups + 3) / 4, n / 128), block, 0, s, g, ep);
     }
     return hipGetLastError();
 }
@@ -736,8 +894,18 @@ struct GramPlan {
     size_t xf, part, total;
 };
 
+// Whether the Gram comes in one launch, from x itself.  Its time grows with every
+// tile's 256 bytes a row, the transpose's and the product's with a large constant
+// (us, both with prev, one launch against several: 1024 channels 10 : 41 at 1021
+// rows, 46 : 67 at 8192; 2048 57 : 65 at 4096, 103 : 85 at 8192; 5120 51 : 76 at
+// 256, 92 : 91 at 1021, 152 : 112 at 2048; 17408 594 : 541 at one row).
+bool takes_gram_few(int rows, int k) {
+    return rows <= 8192 && k <= 8192 && (long long)rows * k * k <= 24LL << 30;
+}
+
 GramPlan gram_plan(int rows, int k) {
-    GramPlan p;
+    GramPlan p{};
+    if (takes_gram_few(rows, k)) return p;
     p.steps = (int)(((long long)rows + 31) / 32);
     const int nt = (k + kTileN - 1) / kTileN, mt = (k + 127) / 128;
     p.tiles = 0;
@@ -745,7 +913,7 @@ GramPlan gram_plan(int rows, int k) {
     p.splits = gemm_splits(p.tiles, p.steps);
     p.xf = 0;
     p.part = align256(frag_bytes(k / 16, p.steps));
-    p.total = p.part + (size_t)p.splits * k * k * 4;
+    p.total = p.part + (p.splits > 1 ? (size_t)p.splits * k * k * 4 : 0);
     return p;
 }
 
@@ -754,7 +922,7 @@ hipError_t gram(const GramPlan& p, Gemm g, hipStream_t s) {
     const Epilogue ep{};
     const dim3 grid(p.tiles, p.splits), block(256);
     hipLaunchKernelGGL((gemm_kernel<T, kOutGram, BF, 4, 1>), grid, block, 0, s, g, ep, ColSum{});
-    hipLaunchKernelGGL((join_kernel<T, true>), dim3((g.gb + 3) / 4, g.ga / 8), block, 0, s, g, ep);
+    if (p.splits > 1) hipLaunchKernelGGL(join_gram_kernel, dim3((g.gb + 7) / 8, g.ga / 8), block, 0, s, g);
     return hipGetLastError();
 }
 
@@ -765,6 +933,15 @@ size_t gram_ws_bytes(int rows, int k) { return gram_plan(rows, k).total; }
 hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, int k,
                        const uint8_t* valid, const float* prev, float* out, void* ws,
                        hipStream_t s) {
+    if (takes_gram_few(rows, k)) {
+        const int nt = k / kGramTile;
+        const dim3 grid(nt * (nt + 1) / 2), block(64 * kGramWaves);
+        if (type == kBf16) hipLaunchKernelGGL(gram_few_kernel<true>, grid, block, 0, s, (const uint16_t*)x, x_stride,
+                                              rows, k, valid, prev, out);
+        else hipLaunchKernelGGL(gram_few_kernel<false>, grid, block, 0, s, (const uint16_t*)x, x_stride, rows, k,
+                                valid, prev, out);
+        return hipGetLastError();
+    }
     const GramPlan p = gram_plan(rows, k);
     uint16_t* xf = (uint16_t*)ws;
     if (p.steps) hipLaunchKernelGGL(transpose_kernel, dim3(p.steps, k / 128), dim3(256), 0, s, (const uint16_t*)x,

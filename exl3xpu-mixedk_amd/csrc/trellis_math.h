@@ -137,20 +137,6 @@ __device__ __forceinline__ float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, 0xf, 0xf, true));
 }
 
-// 4 by 4 transpose among each four neighbouring lanes: afterwards element i of
-// lane 4 a + b is what element b of lane 4 a + i was.
-__device__ __forceinline__ f4 transpose4(f4 v, int lane) {
-    auto move = [](float x, auto c) { return dpp<decltype(c)::value>(x); };
-    using X1 = std::integral_constant<int, 0xB1>;       // lanes 1 0 3 2
-    using X2 = std::integral_constant<int, 0x4E>;       // lanes 2 3 0 1
-    const bool o1 = lane & 1, o2 = lane & 2;
-    // pairs: lane bit 0 with element bit 0, then lane bit 1 with element bit 1
-    const float a = move(o1 ? v[0] : v[1], X1()), b = move(o1 ? v[2] : v[3], X1());
-    v = o1 ? (f4){a, v[1], b, v[3]} : (f4){v[0], a, v[2], b};
-    const float c = move(o2 ? v[0] : v[2], X2()), d = move(o2 ? v[1] : v[3], X2());
-    return o2 ? (f4){c, d, v[2], v[3]} : (f4){v[0], v[1], c, d};
-}
-
 // Largest value of the lanes that differ in bits 4 and 5.
 __device__ __forceinline__ float rows_max(float v) {
     const uint32_t a = __float_as_uint(v);

@@ -20,6 +20,7 @@ cite for these functions.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import sys
@@ -33,6 +34,18 @@ ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _COUNTERS = 16384
 _counters: dict = {}
+_HERE = contextlib.nullcontext()
+
+
+def _stream(dev: torch.device) -> int:
+    """The current stream of dev.  The raw handle comes without a Stream object
+    around it: 0.1 us instead of 2, of the 10 that a call of one token takes."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _on(dev: torch.device):
+    """dev as the current device, where it is not that already."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _counter_words(dev: torch.device, stream: int) -> torch.Tensor:
@@ -128,8 +141,8 @@ def _forward(x, w, bias, act, residual, keep_z):
     res = None if residual is None else _rows(residual, w.n)
     bias = None if bias is None else bias.contiguous()
     L = _hb.lib()
-    with torch.cuda.device(x.device):
-        stream = _hb._stream(x.device)
+    with _on(x.device):
+        stream = _stream(x.device)
         need = L.xtq_linear_ws_bytes(w._p, m, 2 if keep_z else 0)
         ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
         rc = L.xtq_linear_dev(
@@ -170,8 +183,8 @@ class _Linear(torch.autograd.Function):
             if m == 0:
                 return dx, None if dbias is None else dbias.zero_(), dy if want_r else None, None, None
             L = _hb.lib()
-            with torch.cuda.device(dy.device):
-                stream = _hb._stream(dy.device)
+            with _on(dy.device):
+                stream = _stream(dy.device)
                 need = L.xtq_linear_ws_bytes(w._p, m, 1)
                 ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dy.device)
                 rc = L.xtq_linear_bwd_dev(
@@ -272,8 +285,8 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     ids = torch.empty(*x.shape[:-1], top_k, dtype=torch.int32, device=x.device)
     weights = torch.empty(*x.shape[:-1], top_k, dtype=torch.float32, device=x.device)
     L = _hb.lib()
-    with torch.cuda.device(x.device):
-        stream = _hb._stream(x.device)
+    with _on(x.device):
+        stream = _stream(x.device)
         for r in range(0, m, _MOE_ROWS):
             n = min(_MOE_ROWS, m - r)
             need = L.xtq_moe_ws_bytes(n, experts.n, top_k, d, experts.f)
@@ -319,13 +332,13 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
     if out is None:
         out = torch.empty(k, k, dtype=torch.float32, device=x.device)
     L = _hb.lib()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         need = L.xtq_gram_ws_bytes(m, k)
         ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
         rc = L.xtq_gram_dev(_TYPES[x.dtype], rows.data_ptr() if m else None,
                             _stride(rows) if m else k, m, k,
                             None if valid is None else valid.data_ptr(),
                             None if prev is None else prev.data_ptr(), out.data_ptr(),
-                            ws.data_ptr() if need else None, ws.numel(), _hb._stream(x.device))
+                            ws.data_ptr() if need else None, ws.numel(), _stream(x.device))
     _hb._check("xtq_gram_dev", rc)
     return out
