@@ -573,16 +573,22 @@ __global__ __launch_bounds__(256) void transpose_kernel(const uint16_t* __restri
 // 4 r .. + 3, of the eight rows 8 q .. 8 q + 7 of a 32-row step, and what it then
 // holds of channel 4 r + j is its part of an MFMA operand whose index r stands
 // for that channel: the transpose is 16 byte permutes between a lane's own
-// registers.  Its eight waves take a step each in turn and meet in LDS, in an
-// order that the number of rows fixes.
-constexpr int kGramTile = 64, kGramWaves = 8;
+// registers.  Its W waves take a step each in turn and meet in LDS, in an order
+// that the number of rows fixes.  Eight waves, 64 KiB of LDS and 125 registers
+// let two workgroups share a compute unit: one loads while the other multiplies
+// (with a wave's next step fetched ahead, 160 registers and one workgroup, 5120
+// channels took 129 us at 1021 rows and not 92, and 65 at one row, not the 40
+// that its 210 MB take to copy).  Where there is a compute unit for every tile,
+// sixteen waves halve the loads that wait for each other (1024 channels by 1021
+// rows that no cache holds: under 10.5 us, of eight waves 18).
+constexpr int kGramTile = 64;
 
-template <bool BF>
-__global__ __launch_bounds__(64 * kGramWaves, 2) void gram_few_kernel(const uint16_t* __restrict__ x, long long stride,
-                                                                      int rows, int dim,
-                                                                      const uint8_t* __restrict__ valid,
-                                                                      const float* prev, float* out) {
-    __shared__ __align__(16) f4 lds[kGramWaves / 2][16][64];
+template <bool BF, int W>
+__global__ __launch_bounds__(64 * W, 4) void gram_few_kernel(const uint16_t* __restrict__ x, long long stride,
+                                                              int rows, int dim,
+                                                              const uint8_t* __restrict__ valid,
+                                                              const float* prev, float* out) {
+    __shared__ __align__(16) f4 lds[W / 2][16][64];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tm = 0, tn = xcd_order(blockIdx.x, gridDim.x);
@@ -595,20 +601,32 @@ __global__ __launch_bounds__(64 * kGramWaves, 2) void gram_few_kernel(const uint
     const int steps = (int)(((long long)rows + 31) / 32);
     u2 a[8], b[8];
     auto load = [&](int s) {
+        u2 mask = {~0u, ~0u};           // a byte for each of the lane's rows
+        if (valid) {
+            const int row = s * 32 + 8 * q;
+            if (row + 8 <= rows) mask = *(const u2_a1*)(valid + row);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (row + e >= rows || !valid[row + e]) mask[e >> 2] &= ~(0xFFu << (8 * (e & 3)));
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int row = s * 32 + 8 * q + e;
-            a[e] = b[e] = (u2){0u, 0u};
-            if (row < rows && (!valid || valid[row])) {
-                a[e] = *(const u2_a2*)(xa + row * (size_t)stride);
-                b[e] = *(const u2_a2*)(xb + row * (size_t)stride);
+            const int row = s * 32 + 8 * q + e, at = row < rows ? row : rows - 1;
+            const bool keep = row < rows && (mask[e >> 2] >> (8 * (e & 3)) & 0xFFu);
+            a[e] = *(const u2_a2*)(xa + at * (size_t)stride);
+            b[e] = *(const u2_a2*)(xb + at * (size_t)stride);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[e][i] = keep ? a[e][i] : 0u;
+                b[e][i] = keep ? b[e][i] : 0u;
             }
         }
     };
     f4 acc[4][4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i >> 2][i & 3] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = wv; s < steps; s += kGramWaves) {
+    for (int s = wv; s < steps; s += W) {
         load(s);
         u4 fa[4], fb[4];
 #pragma unroll
@@ -624,21 +642,22 @@ __global__ __launch_bounds__(64 * kGramWaves, 2) void gram_few_kernel(const uint
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[j][i] = mfma<BF>(fa[j], fb[i], acc[j][i]);
     }
-    // waves 4 .. 7 to 0 .. 3, these to all
-    if (wv >= kGramWaves / 2)
+    // the upper waves to the lower, these to all
+    if (wv >= W / 2)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) lds[wv - kGramWaves / 2][i][lane] = acc[i >> 2][i & 3];
+        for (int i = 0; i < 16; ++i) lds[wv - W / 2][i][lane] = acc[i >> 2][i & 3];
     __syncthreads();
-    if (wv < kGramWaves / 2)
+    if (wv < W / 2)
 #pragma unroll
         for (int i = 0; i < 16; ++i) lds[wv][i][lane] = acc[i >> 2][i & 3] + lds[wv][i][lane];
     __syncthreads();
-    f4 sum[2];
+    constexpr int N = 16 / W;
+    f4 sum[N];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        sum[i] = lds[0][2 * wv + i][lane];
+    for (int i = 0; i < N; ++i) {
+        sum[i] = lds[0][N * wv + i][lane];
 #pragma unroll
-        for (int w = 1; w < kGramWaves / 2; ++w) sum[i] += lds[w][2 * wv + i][lane];
+        for (int w = 1; w < W / 2; ++w) sum[i] += lds[w][N * wv + i][lane];
     }
     __syncthreads();
     // operand indices 4 q + i and r of products (j, i2) are channels
@@ -646,17 +665,17 @@ __global__ __launch_bounds__(64 * kGramWaves, 2) void gram_few_kernel(const uint
     constexpr int kRow = kGramTile + 4;
     float* const t = (float*)lds;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int at = 2 * wv + n, col = 16 * q + 4 * i + (at >> 2), row = 4 * r + (at & 3);
+            const int at = N * wv + n, col = 16 * q + 4 * i + (at >> 2), row = 4 * r + (at & 3);
             if (tm != tn || col <= row) t[row * kRow + col] = sum[n][i];
             if (tm == tn && col < row) t[col * kRow + row] = sum[n][i];
         }
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int line = 8 * wv + 4 * n + q;
+    for (int n = 0; n < N; ++n) {
+        const int line = 4 * (N * wv + n) + q;
         const size_t at = (size_t)(tm * kGramTile + line) * dim + tn * kGramTile + 4 * r;
         const f4 v = *(const f4*)(t + line * kRow + 4 * r);
         *(f4_a4*)(out + at) = prev ? *(const f4_a4*)(prev + at) + v : v;
@@ -935,11 +954,13 @@ hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, in
                        hipStream_t s) {
     if (takes_gram_few(rows, k)) {
         const int nt = k / kGramTile;
-        const dim3 grid(nt * (nt + 1) / 2), block(64 * kGramWaves);
-        if (type == kBf16) hipLaunchKernelGGL(gram_few_kernel<true>, grid, block, 0, s, (const uint16_t*)x, x_stride,
-                                              rows, k, valid, prev, out);
-        else hipLaunchKernelGGL(gram_few_kernel<false>, grid, block, 0, s, (const uint16_t*)x, x_stride, rows, k,
-                                valid, prev, out);
+        const int tiles = nt * (nt + 1) / 2, waves = tiles > kCUs ? 8 : 16;
+        auto launch = [&](auto* kernel) {
+            hipLaunchKernelGGL(kernel, dim3(tiles), dim3(64 * waves), 0, s, (const uint16_t*)x, x_stride, rows, k,
+                               valid, prev, out);
+        };
+        if (type == kBf16) launch(waves == 8 ? gram_few_kernel<true, 8> : gram_few_kernel<true, 16>);
+        else launch(waves == 8 ? gram_few_kernel<false, 8> : gram_few_kernel<false, 16>);
         return hipGetLastError();
     }
     const GramPlan p = gram_plan(rows, k);

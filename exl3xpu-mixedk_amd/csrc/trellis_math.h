@@ -21,6 +21,7 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 // accesses of any width at any address.
 typedef u4 u4_a2 __attribute__((aligned(2)));
 typedef u2 u2_a2 __attribute__((aligned(2)));
+typedef u2 u2_a1 __attribute__((aligned(1)));
 typedef uint32_t u1_a2 __attribute__((aligned(2)));
 typedef f4 f4_a4 __attribute__((aligned(4)));
 

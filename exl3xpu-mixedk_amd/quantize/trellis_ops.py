@@ -318,7 +318,8 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
     if x.dim() < 1 or not x.shape[-1] or x.shape[-1] % 128:
         raise ValueError(f"x must be [.., k] with k a multiple of 128, got {tuple(x.shape)}")
     k = x.shape[-1]
-    x = x.detach()
+    if x.requires_grad:
+        x = x.detach()
     if valid is not None:
         _like(valid, x, x.shape[:-1], "valid", (torch.bool,))
         valid = valid.contiguous()
