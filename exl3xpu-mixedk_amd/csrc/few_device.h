@@ -52,12 +52,19 @@ struct PairRegs {
     u4 r[(K + 1) / 2];
 };
 
+// Lane's i-th 16-byte piece of a pair (odd K: the upper lanes' last is their first
+// once more).
+template <int K>
+__device__ __forceinline__ int pair_piece(int i, int lane) {
+    const int c = 64 * i + lane;
+    return !(K & 1) || c < 32 * K ? c : lane;
+}
+
 template <int K>
 __device__ __forceinline__ void load_pair(PairRegs<K>& t, const uint8_t* tiles, size_t row_bytes, int lane) {
 #pragma unroll
     for (int i = 0; i < (K + 1) / 2; ++i) {
-        int c = 64 * i + lane;                          // 16-byte piece of the pair
-        if (K & 1) c = c < 32 * K ? c : lane;
+        const int c = pair_piece<K>(i, lane);
         const bool low = c >= 16 * K;
         t.r[i] = *(const u4_a2*)(tiles + (low ? row_bytes : 0) + 16 * (low ? c - 16 * K : c));
     }
@@ -66,8 +73,7 @@ __device__ __forceinline__ void load_pair(PairRegs<K>& t, const uint8_t* tiles, 
 template <int K>
 __device__ __forceinline__ void pair_to_lds(const PairRegs<K>& t, uint8_t* buf, int lane) {
 #pragma unroll
-    for (int i = 0; i < (K + 1) / 2; ++i)
-        if (!(K & 1) || i < K / 2 || lane < 32) *(u4*)(buf + 16 * (64 * i + lane)) = t.r[i];
+    for (int i = 0; i < (K + 1) / 2; ++i) *(u4*)(buf + 16 * pair_piece<K>(i, lane)) = t.r[i];
 }
 
 // Orders a wave's own LDS accesses across its lanes (they execute in order; the
@@ -341,38 +347,30 @@ __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4*
             load(r[1], p0 + 1);
         }
         u4 x[G], lo[G], nx[G], nlo[G];
+        int own[G];
         float f[G];
-        const u4 zero = {0u, 0u, 0u, 0u};
-        // rows past the end have no fragments: zeros
+        // A pair's fragments and its block's shifts.  (What lies in the places of
+        // rows past the end reaches only such rows' sums, which nobody reads.)  From
+        // memory they come a step ahead, and before the trellis words of a later
+        // step: loads arrive in order, so a wait for these behind those would be one
+        // for both; and all of them unconditionally, so that the waits can count.
         auto fetch = [&](u4 (&t)[G], u4 (&u)[G], int p) {
             if constexpr (FUSED) {
-                const bool in = (lane & 15) < a.rows;
-                t[0] = in ? frag[(p - 4 * kb0) * 64 + lane] : zero;
-                if constexpr (LO) u[0] = in ? frag_lo[(p - 4 * kb0) * 64 + lane] : zero;
+                t[0] = frag[(p - 4 * kb0) * 64 + lane];
+                if constexpr (LO) u[0] = frag_lo[(p - 4 * kb0) * 64 + lane];
+                own[0] = shifts[((p >> 2) - kb0) * 16 + (lane & 15)];
             } else {
                 p = p < p1 ? p : p1 - 1;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const bool in = 16 * g + (lane & 15) < a.rows;
-                    t[g] = in ? a.hi[((size_t)g * a.pairs + p) * 64 + lane] : zero;
-                    if constexpr (LO) u[g] = in ? a.lo[((size_t)g * a.pairs + p) * 64 + lane] : zero;
+                    t[g] = a.hi[((size_t)g * a.pairs + p) * 64 + lane];
+                    if constexpr (LO) u[g] = a.lo[((size_t)g * a.pairs + p) * 64 + lane];
+                    own[g] = a.shift[((size_t)g * (a.pairs >> 2) + (p >> 2)) * 16 + (lane & 15)];
                 }
             }
         };
         // pair p lies in its buffer, p + 1 is on its way in r[odd ^ 1], p + 2 in r[odd]
         auto step = [&](int p, int odd) {
-            pair_to_lds<K>(r[odd ^ 1], buf + (odd ^ 1) * kPairBytes<K>, lane);
-            load(r[odd ^ 1], p + 3);
-            if (p == p0 || (p & 3) == 0) {
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    int own = kNoShift;
-                    if (16 * g + (lane & 15) < a.rows)
-                        own = FUSED ? shifts[((p >> 2) - kb0) * 16 + (lane & 15)]
-                                    : a.shift[((size_t)g * (a.pairs >> 2) + (p >> 2)) * 16 + (lane & 15)];
-                    meet(acc[g], shift[g], own, f[g]);
-                }
-            }
             if constexpr (FUSED) {
                 fetch(x, lo, p);
             } else {
@@ -381,8 +379,15 @@ __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4*
                     x[g] = nx[g];
                     if constexpr (LO) lo[g] = nlo[g];
                 }
-                fetch(nx, nlo, p + 1);
             }
+            if (p == p0 || (p & 3) == 0) {
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+                    meet(acc[g], shift[g], 16 * g + (lane & 15) < a.rows ? own[g] : kNoShift, f[g]);
+            }
+            pair_to_lds<K>(r[odd ^ 1], buf + (odd ^ 1) * kPairBytes<K>, lane);
+            if constexpr (!FUSED) fetch(nx, nlo, p + 1);
+            load(r[odd ^ 1], p + 3);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 x[g] = scaled(x[g], f[g]);
