@@ -16,6 +16,15 @@ namespace {
 // at a time, into LDS.  The waves' sums meet in LDS, the workgroups' in scratch,
 // where the last one to arrive adds them in order and finishes the columns.
 // LO: with two terms.
+//
+// The decoding bounds it: 3.85 vector instructions a weight that issue at 33-37 T
+// lane-operations/s (mul1, K = 4) make 9.4 us of the 89 M weights of 17408 by
+// 5120, whose 44.6 MB a copy would move in 9.0; the loop takes that time, and
+// one row 23.5 us in all (48 rows at K = 3: 39.4).  The rest stands before and
+// after it, in cycles of 51,000: 8,200 until the rows are transformed and the
+// first weights there, 5,400 for the slowest wave and the waves' sums, 2,300 to
+// arrive, 4,200 to read the other workgroups' parts and finish.  Small weights
+// are all of that: 5120 by 5120 takes 12.6 us, 5120 by 1024 at K = 7 12.3.
 template <int K, int CODE, int G, bool FUSED, bool LO>
 __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(Weight w, FewArgs a, Epilogue ep) {
     constexpr int W = few_waves(G), N = 8 / W;
