@@ -81,6 +81,10 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(
     }
 }
 
+// Rows that come transformed fill two groups' fragments or four, as many as their
+// kernels read.
+static_assert(kFusedRows >= 16 && kFewRows <= 64, "groups of rows");
+
 template <int K, int CODE>
 hipError_t few_kc(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s) {
     const dim3 grid(w.n / 128, a.splits);
