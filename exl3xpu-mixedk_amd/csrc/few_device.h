@@ -257,10 +257,9 @@ struct FewSource {
     const uint8_t* tiles;
     size_t row_bytes;
     int rows, pairs;                    // pairs: 32-row steps of the weight
-    // FUSED: the rows, transformed here; row i is row list[i] of x (list NULL: i)
+    // FUSED: the rows, transformed here
     const uint16_t* x;
     long long x_stride;
-    const int32_t* list;
     const uint16_t* suh;
     int type;
     uint32_t rinv;                      // item / rows is item * rinv >> 16
@@ -320,8 +319,7 @@ __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4*
                     const int item = t + i * W;
                     if (item >= items) break;
                     const int kbi = item * a.rinv >> 16, row = item - kbi * a.rows;
-                    const size_t at = a.list ? a.list[row] : row;
-                    xw[i] = load_two(a.x + at * a.x_stride + 128 * (kb0 + kbi), lane);
+                    xw[i] = load_two(a.x + (size_t)row * a.x_stride + 128 * (kb0 + kbi), lane);
                     sw[i] = load_two(a.suh + 128 * (kb0 + kbi), lane);
                 }
                 if (t == wv && p0 < p1) {               // behind the first rows' loads

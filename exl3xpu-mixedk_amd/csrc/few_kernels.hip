@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(
     // this workgroup's 32-row steps
     const int s0 = split * a.steps + (split < a.more ? split : a.more), s1 = s0 + a.steps + (split < a.more ? 1 : 0);
     const FewSource src{(const uint8_t*)w.trellis + (size_t)blk * 256 * K, (size_t)nb * 256 * K, ep.rows, w.k / 32,
-                        a.x, a.x_stride, nullptr, w.suh, a.type, a.rinv, a.frag, nullptr, a.shift};
+                        a.x, a.x_stride, w.suh, a.type, a.rinv, a.frag, nullptr, a.shift};
     f4 total[G][N];
     few_sums<K, CODE, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
     // (on their way while the workgroups meet)
@@ -81,10 +81,6 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(
     }
 }
 
-// Rows that come transformed fill two groups' fragments or four, as many as their
-// kernels read.
-static_assert(kFusedRows >= 16 && kFewRows <= 64, "groups of rows");
-
 template <int K, int CODE>
 hipError_t few_kc(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s) {
     const dim3 grid(w.n / 128, a.splits);
@@ -92,7 +88,9 @@ hipError_t few_kc(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStre
         hipLaunchKernelGGL((few_kernel<K, CODE, 1, true, true>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
     else if (!a.frag)
         hipLaunchKernelGGL((few_kernel<K, CODE, 1, true, false>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
-    else if (ep.rows <= 32)
+    else if (a.groups == 1)
+        hipLaunchKernelGGL((few_kernel<K, CODE, 1, false, false>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
+    else if (a.groups == 2)
         hipLaunchKernelGGL((few_kernel<K, CODE, 2, false, false>), grid, dim3(64 * few_waves(2)), 0, s, w, a, ep);
     else
         hipLaunchKernelGGL((few_kernel<K, CODE, 4, false, false>), grid, dim3(64 * few_waves(4)), 0, s, w, a, ep);

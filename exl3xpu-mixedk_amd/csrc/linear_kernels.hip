@@ -739,18 +739,35 @@ void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Parts of the summed dimension, each of 8 steps at least, so that the tiles fill
-// the compute units' two places.
-int gemm_splits(int tiles, int steps) {
-    const int most = steps / 8;
-    int s = tiles >= 2 * kCUs ? 1 : 2 * kCUs / tiles;
-    if (s > most) s = most;
-    return s < 1 ? 1 : s;
-}
+// How a product of `steps` steps is cut: nb groups of 16 rows to a wave's tile,
+// splits of the summed dimension.  The choice is the shortest estimate, from what
+// the kernels measured: a workgroup's step takes 0.62 us (nb 4) or 0.38 (nb 2)
+// alone on a compute unit, two at once 0.72 and 0.46, and where a unit has more to
+// do than those, every two 0.84 and 0.64; parts are written and read at 4 TB/s.  (us with nb 4, nb 2: 5120 by 5120, 333 rows 67 : 56, 1000 rows 92 :
+// 107, 2047 rows 150 : 182; 5120 by 17408, 96 rows 101 : 84, 600 rows 176 : 205.)
+struct Tiling {
+    int nb, tiles, splits;
+};
 
-// Groups of 16 rows of a wave's tile: 4 (128 rows a workgroup), or 2 while that
-// leaves compute units empty.
-int gemm_nb(int rows, int n) { return (n + kTileN - 1) / kTileN * ((rows + 127) / 128) < kCUs ? 2 : 4; }
+Tiling gemm_tiling(int rows, int n, int steps, bool two) {
+    Tiling best{};
+    double least = 0.0;
+    for (int nb = two ? 2 : 4; nb >= 2; nb -= 2) {      // (two terms: the LDS of two workgroups)
+        const int tiles = (n + kTileN - 1) / kTileN * ((rows + 32 * nb - 1) / (32 * nb));
+        const double alone = nb == 4 ? 0.62 : 0.38, pair = nb == 4 ? 0.72 : 0.46, more = nb == 4 ? 0.42 : 0.32;
+        for (int s = 1; s == 1 || (s <= steps / 8 && (s - 1) * tiles < 2 * kCUs); ++s) {
+            const int each = (int)(((long long)tiles * s + kCUs - 1) / kCUs);
+            const double step = each == 1 ? alone : each == 2 ? pair : more * (each % 2 ? each + 0.4 : each);
+            const double us = step * (two ? 2 : 1) * ((steps + s - 1) / s) +
+                              (s > 1 ? 3.0 + 2e-6 * s * rows * n : 0.0);
+            if (!best.nb || us < least) {
+                least = us;
+                best = Tiling{nb, tiles, s};
+            }
+        }
+    }
+    return best;
+}
 
 struct ManyPlan {
     int groups, nb, tiles, splits;
@@ -761,9 +778,10 @@ struct ManyPlan {
 ManyPlan many_plan(int rows, int k, int n, bool colsum, bool two) {
     ManyPlan p;
     p.groups = (rows + 15) / 16;
-    p.nb = two ? 2 : gemm_nb(rows, n);     // (two terms: the LDS of two workgroups)
-    p.tiles = (n + kTileN - 1) / kTileN * ((p.groups + 2 * p.nb - 1) / (2 * p.nb));
-    p.splits = gemm_splits(p.tiles, k / 32);
+    const Tiling t = gemm_tiling(rows, n, k / 32, two);
+    p.nb = t.nb;
+    p.tiles = t.tiles;
+    p.splits = t.splits;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t a = at; at += align256(bytes); return a; };
     p.shift = take((size_t)p.groups * 64);
@@ -832,35 +850,48 @@ __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __re
 }
 
 // Workgroups per 128 columns of a product of few rows: two for each compute
-// unit, each wave with a 32-row step at least.
-int few_splits(int k, int n, int waves) {
+// unit, each wave with a 32-row step at least, and no more than balances what
+// they share, k / 32 steps, with what the last of them adds alone, their parts of
+// every row, 0.01 us each (5120 by 1024: 17 rows 20.0 us, 27.2 with 40 parts; 64
+// rows 27.3, 47.7).
+int few_splits(int rows, int k, int n, int waves) {
     const int most = k / 32 / waves;
     int s = 2 * kCUs / (n / 128);
     if (s > most) s = most;
+    while (s > 1 && (long long)s * s * waves * rows > 4 * k) --s;
     return s < 1 ? 1 : s;
 }
 
+// (5120 by 5120, one launch or two against decoding apart: 17 rows 22 : 42 us, 64
+// rows 35 : 44; 5120 by 1024 20 : 30 and 27 : 32.)
 bool takes_few(int rows, int n, bool two) {
     return rows <= (two ? kFusedRows : kFewRows) && n / 128 <= XTQ_OP_COUNTERS;
 }
 
+// Blocks of rows that a workgroup transforms itself at most, two a wave (us where
+// the product's workgroups transform, and in a launch before it: 5120 by 5120, one
+// row 14.0 : 15.4, four 15.4 : 16.0, six 17.6 : 16.5, sixteen 21.4 : 17.2; 5120 by
+// 17408, one row 27.6 : 27.2, sixteen 45.2 : 29.5).
+constexpr int kFewItems = 16;
+
 int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 struct FewPlan {
-    int splits;
+    int splits, groups;
+    bool apart;
     size_t part, frag, shift, total;
 };
 
-FewPlan few_plan(int rows, int k, int n) {
+FewPlan few_plan(int rows, int k, int n, bool two) {
     FewPlan p;
-    const int g = few_groups(rows);
-    p.splits = few_splits(k, n, few_waves(g));
+    p.groups = few_groups(rows);
+    p.splits = few_splits(rows, k, n, few_waves(p.groups));
+    p.apart = !two && (rows > kFusedRows || rows * (k / 128) > kFewItems * p.splits);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t a = at; at += align256(bytes); return a; };
     p.part = take(p.splits > 1 ? (size_t)p.splits * n * rows * 4 : 0);
-    const bool apart = rows > kFusedRows;
-    p.frag = take(apart ? (size_t)g * k * 32 : 0);
-    p.shift = take(apart ? (size_t)g * k / 2 : 0);
+    p.frag = take(p.apart ? (size_t)p.groups * k * 32 : 0);
+    p.shift = take(p.apart ? (size_t)p.groups * k / 2 : 0);
     p.total = at;
     return p;
 }
@@ -870,7 +901,7 @@ FewPlan few_plan(int rows, int k, int n) {
 size_t linear_ws_bytes(int rows, int k, int n, int backward) {
     if (backward == 1) return many_plan(rows, n, k, true, false).total;
     auto forward = [&](bool two) {
-        return takes_few(rows, n, two) ? few_plan(rows, k, n).total : many_plan(rows, k, n, false, two).total;
+        return takes_few(rows, n, two) ? few_plan(rows, k, n, two).total : many_plan(rows, k, n, false, two).total;
     };
     const size_t one = forward(false);
     if (backward == 0) return one;
@@ -884,14 +915,14 @@ hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_s
     if (takes_few(rows, w.n, two)) {
         static decltype(&launch_few_k2) const few[] = {launch_few_k2, launch_few_k3, launch_few_k4,
                                                        launch_few_k5, launch_few_k6, launch_few_k7};
-        const FewPlan p = few_plan(rows, w.k, w.n);
+        const FewPlan p = few_plan(rows, w.k, w.n, two);
         uint8_t* base = (uint8_t*)ws;
-        FewArgs a{type, two, (const uint16_t*)x, x_stride, nullptr, nullptr, p.splits, w.k / 32 / p.splits,
+        FewArgs a{type, two, (const uint16_t*)x, x_stride, nullptr, nullptr, p.groups, p.splits, w.k / 32 / p.splits,
                   w.k / 32 % p.splits, 65536u / rows + 1, (float*)(base + p.part), counters};
-        if (rows > kFusedRows) {
+        if (p.apart) {
             u4* frag = (u4*)(base + p.frag);
             int32_t* shift = (int32_t*)(base + p.shift);
-            hipLaunchKernelGGL(transform_few_kernel, dim3((w.k / 128 + 3) / 4, 16 * few_groups(rows)),
+            hipLaunchKernelGGL(transform_few_kernel, dim3((w.k / 128 + 3) / 4, 16 * p.groups),
                                dim3(256), 0, s, a.x, x_stride, type, rows, w.k, w.suh, frag, shift);
             a.frag = frag;
             a.shift = shift;
@@ -935,6 +966,15 @@ struct GramPlan {
 // 256, 92 : 91 at 1021, 152 : 112 at 2048; 17408 594 : 541 at one row).
 bool takes_gram_few(int rows, int k) {
     return rows <= 8192 && k <= 8192 && (long long)rows * k * k <= 24LL << 30;
+}
+
+// Parts of the summed dimension, each of 8 steps at least, so that the tiles fill
+// the compute units' two places.
+int gemm_splits(int tiles, int steps) {
+    const int most = steps / 8;
+    int s = tiles >= 2 * kCUs ? 1 : 2 * kCUs / tiles;
+    if (s > most) s = most;
+    return s < 1 ? 1 : s;
 }
 
 GramPlan gram_plan(int rows, int k) {

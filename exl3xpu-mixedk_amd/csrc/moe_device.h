@@ -44,7 +44,6 @@ struct MoeArgs {
 constexpr int kMoeRows = 64;            // rows of a call
 constexpr int kMoeTop = 16;
 constexpr int kMoeExperts = 512;
-constexpr int kMoeFused = 4;            // rows up to which the first product transforms them itself
 constexpr int kMoeRouterCounters = 32;  // one for each 4 rows, one for all
 
 #define XTQ_MOE(C) \

@@ -38,9 +38,10 @@ __device__ __forceinline__ void split_range(int pairs, int splits, int split, in
 }
 
 // Rows of x for the first product, as fragments and what their rounding left,
-// one wave per chunk, weight (gate, up) and 128-column block.  (Each workgroup of
-// the product would do this for its chunk again: one launch less, worth it up to
-// kMoeFused rows.)  Latency bounds it: 8.9 us for 37 rows of 4096 and 4 of 32
+// one wave per chunk, weight (gate, up) and 128-column block.  (For one row the
+// product's workgroups do this themselves, each again: one launch less; us with and
+// without it, 2048 by 1024 and 4096 by 2048: one row 46 : 41 and 52 : 51, two 53 :
+// 52 and 67 : 73, four 72 : 73 and 96 : 107.)  Latency bounds it: 8.9 us for 37 rows of 4096 and 4 of 32
 // experts.
 __global__ __launch_bounds__(256) void moe_x_kernel(MoeArgs a) {
     const int lane = threadIdx.x & 63, nk = a.d / 128, role = blockIdx.y, ch = blockIdx.z;
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(256) void moe_x_kernel(MoeArgs a) {
 }
 
 // One weight's (gate's or up's) 128 columns for a chunk over a part of the summed
-// dimension; the last workgroup of the two weights' parts adds them, applies the
+// dimension (FUSED: of the only row, transformed here); the last workgroup of the two weights' parts adds them, applies the
 // activation and leaves the product's rows as fragments for the second product.
 // The decoding bounds it: 32 experts' gate and up of 4096 by 2048 are 537 M
 // weights, 57 us of vector instructions, of 102 us in all; the compute units
@@ -74,7 +75,6 @@ template <bool FUSED>
 __global__ __launch_bounds__(64 * W, 4) void moe_up_kernel(MoeArgs a) {
     __shared__ __align__(16) u4 lds[(FUSED ? kLds : kLdsApart) / 16];
     __shared__ int32_t shifts[kFewMaxSlice * 16];
-    __shared__ int32_t list[16];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nf = a.f / 128, nk = a.d / 128, ch = blockIdx.z, split = blockIdx.y;
     const int fb = blockIdx.x >> 1, role = blockIdx.x & 1;
@@ -82,13 +82,11 @@ __global__ __launch_bounds__(64 * W, 4) void moe_up_kernel(MoeArgs a) {
     const int rows = c.rows;
     const xtq_moe_weight w = c.w[role];
     if (ch >= *a.nchunks) return;
-    if (FUSED && threadIdx.x < rows) list[threadIdx.x] = c.slots[threadIdx.x] / a.top;
-    if (FUSED) __syncthreads();
     int s0, s1;
     split_range(a.d / 32, a.up_splits, split, s0, s1);
     const u4* hi = FUSED ? nullptr : a.xf + (size_t)(ch * 2 + role) * 2 * nk * 256;
     const FewSource src{(const uint8_t*)w.trellis + (size_t)fb * 256 * w.K, (size_t)nf * 256 * w.K, rows, a.d / 32,
-                        a.x, a.x_stride, list, w.suh, a.type, 65536u / rows + 1, hi,
+                        a.x, a.x_stride, w.suh, a.type, 65536u / rows + 1, hi,
                         FUSED ? nullptr : hi + (size_t)nk * 256,
                         FUSED ? nullptr : a.xs + (size_t)(ch * 2 + role) * nk * 16};
     f4 total[1][1];
@@ -202,7 +200,7 @@ __global__ __launch_bounds__(64 * W, 4) void moe_down_kernel(MoeArgs a) {
     split_range(a.f / 32, a.down_splits, split, s0, s1);
     const u4* hi = a.hf + (size_t)ch * 2 * nf * 256;
     const FewSource src{(const uint8_t*)w.trellis + (size_t)db * 256 * w.K, (size_t)(a.d / 128) * 256 * w.K, c.rows,
-                        a.f / 32, nullptr, 0, nullptr, nullptr, 0, 0, hi, hi + (size_t)nf * 256,
+                        a.f / 32, nullptr, 0, nullptr, 0, 0, hi, hi + (size_t)nf * 256,
                         a.hs + (size_t)ch * nf * 16};
     f4 total[1][1];
     expert_sums<false>(w.K, src, s0, s1, lds, nullptr, total);
@@ -233,7 +231,7 @@ __global__ __launch_bounds__(64 * W, 4) void moe_down_kernel(MoeArgs a) {
 hipError_t XTQ_CAT(launch_moe_code, XTQ_MOE_CODE)(const MoeArgs& a, hipStream_t s) {
     const dim3 block(64 * W), up(2 * (a.f / 128), a.up_splits, a.max_chunks),
         down(a.d / 128, a.down_splits, a.max_chunks);
-    if (a.rows <= kMoeFused) {
+    if (a.rows == 1) {
         hipLaunchKernelGGL((moe_up_kernel<true>), up, block, 0, s, a);
     } else {
         hipLaunchKernelGGL(moe_x_kernel, dim3((a.d / 128 + 3) / 4, 2, a.max_chunks), dim3(256), 0, s, a);

@@ -273,7 +273,7 @@ MoePlan moe_plan(int rows, int experts, int top, int d, int f) {
     p.logits = take((size_t)rows * experts * 4);
     p.nchunks = take(4);
     p.list = take(n * sizeof(MoeChunk));
-    const bool apart = rows > kMoeFused;
+    const bool apart = rows > 1;
     p.xf = take(apart ? n * 4 * d * 32 : 0);
     p.xs = take(apart ? n * 2 * (d / 128) * 64 : 0);
     p.part = take(n * (f / 128) * 2 * p.up_splits * 8192);

@@ -58,10 +58,10 @@ hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long lon
                              void* dbias, int dbias_f32, void* ws, uint32_t* counters,
                              hipStream_t s);
 
-// Products of up to kFewRows rows (few_kernels.hip), one function per K.  Up to
-// kFusedRows rows the product's kernel transforms x itself; more come
-// transformed (transform_few_kernel): fragments frag [group of 16 rows][k/32][64] and
-// their shifts [group][k/128][16].
+// Products of up to kFewRows rows (few_kernels.hip), one function per K.  The
+// kernel transforms up to kFusedRows rows of x itself, or takes them transformed
+// (transform_few_kernel): fragments frag [groups of 16 rows][k/32][64] and their
+// shifts [groups][k/128][16], 1, 2 or 4 groups, all of whose places it reads.
 constexpr int kFewRows = 64;
 constexpr int kFusedRows = 16;
 // Waves of a workgroup: 8, which with their registers make four a SIMD, or 4
@@ -72,8 +72,9 @@ struct FewArgs {
     int two;                            // two terms (up to kFusedRows rows)
     const uint16_t* x;
     long long x_stride;
-    const u4* frag;
+    const u4* frag;                     // NULL: x is transformed by the kernel
     const int32_t* shift;
+    int groups;
     int splits, steps, more;            // 32-row steps of a split; splits with one more
     uint32_t rinv;                      // item / rows is item * rinv >> 16
     float* part;

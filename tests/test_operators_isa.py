@@ -43,7 +43,7 @@ def many(tmp_path_factory):
 
 def test_few_rows_join(few):
     bodies = {k: v for k, v in few.items() if "few_kernel" in k}
-    assert len(bodies) == 12            # three codes; one, one with two terms, two and four groups of rows
+    assert len(bodies) == 15            # three codes; x transformed here, with two terms, and 1, 2, 4 groups apart
     for name, lines in bodies.items():
         assert not any(ln.startswith("buffer_wbl2") for ln in lines), name
         count = [i for i, ln in enumerate(lines) if re.match(r"global_atomic_(add|inc)", ln)]
