@@ -853,7 +853,8 @@ __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __re
 // unit, each wave with a 32-row step at least, and no more than balances what
 // they share, k / 32 steps, with what the last of them adds alone, their parts of
 // every row, 0.01 us each (5120 by 1024: 17 rows 20.0 us, 27.2 with 40 parts; 64
-// rows 27.3, 47.7).
+// rows 27.3, 47.7).  (One workgroup for each: one row of 5120 by 17408 33.2 us, not
+// 27.5; three: 64 rows of 17408 by 5120 61.5, not 51.7.)
 int few_splits(int rows, int k, int n, int waves) {
     const int most = k / 32 / waves;
     int s = 2 * kCUs / (n / 128);

@@ -44,6 +44,11 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// The logit of a key (NaN for NaN's).
+__device__ __forceinline__ float order_value(uint32_t key) {
+    return __uint_as_float(key == 0xFFFFFFFFu ? key : (key & 0x80000000u) ? key ^ 0x80000000u : ~key);
+}
+
 // A row's top-k by a wave: the largest logits, ties to the lowest expert, and
 // their softmax weights over all experts (renorm: over the chosen ones).  N: 64
 // N experts at most.
@@ -81,34 +86,33 @@ __device__ void choose(const MoeArgs& a, int row, int lane) {
         if (lane + 64 * i < a.experts) sum += expf(v[i] - top);
     sum = wave_sum(sum);
     if (__any(nan)) sum = __builtin_nanf("");
-    float chosen = 0.0f, mine = 0.0f;
+    uint32_t mine = 0u;
     int id = 0;
     for (int j = 0; j < a.top; ++j) {
         uint32_t best = 0u;
 #pragma unroll
         for (int i = 0; i < N; ++i) best = key[i] > best ? key[i] : best;
         best = wave_max_u32(best);
-        int e = 0;
         bool found = false;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const unsigned long long at = __ballot(key[i] == best && lane + 64 * i < a.experts);
             if (at && !found) {
                 const int l = __builtin_ctzll(at);
-                e = l + 64 * i;
                 found = true;
-                const float p = expf(__shfl(v[i], l) - top) / sum;
-                chosen += p;
                 if (lane == j) {
-                    mine = p;
-                    id = e;
+                    mine = best;
+                    id = l + 64 * i;
                 }
                 if (lane == l) key[i] = 0u;
             }
         }
     }
+    // (the choice is a chain of maxima; what it weighs is found for all at once)
+    const float p = lane < a.top ? expf(order_value(mine) - top) / sum : 0.0f;
+    const float chosen = wave_sum(p);
     if (lane < a.top) {
-        const float w = a.renorm ? mine / chosen : mine;
+        const float w = a.renorm ? p / chosen : p;
         __hip_atomic_store(a.ids + row * a.top + lane, id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         a.weights[row * a.top + lane] = w;
     }
