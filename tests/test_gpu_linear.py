@@ -68,6 +68,30 @@ def test_linear_codes(xt, oracle_mod, K, code, m):
     assert float(R.row_errors(dx, dy.cpu().double() @ W.t()).max()) <= _tol(torch.float16)
 
 
+@pytest.mark.parametrize("K", range(2, 8))
+@pytest.mark.parametrize("code", sorted(R.CODES))
+def test_linear_rows_apart(xt, oracle_mod, K, code):
+    """Few rows that are transformed before the product's launch, in one, two and four groups of 16, places of the
+    last group left over."""
+    k, n = 1280, 128
+    w = R.random_weight(k, n, K, 3 * K)
+    W = R.dense(oracle_mod, *w, K, code)
+    for m in (9, 30, 50):
+        x = _x(m, k, torch.bfloat16, m + K)
+        y = xt.linear(x, xt.TrellisLinear(*w, K, code=code))
+        assert float(R.row_errors(y, x.cpu().double() @ W).max()) <= _tol(torch.bfloat16)
+
+
+@pytest.mark.parametrize("m,k,n", [(9000, 128, 1152), (3000, 2048, 384), (1815, 4096, 2176)])
+def test_linear_cuts(xt, oracle_mod, m, k, n):
+    """Every way in which a product of many rows is cut: both heights of tile, whole and in parts."""
+    w = R.random_weight(k, n, 4, 5)
+    W = R.dense(oracle_mod, *w, 4, "exl3_mul1").cuda()
+    x = _x(m, k, torch.float16, m, spread=0.5)
+    y = xt.linear(x, xt.TrellisLinear(*w, 4))
+    assert float(R.row_errors(y.cpu(), (x.double() @ W).cpu()).max()) <= _tol(torch.float16)
+
+
 @pytest.mark.parametrize("act", ("none", "relu", "silu", "gelu"))
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 @pytest.mark.parametrize("m,with_bias,with_res", [(5, True, False), (40, False, True), (300, True, True)])
