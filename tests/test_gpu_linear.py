@@ -187,6 +187,32 @@ def test_linear_magnitudes(xt, oracle_mod, m):
         assert bool((got[1::3] == 0).all())
 
 
+@pytest.mark.parametrize("m,step", [(3, 2 ** 31), (70, 2 ** 26)])
+def test_far_rows(xt, m, step):
+    """Rows whose offsets pass 2^32 elements give what the same rows give side by side, bit for bit."""
+    k, n = 256, 384
+    near, res = _x(m, k, torch.float16, 3), _x(m, n, torch.float16, 4)
+    slots = torch.empty(70 * 2 ** 26, dtype=torch.float16, device="cuda")
+    x, r = slots.as_strided((m, k), (step, 1)), slots.as_strided((m, n), (step, 1), 2048)
+    x.copy_(near)
+    r.copy_(res)
+    w = xt.TrellisLinear(*R.random_weight(k, n, 4, 9), 4)
+    assert torch.equal(xt.linear(x, w, residual=r), xt.linear(near, w, residual=res))
+    assert torch.equal(xt.input_gram(x), xt.input_gram(near))
+    x.requires_grad_()
+    far, = torch.autograd.grad(xt.linear(x, w, act="silu"), x, res)
+    near.requires_grad_()
+    side, = torch.autograd.grad(xt.linear(near, w, act="silu"), near, res)
+    assert torch.equal(far, side)
+    if m <= 64:
+        gate, down = xt.TrellisLinear(*R.random_weight(k, n, 3, 1), 3), xt.TrellisLinear(*R.random_weight(n, k, 4, 2), 4)
+        experts = xt.TrellisExperts([gate, gate], [gate, gate], [down, down])
+        router = _x(2, k, torch.float16, 5)
+        with torch.no_grad():
+            assert torch.equal(xt.moe(x, router, experts, 1, residual=x),
+                               xt.moe(near, router, experts, 1, residual=near))
+
+
 @pytest.mark.parametrize("m", (4, 80))
 def test_linear_nonfinite_rows(xt, m):
     """A NaN or an infinity stays in its row."""
