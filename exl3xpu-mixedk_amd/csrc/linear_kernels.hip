@@ -854,17 +854,22 @@ __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __re
 // they share, k / 32 steps, with what the last of them adds alone, their parts of
 // every row, 0.01 us each (5120 by 1024: 17 rows 20.0 us, 27.2 with 40 parts; 64
 // rows 27.3, 47.7).  (One workgroup for each: one row of 5120 by 17408 33.2 us, not
-// 27.5; three: 64 rows of 17408 by 5120 61.5, not 51.7.)
+// 27.5; three: 64 rows of 17408 by 5120 61.5, not 51.7.)  Above 16 rows one is
+// better where that fills them and no wave has more than 16 steps: the joins weigh
+// more (4096 by 4096, 17 rows 17.4 us, 20.2 with two; 48 rows 24.6, 29.2; 17408 by
+// 5120, 23 steps, 36.4, 34.4).
 int few_splits(int rows, int k, int n, int waves) {
     const int most = k / 32 / waves;
     int s = 2 * kCUs / (n / 128);
     if (s > most) s = most;
     while (s > 1 && (long long)s * s * waves * rows > 4 * k) --s;
+    const int one = kCUs / (n / 128);
+    if (rows > 16 && s > one && 5 * one * (n / 128) > 4 * kCUs && k / 32 <= 16 * waves * one) s = one;
     return s < 1 ? 1 : s;
 }
 
-// (5120 by 5120, one launch or two against decoding apart: 17 rows 22 : 42 us, 64
-// rows 35 : 44; 5120 by 1024 20 : 30 and 27 : 32.)
+// (5120 by 5120, one launch or two against decoding apart: 17 rows 20 : 42 us, 64
+// rows 31 : 44; 5120 by 1024 20 : 30 and 27 : 32.)
 bool takes_few(int rows, int n, bool two) {
     return rows <= (two ? kFusedRows : kFewRows) && n / 128 <= XTQ_OP_COUNTERS;
 }
