@@ -1,7 +1,8 @@
 // few_kernels.hip -- linear layers of few rows (up to 64): the weight is decoded
 // on its way to the matrix cores.
 //
-// Built once per width K (XTQ_FEW_K), so that the widths compile side by side.
+// Built once per width K (XTQ_FEW_K), so that the widths compile side by side,
+// and once more (XTQ_FEW_TWO) for two terms of rows that come transformed.
 #include "epilogue.h"
 #include "few_device.h"
 
@@ -35,7 +36,7 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(
     // this workgroup's 32-row steps
     const int s0 = split * a.steps + (split < a.more ? split : a.more), s1 = s0 + a.steps + (split < a.more ? 1 : 0);
     const FewSource src{(const uint8_t*)w.trellis + (size_t)blk * 256 * K, (size_t)nb * 256 * K, ep.rows, w.k / 32,
-                        a.x, a.x_stride, w.suh, a.type, a.rinv, a.frag, nullptr, a.shift};
+                        a.x, a.x_stride, w.suh, a.type, a.rinv, a.frag, a.frag_lo, a.shift};
     f4 total[G][N];
     few_sums<K, CODE, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
     // (on their way while the workgroups meet)
@@ -81,28 +82,39 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(
     }
 }
 
+template <int K, int CODE, int G, bool FUSED, bool LO>
+hipError_t few_launch(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s) {
+    hipLaunchKernelGGL((few_kernel<K, CODE, G, FUSED, LO>), dim3(w.n / 128, a.splits), dim3(64 * few_waves(G)), 0, s,
+                       w, a, ep);
+    return hipGetLastError();
+}
+
 template <int K, int CODE>
 hipError_t few_kc(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s) {
-    const dim3 grid(w.n / 128, a.splits);
-    if (a.two)
-        hipLaunchKernelGGL((few_kernel<K, CODE, 1, true, true>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
-    else if (!a.frag)
-        hipLaunchKernelGGL((few_kernel<K, CODE, 1, true, false>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
-    else if (a.groups == 1)
-        hipLaunchKernelGGL((few_kernel<K, CODE, 1, false, false>), grid, dim3(64 * few_waves(1)), 0, s, w, a, ep);
-    else if (a.groups == 2)
-        hipLaunchKernelGGL((few_kernel<K, CODE, 2, false, false>), grid, dim3(64 * few_waves(2)), 0, s, w, a, ep);
-    else
-        hipLaunchKernelGGL((few_kernel<K, CODE, 4, false, false>), grid, dim3(64 * few_waves(4)), 0, s, w, a, ep);
-    return hipGetLastError();
+#ifdef XTQ_FEW_TWO
+    if (a.groups == 1) return few_launch<K, CODE, 1, false, true>(w, a, ep, s);
+    if (a.groups == 2) return few_launch<K, CODE, 2, false, true>(w, a, ep, s);
+    return few_launch<K, CODE, 4, false, true>(w, a, ep, s);
+#else
+    if (a.two) return few_launch<K, CODE, 1, true, true>(w, a, ep, s);
+    if (!a.frag) return few_launch<K, CODE, 1, true, false>(w, a, ep, s);
+    if (a.groups == 1) return few_launch<K, CODE, 1, false, false>(w, a, ep, s);
+    if (a.groups == 2) return few_launch<K, CODE, 2, false, false>(w, a, ep, s);
+    return few_launch<K, CODE, 4, false, false>(w, a, ep, s);
+#endif
 }
 
 }  // namespace
 
 #define XTQ_CAT2(a, b) a##b
 #define XTQ_CAT(a, b) XTQ_CAT2(a, b)
+#ifdef XTQ_FEW_TWO
+#define XTQ_FEW_NAME launch_few2_k
+#else
+#define XTQ_FEW_NAME launch_few_k
+#endif
 
-hipError_t XTQ_CAT(launch_few_k, XTQ_FEW_K)(const Weight& w, const FewArgs& a, const Epilogue& ep,
+hipError_t XTQ_CAT(XTQ_FEW_NAME, XTQ_FEW_K)(const Weight& w, const FewArgs& a, const Epilogue& ep,
                                             hipStream_t s) {
     if (w.code == kCodeMul1) return few_kc<XTQ_FEW_K, kCodeMul1>(w, a, ep, s);
     if (w.code == kCodeMcg) return few_kc<XTQ_FEW_K, kCodeMcg>(w, a, ep, s);

@@ -832,12 +832,14 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
 }
 
 // Rows to fragments for the products of few rows, a wave for one row's
-// 128-column block.  Rows past the end are zeros.  Latency alone: 2.3 us for 48
-// rows of 5120.
+// 128-column block.  Rows past the end are zeros.  rest (LO): the second terms.
+// Latency alone: 2.3 us for 48 rows of 5120.
+template <bool LO>
 __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __restrict__ x, long long stride,
                                                             int type, int rows, int k,
                                                             const uint16_t* __restrict__ suh,
-                                                            u4* __restrict__ frag, int32_t* __restrict__ shift) {
+                                                            u4* __restrict__ frag, u4* __restrict__ rest,
+                                                            int32_t* __restrict__ shift) {
     const int lane = threadIdx.x & 63, nk = k / 128;
     const int kb = blockIdx.x * 4 + (threadIdx.x >> 6), row = blockIdx.y;
     if (kb >= nk) return;
@@ -845,7 +847,8 @@ __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __re
     if (row < rows) unpack_two(load_two(x + (size_t)row * stride + 128 * kb, lane), type, a, b);
     unpack_two(load_two(suh + 128 * kb, lane), kF16, sa, sb);
     const size_t at = (size_t)(row >> 4) * nk + kb;
-    const int sh = row_to_frags<false>(a * sa, b * sb, lane, row & 15, (uint32_t*)(frag + at * 256), nullptr);
+    const int sh = row_to_frags<LO>(a * sa, b * sb, lane, row & 15, (uint32_t*)(frag + at * 256),
+                                    LO ? (uint32_t*)(rest + at * 256) : nullptr);
     if (lane == 0) shift[at * 16 + (row & 15)] = sh;
 }
 
@@ -870,9 +873,7 @@ int few_splits(int rows, int k, int n, int waves) {
 
 // (5120 by 5120, one launch or two against decoding apart: 17 rows 20 : 42 us, 64
 // rows 31 : 44; 5120 by 1024 20 : 30 and 27 : 32.)
-bool takes_few(int rows, int n, bool two) {
-    return rows <= (two ? kFusedRows : kFewRows) && n / 128 <= XTQ_OP_COUNTERS;
-}
+bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_COUNTERS; }
 
 // Blocks of rows that a workgroup transforms itself at most, two a wave (us where
 // the product's workgroups transform, and in a launch before it: 5120 by 5120, one
@@ -885,18 +886,19 @@ int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 struct FewPlan {
     int splits, groups;
     bool apart;
-    size_t part, frag, shift, total;
+    size_t part, frag, rest, shift, total;
 };
 
 FewPlan few_plan(int rows, int k, int n, bool two) {
     FewPlan p;
     p.groups = few_groups(rows);
     p.splits = few_splits(rows, k, n, few_waves(p.groups));
-    p.apart = !two && (rows > kFusedRows || rows * (k / 128) > kFewItems * p.splits);
+    p.apart = rows > kFusedRows || rows * (k / 128) > kFewItems * p.splits;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t a = at; at += align256(bytes); return a; };
     p.part = take(p.splits > 1 ? (size_t)p.splits * n * rows * 4 : 0);
     p.frag = take(p.apart ? (size_t)p.groups * k * 32 : 0);
+    p.rest = take(p.apart && two ? (size_t)p.groups * k * 32 : 0);
     p.shift = take(p.apart ? (size_t)p.groups * k / 2 : 0);
     p.total = at;
     return p;
@@ -904,36 +906,32 @@ FewPlan few_plan(int rows, int k, int n, bool two) {
 
 }  // namespace
 
-size_t linear_ws_bytes(int rows, int k, int n, int backward) {
-    if (backward == 1) return many_plan(rows, n, k, true, false).total;
-    auto forward = [&](bool two) {
-        return takes_few(rows, n, two) ? few_plan(rows, k, n, two).total : many_plan(rows, k, n, false, two).total;
-    };
-    const size_t one = forward(false);
-    if (backward == 0) return one;
-    const size_t two = forward(true);   // (the activation decides which it is)
-    return one > two ? one : two;
+size_t linear_ws_bytes(int rows, int k, int n, bool backward, bool two) {
+    if (backward) return many_plan(rows, n, k, true, false).total;
+    return takes_few(rows, n) ? few_plan(rows, k, n, two).total : many_plan(rows, k, n, false, two).total;
 }
 
 hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
-                         const Epilogue& ep, void* ws, uint32_t* counters, hipStream_t s) {
-    const bool two = two_terms(type, ep.act, ep.z != nullptr);
-    if (takes_few(rows, w.n, two)) {
+                         const Epilogue& ep, bool two, void* ws, uint32_t* counters, hipStream_t s) {
+    if (takes_few(rows, w.n)) {
         static decltype(&launch_few_k2) const few[] = {launch_few_k2, launch_few_k3, launch_few_k4,
-                                                       launch_few_k5, launch_few_k6, launch_few_k7};
+                                                       launch_few_k5, launch_few_k6, launch_few_k7},
+                                              few2[] = {launch_few2_k2, launch_few2_k3, launch_few2_k4,
+                                                        launch_few2_k5, launch_few2_k6, launch_few2_k7};
         const FewPlan p = few_plan(rows, w.k, w.n, two);
         uint8_t* base = (uint8_t*)ws;
-        FewArgs a{type, two, (const uint16_t*)x, x_stride, nullptr, nullptr, p.groups, p.splits, w.k / 32 / p.splits,
-                  w.k / 32 % p.splits, 65536u / rows + 1, (float*)(base + p.part), counters};
-        if (p.apart) {
-            u4* frag = (u4*)(base + p.frag);
-            int32_t* shift = (int32_t*)(base + p.shift);
-            hipLaunchKernelGGL(transform_few_kernel, dim3((w.k / 128 + 3) / 4, 16 * p.groups),
-                               dim3(256), 0, s, a.x, x_stride, type, rows, w.k, w.suh, frag, shift);
-            a.frag = frag;
-            a.shift = shift;
-        }
-        return few[w.K - 2](w, a, ep, s);
+        FewArgs a{type, two, (const uint16_t*)x, x_stride, nullptr, nullptr, nullptr, p.groups, p.splits,
+                  w.k / 32 / p.splits, w.k / 32 % p.splits, 65536u / rows + 1, (float*)(base + p.part), counters};
+        if (!p.apart) return few[w.K - 2](w, a, ep, s);
+        u4 *frag = (u4*)(base + p.frag), *rest = two ? (u4*)(base + p.rest) : nullptr;
+        int32_t* shift = (int32_t*)(base + p.shift);
+        hipLaunchKernelGGL(two ? transform_few_kernel<true> : transform_few_kernel<false>,
+                           dim3((w.k / 128 + 3) / 4, 16 * p.groups), dim3(256), 0, s, a.x, x_stride, type, rows, w.k,
+                           w.suh, frag, rest, shift);
+        a.frag = frag;
+        a.frag_lo = rest;
+        a.shift = shift;
+        return (two ? few2 : few)[w.K - 2](w, a, ep, s);
     }
     const Source src{(const uint16_t*)x, x_stride, nullptr, 0, w.suh, type, rows, w.k};
     return type == kBf16 ? many<kBf16>(w, 0, src, ep, nullptr, 0, two, ws, s)

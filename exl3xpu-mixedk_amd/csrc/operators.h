@@ -39,20 +39,23 @@ struct Epilogue {
     int rows, cols;
 };
 
-// Whether a product's rows enter with 22 bits, as two fp16 terms: where a slope
-// will be taken at its results and an error of 2^-12 of a row's norm is not
-// below the gradient's own roundoff.  relu's slope jumps at zero: results that
-// near to it take the wrong side, e of them for an error e, and the gradient is
-// off by the root of that.  The other slopes move by about e, which bf16's 2^-9
-// hides and fp16's 2^-12 does not.
-inline bool two_terms(int type, int act, bool keeps_z) {
-    return keeps_z && (act == kActRelu || (type == kF16 && act != kActNone));
-}
+// Whether a product's rows enter with 22 bits, as two fp16 terms, and not with
+// the 11 of one.  fp16: one rounding of the rows is as large as the result's own
+// (together 1.4 times the error of that alone), so only the result's is left.
+// bf16 results are rounded to 8 bits, beside which the rows' 11 do not show
+// (0.0017 of a result's norm with one term and with two); but relu's slope jumps
+// at zero: results that near to it take the wrong side, e of them for an error
+// e, and the gradient is off by the root of that, so relu's rows have 22 bits in
+// either type.  It does not go by whether z is kept: a call's results are the
+// same with a gradient and without.  fast: the caller's choice of one term, which
+// halves the work of the matrix cores (us with one and with two: 17408 by 5120, 1
+// row 24.2 : 27.2, 48 rows 43.8 : 50.4; 5120 by 17408, 333 rows 130 : 170, 4096
+// rows 722 : 1236).
+inline bool two_terms(int type, int act, bool fast) { return !fast && (type == kF16 || act == kActRelu); }
 
-// backward: 0 forward, 1 gradient, 2 forward with two terms.
-size_t linear_ws_bytes(int rows, int k, int n, int backward);
+size_t linear_ws_bytes(int rows, int k, int n, bool backward, bool two);
 hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
-                         const Epilogue& ep, void* ws, uint32_t* counters, hipStream_t s);
+                         const Epilogue& ep, bool two, void* ws, uint32_t* counters, hipStream_t s);
 hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long long dy_stride,
                              const void* z, int act, int rows, void* dx, long long dx_stride,
                              void* dbias, int dbias_f32, void* ws, uint32_t* counters,
@@ -69,10 +72,10 @@ constexpr int kFusedRows = 16;
 constexpr int few_waves(int G) { return G == 1 ? 8 : 4; }
 struct FewArgs {
     int type;
-    int two;                            // two terms (up to kFusedRows rows)
+    int two;                            // two terms
     const uint16_t* x;
     long long x_stride;
-    const u4* frag;                     // NULL: x is transformed by the kernel
+    const u4 *frag, *frag_lo;           // NULL: x is transformed by the kernel; lo: the second terms
     const int32_t* shift;
     int groups;
     int splits, steps, more;            // 32-row steps of a split; splits with one more
@@ -81,7 +84,8 @@ struct FewArgs {
     uint32_t* counters;
 };
 #define XTQ_FEW(K) \
-    hipError_t launch_few_k##K(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s);
+    hipError_t launch_few_k##K(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s); \
+    hipError_t launch_few2_k##K(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s);
 XTQ_FEW(2) XTQ_FEW(3) XTQ_FEW(4) XTQ_FEW(5) XTQ_FEW(6) XTQ_FEW(7)
 #undef XTQ_FEW
 

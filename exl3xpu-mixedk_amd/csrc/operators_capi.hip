@@ -68,7 +68,11 @@ int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int what) {
     if (what < XTQ_LINEAR_FORWARD || what > XTQ_LINEAR_TRAIN) return -15;
     if (!w || w->k <= 0 || w->n <= 0 || w->k % 128 || w->n % 128 || rows < 0 || rows > kMaxRows)
         return -6;
-    return rows ? (int64_t)xtq::linear_ws_bytes(rows, w->k, w->n, what) : 0;
+    if (!rows) return 0;
+    // (the type and the activation decide which of the two it is)
+    const size_t one = xtq::linear_ws_bytes(rows, w->k, w->n, what == XTQ_LINEAR_GRADIENT, false),
+                 two = xtq::linear_ws_bytes(rows, w->k, w->n, what == XTQ_LINEAR_GRADIENT, true);
+    return (int64_t)(one > two ? one : two);
 }
 
 int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_stride, int rows,
@@ -78,6 +82,8 @@ int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_strid
     xtq::Weight wt;
     int rc = check_weight(w, &wt);
     if (rc) return rc;
+    const bool fast = type & XTQ_FAST;
+    type &= ~XTQ_FAST;
     if ((type != XTQ_BF16 && type != XTQ_F16) || act < XTQ_ACT_NONE || act > XTQ_ACT_GELU) return 15;
     if (rows < 0 || rows > kMaxRows) return 6;
     if (rows == 0) return 0;
@@ -86,8 +92,8 @@ int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_strid
     if (res && (rc = check_rows(res, res_stride, wt.n))) return rc;
     if (!aligned(z, 2) || !aligned(bias, bias_f32 ? 4 : 2)) return 12;
     if (!counters || !aligned(counters, 4)) return 12;
-    const int what = xtq::two_terms(type, act, z != nullptr) ? XTQ_LINEAR_TRAIN : XTQ_LINEAR_FORWARD;
-    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, what)))) return rc;
+    const bool two = xtq::two_terms(type, act, fast);
+    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, false, two)))) return rc;
     xtq::Epilogue ep{};
     ep.colscale = wt.svh;
     ep.scale = wt.scale;
@@ -101,7 +107,7 @@ int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_strid
     ep.y_stride = y_stride;
     ep.rows = rows;
     ep.cols = wt.n;
-    return status(xtq::launch_linear(wt, type, x, x_stride, rows, ep, ws, counters,
+    return status(xtq::launch_linear(wt, type, x, x_stride, rows, ep, two, ws, counters,
                                      (hipStream_t)stream), "linear");
 }
 
@@ -119,7 +125,7 @@ int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy
     if (act != XTQ_ACT_NONE && (!z || !aligned(z, 2))) return 12;
     if (!aligned(dbias, bias_f32 ? 4 : 2)) return 12;
     if (!counters || !aligned(counters, 4)) return 12;
-    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, XTQ_LINEAR_GRADIENT)))) return rc;
+    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, true, false)))) return rc;
     return status(xtq::launch_linear_bwd(wt, type, dy, dy_stride, z, act, rows, dx, dx_stride, dbias,
                                          bias_f32, ws, counters, (hipStream_t)stream), "linear_bwd");
 }

@@ -32,6 +32,7 @@ import hip_backend as _hb  # noqa: E402
 
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_FAST = 16
 _COUNTERS = 16384
 _counters: dict = {}
 _HERE = contextlib.nullcontext()
@@ -102,8 +103,8 @@ class TrellisLinear:
         return cls(r["trellis"].to(device), r["suh"].to(device).half(), r["svh"].to(device).half(),
                    r["K"], code=r["code"], scale=1.0 if r["channel_scales"] else r["Wscale"])
 
-    def __call__(self, x, bias=None, act="none", residual=None):
-        return linear(x, self, bias=bias, act=act, residual=residual)
+    def __call__(self, x, bias=None, act="none", residual=None, fast=False):
+        return linear(x, self, bias=bias, act=act, residual=residual, fast=fast)
 
 
 def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -131,7 +132,7 @@ def _like(t: torch.Tensor, x: torch.Tensor, shape, name: str, dtypes) -> None:
                          f"{x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
-def _forward(x, w, bias, act, residual, keep_z):
+def _forward(x, w, bias, act, residual, fast, keep_z):
     rows = _rows(x, w.k)
     m = rows.shape[0]
     y = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
@@ -146,7 +147,7 @@ def _forward(x, w, bias, act, residual, keep_z):
         need = L.xtq_linear_ws_bytes(w._p, m, 2 if keep_z else 0)
         ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
         rc = L.xtq_linear_dev(
-            w._p, _TYPES[x.dtype], rows.data_ptr(), _stride(rows), m,
+            w._p, _TYPES[x.dtype] | fast, rows.data_ptr(), _stride(rows), m,
             None if bias is None else bias.data_ptr(), int(bias is not None and
                                                            bias.dtype == torch.float32), act,
             None if res is None else res.data_ptr(), 0 if res is None else _stride(res),
@@ -158,9 +159,9 @@ def _forward(x, w, bias, act, residual, keep_z):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, bias, residual, w, act):
+    def forward(ctx, x, bias, residual, w, act, fast):
         need = ctx.needs_input_grad[0] or (bias is not None and ctx.needs_input_grad[1])
-        y, z = _forward(x, w, bias, act, residual, need and act != 0)
+        y, z = _forward(x, w, bias, act, residual, fast, need and act != 0)
         ctx.w, ctx.act, ctx.shape = w, act, x.shape
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.save_for_backward(z)
@@ -181,7 +182,7 @@ class _Linear(torch.autograd.Function):
             if want_b:
                 dbias = torch.empty(w.n, dtype=ctx.bias_dtype, device=dy.device)
             if m == 0:
-                return dx, None if dbias is None else dbias.zero_(), dy if want_r else None, None, None
+                return dx, None if dbias is None else dbias.zero_(), dy if want_r else None, None, None, None
             L = _hb.lib()
             with _on(dy.device):
                 stream = _stream(dy.device)
@@ -195,30 +196,35 @@ class _Linear(torch.autograd.Function):
                     int(ctx.bias_dtype == torch.float32), ws.data_ptr(), ws.numel(),
                     _counter_words(dy.device, stream).data_ptr(), stream)
             _hb._check("xtq_linear_bwd_dev", rc)
-        return dx, dbias, dy if want_r else None, None, None
+        return dx, dbias, dy if want_r else None, None, None, None
 
 
 def linear(x: torch.Tensor, w: TrellisLinear, bias: torch.Tensor | None = None,
-           act: str = "none", residual: torch.Tensor | None = None) -> torch.Tensor:
+           act: str = "none", residual: torch.Tensor | None = None,
+           fast: bool = False) -> torch.Tensor:
     """act(x W + bias) + residual for x [.., k] (bfloat16 or float16) -> [.., n]
     in x's type.  act: none, relu, silu or gelu (erf).  bias [n] has x's type or
     fp32, residual y's shape and x's type.  Differentiable in x, bias and
-    residual (once; the weight is frozen)."""
+    residual (once; the weight is frozen); the same result with a gradient and
+    without.  x enters the product with 22 bits for float16 and for relu, and with
+    11 otherwise, which a bfloat16 result's 8 hide.  fast: with 11 bits always, at
+    half the matrix work: float16 results are then off by 1.4 times their own
+    rounding, and relu's gradient takes some slopes on the wrong side of zero."""
     if x.dtype not in _TYPES:
         raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
     if x.device != w.device:
         raise ValueError(f"x must be on {w.device}, got {x.device}")
     if x.dim() < 1 or x.shape[-1] != w.k:
         raise ValueError(f"x must be [.., {w.k}], got {tuple(x.shape)}")
-    a = _check_act(act)
+    a, fast = _check_act(act), _FAST if fast else 0
     if bias is not None:
         _like(bias, x, (w.n,), "bias", (x.dtype, torch.float32))
     if residual is not None:
         _like(residual, x, (*x.shape[:-1], w.n), "residual", (x.dtype,))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (x, bias, residual)):
-        return _Linear.apply(x, bias, residual, w, a)
-    return _forward(x, w, bias, a, residual, False)[0]
+        return _Linear.apply(x, bias, residual, w, a, fast)
+    return _forward(x, w, bias, a, residual, fast, False)[0]
 
 
 _MOE_ROWS = 64

@@ -339,7 +339,7 @@ typedef struct xtq_weight {
     const char* code;
 } xtq_weight;
 
-enum { XTQ_BF16 = 0, XTQ_F16 = 1 };
+enum { XTQ_BF16 = 0, XTQ_F16 = 1, XTQ_FAST = 16 };
 enum { XTQ_ACT_NONE = 0, XTQ_ACT_RELU = 1, XTQ_ACT_SILU = 2, XTQ_ACT_GELU = 3 };
 enum { XTQ_OP_COUNTERS = 16384 };
 enum { XTQ_LINEAR_FORWARD = 0, XTQ_LINEAR_GRADIENT = 1, XTQ_LINEAR_TRAIN = 2 };
@@ -350,11 +350,14 @@ enum { XTQ_LINEAR_FORWARD = 0, XTQ_LINEAR_GRADIENT = 1, XTQ_LINEAR_TRAIN = 2 };
  *   act    XTQ_ACT_*; gelu is the erf form
  *   res    [rows][n], or NULL; may be y itself
  *   z      [rows][n] contiguous (out): x W + bias, for xtq_linear_bwd_dev; or NULL.
- *          With z, and act relu or (for XTQ_F16) silu or gelu, x enters the
- *          product with 22 bits instead of 11, since slopes will be taken at z.
+ * x enters the product with 22 bits for XTQ_F16 and for relu, and with 11
+ * otherwise, beside which a bf16 result's 8 count alone.  y is the same with and
+ * without z.  type | XTQ_FAST: with 11 bits always, at half the matrix work; fp16
+ * results are then off by 1.4 times their own rounding, and relu's gradient takes
+ * the wrong slope where z is within 2^-12 of a row's norm of zero.
  * At most 1,048,560 rows.  xtq_linear_ws_bytes: the scratch of xtq_linear_dev
  * without z (XTQ_LINEAR_FORWARD) or with it (XTQ_LINEAR_TRAIN, never less), or of
- * xtq_linear_bwd_dev (XTQ_LINEAR_GRADIENT).
+ * xtq_linear_bwd_dev (XTQ_LINEAR_GRADIENT), for either type.
  */
 XTQ_API int64_t xtq_linear_ws_bytes(const xtq_weight* w, int rows, int what);
 XTQ_API int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t x_stride,
