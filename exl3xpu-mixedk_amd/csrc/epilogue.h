@@ -89,7 +89,10 @@ __device__ __forceinline__ Columns<N> load_columns(const Epilogue& ep, int col) 
 }
 
 // Scales, bias, activation and residual of N columns of a row, and their store
-// (v: transformed sums).
+// (v: transformed sums).  y comes of the unrounded z; the z that is kept for the
+// gradient has the activations' type, as they are kept themselves: a slope taken
+// at it is off by |z act''(z)| <= 0.32 times z's relative rounding, which adds 6 %
+// at most to the error that the gradient's own rounding leaves.
 template <int T, int N>
 __device__ __forceinline__ void finish_cols(const float* v, const Columns<N>& c, const Epilogue& ep, int row,
                                             int col) {

@@ -907,7 +907,7 @@ FewPlan few_plan(int rows, int k, int n, bool two) {
 }  // namespace
 
 size_t linear_ws_bytes(int rows, int k, int n, bool backward, bool two) {
-    if (backward) return many_plan(rows, n, k, true, false).total;
+    if (backward) return many_plan(rows, n, k, true, two).total;
     return takes_few(rows, n) ? few_plan(rows, k, n, two).total : many_plan(rows, k, n, false, two).total;
 }
 
@@ -940,7 +940,7 @@ hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_s
 
 hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long long dy_stride,
                              const void* z, int act, int rows, void* dx, long long dx_stride,
-                             void* dbias, int dbias_f32, void* ws, uint32_t* counters,
+                             void* dbias, int dbias_f32, bool two, void* ws, uint32_t* counters,
                              hipStream_t s) {
     (void)counters;
     const Source src{(const uint16_t*)dy, dy_stride, act == kActNone ? nullptr : (const uint16_t*)z, act,
@@ -952,8 +952,8 @@ hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long lon
     ep.y_stride = dx_stride;
     ep.rows = rows;
     ep.cols = w.k;
-    return type == kBf16 ? many<kBf16>(w, 1, src, ep, dbias, dbias_f32, false, ws, s)
-                         : many<kF16>(w, 1, src, ep, dbias, dbias_f32, false, ws, s);
+    return type == kBf16 ? many<kBf16>(w, 1, src, ep, dbias, dbias_f32, two, ws, s)
+                         : many<kF16>(w, 1, src, ep, dbias, dbias_f32, two, ws, s);
 }
 
 namespace {

@@ -39,7 +39,7 @@ struct Epilogue {
     int rows, cols;
 };
 
-// Whether a product's rows enter with 22 bits, as two fp16 terms, and not with
+// Whether a forward product's rows enter with 22 bits, as two fp16 terms, and not with
 // the 11 of one.  fp16: one rounding of the rows is as large as the result's own
 // (together 1.4 times the error of that alone), so only the result's is left.
 // bf16 results are rounded to 8 bits, beside which the rows' 11 do not show
@@ -53,12 +53,15 @@ struct Epilogue {
 // rows 722 : 1236).
 inline bool two_terms(int type, int act, bool fast) { return !fast && (type == kF16 || act == kActRelu); }
 
+// The same for a gradient's product: no slope is taken at what it gives.
+inline bool two_terms_gradient(int type, bool fast) { return !fast && type == kF16; }
+
 size_t linear_ws_bytes(int rows, int k, int n, bool backward, bool two);
 hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
                          const Epilogue& ep, bool two, void* ws, uint32_t* counters, hipStream_t s);
 hipError_t launch_linear_bwd(const Weight& w, int type, const void* dy, long long dy_stride,
                              const void* z, int act, int rows, void* dx, long long dx_stride,
-                             void* dbias, int dbias_f32, void* ws, uint32_t* counters,
+                             void* dbias, int dbias_f32, bool two, void* ws, uint32_t* counters,
                              hipStream_t s);
 
 // Products of up to kFewRows rows (few_kernels.hip), one function per K.  The

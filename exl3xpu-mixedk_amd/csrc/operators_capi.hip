@@ -117,6 +117,8 @@ int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy
     xtq::Weight wt;
     int rc = check_weight(w, &wt);
     if (rc) return rc;
+    const bool fast = type & XTQ_FAST;
+    type &= ~XTQ_FAST;
     if ((type != XTQ_BF16 && type != XTQ_F16) || act < XTQ_ACT_NONE || act > XTQ_ACT_GELU) return 15;
     if (rows <= 0 || rows > kMaxRows) return 6;
     if ((rc = check_rows(dy, dy_stride, wt.n))) return rc;
@@ -125,9 +127,10 @@ int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy
     if (act != XTQ_ACT_NONE && (!z || !aligned(z, 2))) return 12;
     if (!aligned(dbias, bias_f32 ? 4 : 2)) return 12;
     if (!counters || !aligned(counters, 4)) return 12;
-    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, true, false)))) return rc;
+    const bool two = xtq::two_terms_gradient(type, fast);
+    if ((rc = check_ws(ws, ws_bytes, xtq::linear_ws_bytes(rows, wt.k, wt.n, true, two)))) return rc;
     return status(xtq::launch_linear_bwd(wt, type, dy, dy_stride, z, act, rows, dx, dx_stride, dbias,
-                                         bias_f32, ws, counters, (hipStream_t)stream), "linear_bwd");
+                                         bias_f32, two, ws, counters, (hipStream_t)stream), "linear_bwd");
 }
 
 int xtq_moe_table(const xtq_weight* weights, int experts, xtq_moe_weight* table) {

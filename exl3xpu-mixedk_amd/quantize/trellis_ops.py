@@ -162,7 +162,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, bias, residual, w, act, fast):
         need = ctx.needs_input_grad[0] or (bias is not None and ctx.needs_input_grad[1])
         y, z = _forward(x, w, bias, act, residual, fast, need and act != 0)
-        ctx.w, ctx.act, ctx.shape = w, act, x.shape
+        ctx.w, ctx.act, ctx.fast, ctx.shape = w, act, fast, x.shape
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.save_for_backward(z)
         return y
@@ -189,7 +189,7 @@ class _Linear(torch.autograd.Function):
                 need = L.xtq_linear_ws_bytes(w._p, m, 1)
                 ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dy.device)
                 rc = L.xtq_linear_bwd_dev(
-                    w._p, _TYPES[dy.dtype], rows.data_ptr(), _stride(rows),
+                    w._p, _TYPES[dy.dtype] | ctx.fast, rows.data_ptr(), _stride(rows),
                     None if z is None else z.data_ptr(), ctx.act, m,
                     None if dx is None else dx.data_ptr(), w.k,
                     None if dbias is None else dbias.data_ptr(),
@@ -207,9 +207,10 @@ def linear(x: torch.Tensor, w: TrellisLinear, bias: torch.Tensor | None = None,
     fp32, residual y's shape and x's type.  Differentiable in x, bias and
     residual (once; the weight is frozen); the same result with a gradient and
     without.  x enters the product with 22 bits for float16 and for relu, and with
-    11 otherwise, which a bfloat16 result's 8 hide.  fast: with 11 bits always, at
-    half the matrix work: float16 results are then off by 1.4 times their own
-    rounding, and relu's gradient takes some slopes on the wrong side of zero."""
+    11 otherwise, which a bfloat16 result's 8 hide; the gradient's product likewise
+    (float16: 22).  fast: with 11 bits always, at half the matrix work: float16
+    results and gradients are then off by 1.4 times their own rounding, and relu's
+    gradient takes some slopes on the wrong side of zero."""
     if x.dtype not in _TYPES:
         raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
     if x.device != w.device:

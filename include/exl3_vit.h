@@ -371,6 +371,8 @@ XTQ_API int xtq_linear_dev(const xtq_weight* w, int type, const void* x, int64_t
  *   z      as the forward call wrote it (unused for XTQ_ACT_NONE)
  *   dx     or NULL (then only dbias is computed)
  *   dbias  [n] (out) fp32 or of the activations' type as bias_f32 says, or NULL
+ * dz enters the product with 22 bits for XTQ_F16, and with 11 for XTQ_BF16 or
+ * type | XTQ_FAST.
  */
 XTQ_API int xtq_linear_bwd_dev(const xtq_weight* w, int type, const void* dy, int64_t dy_stride,
                                const void* z, int act, int rows, void* dx, int64_t dx_stride,
