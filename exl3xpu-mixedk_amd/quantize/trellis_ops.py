@@ -26,6 +26,7 @@ import os
 import sys
 
 import torch
+import torch.autograd.forward_ad as _fad
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import hip_backend as _hb  # noqa: E402
@@ -132,6 +133,14 @@ def _like(t: torch.Tensor, x: torch.Tensor, shape, name: str, dtypes) -> None:
                          f"{x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
+def _no_tangents(name: str, *tensors) -> None:
+    """Raises for tensors that carry a forward-mode derivative: a kernel reads their
+    values alone, and the result's missing tangent would read as zero."""
+    if _fad._current_level >= 0 and any(t is not None and _fad.unpack_dual(t).tangent is not None
+                                        for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def _forward(x, w, bias, act, residual, fast, keep_z):
     rows = _rows(x, w.k)
     m = rows.shape[0]
@@ -171,6 +180,7 @@ class _Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         z, = ctx.saved_tensors
+        _no_tangents("linear's gradient", dy)
         w = ctx.w
         want_x, want_b, want_r = ctx.needs_input_grad[:3]
         dx = dbias = None
@@ -205,7 +215,7 @@ def linear(x: torch.Tensor, w: TrellisLinear, bias: torch.Tensor | None = None,
     """act(x W + bias) + residual for x [.., k] (bfloat16 or float16) -> [.., n]
     in x's type.  act: none, relu, silu or gelu (erf).  bias [n] has x's type or
     fp32, residual y's shape and x's type.  Differentiable in x, bias and
-    residual (once; the weight is frozen); the same result with a gradient and
+    residual (once, in reverse mode; the weight is frozen); the same result with a gradient and
     without.  x enters the product with 22 bits for float16 and for relu, and with
     11 otherwise, which a bfloat16 result's 8 hide; the gradient's product likewise
     (float16: 22).  fast: with 11 bits always, at half the matrix work: float16
@@ -218,6 +228,7 @@ def linear(x: torch.Tensor, w: TrellisLinear, bias: torch.Tensor | None = None,
     if x.dim() < 1 or x.shape[-1] != w.k:
         raise ValueError(f"x must be [.., {w.k}], got {tuple(x.shape)}")
     a, fast = _check_act(act), _FAST if fast else 0
+    _no_tangents("linear", x, bias, residual)
     if bias is not None:
         _like(bias, x, (w.n,), "bias", (x.dtype, torch.float32))
     if residual is not None:
@@ -283,6 +294,7 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     if valid is not None:
         _like(valid, x, x.shape[:-1], "valid", (torch.bool,))
         valid = valid.contiguous()
+    _no_tangents("moe", x, router, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, router, residual)):
         raise NotImplementedError("moe has no gradient: call it under torch.no_grad()")
     rows, router = _rows(x, d), router.contiguous()
@@ -325,6 +337,7 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
     if x.dim() < 1 or not x.shape[-1] or x.shape[-1] % 128:
         raise ValueError(f"x must be [.., k] with k a multiple of 128, got {tuple(x.shape)}")
     k = x.shape[-1]
+    _no_tangents("input_gram", x, prev, out)
     if x.requires_grad:
         x = x.detach()
     if valid is not None:
