@@ -329,7 +329,7 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
     float16) that valid [..] (bool) keeps, as fp32 [k, k]: the input Gram that
     quantize_linear takes as H_x.  Tokens left out may hold anything.  prev: the
     Gram so far (None: zero); out: where to write (prev itself accumulates in
-    place)."""
+    place).  No gradient."""
     if x.dtype not in _TYPES:
         raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
     if not x.is_cuda:
@@ -338,8 +338,8 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
         raise ValueError(f"x must be [.., k] with k a multiple of 128, got {tuple(x.shape)}")
     k = x.shape[-1]
     _no_tangents("input_gram", x, prev, out)
-    if x.requires_grad:
-        x = x.detach()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, prev, out)):
+        raise NotImplementedError("input_gram has no gradient: call it under torch.no_grad()")
     if valid is not None:
         _like(valid, x, x.shape[:-1], "valid", (torch.bool,))
         valid = valid.contiguous()

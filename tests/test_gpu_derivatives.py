@@ -61,3 +61,14 @@ def test_forward_mode_over_a_gradient_is_refused(xt):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, fad.make_dual(dy, dy), retain_graph=True)
         torch.autograd.grad(y, x, dy)
+
+
+@pytest.mark.parametrize("name", ("moe x", "moe router", "moe residual", "input_gram x", "input_gram prev",
+                                  "input_gram out"))
+def test_gradient_is_refused(xt, name):
+    value, call = _calls(xt)[name]
+    value = value.clone().requires_grad_()
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        call(value)
+    with torch.no_grad():
+        call(value)
