@@ -350,7 +350,8 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
                 raise ValueError(f"{name} must be contiguous")
     rows = _rows(x, k)
     m = rows.shape[0]
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(k, k, dtype=torch.float32, device=x.device)
     L = _hb.lib()
     with _on(x.device):
@@ -362,4 +363,6 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
                             None if prev is None else prev.data_ptr(), out.data_ptr(),
                             ws.data_ptr() if need else None, ws.numel(), _stream(x.device))
     _hb._check("xtq_gram_dev", rc)
+    if given and not out.is_inference():        # written behind autograd's back: whoever kept it has to know
+        torch.autograd.graph.increment_version(out)
     return out

@@ -72,3 +72,25 @@ def test_gradient_is_refused(xt, name):
         call(value)
     with torch.no_grad():
         call(value)
+
+
+def test_out_is_an_inplace_write_to_autograd(xt):
+    """A backward pass that kept the Gram so far has to find that it changed."""
+    x, gram = _half(3, 256), torch.zeros(256, 256, device="cuda")
+    scale = torch.ones(256, 256, device="cuda", requires_grad=True)
+    loss = (scale * gram).sum()
+    before = gram._version
+    xt.input_gram(x, prev=gram, out=gram)
+    assert gram._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    whole = torch.zeros(2, 256, 256, device="cuda")
+    loss = (scale * whole[0]).sum()
+    xt.input_gram(x, out=whole[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        kept = torch.zeros(256, 256, device="cuda")
+        assert xt.input_gram(x, prev=kept, out=kept) is kept
+        xt.input_gram(x, prev=gram, out=gram)
+    assert torch.equal(kept, xt.input_gram(x, out=kept))
