@@ -212,6 +212,10 @@ int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, int k, con
     int rc;
     if (rows && (rc = check_rows(x, x_stride, k))) return rc;
     if (!out || !aligned(out, 4) || !aligned(prev, 4)) return 12;
+    if (prev && prev != out) {          // an element would be read after another's place was written over it
+        const uintptr_t a = (uintptr_t)prev, b = (uintptr_t)out;
+        if ((a < b ? b - a : a - b) < (uintptr_t)k * k * 4) return 12;
+    }
     if ((rc = check_ws(ws, ws_bytes, xtq::gram_ws_bytes(rows, k)))) return rc;
     return status(xtq::launch_gram(type, x, x_stride, rows, k, valid, prev, out, ws,
                                    (hipStream_t)stream), "gram");

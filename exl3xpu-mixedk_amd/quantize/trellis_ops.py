@@ -348,6 +348,8 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
             _like(t, x, (k, k), name, (torch.float32,))
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
+    if prev is not None and out is not None and 0 < abs(prev.data_ptr() - out.data_ptr()) < 4 * k * k:
+        raise ValueError("prev and out must be one tensor's memory or apart")
     rows = _rows(x, k)
     m = rows.shape[0]
     given = out is not None

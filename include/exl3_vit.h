@@ -419,7 +419,7 @@ XTQ_API int xtq_moe_dev(const xtq_moe_weight* table, int experts, int d, int f, 
  * out = prev + X^T X, [k][k] fp32, over the rows of x [rows][k] whose valid byte
  * is not zero (all rows for valid NULL; the others are not looked at): the input
  * Gram that quantize_linear takes (quantize.py:750).  prev NULL: zero; it may be
- * out itself.  Zero rows give prev or zero.  At most 2^30 rows.
+ * out itself, but not overlap it otherwise (status 12).  Zero rows give prev or zero.  At most 2^30 rows.
  */
 XTQ_API int64_t xtq_gram_ws_bytes(int rows, int k);
 XTQ_API int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, int k,
