@@ -267,6 +267,15 @@ class TrellisExperts:
         _hb._check("xtq_moe_table", _hb.lib().xtq_moe_table(host, n, words.data_ptr()))
         self.n, self.table = n, words.to(self.device)
         self._code = _hb.code_name(self.code).encode()
+        self._rows: dict = {}               # by top_k: tokens that one call takes
+
+
+def _moe_rows(experts: int, top_k: int, d: int, f: int) -> int:
+    """The most tokens that a call of xtq_moe_dev takes: its workgroups count
+    themselves in XTQ_OP_COUNTERS words, which many experts' wide layers use up
+    before 64 tokens.  0: not even one."""
+    need = _hb.lib().xtq_moe_ws_bytes
+    return next((r for r in range(_MOE_ROWS, 0, -1) if need(r, experts, top_k, d, f) >= 0), 0)
 
 
 def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: int,
@@ -278,7 +287,8 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     type or fp32; renorm divides the weights by their sum.  Tokens that valid [..]
     (bool) leaves out are not looked at: their result is the residual or 0.
     return_routing: also the expert numbers int32 [.., top_k] (-1 where left out)
-    and weights fp32.  More than 64 tokens run 64 at a time.  No gradient."""
+    and weights fp32.  More than 64 tokens run 64 at a time, fewer where many
+    experts' wide layers take more counters than there are.  No gradient."""
     if x.dtype not in _TYPES:
         raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
     if x.device != experts.device:
@@ -297,6 +307,11 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     _no_tangents("moe", x, router, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, router, residual)):
         raise NotImplementedError("moe has no gradient: call it under torch.no_grad()")
+    most = experts._rows.get(top_k)
+    if most is None:
+        most = experts._rows[top_k] = _moe_rows(experts.n, top_k, d, experts.f)
+    if not most:
+        raise ValueError(f"{top_k} experts of {d} by {experts.f} a token are more than a call can count")
     rows, router = _rows(x, d), router.contiguous()
     res = None if residual is None else _rows(residual, d)
     m = rows.shape[0]
@@ -306,8 +321,8 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     L = _hb.lib()
     with _on(x.device):
         stream = _stream(x.device)
-        for r in range(0, m, _MOE_ROWS):
-            n = min(_MOE_ROWS, m - r)
+        for r in range(0, m, most):
+            n = min(most, m - r)
             need = L.xtq_moe_ws_bytes(n, experts.n, top_k, d, experts.f)
             ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
             rc = L.xtq_moe_dev(
