@@ -54,13 +54,14 @@ def _counter_words(dev: torch.device, stream: int) -> torch.Tensor:
     """The zeroed words a call counts its finished parts in: one set per stream,
     since calls on one stream never overlap (every call leaves them zero).  A
     captured call gets a set of its own, cleared inside the graph, because the
-    graph may be replayed on any stream."""
+    graph may be replayed on any stream; the caller keeps it until its kernels
+    are recorded."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(_COUNTERS, dtype=torch.int32, device=dev)
     key = (dev.index, stream)
     t = _counters.get(key)
-    if t is None:
-        t = _counters[key] = torch.zeros(_COUNTERS, dtype=torch.int32, device=dev)
+    if t is None:                       # (of two threads that come here at once, one's set stays)
+        t = _counters.setdefault(key, torch.zeros(_COUNTERS, dtype=torch.int32, device=dev))
     return t
 
 
@@ -154,6 +155,7 @@ def _forward(x, w, bias, act, residual, fast, keep_z):
     with _on(x.device):
         stream = _stream(x.device)
         need = L.xtq_linear_ws_bytes(w._p, m, 2 if keep_z else 0)
+        words = _counter_words(x.device, stream)
         ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
         rc = L.xtq_linear_dev(
             w._p, _TYPES[x.dtype] | fast, rows.data_ptr(), _stride(rows), m,
@@ -161,7 +163,7 @@ def _forward(x, w, bias, act, residual, fast, keep_z):
                                                            bias.dtype == torch.float32), act,
             None if res is None else res.data_ptr(), 0 if res is None else _stride(res),
             None if z is None else z.data_ptr(), y.data_ptr(), w.n, ws.data_ptr(), ws.numel(),
-            _counter_words(x.device, stream).data_ptr(), stream)
+            words.data_ptr(), stream)
     _hb._check("xtq_linear_dev", rc)
     return y, z
 
@@ -197,6 +199,7 @@ class _Linear(torch.autograd.Function):
             with _on(dy.device):
                 stream = _stream(dy.device)
                 need = L.xtq_linear_ws_bytes(w._p, m, 1)
+                words = _counter_words(dy.device, stream)
                 ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dy.device)
                 rc = L.xtq_linear_bwd_dev(
                     w._p, _TYPES[dy.dtype] | ctx.fast, rows.data_ptr(), _stride(rows),
@@ -204,7 +207,7 @@ class _Linear(torch.autograd.Function):
                     None if dx is None else dx.data_ptr(), w.k,
                     None if dbias is None else dbias.data_ptr(),
                     int(ctx.bias_dtype == torch.float32), ws.data_ptr(), ws.numel(),
-                    _counter_words(dy.device, stream).data_ptr(), stream)
+                    words.data_ptr(), stream)
             _hb._check("xtq_linear_bwd_dev", rc)
         return dx, dbias, dy if want_r else None, None, None, None
 
@@ -321,6 +324,7 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     L = _hb.lib()
     with _on(x.device):
         stream = _stream(x.device)
+        words = _counter_words(x.device, stream)        # (of all batches: they follow each other)
         for r in range(0, m, most):
             n = min(most, m - r)
             need = L.xtq_moe_ws_bytes(n, experts.n, top_k, d, experts.f)
@@ -333,7 +337,7 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
                 None if res is None else res.data_ptr() + 2 * r * _stride(res),
                 0 if res is None else _stride(res), y.data_ptr() + 2 * r * d, d,
                 ids.data_ptr() + 4 * r * top_k, weights.data_ptr() + 4 * r * top_k, ws.data_ptr(),
-                ws.numel(), _counter_words(x.device, stream).data_ptr(), stream)
+                ws.numel(), words.data_ptr(), stream)
             _hb._check("xtq_moe_dev", rc)
     return (y, ids, weights) if return_routing else y
 
