@@ -89,9 +89,13 @@ hipError_t few_launch(const Weight& w, const FewArgs& a, const Epilogue& ep, hip
     return hipGetLastError();
 }
 
+// (Rows and fragments are held against each other here once more: the kernels
+// themselves take them as they come.)
 template <int K, int CODE>
 hipError_t few_kc(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s) {
+    if (ep.rows > (a.frag ? 16 * a.groups : kFusedRows)) return hipErrorInvalidValue;
 #ifdef XTQ_FEW_TWO
+    if (!a.frag || !a.frag_lo) return hipErrorInvalidValue;
     if (a.groups == 1) return few_launch<K, CODE, 1, false, true>(w, a, ep, s);
     if (a.groups == 2) return few_launch<K, CODE, 2, false, true>(w, a, ep, s);
     return few_launch<K, CODE, 4, false, true>(w, a, ep, s);

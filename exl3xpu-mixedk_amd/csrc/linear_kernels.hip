@@ -881,7 +881,18 @@ bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_C
 // 17408, one row 27.6 : 27.2, sixteen 45.2 : 29.5).
 constexpr int kFewItems = 16;
 
-int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+constexpr int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+// The kernels read every place of their groups, so there is one for each row, in a
+// number that has a kernel; one group where the kernel transforms the rows.
+constexpr bool groups_fit() {
+    for (int r = 1; r <= kFewRows; ++r) {
+        const int g = few_groups(r);
+        if (16 * g < r || (g != 1 && g != 2 && g != 4) || (r <= kFusedRows && g != 1)) return false;
+    }
+    return true;
+}
+static_assert(groups_fit(), "groups of fragments that the kernels of few rows read");
 
 struct FewPlan {
     int splits, groups;
