@@ -1287,7 +1287,7 @@ const char* xtq_vit_strerror(int rc) {
         case 3: return "XTQ_VIT_DEVIDX names no device";
         case 4: return "HIP runtime error during a run";
         case 5: return "request exceeds XTQ_VIT_MAXBYTES or XTQ_VIT_DEV_MAXBYTES";
-        case 6: return "sequence count out of range (XTQ_VIT_MAXSEQ for host pointers)";
+        case 6: return "sizes or sequence count out of range (XTQ_VIT_MAXSEQ for host pointers)";
         case 8: return "unsupported code";
         case 9: return "unsupported K";
         case 10: return "pivot or margin out of range";
