@@ -327,8 +327,13 @@ XTQ_API int xtq_had128_both_dev(const float* d_h, const float* d_in, float* d_ou
  *     call; every call leaves them zero.  Not shared with a call that may run at
  *     the same time.
  *   - a NaN or an infinity in a row spreads over that row's results (as NaN,
- *     mostly: the transforms take differences), never to other rows'.
- *   - zero rows: nothing is enqueued, status 0.
+ *     mostly: the transforms take differences), never to other rows'.  Sums of
+ *     128 values are taken in fp32 before the scales svh: rows (times suh) and
+ *     results (over svh and scale) are taken up to 2^120; past it they may
+ *     overflow where the product itself does not (bf16 alone reaches so far).
+ *   - zero rows: nothing is enqueued, status 0, by xtq_linear_dev and xtq_moe_dev.
+ *     xtq_gram_dev then writes prev or zero; xtq_linear_bwd_dev takes one row at
+ *     least (status 6).
  */
 typedef struct xtq_weight {
     const int16_t* trellis;   /* [k/16][n/16][16K] device */
