@@ -18,14 +18,20 @@ namespace {
 // where the last one to arrive adds them in order and finishes the columns.
 // LO: with two terms.
 //
-// The decoding bounds it: 3.85 vector instructions a weight that issue at 33-37 T
-// lane-operations/s (mul1, K = 4) make 9.4 us of the 89 M weights of 17408 by
-// 5120, whose 44.6 MB a copy would move in 9.0; the loop takes that time, and
-// one row 23.5 us in all (48 rows at K = 3: 39.4).  The rest stands before and
-// after it, in cycles of 51,000: 8,200 until the rows are transformed and the
-// first weights there, 5,400 for the slowest wave and the waves' sums, 2,300 to
-// arrive, 4,200 to read the other workgroups' parts and finish.  Small weights
-// are all of that: 5120 by 5120 takes 12.6 us, 5120 by 1024 at K = 7 12.3.
+// The decoding bounds it.  One row of 17408 by 5120 at K = 4 (22.9 us; 44.6 MB that
+// a copy would move in 9.0) is 7.0 M wave instructions, 5.0 a weight, 3.85 of which
+// issue at 33-37 T lane-operations/s: 27,400 cycles of every SIMD, 12.3 us.  By
+// clocks of all waves, 51,000 cycles from a wave's start: 7,600 until the row is
+// transformed and the first weights lie in LDS (12,100 for the last wave), 31,000
+// more until the last wave has multiplied, 2,100 for the waves' sums, 1,000 to
+// store them, 1,800 to arrive, 3,100 to read the other workgroups' parts and
+// finish.  In the 31,000 the two workgroups of a compute unit
+// go one after the other more than side by side: the first is through its 8 blocks
+// at 14,300, the second at 32,400, and each then transforms the row's 4 further
+// blocks (few_slice) and starts its loads anew, 5,900 cycles that only the
+// neighbour's decoding can hide, and the last of them nothing.
+// 5120 by 5120 takes 12.6 us: 6,300 cycles (9,000) until the loop, 8,100 in it, 2,500,
+// 1,000 and 2,300 for sums, parts and arrival, 2,200 to finish.
 template <int K, int CODE, int G, bool FUSED, bool LO>
 __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void few_kernel(Weight w, FewArgs a, Epilogue ep) {
     constexpr int W = few_waves(G), N = 8 / W;

@@ -872,13 +872,17 @@ int few_splits(int rows, int k, int n, int waves) {
 }
 
 // (5120 by 5120, one launch or two against decoding apart: 17 rows 20 : 42 us, 64
-// rows 31 : 44; 5120 by 1024 20 : 30 and 27 : 32.)
+// rows 31 : 44; 5120 by 1024 20 : 30 and 27 : 32; with two terms 24 : 43, 35 : 43, 23 :
+// 34 and, at K = 7, whose 64 rows of two terms spill, 38 : 37.)
 bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_COUNTERS; }
 
 // Blocks of rows that a workgroup transforms itself at most, two a wave (us where
 // the product's workgroups transform, and in a launch before it: 5120 by 5120, one
 // row 14.0 : 15.4, four 15.4 : 16.0, six 17.6 : 16.5, sixteen 21.4 : 17.2; 5120 by
-// 17408, one row 27.6 : 27.2, sixteen 45.2 : 29.5).
+// 17408, one row 27.6 : 27.2, sixteen 45.2 : 29.5; with two terms 5120 by 5120, one
+// row 15.3 : 16.8, six 17.7 : 17.8, sixteen 22.0 : 19.2; 5120 by 17408 29.4 : 28.4,
+// 48.3 : 30.5.  These and few_splits' are graphs replayed, which clear the counters
+// before each product; the kernel of one row of 5120 by 5120 alone takes 12.6).
 constexpr int kFewItems = 16;
 
 constexpr int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
