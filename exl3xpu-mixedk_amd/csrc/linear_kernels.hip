@@ -743,8 +743,10 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 // splits of the summed dimension.  The choice is the shortest estimate, from what
 // the kernels measured: a workgroup's step takes 0.62 us (nb 4) or 0.38 (nb 2)
 // alone on a compute unit, two at once 0.72 and 0.46, and where a unit has more to
-// do than those, every two 0.84 and 0.64; parts are written and read at 4 TB/s.  (us with nb 4, nb 2: 5120 by 5120, 333 rows 67 : 56, 1000 rows 92 :
-// 107, 2047 rows 150 : 182; 5120 by 17408, 96 rows 101 : 84, 600 rows 176 : 205.)
+// do than those, every two 0.84 and 0.64; parts are written and read at 4 TB/s.  (us of
+// whole calls in replayed graphs with nb 4, nb 2: 5120 by 5120, 333 rows 67 : 56, 1000
+// rows 92 : 107, 2047 rows 150 : 182; 5120 by 17408, 96 rows 101 : 84, 600 rows 176 :
+// 205.)
 struct Tiling {
     int nb, tiles, splits;
 };
@@ -881,8 +883,9 @@ bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_C
 // row 14.0 : 15.4, four 15.4 : 16.0, six 17.6 : 16.5, sixteen 21.4 : 17.2; 5120 by
 // 17408, one row 27.6 : 27.2, sixteen 45.2 : 29.5; with two terms 5120 by 5120, one
 // row 15.3 : 16.8, six 17.7 : 17.8, sixteen 22.0 : 19.2; 5120 by 17408 29.4 : 28.4,
-// 48.3 : 30.5.  These and few_splits' are graphs replayed, which clear the counters
-// before each product; the kernel of one row of 5120 by 5120 alone takes 12.6).
+// 48.3 : 30.5.  These, few_splits' and takes_few's with two terms are graphs
+// replayed, which clear the counters before each product; the kernel of one row of
+// 5120 by 5120 alone takes 12.6).
 constexpr int kFewItems = 16;
 
 constexpr int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }

@@ -39,8 +39,8 @@ __device__ __forceinline__ void split_range(int pairs, int splits, int split, in
 
 // Rows of x for the first product, as fragments and what their rounding left,
 // one wave per chunk, weight (gate, up) and 128-column block.  (For one row the
-// product's workgroups do this themselves, each again: one launch less; us with and
-// without it, 2048 by 1024 and 4096 by 2048: one row 46 : 41 and 52 : 51, two 53 :
+// product's workgroups do this themselves, each again: one launch less; us of
+// whole layers in replayed graphs with and without it, 2048 by 1024 and 4096 by 2048: one row 46 : 41 and 52 : 51, two 53 :
 // 52 and 67 : 73, four 72 : 73 and 96 : 107.)  Latency bounds it: 8.9 us for 37 rows of 4096 and 4 of 32
 // experts.
 __global__ __launch_bounds__(256) void moe_x_kernel(MoeArgs a) {
