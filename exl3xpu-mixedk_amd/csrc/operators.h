@@ -1,6 +1,7 @@
 // operators.h -- internal launch interface of the operators on trellis-coded
-// weights (linear layer, mixture layer, input Gram).  The exported entry points
-// live in operators_capi.hip and are declared in include/exl3_vit.h.
+// weights (linear layer, mixture layer, input Gram) and of the norms around them.
+// The exported entry points live in operators_capi.hip and are declared in
+// include/exl3_vit.h.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -96,6 +97,43 @@ struct MoeArgs;
 size_t moe_ws_bytes(int rows, int experts, int top, int d, int f);
 size_t moe_counters(int rows, int experts, int top, int d, int f);
 hipError_t launch_moe(MoeArgs a, void* ws, hipStream_t s);
+
+// Norms of rows and the residual sum between blocks (norm_kernels.hip; the C-ABI's
+// numbers).  kind and post: the norm of y and of x before it, or none.
+enum NormKind { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
+enum GateAct { kGateNone = 0, kGateSigmoid = 1, kGateSilu = 2 };
+struct NormParam {
+    const void* p;                      // [d] or NULL
+    int f32;                            // fp32, else of the rows' type
+};
+struct NormArgs {
+    int rows, d, kind, post, gate_act;
+    float eps, post_eps, scale_number;  // the number scales where there is no tensor
+    NormParam weight, bias, scale, post_weight, post_bias;
+    const uint16_t *x, *res, *gate;     // res NULL: y is x, and not written
+    long long x_stride, res_stride, gate_stride;
+    uint16_t *y, *h;
+    long long y_stride, h_stride;
+    float* stats;                       // [rows][4] or NULL: mean and factor of x's norm, of y's
+};
+enum NormSumOf { kSumWeight, kSumBias, kSumScale, kSumPostWeight, kSumPostBias, kNormSums };
+struct NormSum {
+    void* p;                            // [d] or NULL
+    int f32;
+};
+struct NormGradArgs {
+    NormArgs f;
+    const uint16_t *dy, *dh;            // NULL: zero
+    long long dy_stride, dh_stride;
+    uint16_t *dx, *dres, *dgate;        // [rows][d] or NULL
+    NormSum dparam[kNormSums];
+    int place[kNormSums];               // of the sums in part
+    float* part;                        // [place][workgroup][d]
+};
+constexpr int kNormMaxD = 32768;        // 16 waves of four eights a lane
+hipError_t launch_norm(const NormArgs& a, int type, hipStream_t s);
+size_t norm_bwd_ws_bytes(int rows, int d, int sums);
+hipError_t launch_norm_bwd(NormGradArgs a, int type, void* ws, hipStream_t s);
 
 size_t gram_ws_bytes(int rows, int k);
 hipError_t launch_gram(int type, const void* x, long long x_stride, int rows, int k,

@@ -1,5 +1,5 @@
-// operators_capi.hip -- C entries of the operators on trellis weights (declared
-// in include/exl3_vit.h): arguments are checked on the host against everything
+// operators_capi.hip -- C entries of the operators on trellis weights and of the
+// norms around them (declared in include/exl3_vit.h): arguments are checked on the host against everything
 // the kernels assume, then the kernels are enqueued.  No state is kept between
 // calls and nothing is locked.
 #include <stdio.h>
@@ -58,6 +58,47 @@ bool moe_sizes(int rows, int experts, int top, int d, int f) {
            top <= xtq::kMoeTop && top <= experts && d > 0 && f > 0 && d % 128 == 0 && f % 128 == 0 &&
            d <= (1 << 20) && f <= (1 << 20) &&
            (rows == 0 || xtq::moe_counters(rows, experts, top, d, f) <= XTQ_OP_COUNTERS);
+}
+
+// A norm's structure and inputs, and what the kernels take of them.
+int check_norm(const xtq_norm* p, int type, int rows, int d, const void* x, int64_t x_stride, const void* res,
+               int64_t res_stride, const void* gate, int64_t gate_stride, xtq::NormArgs* out) {
+    if (!p) return 12;
+    if (type != XTQ_BF16 && type != XTQ_F16) return 15;
+    for (int k : {p->kind, p->post})
+        if (k < XTQ_NORM_NONE || k > XTQ_NORM_LAYER) return 15;
+    if (p->gate_act < XTQ_GATE_NONE || p->gate_act > XTQ_GATE_SILU) return 15;
+    if (!res && (!p->kind || p->post || gate || p->scale)) return 15;       // nothing that they would be of
+    if (d <= 0 || d > xtq::kNormMaxD || rows < 0 || rows > (1 << 30)) return 6;
+    xtq::NormArgs a{};
+    struct { const void* p; int bit; xtq::NormParam* to; } params[] = {
+        {p->weight, XTQ_NORM_WEIGHT_F32, &a.weight}, {p->bias, XTQ_NORM_BIAS_F32, &a.bias},
+        {p->scale, XTQ_NORM_SCALE_F32, &a.scale}, {p->post_weight, XTQ_NORM_POST_WEIGHT_F32, &a.post_weight},
+        {p->post_bias, XTQ_NORM_POST_BIAS_F32, &a.post_bias}};
+    for (auto& q : params) {
+        *q.to = xtq::NormParam{q.p, (p->f32 & q.bit) != 0};
+        if (!aligned(q.p, q.to->f32 ? 4 : 2)) return 12;
+    }
+    int rc;
+    if (rows && (rc = check_rows(x, x_stride, d))) return rc;
+    if (rows && res && (rc = check_rows(res, res_stride, d))) return rc;
+    if (rows && gate && (rc = check_rows(gate, gate_stride, d))) return rc;
+    a.rows = rows;
+    a.d = d;
+    a.kind = p->kind;
+    a.post = p->post;
+    a.gate_act = p->gate_act;
+    a.eps = p->eps;
+    a.post_eps = p->post_eps;
+    a.scale_number = p->scale_number;
+    a.x = (const uint16_t*)x;
+    a.x_stride = x_stride;
+    a.res = (const uint16_t*)res;
+    a.res_stride = res_stride;
+    a.gate = (const uint16_t*)gate;
+    a.gate_stride = gate_stride;
+    *out = a;
+    return 0;
 }
 
 }  // namespace
@@ -219,6 +260,66 @@ int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, int k, con
     if ((rc = check_ws(ws, ws_bytes, xtq::gram_ws_bytes(rows, k)))) return rc;
     return status(xtq::launch_gram(type, x, x_stride, rows, k, valid, prev, out, ws,
                                    (hipStream_t)stream), "gram");
+}
+
+int xtq_norm_dev(const xtq_norm* p, int type, int rows, int d, const void* x, int64_t x_stride, const void* res,
+                 int64_t res_stride, const void* gate, int64_t gate_stride, void* y, int64_t y_stride, void* h,
+                 int64_t h_stride, float* stats, void* stream) {
+    xtq::NormArgs a;
+    int rc = check_norm(p, type, rows, d, x, x_stride, res, res_stride, gate, gate_stride, &a);
+    if (rc) return rc;
+    if (rows == 0) return 0;
+    if (res && (rc = check_rows(y, y_stride, d))) return rc;
+    if (a.kind && (rc = check_rows(h, h_stride, d))) return rc;
+    if (!aligned(stats, 16)) return 12;
+    a.y = (uint16_t*)y;
+    a.y_stride = y_stride;
+    a.h = (uint16_t*)h;
+    a.h_stride = h_stride;
+    a.stats = stats;
+    return status(xtq::launch_norm(a, type, (hipStream_t)stream), "norm");
+}
+
+int64_t xtq_norm_bwd_ws_bytes(int rows, int d, int sums) {
+    if (d <= 0 || d > xtq::kNormMaxD || rows < 0 || rows > (1 << 30) || sums < 0 || sums > xtq::kNormSums) return -6;
+    return (int64_t)xtq::norm_bwd_ws_bytes(rows, d, sums);
+}
+
+int xtq_norm_bwd_dev(const xtq_norm* p, int type, int rows, int d, const void* x, int64_t x_stride, const void* res,
+                     int64_t res_stride, const void* gate, int64_t gate_stride, const float* stats, const void* dy,
+                     int64_t dy_stride, const void* dh, int64_t dh_stride, void* dx, void* dres, void* dgate,
+                     void* const dparam[5], void* ws, int64_t ws_bytes, void* stream) {
+    if (rows == 0) return 6;
+    xtq::NormGradArgs a{};
+    int rc = check_norm(p, type, rows, d, x, x_stride, res, res_stride, gate, gate_stride, &a.f);
+    if (rc) return rc;
+    if (!stats || !aligned(stats, 16) || !dparam) return 12;
+    if (dy && (rc = check_rows(dy, dy_stride, d))) return rc;
+    if (dh && (rc = check_rows(dh, dh_stride, d))) return rc;
+    if ((dy && !res) || (dh && !a.f.kind) || (dres && !res) || (dgate && !gate)) return 15;
+    if (!aligned(dx, 2) || !aligned(dres, 2) || !aligned(dgate, 2)) return 12;
+    // (what is not there has no gradient)
+    const bool there[] = {a.f.kind != 0, a.f.kind != 0, res != nullptr, a.f.post != 0, a.f.post != 0};
+    const int f32[] = {a.f.weight.f32, a.f.bias.f32, a.f.scale.f32, a.f.post_weight.f32, a.f.post_bias.f32};
+    int sums = 0;
+    for (int k = 0; k < xtq::kNormSums; ++k) {
+        if (!dparam[k]) continue;
+        if (!there[k]) return 15;
+        if (!aligned(dparam[k], f32[k] ? 4 : 2)) return 12;
+        a.dparam[k] = xtq::NormSum{dparam[k], f32[k]};
+        ++sums;
+    }
+    if (!dx && !dres && !dgate && !sums) return 12;
+    if ((rc = check_ws(ws, ws_bytes, xtq::norm_bwd_ws_bytes(rows, d, sums)))) return rc;
+    a.f.stats = const_cast<float*>(stats);
+    a.dy = (const uint16_t*)dy;
+    a.dy_stride = dy_stride;
+    a.dh = (const uint16_t*)dh;
+    a.dh_stride = dh_stride;
+    a.dx = (uint16_t*)dx;
+    a.dres = (uint16_t*)dres;
+    a.dgate = (uint16_t*)dgate;
+    return status(xtq::launch_norm_bwd(a, type, ws, (hipStream_t)stream), "norm_bwd");
 }
 
 }  // extern "C"

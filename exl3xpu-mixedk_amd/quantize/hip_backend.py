@@ -43,6 +43,15 @@ class TrellisWeight(ctypes.Structure):
                 ("K", ctypes.c_int32), ("code", ctypes.c_char_p)]
 
 
+class NormParams(ctypes.Structure):
+    """xtq_norm of include/exl3_vit.h."""
+    _fields_ = [("kind", ctypes.c_int32), ("post", ctypes.c_int32), ("gate_act", ctypes.c_int32),
+                ("f32", ctypes.c_int32), ("eps", ctypes.c_float), ("post_eps", ctypes.c_float),
+                ("scale_number", ctypes.c_float), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("post_weight", ctypes.c_void_p),
+                ("post_bias", ctypes.c_void_p)]
+
+
 def lib():
     """Load libexl3vit.so once; raises if it has not been built."""
     global _LIB
@@ -90,6 +99,12 @@ def lib():
         L.xtq_gram_ws_bytes.argtypes = [i32, i32]
         L.xtq_gram_ws_bytes.restype = ll
         L.xtq_gram_dev.argtypes = [i32, vp, ll, i32, i32, vp, vp, vp, vp, ll, vp]
+        np_ = ctypes.POINTER(NormParams)
+        L.xtq_norm_dev.argtypes = [np_, i32, i32, i32, vp, ll, vp, ll, vp, ll, vp, ll, vp, ll, vp, vp]
+        L.xtq_norm_bwd_ws_bytes.argtypes = [i32, i32, i32]
+        L.xtq_norm_bwd_ws_bytes.restype = ll
+        L.xtq_norm_bwd_dev.argtypes = [np_, i32, i32, i32, vp, ll, vp, ll, vp, ll, vp, vp, ll, vp, ll, vp,
+                                       vp, vp, vp, vp, ll, vp]
         L.xtq_vit_scratch_per_seq.argtypes = [i32]
         L.xtq_vit_scratch_per_seq.restype = i64
         L.xtq_vit_chunk_seqs.argtypes = [i32, i32, ctypes.POINTER(ctypes.c_int)]
@@ -109,7 +124,8 @@ def lib():
                    "xtq_trellis_unpack_dev", "xtq_trellis_pack64_dev",
                    "xtq_trellis_unpack64_dev", "xtq_vit_get_lut", "xtq_had128_left_dev",
                    "xtq_had128_right_dev", "xtq_had128_both_dev", "xtq_linear_dev",
-                   "xtq_linear_bwd_dev", "xtq_gram_dev", "xtq_moe_table", "xtq_moe_dev"):
+                   "xtq_linear_bwd_dev", "xtq_gram_dev", "xtq_moe_table", "xtq_moe_dev",
+                   "xtq_norm_dev", "xtq_norm_bwd_dev"):
             getattr(L, fn).restype = i32
         _LIB = L
     return _LIB

@@ -387,3 +387,145 @@ def input_gram(x: torch.Tensor, valid: torch.Tensor | None = None,
     if given and not out.is_inference():        # written behind autograd's back: whoever kept it has to know
         torch.autograd.graph.increment_version(out)
     return out
+
+
+NORMS = {None: 0, "rms": 1, "layer": 2}
+GATES = {"none": 0, "sigmoid": 1, "silu": 2}
+_MAX_D = 32768
+_PARAMS = ("weight", "bias", "scale", "post_weight", "post_bias")
+
+
+def _norm_rows(t, d):
+    """Address and stride of rows (None: none)."""
+    return (None, 0) if t is None else (t.data_ptr(), _stride(t))
+
+
+def _norm_struct(cfg, params):
+    kind, post, gate_act, eps, post_eps, number = cfg
+    f32 = sum(1 << i for i, p in enumerate(params) if p is not None and p.dtype == torch.float32)
+    return _hb.NormParams(kind, post, gate_act, f32, eps, post_eps, number,
+                          *(None if p is None else p.data_ptr() for p in params))
+
+
+def _norm_forward(x, res, gate, params, cfg, keep):
+    d = x.shape[-1]
+    y = None if res is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if cfg[0] else None
+    rows = _rows(x, d)
+    m = rows.shape[0]
+    stats = torch.empty(m, 4, dtype=torch.float32, device=x.device) if keep else None
+    if m == 0:
+        return y, h, stats
+    res, gate = (None if t is None else _rows(t, d) for t in (res, gate))
+    params = [None if p is None else p.contiguous() for p in params]
+    with _on(x.device):
+        rc = _hb.lib().xtq_norm_dev(
+            ctypes.byref(_norm_struct(cfg, params)), _TYPES[x.dtype], m, d, *_norm_rows(rows, d),
+            *_norm_rows(res, d), *_norm_rows(gate, d), None if y is None else y.data_ptr(), d,
+            None if h is None else h.data_ptr(), d, None if stats is None else stats.data_ptr(),
+            _stream(x.device))
+    _hb._check("xtq_norm_dev", rc)
+    return y, h, stats
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, res, gate, weight, bias, scale, post_weight, post_bias, cfg):
+        params = (weight, bias, scale, post_weight, post_bias)
+        y, h, stats = _norm_forward(x, res, gate, params, cfg, True)
+        ctx.cfg = cfg
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, res, gate, *params, stats)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        x, res, gate, *params, stats = ctx.saved_tensors
+        _no_tangents("the norm's gradient", dy, dh)
+        want = ctx.needs_input_grad[:8]
+        d = x.shape[-1]
+        rows = _rows(x, d)
+        m = rows.shape[0]
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if w else None
+                 for w, t in zip(want, (x, res, gate, *params))]
+        if m == 0:
+            return (*(g if g is None else g.zero_() for g in grads), None)
+        res, gate, dy, dh = (None if t is None else _rows(t, d) for t in (res, gate, dy, dh))
+        params = [None if p is None else p.contiguous() for p in params]
+        L = _hb.lib()
+        out = [None if g is None else g.data_ptr() for g in grads]
+        with _on(x.device):
+            need = L.xtq_norm_bwd_ws_bytes(m, d, sum(p is not None for p in out[3:]))
+            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+            rc = L.xtq_norm_bwd_dev(
+                ctypes.byref(_norm_struct(ctx.cfg, params)), _TYPES[x.dtype], m, d, *_norm_rows(rows, d),
+                *_norm_rows(res, d), *_norm_rows(gate, d), stats.data_ptr(), *_norm_rows(dy, d),
+                *_norm_rows(dh, d), *out[:3], (ctypes.c_void_p * 5)(*out[3:]), ws.data_ptr(), ws.numel(),
+                _stream(x.device))
+        _hb._check("xtq_norm_bwd_dev", rc)
+        return (*grads, None)
+
+
+def _norm(name, x, res, gate, params, kind, post, gate_act, eps, post_eps, number):
+    if x.dtype not in _TYPES:
+        raise ValueError(f"{name}'s rows must be bfloat16 or float16, got {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{name}'s rows must be a HIP device tensor, got {x.device}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MAX_D:
+        raise ValueError(f"{name}'s rows must be [.., 1 to {_MAX_D}], got {tuple(x.shape)}")
+    for t, what in ((res, "residual"), (gate, "gate")):
+        if t is not None:
+            _like(t, x, x.shape, what, (x.dtype,))
+    for t, what in zip(params, _PARAMS):
+        if t is not None:
+            _like(t, x, x.shape[-1:], what, (x.dtype, torch.float32))
+    for k in (kind, post):
+        if k not in NORMS:
+            raise ValueError(f"norm {k!r} not in {tuple(NORMS)}")
+    if gate_act not in GATES:
+        raise ValueError(f"gate_act {gate_act!r} not in {tuple(GATES)}")
+    if not (eps >= 0 and post_eps >= 0):
+        raise ValueError(f"eps must be at least 0, got {eps}, {post_eps}")
+    if (kind is None and any(t is not None for t in params[:2])) or \
+            (post is None and any(t is not None for t in params[3:])):
+        raise ValueError("weights and biases are of a norm that there is")
+    tensors = (x, res, gate, *params)
+    _no_tangents(name, *tensors)
+    cfg = (NORMS[kind], NORMS[post], GATES[gate_act], float(eps), float(post_eps), float(number))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return _Norm.apply(*tensors, cfg)
+    return _norm_forward(x, res, gate, params, cfg, False)[:2]
+
+
+def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+         kind: str = "rms", eps: float = 1e-6) -> torch.Tensor:
+    """The norm of each row of x [.., d] (bfloat16 or float16, d up to 32768), in x's
+    type: (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias for "layer", the
+    same without the mean for "rms".  weight and bias [d] have x's type or fp32 (None:
+    1 and 0).  Differentiable in all three (once, in reverse mode).  A row's result is
+    the same whatever rows are beside it."""
+    if kind is None:
+        raise ValueError("kind must be 'rms' or 'layer'")
+    return _norm("norm", x, None, None, (weight, bias, None, None, None), kind, None, "none", eps, eps, 1.0)[1]
+
+
+def residual_norm(block: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
+                  bias: torch.Tensor | None = None, kind: str | None = "rms", eps: float = 1e-6,
+                  gate: torch.Tensor | None = None, gate_act: str = "none", scale=None,
+                  post: str | None = None, post_weight: torch.Tensor | None = None,
+                  post_bias: torch.Tensor | None = None, post_eps: float | None = None):
+    """What lies between two blocks, in one pass: with p the post norm of the block's
+    result (post: "rms", "layer" or None: the result itself),
+        y = residual + scale * act(gate) * p,    h = norm(y, weight, bias, kind, eps),
+    returned as (y, h), h None for kind None.  block, residual and gate [.., d] have one
+    shape and type; gate_act: none (the gate itself), sigmoid or silu; scale is a number
+    or [d]; scale, weights and biases [d] have the block's type or fp32.  h comes of y
+    before y is rounded.  Differentiable in every tensor (once, in reverse mode)."""
+    number = 1.0
+    if scale is not None and not isinstance(scale, torch.Tensor):
+        number, scale = float(scale), None
+    if not isinstance(residual, torch.Tensor):
+        raise ValueError("residual must be a tensor")
+    return _norm("residual_norm", block, residual, gate, (weight, bias, scale, post_weight, post_bias), kind,
+                 post, gate_act, eps, eps if post_eps is None else post_eps, number)

@@ -432,6 +432,60 @@ XTQ_API int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, in
                          int64_t ws_bytes, void* stream);
 
 /*
+ * Norms of rows, and the residual sum between two blocks.  Of a block's result x,
+ * its residual res, gate and scale, all rows [rows][d]:
+ *   p = post norm of x (or x),  y = res + scale * ga(gate) * p,  h = norm of y,
+ * where the norm of t is (t - mean) / sqrt(mean of (t - mean)^2 + eps) * weight +
+ * bias, with mean = 0 for XTQ_NORM_RMS.  res NULL: y is x itself and is not written
+ * (the plain norm; post is XTQ_NORM_NONE then, gate and scale NULL).
+ *   kind, post   XTQ_NORM_*; kind XTQ_NORM_NONE: no h
+ *   gate         or NULL (factor 1); gate_act: XTQ_GATE_NONE (the gate itself),
+ *                XTQ_GATE_SIGMOID or XTQ_GATE_SILU of it
+ *   scale        [d], or NULL: scale_number for all channels
+ *   weight, bias, post_weight, post_bias   [d] or NULL (1 and 0)
+ *   f32          bits XTQ_NORM_*_F32: that parameter is fp32, else of the rows' type
+ *   stats        [rows][4] fp32 (out), 16-byte aligned, for xtq_norm_bwd_dev; or NULL
+ * Stream-ordered, as the operators above are, with their types and strides; no
+ * scratch, no counters.  Sums are fp32 and in an order that d alone fixes, so a row's
+ * results do not depend on the other rows; h comes of y before y is rounded.  Squares
+ * are fp32: rows are taken up to 2^63.  d up to 32,768, at most 2^30 rows; zero
+ * rows: nothing is enqueued.
+ */
+enum { XTQ_NORM_NONE = 0, XTQ_NORM_RMS = 1, XTQ_NORM_LAYER = 2 };
+enum { XTQ_GATE_NONE = 0, XTQ_GATE_SIGMOID = 1, XTQ_GATE_SILU = 2 };
+enum { XTQ_NORM_WEIGHT_F32 = 1, XTQ_NORM_BIAS_F32 = 2, XTQ_NORM_SCALE_F32 = 4,
+       XTQ_NORM_POST_WEIGHT_F32 = 8, XTQ_NORM_POST_BIAS_F32 = 16 };
+typedef struct xtq_norm {
+    int32_t kind, post, gate_act, f32;
+    float eps, post_eps, scale_number;
+    const void *weight, *bias, *scale, *post_weight, *post_bias;
+} xtq_norm;
+
+XTQ_API int xtq_norm_dev(const xtq_norm* p, int type, int rows, int d, const void* x,
+                         int64_t x_stride, const void* res, int64_t res_stride, const void* gate,
+                         int64_t gate_stride, void* y, int64_t y_stride, void* h,
+                         int64_t h_stride, float* stats, void* stream);
+
+/*
+ * Gradients of xtq_norm_dev: of the inputs as they were given to it, its stats, and
+ * the gradients of its results.
+ *   dy, dh             [rows][d], or NULL: zero
+ *   dx, dres, dgate    [rows][d] contiguous (out), each or NULL
+ *   dparam             gradients [d] (out) of weight, bias, scale, post_weight and
+ *                      post_bias, in this order, each or NULL, fp32 or of the rows'
+ *                      type as p->f32 says of the parameter
+ * ws: xtq_norm_bwd_ws_bytes of the number of dparam's entries that are not NULL.
+ * Sums over rows are fp32, in an order that rows and d fix.  Zero rows: status 6.
+ */
+XTQ_API int64_t xtq_norm_bwd_ws_bytes(int rows, int d, int sums);
+XTQ_API int xtq_norm_bwd_dev(const xtq_norm* p, int type, int rows, int d, const void* x,
+                             int64_t x_stride, const void* res, int64_t res_stride,
+                             const void* gate, int64_t gate_stride, const float* stats,
+                             const void* dy, int64_t dy_stride, const void* dh,
+                             int64_t dh_stride, void* dx, void* dres, void* dgate,
+                             void* const dparam[5], void* ws, int64_t ws_bytes, void* stream);
+
+/*
  * Copies the fp32 decode table of `code` (65536 entries) into host memory
  * (the values get_lut returns, quantize.py:90-97).
  */
