@@ -1,0 +1,526 @@
+// gated_kernels.hip -- the gated projection act(x Wg + bg) (x Wu + bu) on two trellis
+// weights for many rows, and its gradient.
+//
+// Forward: the columns of both weights lie in one operand, 128 of gate beside 128 of
+// up, so that a tile of 256 columns holds both factors of 128 results: its waves hand
+// each other what they need in LDS, and only the product leaves.  Each weight has its
+// own row signs and scales, so the rows come in two transforms, and a wave reads that
+// of its own weight.
+//
+// Gradient: with dg = dy zu act'(zg), du = dy act(zg), dx = dg Wg^T + du Wu^T is one
+// product over both weights' columns one after the other, in parts that lie in one
+// weight each: the parts are transformed apart and added.
+#include "few_device.h"
+#include "product_device.h"
+
+#pragma clang fp contract(off)
+
+namespace xtq {
+namespace {
+
+// Fused epilogue or parts for gated_join_kernel.
+enum GatedOut { kGatedFinish, kGatedParts };
+
+struct GatedGemm {
+    const uint16_t* A;                  // both weights, 8 groups of one, 8 of the other
+    const uint16_t *B[2], *B2[2];       // the rows transformed for each; second terms
+    const int32_t* rowexp[2];
+    int nb, gb;                         // blocks of 128 columns, groups of 16 rows
+    int steps, tiles, splits;
+    float* part;                        // [splits][2 nb][gb][8][64][4]
+};
+
+template <int T>
+__device__ __forceinline__ void role_columns(Columns<4> (&c)[8], const GatedArgs& a, int role, int blk, int lane) {
+    Epilogue ep{};
+    ep.colscale = a.w[role].svh;
+    ep.scale = a.w[role].scale;
+    ep.bias = a.bias[role];
+    ep.bias_f32 = a.bias_f32[role];
+    unit_columns<T>(c, ep, blk, lane);
+}
+
+// Transform, scales and bias of a unit of one weight, in place, and its z's store.
+__device__ __forceinline__ void finish_role(f4* v, const Columns<4> (&c)[8], const GatedArgs& a, const GatedGemm& g,
+                                            int role, int grp, int blk, int lane) {
+    transform_unit(v);
+    const int row = grp * 16 + (lane & 15), e = g.rowexp[role][row];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = ldexpf(v[j][i], e) * c[j].scale[i] + c[j].bias[i];
+    if (a.z && row < a.rows) {
+        float* z = a.z + ((size_t)role * a.rows + row) * a.w[0].n + blk * 128 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *(f4_a4*)(z + 16 * j) = v[j];
+    }
+}
+
+// act(gate) up of a unit, and its store.
+template <int T>
+__device__ __forceinline__ void store_gated(const f4* gate, const f4* up, const GatedArgs& a, int grp, int blk,
+                                            int lane) {
+    const int row = grp * 16 + (lane & 15);
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float o[4] = {gate[j][0], gate[j][1], gate[j][2], gate[j][3]};
+        activate<4>(o, a.act);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= up[j][i];
+        store16<T, 4>(a.y + (size_t)row * a.y_stride + blk * 128 + 16 * j + 4 * (lane >> 4), o);
+    }
+}
+
+// The product of fragments (gemm_kernel of linear_kernels.hip) with each wave's rows
+// those of its weight.
+template <int T, int OUT, int NB, int TERMS>
+__global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedArgs a) {
+    constexpr int kFrags = 16 + 4 * NB * TERMS, kOwn = 4 + NB * TERMS;
+    constexpr int kBuffers = kFrags > 24 ? 2 : 3;
+    __shared__ __align__(1024) uint8_t lds[kBuffers][kFrags * kFragBytes];
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), role = wv & 1, wm = wv >> 1;
+    const int tile = xcd_order(blockIdx.x, g.tiles);
+    const int mt = (g.gb + 2 * NB - 1) / (2 * NB), band = tile / (g.nb * kBand);
+    const int high = mt - band * kBand < kBand ? mt - band * kBand : kBand, in = tile - band * g.nb * kBand;
+    const int tn = in / high, tm = band * kBand + in - tn * high;
+    const int split = blockIdx.y;
+    const int s0 = (int)((long long)g.steps * split / g.splits);
+    const int s1 = (int)((long long)g.steps * (split + 1) / g.splits);
+
+    // this wave's fragments of a step: a quarter of A's 16 and of each B's 2 NB
+    const uint16_t* fa = g.A + (size_t)tn * g.steps * 8192 + wv * 2048 + lane * 8;
+    const int gb0 = tm * 2 * NB;        // first group of rows
+    const size_t at_b = ((size_t)(gb0 >> 4) * g.steps * 16 + (gb0 & 15) + wv * (NB / 2)) * 512 + lane * 8;
+    auto load = [&](int s) {
+        uint8_t* l = lds[(s - s0) % kBuffers];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_global_load_lds((global_void*)(fa + (size_t)s * 8192 + i * 512),
+                                             (lds_void*)(l + (wv * 4 + i) * kFragBytes), 16, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+                for (int i = 0; i < NB / 2; ++i)
+                    __builtin_amdgcn_global_load_lds(
+                        (global_void*)((t ? g.B2[r] : g.B[r]) + at_b + (size_t)s * 8192 + i * 512),
+                        (lds_void*)(l + (16 + 2 * NB * (r * TERMS + t) + wv * (NB / 2) + i) * kFragBytes), 16, 0, 0);
+    };
+    // All waves' pieces of the next step are in LDS, and all waves have read this
+    // one (their reads were waited for before they came here).
+    auto meet_up = [&](bool more) {
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kOwn) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    f4 acc[8][NB];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[j][b] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kAhead = kBuffers - 1;        // steps on their way beside the one that is multiplied
+    load(s0);
+    if (kAhead > 1 && s0 + 1 < s1) load(s0 + 1);
+    meet_up(kAhead > 1 && s0 + 1 < s1);
+    for (int s = s0; s < s1; ++s) {
+        if (s + kAhead < s1) load(s + kAhead);
+        u4 fr[8], b[TERMS][NB];
+        const uint8_t* l = lds[(s - s0) % kBuffers] + lane * 16;
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                b[t][i] = *(const u4*)(l + (16 + 2 * NB * (role * TERMS + t) + wm * NB + i) * kFragBytes);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) fr[j] = *(const u4*)(l + (role * 8 + j) * kFragBytes);
+        __builtin_amdgcn_sched_barrier(0);      // all reads under way before the first product
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+                for (int i = 0; i < NB; ++i) acc[j][i] = mfma<false>(fr[j], b[t][i], acc[j][i]);
+        __builtin_amdgcn_sched_barrier(0);      // none after the others have met
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        meet_up(kAhead > 1 && s + kAhead < s1);
+    }
+    if constexpr (OUT == kGatedParts) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int grp = gb0 + wm * NB + b;
+            if (grp >= g.gb) continue;
+            f4* o = (f4*)g.part + (((size_t)split * 2 * g.nb + 2 * tn + role) * g.gb + grp) * 512 + lane;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j * 64] = acc[j][b];
+        }
+        return;
+    }
+    // Of each two units a wave keeps one and gives the other's factor to the wave of
+    // the other weight.  (Rows past the last group are finished like others, from what
+    // their places hold, and not stored; the exponents' places are there for all of
+    // a tile's groups.)
+    Columns<4> cols[8];
+    role_columns<T>(cols, a, role, tn, lane);
+    f4* const give = (f4*)lds + (size_t)wv * (NB / 2) * 512 + lane;
+    const f4* const take = (const f4*)lds + (size_t)(wv ^ 1) * (NB / 2) * 512 + lane;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        f4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = acc[j][b];
+        finish_role(v, cols, a, g, role, gb0 + wm * NB + b, tn, lane);
+        // wave `role` keeps units b with b % 2 == role
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if ((b & 1) != role) give[(b >> 1) * 512 + j * 64] = v[j];
+            else acc[j][b & ~1] = v[j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; b += 2) {
+        f4 mine[8], other[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            mine[j] = acc[j][b];
+            other[j] = take[(b >> 1) * 512 + j * 64];
+        }
+        const int grp = gb0 + wm * NB + b + role;
+        if (role == 0) store_gated<T>(mine, other, a, grp, tn, lane);
+        else store_gated<T>(other, mine, a, grp, tn, lane);
+    }
+}
+
+// Joins the splits' parts of both weights, a workgroup of one wave one unit.
+template <int T>
+__global__ __launch_bounds__(64) void gated_join_kernel(GatedGemm g, GatedArgs a) {
+    const int lane = threadIdx.x, grp = blockIdx.x, blk = blockIdx.y;
+    const Gemm parts{nullptr, nullptr, nullptr, 16 * g.nb, g.gb, g.steps, g.tiles, g.splits, g.part, nullptr, nullptr, 0};
+    f4 v[2][8];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        sum_splits<4>(v[r], parts, grp, 2 * blk + r, lane, 0, g.splits);
+        Columns<4> cols[8];
+        role_columns<T>(cols, a, r, blk, lane);
+        finish_role(v[r], cols, a, g, r, grp, blk, lane);
+    }
+    store_gated<T>(v[0], v[1], a, grp, blk, lane);
+}
+
+// ------------------------------------------------------------------ gradient
+struct GatedSource {
+    const uint16_t* dy;
+    long long dy_stride;
+    const float* z;                     // [2][rows][n]
+    const uint16_t* svh[2];
+    int type, act, rows, n;
+};
+
+// Eight values of dg and du of a row.
+__device__ __forceinline__ void gated_slopes(const GatedSource& s, size_t row, int col, float* dg, float* du) {
+    float d[8];
+    unpack8(*(const u4_a2*)(s.dy + row * (size_t)s.dy_stride + col), s.type, d);
+    const float* zg = s.z + row * (size_t)s.n + col;
+    const float* zu = zg + (size_t)s.rows * s.n;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const f4 a = *(const f4_a4*)(zg + 4 * h), b = *(const f4_a4*)(zu + 4 * h);
+        float v[4] = {a[0], a[1], a[2], a[3]};
+        activate<4>(v, s.act);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            dg[4 * h + i] = d[4 * h + i] * b[i] * act_slope(a[i], s.act);
+            du[4 * h + i] = d[4 * h + i] * v[i];
+        }
+    }
+}
+
+// As row_exponents of linear_kernels.hip, for both weights' rows at once.
+__global__ __launch_bounds__(256) void gated_exponents_kernel(GatedSource s, int32_t* __restrict__ shift,
+                                                              int32_t* __restrict__ rowexp, int places) {
+    __shared__ float part[2][4];
+    const int row = blockIdx.x;
+    float top[2] = {0.0f, 0.0f};
+    for (int c = threadIdx.x * 8; c < s.n; c += 2048) {
+        float v[2][8];
+        gated_slopes(s, row, c, v[0], v[1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float t[8];
+            unpack8(*(const u4_a2*)(s.svh[r] + c), kF16, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top[r] = fmaxf(top[r], fabsf(v[r][i] * t[i]));
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        top[r] = wave_max(top[r]);
+        if ((threadIdx.x & 63) == 0) part[r][threadIdx.x >> 6] = top[r];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const float* p = part[threadIdx.x];
+        const int sh = shift_to(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), 7);
+        shift[threadIdx.x * places + row] = sh;
+        rowexp[threadIdx.x * places + row] = -sh - 7;
+    }
+}
+
+// dg's and du's rows to fragments, one behind the other in the summed dimension, a
+// wave 16 rows of one 128-column block of both; the biases' gradients' sums beside.
+__global__ __launch_bounds__(256) void gated_transform_kernel(GatedSource s, const int32_t* __restrict__ shift,
+                                                              int places, uint16_t* __restrict__ frags,
+                                                              uint16_t* __restrict__ rest,
+                                                              float* __restrict__ colsum) {
+    const int lane = threadIdx.x & 63, nblk = s.n / 128;
+    const int blk = blockIdx.x * 4 + (threadIdx.x >> 6), grp = blockIdx.y;
+    if (blk >= nblk) return;
+    const int q = lane >> 4, row = grp * 16 + (lane & 15);
+    float v[2][32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0.0f;
+    if (row < s.rows) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) gated_slopes(s, row, 128 * blk + 32 * p + 8 * q, v[0] + 8 * p, v[1] + 8 * p);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        if (colsum) rows_sum(v[r], lane, colsum + ((size_t)grp * 2 + r) * s.n + 128 * blk);
+        if (!frags) continue;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            float c[8];
+            unpack8(*(const u4_a2*)(s.svh[r] + 128 * blk + 32 * p + 8 * q), kF16, c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[r][8 * p + i] *= c[i];
+        }
+        rows_to_frags(v[r], row < s.rows ? shift[r * places + row] : 0, lane, grp, 4 * (r * nblk + blk), 8 * nblk, frags,
+                      rest);
+    }
+}
+
+__global__ __launch_bounds__(256) void gated_column_sums_kernel(ColSum a) {
+    __shared__ float part[256];
+    column_sums(a, blockIdx.x, part);
+}
+
+// dx's units: each weight's parts added and transformed, times its scales, and both added.
+template <int T>
+__global__ __launch_bounds__(64) void gated_dx_kernel(Gemm g, GatedGradArgs a, const int32_t* __restrict__ rowexp,
+                                                      int places) {
+    const int lane = threadIdx.x, grp = blockIdx.x, blk = blockIdx.y, row = grp * 16 + (lane & 15);
+    f4 v[2][8];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        sum_splits<4>(v[r], g, grp, blk, lane, r * (g.splits / 2), (r + 1) * (g.splits / 2));
+        transform_unit(v[r]);
+        Epilogue ep{};
+        ep.colscale = a.w[r].suh;
+        ep.scale = a.w[r].scale;
+        Columns<4> cols[8];
+        unit_columns<T>(cols, ep, blk, lane);
+        const int e = row < a.rows ? rowexp[r * places + row] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][j][i] = ldexpf(v[r][j][i], e) * cols[j].scale[i];
+    }
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const f4 t = v[0][j] + v[1][j];
+        const float o[4] = {t[0], t[1], t[2], t[3]};
+        store16<T, 4>(a.dx + (size_t)row * a.dx_stride + blk * 128 + 16 * j + 4 * (lane >> 4), o);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+struct Taker {
+    size_t at = 0;
+    size_t operator()(size_t bytes) {
+        const size_t a = at;
+        at += align256(bytes);
+        return a;
+    }
+};
+
+struct FewPlan {
+    int groups, splits;
+    bool apart;
+    size_t part, frag, rest, shift, total;
+};
+
+bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_COUNTERS; }
+
+FewPlan few_plan(int rows, int k, int n, bool two) {
+    FewPlan p;
+    p.groups = few_groups(rows);
+    p.splits = few_splits(rows, k, 2 * n, few_waves(p.groups));
+    p.apart = rows > kFusedRows || rows * (k / 128) > 16 * p.splits;
+    Taker take;
+    p.part = take((size_t)p.splits * 2 * n * rows * 4);
+    p.frag = take(p.apart ? (size_t)2 * p.groups * k * 32 : 0);
+    p.rest = take(p.apart && two ? (size_t)2 * p.groups * k * 32 : 0);
+    p.shift = take(p.apart ? (size_t)2 * p.groups * k / 2 : 0);
+    p.total = take.at;
+    return p;
+}
+
+struct ManyPlan {
+    int groups, places, nb, tiles, splits;
+    size_t shift, rowexp, xf[2], x2[2], wf, part, total;
+};
+
+ManyPlan many_plan(int rows, int k, int n, bool two) {
+    ManyPlan p;
+    p.groups = (rows + 15) / 16;
+    p.places = (p.groups + 15) / 16 * 256;      // whole tiles' rows
+    const Tiling t = gemm_tiling(rows, 2 * n, k / 32, two);
+    p.nb = t.nb;
+    p.tiles = t.tiles;
+    p.splits = t.splits;
+    Taker take;
+    p.shift = take((size_t)2 * p.places * 4);
+    p.rowexp = take((size_t)2 * p.places * 4);
+    for (int r = 0; r < 2; ++r) {
+        p.xf[r] = take(frag_bytes(p.groups, k / 32));
+        p.x2[r] = take(two ? frag_bytes(p.groups, k / 32) : 0);
+    }
+    p.wf = take(frag_bytes(2 * n / 16, k / 32));
+    p.part = take(p.splits > 1 ? (size_t)p.splits * p.groups * 64 * 2 * n : 0);
+    p.total = take.at;
+    return p;
+}
+
+template <int T>
+hipError_t many(const GatedArgs& a, void* ws, hipStream_t s) {
+    const int k = a.w[0].k, n = a.w[0].n;
+    const ManyPlan p = many_plan(a.rows, k, n, a.two);
+    uint8_t* base = (uint8_t*)ws;
+    GatedGemm g{};
+    g.A = (uint16_t*)(base + p.wf);
+    g.nb = n / 128;
+    g.gb = p.groups;
+    g.steps = k / 32;
+    g.tiles = p.tiles;
+    g.splits = p.splits;
+    g.part = (float*)(base + p.part);
+    for (int r = 0; r < 2; ++r) {
+        int32_t *shift = (int32_t*)(base + p.shift) + r * p.places, *rowexp = (int32_t*)(base + p.rowexp) + r * p.places;
+        uint16_t *xf = (uint16_t*)(base + p.xf[r]), *x2 = a.two ? (uint16_t*)(base + p.x2[r]) : nullptr;
+        const Source src{a.x, a.x_stride, nullptr, 0, a.w[r].suh, T, a.rows, k};
+        prepare(a.w[r], 0, Prepare{(uint16_t*)(base + p.wf), FragPlace{r, 0, k / 32}, (k / 16) * (n / 16) / 32, src, shift,
+                                   rowexp}, s);
+        transform_rows(src, shift, xf, x2, nullptr, s);
+        g.B[r] = xf;
+        g.B2[r] = x2;
+        g.rowexp[r] = rowexp;
+    }
+    const dim3 grid(p.tiles, p.splits), block(256);
+    auto gemm = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, g, a); };
+    if (p.splits == 1) {
+        if (a.two) gemm(gated_gemm_kernel<T, kGatedFinish, 2, 2>);
+        else if (p.nb == 4) gemm(gated_gemm_kernel<T, kGatedFinish, 4, 1>);
+        else gemm(gated_gemm_kernel<T, kGatedFinish, 2, 1>);
+    } else {
+        if (a.two) gemm(gated_gemm_kernel<T, kGatedParts, 2, 2>);
+        else if (p.nb == 4) gemm(gated_gemm_kernel<T, kGatedParts, 4, 1>);
+        else gemm(gated_gemm_kernel<T, kGatedParts, 2, 1>);
+        hipLaunchKernelGGL((gated_join_kernel<T>), dim3(p.groups, n / 128), dim3(64), 0, s, g, a);
+    }
+    return hipGetLastError();
+}
+
+struct GradPlan {
+    int groups, places, nb, tiles, splits;      // splits: of both weights together
+    size_t shift, rowexp, zf, z2, wf, part, colsum, total;
+};
+
+GradPlan grad_plan(int rows, int k, int n, bool two) {
+    GradPlan p;
+    p.groups = (rows + 15) / 16;
+    p.places = p.groups * 16;
+    const Tiling t = gemm_tiling(rows, k, n / 32, two);
+    p.nb = t.nb;
+    p.tiles = t.tiles;
+    p.splits = 2 * t.splits;
+    Taker take;
+    p.shift = take((size_t)2 * p.places * 4);
+    p.rowexp = take((size_t)2 * p.places * 4);
+    p.zf = take(frag_bytes(p.groups, n / 16));
+    p.z2 = take(two ? frag_bytes(p.groups, n / 16) : 0);
+    p.wf = take(frag_bytes(k / 16, n / 16));
+    p.part = take((size_t)p.splits * p.groups * 64 * k);
+    p.colsum = take((size_t)p.groups * 2 * n * 4);
+    p.total = take.at;
+    return p;
+}
+
+template <int T>
+hipError_t gradient(const GatedGradArgs& a, void* ws, hipStream_t s) {
+    const int k = a.w[0].k, n = a.w[0].n;
+    const GradPlan p = grad_plan(a.rows, k, n, a.two);
+    uint8_t* base = (uint8_t*)ws;
+    int32_t *shift = (int32_t*)(base + p.shift), *rowexp = (int32_t*)(base + p.rowexp);
+    uint16_t *wf = (uint16_t*)(base + p.wf), *zf = (uint16_t*)(base + p.zf), *z2 = a.two ? (uint16_t*)(base + p.z2) : nullptr;
+    const bool sum = a.dbias[0] || a.dbias[1];
+    float* colsum = sum ? (float*)(base + p.colsum) : nullptr;
+    const GatedSource src{a.dy, a.dy_stride, a.z, {a.w[0].svh, a.w[1].svh}, T, a.act, a.rows, n};
+    const ColSum sums{colsum, p.groups, 2 * n, T, a.bias_f32[0], a.dbias[0], n, a.bias_f32[1], a.dbias[1]};
+    const int adders = sum ? 2 * n / 64 : 0;
+    const dim3 rows_grid((n / 128 + 3) / 4, p.groups);
+    if (!a.dx) {
+        hipLaunchKernelGGL(gated_transform_kernel, rows_grid, dim3(256), 0, s, src, shift, p.places, (uint16_t*)nullptr,
+                           (uint16_t*)nullptr, colsum);
+        hipLaunchKernelGGL(gated_column_sums_kernel, dim3(adders), dim3(256), 0, s, sums);
+        return hipGetLastError();
+    }
+    for (int r = 0; r < 2; ++r)
+        prepare(a.w[r], 1, Prepare{wf, FragPlace{-1, r * (n / 32), n / 16}, (k / 16) * (n / 16) / 32, Source{}, nullptr,
+                                   nullptr}, s);
+    hipLaunchKernelGGL(gated_exponents_kernel, dim3(a.rows), dim3(256), 0, s, src, shift, rowexp, p.places);
+    hipLaunchKernelGGL(gated_transform_kernel, rows_grid, dim3(256), 0, s, src, (const int32_t*)shift, p.places, zf, z2, colsum);
+    const Gemm g{wf, zf, z2, k / 16, p.groups, n / 16, p.tiles, p.splits, (float*)(base + p.part), nullptr, nullptr, 0};
+    const hipError_t e = launch_parts(g, T, p.nb, a.two, sums, adders, s);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((gated_dx_kernel<T>), dim3(p.groups, k / 128), dim3(64), 0, s, g, a, (const int32_t*)rowexp, p.places);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t gated_ws_bytes(int rows, int k, int n, bool two) {
+    return takes_few(rows, n) ? few_plan(rows, k, n, two).total : many_plan(rows, k, n, two).total;
+}
+
+size_t gated_bwd_ws_bytes(int rows, int k, int n, bool two) { return grad_plan(rows, k, n, two).total; }
+
+hipError_t launch_gated(const GatedArgs& a, void* ws, uint32_t* counters, hipStream_t s) {
+    const int k = a.w[0].k, n = a.w[0].n;
+    if (!takes_few(a.rows, n)) return a.type == kBf16 ? many<kBf16>(a, ws, s) : many<kF16>(a, ws, s);
+    const FewPlan p = few_plan(a.rows, k, n, a.two);
+    uint8_t* base = (uint8_t*)ws;
+    GatedFew f{nullptr, nullptr, nullptr, p.groups, p.splits, (float*)(base + p.part), counters};
+    if (p.apart) {
+        u4 *frag = (u4*)(base + p.frag), *rest = a.two ? (u4*)(base + p.rest) : nullptr;
+        int32_t* shift = (int32_t*)(base + p.shift);
+        transform_few(a.two, a.x, a.x_stride, a.type, a.rows, k, p.groups, a.w[0].suh, a.w[1].suh, frag, rest, shift, s);
+        f.frag = frag;
+        f.frag_lo = rest;
+        f.shift = shift;
+    }
+    static decltype(&launch_gated_few_code0) const few[] = {launch_gated_few_code0, launch_gated_few_code1,
+                                                            launch_gated_few_code2};
+    return few[a.w[0].code](a, f, s);
+}
+
+hipError_t launch_gated_bwd(const GatedGradArgs& a, void* ws, hipStream_t s) {
+    return a.type == kBf16 ? gradient<kBf16>(a, ws, s) : gradient<kF16>(a, ws, s);
+}
+
+}  // namespace xtq

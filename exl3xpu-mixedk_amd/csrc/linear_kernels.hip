@@ -16,50 +16,13 @@
 // arithmetic.  16 fragments of a step lie side by side (frag_at), the rows or
 // columns of a workgroup's tile: it reads two streams of 16 KiB pieces, and not
 // 32 of 1 KiB from as many pages.
-#include "epilogue.h"
 #include "few_device.h"
-#include "operators.h"
+#include "product_device.h"
 
 #pragma clang fp contract(off)
 
 namespace xtq {
 namespace {
-
-constexpr int kFragBytes = 1024;
-
-// Where fragment `step` of group `grp` starts, in elements.  Groups come in
-// sixteens; scratch is sized for whole ones, and what is not written there
-// reaches no result.
-__host__ __device__ __forceinline__ size_t frag_at(size_t grp, size_t step, size_t steps) {
-    return (((grp >> 4) * steps + step) * 16 + (grp & 15)) * 512;
-}
-
-// Bytes of `groups` groups' fragments.
-size_t frag_bytes(size_t groups, size_t steps) { return (groups + 15) / 16 * 16 * steps * kFragBytes; }
-
-__device__ __forceinline__ void unpack8(u4 w, int type, float* v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (type == kBf16) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        } else {
-            v[2 * i] = half_bits(w[i] & 0xFFFFu);
-            v[2 * i + 1] = half_bits(w[i] >> 16);
-        }
-    }
-}
-
-// Input of a product: activations, or (z set) a gradient dy times the
-// activation's slope at the saved z.
-struct Source {
-    const uint16_t* x;
-    long long stride;
-    const uint16_t* z;          // [rows][cols] or NULL
-    int act;
-    const uint16_t* colscale;   // fp16 per column
-    int type, rows, cols;
-};
 
 // Eight consecutive values of a row before its column scales.
 __device__ __forceinline__ void load8(const Source& s, size_t row, int col, float* v) {
@@ -106,73 +69,10 @@ __global__ __launch_bounds__(256) void transform_kernel(Source s, const int32_t*
 #pragma unroll
         for (int p = 0; p < 4; ++p) load8(s, row, 128 * blk + 32 * p + 8 * q, v + 8 * p);
     }
-    if (colsum) {
-        float* out = colsum + (size_t)grp * s.cols + 128 * blk;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float t = v[i];
-            t += dpp<0xB1>(t);          // lanes 1 0 3 2
-            t += dpp<0x4E>(t);          // lanes 2 3 0 1
-            t += dpp<0x141>(t);         // mirrored in eights, then in sixteens
-            t += dpp<0x140>(t);
-            if ((lane & 15) == 0) out[32 * (i >> 3) + 8 * q + (i & 7)] = t;
-        }
-    }
+    if (colsum) rows_sum(v, lane, colsum + (size_t)grp * s.cols + 128 * blk);
 #pragma unroll
     for (int p = 0; p < 4; ++p) scale8(s.colscale, 128 * blk + 32 * p + 8 * q, v + 8 * p);
-#pragma unroll
-    for (int b = 1; b < 32; b <<= 1)
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (!(i & b)) {
-                const float a = v[i], c = v[i | b];
-                v[i] = a + c;
-                v[i | b] = a - c;
-            }
-    const int sh = row < s.rows ? shift[row] : 0;
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-        cross_pair<16>(v[i], v[i + 1]);
-        cross_pair<32>(v[i], v[i + 1]);
-        v[i] = ldexpf(v[i], sh);
-        v[i + 1] = ldexpf(v[i + 1], sh);
-    }
-    uint16_t* out = frags + lane * 8;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        h8 o;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = (_Float16)v[8 * p + i];
-        *(h8*)(out + frag_at(grp, 4 * blk + p, 4 * nblk)) = o;
-        if (rest) {
-            h8 l;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) l[i] = (_Float16)(v[8 * p + i] - (float)o[i]);
-            *(h8*)(rest + lane * 8 + frag_at(grp, 4 * blk + p, 4 * nblk)) = l;
-        }
-    }
-}
-
-// Column sums' last step: out[c] = sum of part[g][c] over the groups, in an
-// order that their number fixes: four threads a column take every fourth group.
-struct ColSum {
-    const float* part;
-    int groups, cols, type, f32;
-    void* out;
-};
-
-__device__ void column_sums(const ColSum& a, int block, float* part) {
-    const int c = block * 64 + (threadIdx.x & 63), wv = threadIdx.x >> 6;
-    float t = 0.0f;
-    if (c < a.cols)
-#pragma unroll 8
-        for (int g = wv; g < a.groups; g += 4) t += a.part[(size_t)g * a.cols + c];
-    part[threadIdx.x] = t;
-    __syncthreads();
-    if (wv || c >= a.cols) return;
-    t = (part[c & 63] + part[64 + (c & 63)]) + (part[128 + (c & 63)] + part[192 + (c & 63)]);
-    if (a.f32) ((float*)a.out)[c] = t;
-    else ((uint16_t*)a.out)[c] = (uint16_t)(a.type == kBf16 ? to16<kBf16>(t) : to16<kF16>(t));
+    rows_to_frags(v, row < s.rows ? shift[row] : 0, lane, grp, 4 * blk, 4 * nblk, frags, rest);
 }
 
 __global__ __launch_bounds__(256) void column_sums_kernel(ColSum a) {
@@ -214,11 +114,12 @@ __device__ void row_exponents(const Source& s, int row, int32_t* __restrict__ sh
 // takes 8 by 4 tiles (along the summed dimension by the other), the trellis
 // words staged in LDS.  Memory bounds it: 5120 by 17408 at K = 4 reads 45 MB and
 // writes 178 in 50 us, 4.5 TB/s (a copy moves 4.97).  The workgroups past `decoders` find the exponents of the
-// source's rows, which nothing here waits for.
+// source's rows, which nothing here waits for.  place: where the fragments lie
+// among those of another weight.
 template <int K, int CODE, int BWD>
 __global__ __launch_bounds__(256) void prepare_kernel(const int16_t* __restrict__ trellis, int tk, int tn,
-                                                      uint16_t* __restrict__ frags, int decoders, Source src,
-                                                      int32_t* __restrict__ shift,
+                                                      uint16_t* __restrict__ frags, FragPlace place, int decoders,
+                                                      Source src, int32_t* __restrict__ shift,
                                                       int32_t* __restrict__ rowexp) {
     if ((int)blockIdx.x >= decoders) return row_exponents(src, blockIdx.x - decoders, shift, rowexp);
     constexpr int TW = 8 * K;                           // words of a tile
@@ -249,9 +150,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(const int16_t* __restrict_
         u4 o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = code_pair<CODE>(st[2 * j], st[2 * j + 1]);
-        const size_t g = BWD ? i0 + wv : j0 + wv;
-        const size_t np = (BWD ? tn : tk) / 2, f = (BWD ? j0 : i0) / 2 + p;
-        *(u4*)(frags + frag_at(g, f, np) + lane * 8) = o;
+        size_t g = BWD ? i0 + wv : j0 + wv;
+        if (place.half >= 0) g = (g >> 3) * 16 + 8 * place.half + (g & 7);
+        const size_t f = place.step + (BWD ? j0 : i0) / 2 + p;
+        *(u4*)(frags + frag_at(g, f, place.steps) + lane * 8) = o;
     }
 }
 
@@ -265,42 +167,9 @@ __global__ __launch_bounds__(256) void prepare_kernel(const int16_t* __restrict_
 // overlap with the other's products.  (One workgroup of 8 waves and 256 by 256,
 // its fragments fetched a step ahead: the epilogue, 17 us a tile, stood alone.)
 // 4096 rows by 5120 by 17408 with the epilogue: 666 us, 1.10 PFLOP/s; the library's
-// product of the same size alone takes 594, 8192 cubed runs at 1.29.
-constexpr int kTileN = 256;
-
-// Workgroups go round robin over the 8 XCDs, each with an L2 of its own: an XCD
-// gets a run of tiles that lie side by side, in bands of kBand rows of tiles.
-constexpr int kXcds = 8;
-constexpr int kBand = 8;
-
-__device__ __forceinline__ int xcd_order(int id, int all) {
-    const int x = id % kXcds, each = all / kXcds, more = all % kXcds;
-    return x * each + (x < more ? x : more) + id / kXcds;
-}
-
+// product of the same size alone takes 594, 8192 cubed runs at 1.29.  (A tile's
+// columns: kTileN; tiles in bands of kBand rows of tiles by XCD.)
 enum GemmOut { kOutEpilogue, kOutPartial, kOutGram };
-
-struct Gemm {
-    const uint16_t *A, *B, *B2;         // B2: B's second terms (TERMS 2)
-    int ga, gb;                         // 16-wide groups of columns, rows
-    int steps;                          // 32-wide steps of the summed dimension
-    int tiles, splits;                  // splits of the summed dimension
-    float* part;                        // partial: [splits][blocks of 128][gb][8][64][4]
-    const float* prev;                  // Gram
-    float* out;
-    int dim;
-};
-
-template <bool BF>
-__device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
-    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a),
-                                                                    __builtin_bit_cast(b8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a),
-                                                       __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
-
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
 
 // out = prev + sums of 32 rows by 128 columns of the Gram, at and below the
 // diagonal and mirrored.  They go through t, 32 lines in LDS that only this wave
@@ -504,29 +373,6 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epilogue ep, ColSu
     }
 }
 
-// The sum over the splits of a unit (128 columns by 16 rows), in order, U of
-// them in flight for each register.
-template <int U>
-__device__ __forceinline__ void sum_splits(f4 (&v)[8], const Gemm& g, int grp, int blk, int lane) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-    const f4* p = (const f4*)g.part + ((size_t)blk * g.gb + grp) * 512 + lane;
-    const size_t stride = (size_t)(g.ga / 8) * g.gb * 512;
-    for (int s = 0; s < g.splits; s += U) {
-        f4 t[U][8];
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) t[i][j] = p[(s + i < g.splits ? s + i : s) * stride + j * 64];
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (s + i < g.splits) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] += t[i][j];
-            }
-    }
-}
-
 // Joins the splits' partial products and finishes them, a workgroup of one wave
 // one unit: units are few, so each may land where there is room (four waves a
 // workgroup: 15.9 us, not 14.6, for 333 rows by 6144 columns in three parts, whose
@@ -536,7 +382,7 @@ template <int T>
 __global__ __launch_bounds__(64) void join_kernel(Gemm g, Epilogue ep) {
     const int lane = threadIdx.x, grp = blockIdx.x, blk = blockIdx.y;
     f4 v[8];
-    sum_splits<4>(v, g, grp, blk, lane);
+    sum_splits<4>(v, g, grp, blk, lane, 0, g.splits);
     Columns<4> cols[8];
     unit_columns<T>(cols, ep, blk, lane);
     finish_unit<T>(v, cols, ep, grp, blk, lane);
@@ -548,8 +394,8 @@ __global__ __launch_bounds__(256) void join_gram_kernel(Gemm g) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, grp = (blockIdx.x * 4 + wv) * 2, blk = blockIdx.y;
     if (grp >= g.gb || blk * 128 > grp * 16 + 31) return;       // (above the diagonal)
     f4 v[2][8];
-    sum_splits<2>(v[0], g, grp, blk, lane);
-    sum_splits<2>(v[1], g, grp + 1, blk, lane);
+    sum_splits<2>(v[0], g, grp, blk, lane, 0, g.splits);
+    sum_splits<2>(v[1], g, grp + 1, blk, lane, 0, g.splits);
     finish_gram(v, t[wv], g, grp, blk, lane);
 }
 
@@ -702,21 +548,14 @@ __global__ __launch_bounds__(64 * W, 4) void gram_few_kernel(const uint16_t* __r
     }
 }
 
-struct Prepare {
-    uint16_t* frags;
-    int decoders;
-    Source src;
-    int32_t *shift, *rowexp;
-};
-
 template <int K, int CODE>
 void prepare_kc(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     const int tk = w.k / 16, tn = w.n / 16;
     const dim3 grid(p.decoders + p.src.rows);
     if (bwd) hipLaunchKernelGGL((prepare_kernel<K, CODE, 1>), grid, dim3(256), 0, s, w.trellis, tk, tn, p.frags,
-                                p.decoders, p.src, p.shift, p.rowexp);
+                                p.place, p.decoders, p.src, p.shift, p.rowexp);
     else hipLaunchKernelGGL((prepare_kernel<K, CODE, 0>), grid, dim3(256), 0, s, w.trellis, tk, tn, p.frags,
-                            p.decoders, p.src, p.shift, p.rowexp);
+                            p.place, p.decoders, p.src, p.shift, p.rowexp);
 }
 
 template <int K>
@@ -725,6 +564,8 @@ void prepare_k(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     else if (w.code == kCodeMcg) prepare_kc<K, kCodeMcg>(w, bwd, p, s);
     else prepare_kc<K, kCode3Inst>(w, bwd, p, s);
 }
+
+}  // namespace
 
 void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     switch (w.K) {
@@ -737,8 +578,6 @@ void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     }
 }
 
-size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
-
 // How a product of `steps` steps is cut: nb groups of 16 rows to a wave's tile,
 // splits of the summed dimension.  The choice is the shortest estimate, from what
 // the kernels measured: a workgroup's step takes 0.62 us (nb 4) or 0.38 (nb 2)
@@ -747,10 +586,6 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 // whole calls in replayed graphs with nb 4, nb 2: 5120 by 5120, 333 rows 67 : 56, 1000
 // rows 92 : 107, 2047 rows 150 : 182; 5120 by 17408, 96 rows 101 : 84, 600 rows 176 :
 // 205.)
-struct Tiling {
-    int nb, tiles, splits;
-};
-
 Tiling gemm_tiling(int rows, int n, int steps, bool two) {
     Tiling best{};
     double least = 0.0;
@@ -770,6 +605,8 @@ Tiling gemm_tiling(int rows, int n, int steps, bool two) {
     }
     return best;
 }
+
+namespace {
 
 struct ManyPlan {
     int groups, nb, tiles, splits;
@@ -797,6 +634,31 @@ ManyPlan many_plan(int rows, int k, int n, bool colsum, bool two) {
     return p;
 }
 
+template <int T>
+void launch_parts_of(const Gemm& g, int nb, bool two, const ColSum& sums, int adders, hipStream_t s) {
+    const dim3 grid(g.tiles + adders, g.splits), block(256);
+    const Epilogue ep{};
+    if (two) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 2>), grid, block, 0, s, g, ep, sums);
+    else if (nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 4, 1>), grid, block, 0, s, g, ep, sums);
+    else hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 1>), grid, block, 0, s, g, ep, sums);
+}
+
+}  // namespace
+
+void transform_rows(const Source& src, const int32_t* shift, uint16_t* frags, uint16_t* rest, float* colsum,
+                    hipStream_t s) {
+    hipLaunchKernelGGL(transform_kernel, dim3((src.cols / 128 + 3) / 4, (src.rows + 15) / 16), dim3(256), 0, s, src,
+                       shift, frags, rest, colsum);
+}
+
+hipError_t launch_parts(const Gemm& g, int type, int nb, bool two, const ColSum& sums, int adders, hipStream_t s) {
+    if (type == kBf16) launch_parts_of<kBf16>(g, nb, two, sums, adders, s);
+    else launch_parts_of<kF16>(g, nb, two, sums, adders, s);
+    return hipGetLastError();
+}
+
+namespace {
+
 // The product of a source's rows with a weight (bwd: its transpose).
 template <int T>
 hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* dbias, int dbias_f32,
@@ -808,10 +670,9 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
     uint16_t *xf = (uint16_t*)(base + p.xf), *x2 = two ? (uint16_t*)(base + p.x2) : nullptr, *wf = (uint16_t*)(base + p.wf);
     float* colsum = dbias ? (float*)(base + p.colsum) : nullptr;
     const int decoders = ep.y ? (w.k / 16) * (w.n / 16) / 32 : 0;
-    prepare(w, bwd, Prepare{wf, decoders, src, shift, rowexp}, s);
-    hipLaunchKernelGGL(transform_kernel, dim3((k / 128 + 3) / 4, p.groups), dim3(256), 0, s, src,
-                       (const int32_t*)shift, xf, x2, colsum);
-    const ColSum sums{colsum, p.groups, k, T, dbias_f32, dbias};
+    prepare(w, bwd, Prepare{wf, FragPlace{-1, 0, k / 32}, decoders, src, shift, rowexp}, s);
+    transform_rows(src, shift, xf, x2, colsum, s);
+    const ColSum sums{colsum, p.groups, k, T, dbias_f32, dbias, k, 0, nullptr};
     const int adders = dbias ? (k + 63) / 64 : 0;
     if (!ep.y) {
         hipLaunchKernelGGL(column_sums_kernel, dim3(adders), dim3(256), 0, s, sums);
@@ -825,9 +686,8 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
         else if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 4, 1>), grid, block, 0, s, g, ep, sums);
         else hipLaunchKernelGGL((gemm_kernel<T, kOutEpilogue, false, 2, 1>), grid, block, 0, s, g, ep, sums);
     } else {
-        if (two) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 2>), grid, block, 0, s, g, ep, sums);
-        else if (p.nb == 4) hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 4, 1>), grid, block, 0, s, g, ep, sums);
-        else hipLaunchKernelGGL((gemm_kernel<T, kOutPartial, false, 2, 1>), grid, block, 0, s, g, ep, sums);
+        const hipError_t e = launch_parts(g, T, p.nb, two, sums, adders, s);
+        if (e != hipSuccess) return e;
         hipLaunchKernelGGL((join_kernel<T>), dim3(p.groups, n / 128), dim3(64), 0, s, g, ep);
     }
     return hipGetLastError();
@@ -840,6 +700,7 @@ template <bool LO>
 __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __restrict__ x, long long stride,
                                                             int type, int rows, int k,
                                                             const uint16_t* __restrict__ suh,
+                                                            const uint16_t* __restrict__ suh2,
                                                             u4* __restrict__ frag, u4* __restrict__ rest,
                                                             int32_t* __restrict__ shift) {
     const int lane = threadIdx.x & 63, nk = k / 128;
@@ -847,11 +708,20 @@ __global__ __launch_bounds__(256) void transform_few_kernel(const uint16_t* __re
     if (kb >= nk) return;
     float a = 0.0f, b = 0.0f, sa, sb;
     if (row < rows) unpack_two(load_two(x + (size_t)row * stride + 128 * kb, lane), type, a, b);
-    unpack_two(load_two(suh + 128 * kb, lane), kF16, sa, sb);
-    const size_t at = (size_t)(row >> 4) * nk + kb;
+    unpack_two(load_two((blockIdx.z ? suh2 : suh) + 128 * kb, lane), kF16, sa, sb);
+    const size_t at = (size_t)(blockIdx.z * (gridDim.y >> 4) + (row >> 4)) * nk + kb;
     const int sh = row_to_frags<LO>(a * sa, b * sb, lane, row & 15, (uint32_t*)(frag + at * 256),
                                     LO ? (uint32_t*)(rest + at * 256) : nullptr);
     if (lane == 0) shift[at * 16 + (row & 15)] = sh;
+}
+
+}  // namespace
+
+void transform_few(bool two, const void* x, long long x_stride, int type, int rows, int k, int groups,
+                   const uint16_t* suh, const uint16_t* suh2, u4* frag, u4* rest, int32_t* shift, hipStream_t s) {
+    hipLaunchKernelGGL(two ? transform_few_kernel<true> : transform_few_kernel<false>,
+                       dim3((k / 128 + 3) / 4, 16 * groups, suh2 ? 2 : 1), dim3(256), 0, s, (const uint16_t*)x, x_stride,
+                       type, rows, k, suh, suh2, frag, rest, shift);
 }
 
 // Workgroups per 128 columns of a product of few rows: two for each compute
@@ -873,6 +743,8 @@ int few_splits(int rows, int k, int n, int waves) {
     return s < 1 ? 1 : s;
 }
 
+namespace {
+
 // (5120 by 5120, one launch or two against decoding apart: 17 rows 20 : 42 us, 64
 // rows 31 : 44; 5120 by 1024 20 : 30 and 27 : 32; with two terms 24 : 43, 35 : 43, 23 :
 // 34 and, at K = 7, whose 64 rows of two terms spill, 38 : 37.)
@@ -887,8 +759,6 @@ bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_C
 // replayed, which clear the counters before each product; the kernel of one row of
 // 5120 by 5120 alone takes 12.6).
 constexpr int kFewItems = 16;
-
-constexpr int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 // The kernels read every place of their groups, so there is one for each row, in a
 // number that has a kernel; one group where the kernel transforms the rows.
@@ -943,9 +813,7 @@ hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_s
         if (!p.apart) return few[w.K - 2](w, a, ep, s);
         u4 *frag = (u4*)(base + p.frag), *rest = two ? (u4*)(base + p.rest) : nullptr;
         int32_t* shift = (int32_t*)(base + p.shift);
-        hipLaunchKernelGGL(two ? transform_few_kernel<true> : transform_few_kernel<false>,
-                           dim3((w.k / 128 + 3) / 4, 16 * p.groups), dim3(256), 0, s, a.x, x_stride, type, rows, w.k,
-                           w.suh, frag, rest, shift);
+        transform_few(two, x, x_stride, type, rows, w.k, p.groups, w.suh, nullptr, frag, rest, shift, s);
         a.frag = frag;
         a.frag_lo = rest;
         a.shift = shift;

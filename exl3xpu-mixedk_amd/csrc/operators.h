@@ -57,6 +57,68 @@ inline bool two_terms(int type, int act, bool fast) { return !fast && (type == k
 // The same for a gradient's product: no slope is taken at what it gives.
 inline bool two_terms_gradient(int type, bool fast) { return !fast && type == kF16; }
 
+// Input of a product: activations, or (z set) a gradient dy times the
+// activation's slope at the saved z.
+struct Source {
+    const uint16_t* x;
+    long long stride;
+    const uint16_t* z;          // [rows][cols] or NULL
+    int act;
+    const uint16_t* colscale;   // fp16 per column
+    int type, rows, cols;
+};
+
+// What a weight's way to fragments takes: where they lie among another weight's
+// (half: of the groups of 128, its half of 256, or -1; step: its first of `steps`
+// of the summed dimension), workgroups that decode, and a source whose rows'
+// exponents are found beside.
+struct FragPlace {
+    int half, step, steps;
+};
+struct Prepare {
+    uint16_t* frags;
+    FragPlace place;
+    int decoders;
+    Source src;
+    int32_t *shift, *rowexp;
+};
+void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s);
+// A source's rows to fragments (rest: and what the rounding left; colsum: and their
+// sums by 16 rows, each NULL for none).
+void transform_rows(const Source& src, const int32_t* shift, uint16_t* frags, uint16_t* rest, float* colsum,
+                    hipStream_t s);
+
+struct Tiling {
+    int nb, tiles, splits;
+};
+
+Tiling gemm_tiling(int rows, int n, int steps, bool two);
+
+// Column sums' last step: out[c] = sum of part[g][c] over the groups, in an
+// order that their number fixes: four threads a column take every fourth group.
+struct ColSum {
+    const float* part;
+    int groups, cols, type, f32;
+    void* out;
+    int first, more_f32;                // columns from `first` on are another sum's
+    void* more;
+};
+
+// A product of fragments.
+struct Gemm {
+    const uint16_t *A, *B, *B2;         // B2: B's second terms (TERMS 2)
+    int ga, gb;                         // 16-wide groups of columns, rows
+    int steps;                          // 32-wide steps of the summed dimension
+    int tiles, splits;                  // splits of the summed dimension
+    float* part;                        // partial: [splits][blocks of 128][gb][8][64][4]
+    const float* prev;                  // Gram
+    float* out;
+    int dim;
+};
+// The product's parts, in g.splits runs of the summed dimension, by tiles of nb, and
+// beside them `adders` workgroups of column sums.
+hipError_t launch_parts(const Gemm& g, int type, int nb, bool two, const ColSum& sums, int adders, hipStream_t s);
+
 size_t linear_ws_bytes(int rows, int k, int n, bool backward, bool two);
 hipError_t launch_linear(const Weight& w, int type, const void* x, long long x_stride, int rows,
                          const Epilogue& ep, bool two, void* ws, uint32_t* counters, hipStream_t s);
@@ -92,6 +154,58 @@ struct FewArgs {
     hipError_t launch_few2_k##K(const Weight& w, const FewArgs& a, const Epilogue& ep, hipStream_t s);
 XTQ_FEW(2) XTQ_FEW(3) XTQ_FEW(4) XTQ_FEW(5) XTQ_FEW(6) XTQ_FEW(7)
 #undef XTQ_FEW
+
+// Workgroups per 128 columns and groups of 16 rows of those products, and their rows'
+// way to fragments (suh2: for a second weight too, behind the first's).
+int few_splits(int rows, int k, int n, int waves);
+constexpr int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+void transform_few(bool two, const void* x, long long x_stride, int type, int rows, int k, int groups,
+                   const uint16_t* suh, const uint16_t* suh2, u4* frag, u4* rest, int32_t* shift, hipStream_t s);
+
+// The gated projection act(x Wg + bg) (x Wu + bu) (gated_kernels.hip; up to kFewRows rows
+// gated_few.hip).  Role 0 is the gate, 1 the up weight.
+struct GatedArgs {
+    Weight w[2];                        // one k, n and code
+    int type, rows, act;
+    const uint16_t* x;
+    long long x_stride;
+    const void* bias[2];                // [n] or NULL
+    int bias_f32[2];
+    float* z;                           // [2][rows][n] values before the activation and the product, or NULL
+    uint16_t* y;
+    long long y_stride;
+    bool two;
+};
+struct GatedGradArgs {
+    Weight w[2];
+    int type, rows, act;
+    const uint16_t* dy;
+    long long dy_stride;
+    const float* z;
+    uint16_t* dx;                       // or NULL
+    long long dx_stride;
+    void* dbias[2];                     // or NULL
+    int bias_f32[2];
+    bool two;
+};
+size_t gated_ws_bytes(int rows, int k, int n, bool two);
+size_t gated_bwd_ws_bytes(int rows, int k, int n, bool two);
+hipError_t launch_gated(const GatedArgs& a, void* ws, uint32_t* counters, hipStream_t s);
+hipError_t launch_gated_bwd(const GatedGradArgs& a, void* ws, hipStream_t s);
+
+// Few rows, one function per codebook: frag [role][groups of 16 rows][k/32][64] and
+// shifts as in FewArgs, or NULL (one group: the kernel transforms x).
+struct GatedFew {
+    const u4 *frag, *frag_lo;
+    const int32_t* shift;
+    int groups, splits;
+    float* part;                        // [n/128][role][split][row][128]
+    uint32_t* counters;                 // [n/128]
+};
+#define XTQ_GATED(C) \
+    hipError_t launch_gated_few_code##C(const GatedArgs& a, const GatedFew& f, hipStream_t s);
+XTQ_GATED(0) XTQ_GATED(1) XTQ_GATED(2)
+#undef XTQ_GATED
 
 struct MoeArgs;
 size_t moe_ws_bytes(int rows, int experts, int top, int d, int f);

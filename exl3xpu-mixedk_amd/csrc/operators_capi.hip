@@ -36,6 +36,14 @@ int check_weight(const xtq_weight* w, xtq::Weight* out) {
     return 0;
 }
 
+// A gate's and an up's weights: one shape and code, each its own K.
+int check_pair(const xtq_weight* gate, const xtq_weight* up, xtq::Weight* out) {
+    int rc = check_weight(gate, out);
+    if (rc || (rc = check_weight(up, out + 1))) return rc;
+    if (out[0].code != out[1].code) return 8;
+    return out[0].k != out[1].k || out[0].n != out[1].n ? 6 : 0;
+}
+
 // A matrix of 16-bit elements.
 int check_rows(const void* p, int64_t stride, int cols) {
     if (!p || !aligned(p, 2)) return 12;
@@ -260,6 +268,80 @@ int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, int k, con
     if ((rc = check_ws(ws, ws_bytes, xtq::gram_ws_bytes(rows, k)))) return rc;
     return status(xtq::launch_gram(type, x, x_stride, rows, k, valid, prev, out, ws,
                                    (hipStream_t)stream), "gram");
+}
+
+int64_t xtq_gated_ws_bytes(const xtq_weight* gate, int rows, int gradient) {
+    if (!gate || gate->k <= 0 || gate->n <= 0 || gate->k % 128 || gate->n % 128 || rows < 0 || rows > kMaxRows)
+        return -6;
+    if (!rows) return 0;
+    auto* bytes = gradient ? xtq::gated_bwd_ws_bytes : xtq::gated_ws_bytes;
+    const size_t one = bytes(rows, gate->k, gate->n, false), two = bytes(rows, gate->k, gate->n, true);
+    return (int64_t)(one > two ? one : two);
+}
+
+int xtq_gated_dev(const xtq_weight* gate, const xtq_weight* up, int type, const void* x, int64_t x_stride, int rows,
+                  const void* gate_bias, const void* up_bias, int bias_f32, int act, float* z, void* y,
+                  int64_t y_stride, void* ws, int64_t ws_bytes, uint32_t* counters, void* stream) {
+    xtq::GatedArgs a{};
+    int rc = check_pair(gate, up, a.w);
+    if (rc) return rc;
+    const bool fast = type & XTQ_FAST;
+    type &= ~XTQ_FAST;
+    if ((type != XTQ_BF16 && type != XTQ_F16) || act < XTQ_ACT_NONE || act > XTQ_ACT_GELU) return 15;
+    if (rows < 0 || rows > kMaxRows) return 6;
+    if (rows == 0) return 0;
+    if ((rc = check_rows(x, x_stride, a.w[0].k))) return rc;
+    if ((rc = check_rows(y, y_stride, a.w[0].n))) return rc;
+    a.bias[0] = gate_bias;
+    a.bias[1] = up_bias;
+    for (int r = 0; r < 2; ++r) {
+        a.bias_f32[r] = bias_f32 >> r & 1;
+        if (!aligned(a.bias[r], a.bias_f32[r] ? 4 : 2)) return 12;
+    }
+    if (!aligned(z, 4) || !counters || !aligned(counters, 4)) return 12;
+    a.two = xtq::two_terms(type, act, fast);
+    if ((rc = check_ws(ws, ws_bytes, xtq::gated_ws_bytes(rows, a.w[0].k, a.w[0].n, a.two)))) return rc;
+    a.type = type;
+    a.rows = rows;
+    a.act = act;
+    a.x = (const uint16_t*)x;
+    a.x_stride = x_stride;
+    a.z = z;
+    a.y = (uint16_t*)y;
+    a.y_stride = y_stride;
+    return status(xtq::launch_gated(a, ws, counters, (hipStream_t)stream), "gated");
+}
+
+int xtq_gated_bwd_dev(const xtq_weight* gate, const xtq_weight* up, int type, const void* dy, int64_t dy_stride,
+                      const float* z, int act, int rows, void* dx, int64_t dx_stride, void* dgate_bias,
+                      void* dup_bias, int bias_f32, void* ws, int64_t ws_bytes, void* stream) {
+    xtq::GatedGradArgs a{};
+    int rc = check_pair(gate, up, a.w);
+    if (rc) return rc;
+    const bool fast = type & XTQ_FAST;
+    type &= ~XTQ_FAST;
+    if ((type != XTQ_BF16 && type != XTQ_F16) || act < XTQ_ACT_NONE || act > XTQ_ACT_GELU) return 15;
+    if (rows <= 0 || rows > kMaxRows) return 6;
+    if ((rc = check_rows(dy, dy_stride, a.w[0].n))) return rc;
+    if (!z || !aligned(z, 4) || (!dx && !dgate_bias && !dup_bias)) return 12;
+    if (dx && (rc = check_rows(dx, dx_stride, a.w[0].k))) return rc;
+    a.dbias[0] = dgate_bias;
+    a.dbias[1] = dup_bias;
+    for (int r = 0; r < 2; ++r) {
+        a.bias_f32[r] = bias_f32 >> r & 1;
+        if (!aligned(a.dbias[r], a.bias_f32[r] ? 4 : 2)) return 12;
+    }
+    a.two = xtq::two_terms_gradient(type, fast);
+    if ((rc = check_ws(ws, ws_bytes, xtq::gated_bwd_ws_bytes(rows, a.w[0].k, a.w[0].n, a.two)))) return rc;
+    a.type = type;
+    a.rows = rows;
+    a.act = act;
+    a.dy = (const uint16_t*)dy;
+    a.dy_stride = dy_stride;
+    a.z = z;
+    a.dx = (uint16_t*)dx;
+    a.dx_stride = dx_stride;
+    return status(xtq::launch_gated_bwd(a, ws, (hipStream_t)stream), "gated_bwd");
 }
 
 int xtq_norm_dev(const xtq_norm* p, int type, int rows, int d, const void* x, int64_t x_stride, const void* res,

@@ -99,6 +99,10 @@ def lib():
         L.xtq_gram_ws_bytes.argtypes = [i32, i32]
         L.xtq_gram_ws_bytes.restype = ll
         L.xtq_gram_dev.argtypes = [i32, vp, ll, i32, i32, vp, vp, vp, vp, ll, vp]
+        L.xtq_gated_ws_bytes.argtypes = [wp, i32, i32]
+        L.xtq_gated_ws_bytes.restype = ll
+        L.xtq_gated_dev.argtypes = [wp, wp, i32, vp, ll, i32, vp, vp, i32, i32, vp, vp, ll, vp, ll, vp, vp]
+        L.xtq_gated_bwd_dev.argtypes = [wp, wp, i32, vp, ll, vp, i32, i32, vp, ll, vp, vp, i32, vp, ll, vp]
         np_ = ctypes.POINTER(NormParams)
         L.xtq_norm_dev.argtypes = [np_, i32, i32, i32, vp, ll, vp, ll, vp, ll, vp, ll, vp, ll, vp, vp]
         L.xtq_norm_bwd_ws_bytes.argtypes = [i32, i32, i32]
@@ -125,7 +129,7 @@ def lib():
                    "xtq_trellis_unpack64_dev", "xtq_vit_get_lut", "xtq_had128_left_dev",
                    "xtq_had128_right_dev", "xtq_had128_both_dev", "xtq_linear_dev",
                    "xtq_linear_bwd_dev", "xtq_gram_dev", "xtq_moe_table", "xtq_moe_dev",
-                   "xtq_norm_dev", "xtq_norm_bwd_dev"):
+                   "xtq_gated_dev", "xtq_gated_bwd_dev", "xtq_norm_dev", "xtq_norm_bwd_dev"):
             getattr(L, fn).restype = i32
         _LIB = L
     return _LIB

@@ -242,6 +242,97 @@ def linear(x: torch.Tensor, w: TrellisLinear, bias: torch.Tensor | None = None,
     return _forward(x, w, bias, a, residual, fast, False)[0]
 
 
+def _gated_forward(x, gate, up, biases, act, fast, keep_z):
+    rows = _rows(x, gate.k)
+    m, n = rows.shape[0], gate.n
+    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
+    z = torch.empty(2, m, n, dtype=torch.float32, device=x.device) if keep_z else None
+    if m == 0:
+        return y, z
+    biases = [None if b is None else b.contiguous() for b in biases]
+    L = _hb.lib()
+    with _on(x.device):
+        stream = _stream(x.device)
+        need = L.xtq_gated_ws_bytes(gate._p, m, 0)
+        words = _counter_words(x.device, stream)
+        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+        rc = L.xtq_gated_dev(
+            gate._p, up._p, _TYPES[x.dtype] | fast, rows.data_ptr(), _stride(rows), m,
+            *(None if b is None else b.data_ptr() for b in biases), _f32_bits(biases), act,
+            None if z is None else z.data_ptr(), y.data_ptr(), n, ws.data_ptr(), ws.numel(),
+            words.data_ptr(), stream)
+    _hb._check("xtq_gated_dev", rc)
+    return y, z
+
+
+def _f32_bits(tensors):
+    return sum(1 << i for i, t in enumerate(tensors) if t is not None and t.dtype == torch.float32)
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_bias, up_bias, gate, up, act, fast):
+        y, z = _gated_forward(x, gate, up, (gate_bias, up_bias), act, fast, True)
+        ctx.weights, ctx.act, ctx.fast, ctx.shape = (gate, up), act, fast, x.shape
+        ctx.types = [None if b is None else b.dtype for b in (gate_bias, up_bias)]
+        ctx.save_for_backward(z)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        z, = ctx.saved_tensors
+        _no_tangents("gated's gradient", dy)
+        gate, up = ctx.weights
+        rows = _rows(dy, gate.n)
+        m = rows.shape[0]
+        want = ctx.needs_input_grad[:3]
+        dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device) if want[0] else None
+        dbias = [torch.empty(gate.n, dtype=t, device=dy.device) if w else None for w, t in zip(want[1:], ctx.types)]
+        if m == 0:
+            return (dx, *(None if b is None else b.zero_() for b in dbias), None, None, None, None)
+        L = _hb.lib()
+        with _on(dy.device):
+            need = L.xtq_gated_ws_bytes(gate._p, m, 1)
+            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dy.device)
+            rc = L.xtq_gated_bwd_dev(
+                gate._p, up._p, _TYPES[dy.dtype] | ctx.fast, rows.data_ptr(), _stride(rows), z.data_ptr(),
+                ctx.act, m, None if dx is None else dx.data_ptr(), gate.k,
+                *(None if b is None else b.data_ptr() for b in dbias), _f32_bits(dbias), ws.data_ptr(),
+                ws.numel(), _stream(dy.device))
+        _hb._check("xtq_gated_bwd_dev", rc)
+        return dx, *dbias, None, None, None, None
+
+
+def gated(x: torch.Tensor, gate: TrellisLinear, up: TrellisLinear, gate_bias: torch.Tensor | None = None,
+          up_bias: torch.Tensor | None = None, act: str = "silu", fast: bool = False) -> torch.Tensor:
+    """act(x Wg + gate_bias) * (x Wu + up_bias) for x [.., k] (bfloat16 or float16) ->
+    [.., n] in x's type: a gated block's first half, whose second is linear's.  gate and
+    up have one shape and code, each its own K.  act: none, relu, silu or gelu (erf).
+    Biases [n] have x's type or fp32.  Differentiable in x and the biases (once, in
+    reverse mode; the weights are frozen), which keeps both factors in fp32; the same
+    result with a gradient and without.  x enters the products, and the gradient its
+    own, with as many bits as linear's; fast as there."""
+    if x.dtype not in _TYPES:
+        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if (up.k, up.n) != (gate.k, gate.n) or up.device != gate.device or \
+            _hb.code_name(up.code) != _hb.code_name(gate.code):
+        raise ValueError(f"up must be [{gate.k}, {gate.n}] {gate.code} on {gate.device}, got "
+                         f"[{up.k}, {up.n}] {up.code} on {up.device}")
+    if x.device != gate.device:
+        raise ValueError(f"x must be on {gate.device}, got {x.device}")
+    if x.dim() < 1 or x.shape[-1] != gate.k:
+        raise ValueError(f"x must be [.., {gate.k}], got {tuple(x.shape)}")
+    a, fast = _check_act(act), _FAST if fast else 0
+    _no_tangents("gated", x, gate_bias, up_bias)
+    for b, name in ((gate_bias, "gate_bias"), (up_bias, "up_bias")):
+        if b is not None:
+            _like(b, x, (gate.n,), name, (x.dtype, torch.float32))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate_bias, up_bias)):
+        return _Gated.apply(x, gate_bias, up_bias, gate, up, a, fast)
+    return _gated_forward(x, gate, up, (gate_bias, up_bias), a, fast, False)[0]
+
+
 _MOE_ROWS = 64
 
 
@@ -402,8 +493,7 @@ def _norm_rows(t, d):
 
 def _norm_struct(cfg, params):
     kind, post, gate_act, eps, post_eps, number = cfg
-    f32 = sum(1 << i for i, p in enumerate(params) if p is not None and p.dtype == torch.float32)
-    return _hb.NormParams(kind, post, gate_act, f32, eps, post_eps, number,
+    return _hb.NormParams(kind, post, gate_act, _f32_bits(params), eps, post_eps, number,
                           *(None if p is None else p.data_ptr() for p in params))
 
 

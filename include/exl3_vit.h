@@ -432,6 +432,36 @@ XTQ_API int xtq_gram_dev(int type, const void* x, int64_t x_stride, int rows, in
                          int64_t ws_bytes, void* stream);
 
 /*
+ * The gated projection y = act(x Wg + bg) * (x Wu + bu) for x [rows][k], y [rows][n].
+ * gate and up have one k, n and code, each its own K (else 6, 8).
+ *   gate_bias, up_bias  [n] or NULL; fp32 where bit 0 (gate) or 1 (up) of bias_f32
+ *                       is set, else of the activations' type
+ *   z                   [2][rows][n] fp32 (out): x Wg + bg and x Wu + bu, for
+ *                       xtq_gated_bwd_dev; or NULL
+ * x enters the products with as many bits as in xtq_linear_dev, and y is the same
+ * with and without z; type | XTQ_FAST as there.  At most 1,048,560 rows.
+ * xtq_gated_ws_bytes: the scratch of either entry (gradient != 0: of the gradient), by
+ * one weight's sizes, for either type.
+ */
+XTQ_API int64_t xtq_gated_ws_bytes(const xtq_weight* gate, int rows, int gradient);
+XTQ_API int xtq_gated_dev(const xtq_weight* gate, const xtq_weight* up, int type, const void* x,
+                          int64_t x_stride, int rows, const void* gate_bias, const void* up_bias,
+                          int bias_f32, int act, float* z, void* y, int64_t y_stride, void* ws,
+                          int64_t ws_bytes, uint32_t* counters, void* stream);
+
+/*
+ * Gradient of xtq_gated_dev: with dg = dy zu act'(zg) and du = dy act(zg),
+ * dx = dg Wg^T + du Wu^T [rows][k], dgate_bias and dup_bias the sums of dg's and du's
+ * rows, each or NULL.  z as the forward call wrote it.  dg and du enter the product
+ * with 22 bits for XTQ_F16, and with 11 for XTQ_BF16 or type | XTQ_FAST.  Zero rows:
+ * status 6.
+ */
+XTQ_API int xtq_gated_bwd_dev(const xtq_weight* gate, const xtq_weight* up, int type,
+                              const void* dy, int64_t dy_stride, const float* z, int act, int rows,
+                              void* dx, int64_t dx_stride, void* dgate_bias, void* dup_bias,
+                              int bias_f32, void* ws, int64_t ws_bytes, void* stream);
+
+/*
  * Norms of rows, and the residual sum between two blocks.  Of a block's result x,
  * its residual res, gate and scale, all rows [rows][d]:
  *   p = post norm of x (or x),  y = res + scale * ga(gate) * p,  h = norm of y,

@@ -23,7 +23,7 @@ def _norm(hb, params=None, **kw):  # noqa: F811
 
 def _bwd(hb, params=None, dparam=(P, None, P, P, None), **kw):  # noqa: F811
     a = dict(type=0, rows=5, d=100, x=P, xs=100, res=P, rs=100, gate=P, gs=100, stats=P, dy=P, dys=100, dh=P, dhs=100,
-             dx=P, dres=P, dgate=P, dparam=(ctypes.c_void_p * 5)(*dparam), ws=P, nws=1 << 40, stream=None)
+             dx=P, dres=P, dgate=P, dparam=dparam and (ctypes.c_void_p * 5)(*dparam), ws=P, nws=1 << 40, stream=None)
     a.update(kw)
     return hb.lib().xtq_norm_bwd_dev(ctypes.byref(_params(hb) if params is None else params), *a.values())
 
