@@ -19,6 +19,10 @@ namespace {
 // Rows of 16 lanes (four a wave), of a wave, of a workgroup.
 enum Mode { kSub, kWave, kBlock };
 
+// Waves that share a row at most: three a SIMD, whose 168 registers hold, of a
+// gradient, eight channels' parameters and sums and two rows' inputs.
+constexpr int kRowWaves = 12;
+
 template <int T>
 __device__ __forceinline__ void unpack(u4 w, float* v) {
 #pragma unroll
@@ -28,14 +32,29 @@ __device__ __forceinline__ void unpack(u4 w, float* v) {
     }
 }
 
-// Eight values of a row, `n` of which (at most 8) lie inside it; the others are 0.
-__device__ __forceinline__ u4 load8(const uint16_t* p, int n) {
-    if (n >= 8) return *(const u4_a2*)p;
+// Eight values of a row from column `col` on, on their way: every lane loads 16 bytes
+// inside the row, those at its end where its own reach past it, and in_place brings
+// them home once they are there.  (A load under a condition is waited for where the
+// branches meet: the gradient of 8191 rows of 5120 took 215 us so, and not 152.)
+template <int MODE>
+__device__ __forceinline__ u4 load8(const uint16_t* row, int col, int d) {
+    if (MODE != kSub || d >= 8) return *(const u4_a2*)(row + (col < d - 8 ? col : d - 8));
     u4 w = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    for (int i = 1; i < 8; ++i)
+        if (8 - i <= d) w[i >> 1] |= (uint32_t)row[d - 8 + i] << (16 * (i & 1));
     return w;
+}
+
+// The `n` last of eight values (all for 8 and more, none for less than 1) to the
+// front, zeros behind them.
+__device__ __forceinline__ void in_place(u4& w, int n) {
+    if (n >= 8) return;
+    const int by = 16 * (8 - (n > 0 ? n : 0));
+    uint64_t lo = (uint64_t)w[0] | (uint64_t)w[1] << 32, hi = (uint64_t)w[2] | (uint64_t)w[3] << 32;
+    lo = by >= 128 ? 0 : by >= 64 ? hi >> (by - 64) : lo >> by | hi << (64 - by);
+    hi = by >= 64 ? 0 : hi >> by;
+    w = (u4){(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 
 template <int T>
@@ -52,43 +71,41 @@ __device__ __forceinline__ void store8(uint16_t* p, int n, const float* v) {
         if (i < n) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
 }
 
-// Eight channels of a parameter (of the rows' type or fp32), `missing` where there is none.
-template <int T>
-__device__ __forceinline__ void param8(const NormParam& p, int col, int n, float missing, float* v) {
+// Eight channels of a parameter (of the rows' type or fp32) from `col` on, `missing`
+// where there is none.  Those past the end are any finite numbers.
+template <int T, int MODE>
+__device__ __forceinline__ void param8(const NormParam& p, int col, int d, float missing, float* v) {
+    if (!p.p) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = missing;
-    if (!p.p || n <= 0) return;
-    if (p.f32) {
-        const float* f = (const float*)p.p + col;
-        if (n >= 8) {
-            const f4 a = *(const f4_a4*)f, b = *(const f4_a4*)(f + 4);
+        for (int i = 0; i < 8; ++i) v[i] = missing;
+    } else if (!p.f32) {
+        u4 w = load8<MODE>((const uint16_t*)p.p, col, d);
+        in_place(w, d - col);
+        unpack<T>(w, v);
+    } else if (d & 7) {
+        const float* f = (const float*)p.p;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = a[i];
-                v[4 + i] = b[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n) v[i] = f[i];
-        }
+        for (int i = 0; i < 8; ++i) v[i] = f[col + i < d ? col + i : d - 1];
     } else {
-        unpack<T>(load8((const uint16_t*)p.p + col, n), v);
+        const float* f = (const float*)p.p + (col < d ? col : 0);
+        const f4 a = *(const f4_a4*)f, b = *(const f4_a4*)(f + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
     }
 }
 
-// Gate's factor and its slope.
-__device__ __forceinline__ float gate_value(float g, int act) {
-    if (act == kGateNone) return g;
-    const float s = fast_rcp(1.0f + fast_exp(-g));
-    return act == kGateSigmoid ? s : g * s;
-}
-__device__ __forceinline__ float gate_slope(float g, int act) {
-    if (act == kGateNone) return 1.0f;
-    if (act == kGateSilu) return act_slope(g, kActSilu);
-    // s (1 - s) without the difference, which loses s's neighbourhood of 1
-    const float e = fast_exp(-fabsf(g)), r = fast_rcp(1.0f + e);
-    return e * r * r;
+// Gate's factor, and its slope.  s (1 - s) comes without the difference, which loses
+// s's neighbourhood of 1.
+__device__ __forceinline__ void gate_at(float g, int act, float& value, float& slope) {
+    value = g;
+    slope = 1.0f;
+    if (act == kGateNone) return;
+    const float e = fast_exp(-fabsf(g)), r = fast_rcp(1.0f + e), s = g < 0.0f ? e * r : r, t = e * r * r;
+    value = act == kGateSigmoid ? s : g * s;
+    slope = act == kGateSigmoid ? t : __builtin_fmaf(g, t, s);
 }
 
 // Sum over the lanes of 16, of the wave.
@@ -158,7 +175,7 @@ __device__ __forceinline__ void row_stats(Group<MODE>& g, const float (&t)[V][8]
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += t[v][i];
+            for (int i = 0; i < 8; ++i) s += (v * g.width + g.lane) * 8 + i < d ? t[v][i] : 0.0f;
         mean = g.sum(s) / (float)d;
     }
     s = 0.0f;
@@ -173,7 +190,7 @@ __device__ __forceinline__ void row_stats(Group<MODE>& g, const float (&t)[V][8]
 }
 
 template <int T, int MODE, int V>
-__global__ __launch_bounds__(MODE == kBlock ? 1024 : 256) void norm_kernel(NormArgs a) {
+__global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_kernel(NormArgs a) {
     Group<MODE> g;
     const int row = MODE == kSub ? blockIdx.x * 16 + (threadIdx.x >> 4)
                                  : MODE == kWave ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
@@ -185,15 +202,18 @@ __global__ __launch_bounds__(MODE == kBlock ? 1024 : 256) void norm_kernel(NormA
     for (int v = 0; v < V; ++v) {
         col[v] = (v * g.width + g.lane) * 8;
         n[v] = in ? a.d - col[v] : 0;
-        wx[v] = load8(a.x + at * a.x_stride + col[v], n[v]);
-        wr[v] = a.res ? load8(a.res + at * a.res_stride + col[v], n[v]) : (u4){0u, 0u, 0u, 0u};
-        if (a.gate) wg[v] = load8(a.gate + at * a.gate_stride + col[v], n[v]);
+        wx[v] = load8<MODE>(a.x + at * a.x_stride, col[v], a.d);
+        if (a.res) wr[v] = load8<MODE>(a.res + at * a.res_stride, col[v], a.d);
+        if (a.gate) wg[v] = load8<MODE>(a.gate + at * a.gate_stride, col[v], a.d);
     }
     float t[V][8];
 #pragma unroll
-    for (int v = 0; v < V; ++v) unpack<T>(wx[v], t[v]);
+    for (int v = 0; v < V; ++v) {
+        in_place(wx[v], n[v]);
+        unpack<T>(wx[v], t[v]);
+    }
     float mean, rstd;
-    f4 stats = {0.0f, 0.0f, 0.0f, 0.0f};
+    f4 stats = {0.0f, 1.0f, 0.0f, 1.0f};
     if (a.post) {
         row_stats<MODE, V>(g, t, a.d, a.post, a.post_eps, mean, rstd);
         stats[0] = mean;
@@ -201,8 +221,8 @@ __global__ __launch_bounds__(MODE == kBlock ? 1024 : 256) void norm_kernel(NormA
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float w[8], b[8];
-            param8<T>(a.post_weight, col[v], n[v], 1.0f, w);
-            param8<T>(a.post_bias, col[v], n[v], 0.0f, b);
+            param8<T, MODE>(a.post_weight, col[v], a.d, 1.0f, w);
+            param8<T, MODE>(a.post_bias, col[v], a.d, 0.0f, b);
 #pragma unroll
             for (int i = 0; i < 8; ++i) t[v][i] = (t[v][i] - mean) * rstd * w[i] + b[i];
         }
@@ -210,14 +230,19 @@ __global__ __launch_bounds__(MODE == kBlock ? 1024 : 256) void norm_kernel(NormA
     if (a.res) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float s[8], r[8], y[8];
-            param8<T>(a.scale, col[v], n[v], a.scale_number, s);
+            float s[8], r[8];
+            param8<T, MODE>(a.scale, col[v], a.d, a.scale_number, s);
+            in_place(wr[v], n[v]);
             unpack<T>(wr[v], r);
             if (a.gate) {
-                float e[8];
+                float e[8], slope;
+                in_place(wg[v], n[v]);
                 unpack<T>(wg[v], e);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[v][i] *= gate_value(e[i], a.gate_act);
+                for (int i = 0; i < 8; ++i) {
+                    gate_at(e[i], a.gate_act, e[i], slope);
+                    t[v][i] *= e[i];
+                }
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) t[v][i] = r[i] + s[i] * t[v][i];
@@ -231,8 +256,8 @@ __global__ __launch_bounds__(MODE == kBlock ? 1024 : 256) void norm_kernel(NormA
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float w[8], b[8];
-            param8<T>(a.weight, col[v], n[v], 1.0f, w);
-            param8<T>(a.bias, col[v], n[v], 0.0f, b);
+            param8<T, MODE>(a.weight, col[v], a.d, 1.0f, w);
+            param8<T, MODE>(a.bias, col[v], a.d, 0.0f, b);
 #pragma unroll
             for (int i = 0; i < 8; ++i) t[v][i] = (t[v][i] - mean) * rstd * w[i] + b[i];
             if (n[v] > 0) store8<T>(a.h + at * a.h_stride + col[v], n[v], t[v]);
@@ -241,187 +266,322 @@ __global__ __launch_bounds__(MODE == kBlock ? 1024 : 256) void norm_kernel(NormA
     if (a.stats && in && g.lane == 0) *(f4*)(a.stats + 4 * at) = stats;
 }
 
+// Parameters of eight channels, as a gradient's rows use them.
+struct Channels {
+    float w[8], s[8], pw[8], pb[8];
+};
+
+// What a gradient is of: the plain norm, a residual sum, one with a gate.
+enum GradOf { kPlain, kResidual, kWithGate };
+
+template <int T, int MODE, int OF>
+__device__ __forceinline__ void load_channels(Channels& c, const NormArgs& a, int col) {
+    param8<T, MODE>(a.weight, col, a.d, 1.0f, c.w);
+    if constexpr (OF != kPlain) {
+        param8<T, MODE>(a.scale, col, a.d, a.scale_number, c.s);
+        param8<T, MODE>(a.post_weight, col, a.d, 1.0f, c.pw);
+        param8<T, MODE>(a.post_bias, col, a.d, 0.0f, c.pb);
+    }
+}
+
+// Eight channels of a row's inputs.
+struct Raw {
+    u4 x, r, g, y, h;
+};
+
+template <int MODE, int OF>
+__device__ __forceinline__ void load_raw(Raw& t, const NormGradArgs& a, size_t at, int col) {
+    const u4 zero = {0u, 0u, 0u, 0u};
+    t.x = load8<MODE>(a.f.x + at * a.f.x_stride, col, a.f.d);
+    t.h = a.dh ? load8<MODE>(a.dh + at * a.dh_stride, col, a.f.d) : zero;
+    if constexpr (OF != kPlain) {
+        t.r = load8<MODE>(a.f.res + at * a.f.res_stride, col, a.f.d);
+        t.y = a.dy ? load8<MODE>(a.dy + at * a.dy_stride, col, a.f.d) : zero;
+    }
+    if constexpr (OF == kWithGate) t.g = load8<MODE>(a.f.gate + at * a.f.gate_stride, col, a.f.d);
+}
+
+template <int OF>
+__device__ __forceinline__ void raw_in_place(Raw& t, int n) {
+    in_place(t.x, n);
+    in_place(t.h, n);
+    if constexpr (OF != kPlain) {
+        in_place(t.r, n);
+        in_place(t.y, n);
+    }
+    if constexpr (OF == kWithGate) in_place(t.g, n);
+}
+
+// Tells the compiler nothing of what the inputs are, so that what was computed of
+// them before is not kept in registers until it is needed once more.
+template <int OF>
+__device__ __forceinline__ void forget(Raw& t) {
+    asm volatile("" : "+v"(t.x), "+v"(t.h));
+    if constexpr (OF != kPlain) asm volatile("" : "+v"(t.r), "+v"(t.y));
+    if constexpr (OF == kWithGate) asm volatile("" : "+v"(t.g));
+}
+
+// i-th of eight values.
+template <int T>
+__device__ __forceinline__ float pick(const u4& w, int i) {
+    return from16<T>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu);
+}
+
+// Eight gates' factors and slopes.
+struct Gate {
+    float ga[8], slope[8];
+};
+
+template <int T, int OF>
+__device__ __forceinline__ void gates(Gate& e, const Raw& t, int act) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        e.ga[i] = e.slope[i] = 1.0f;
+        if constexpr (OF == kWithGate) gate_at(pick<T>(t.g, i), act, e.ga[i], e.slope[i]);
+    }
+}
+
+// What a row's i-th channel is forward: x^, p, q, t^, and c = dh w.  (A norm that is
+// not there has mean 0 and factor 1.)
+struct Forward {
+    float hat, p, q, that, dh, c;
+};
+
+template <int T, int OF, bool BIAS>
+__device__ __forceinline__ Forward again(const Raw& t, int i, const Gate& e, const Channels& ch, const f4& stats) {
+    Forward f;
+    f.p = pick<T>(t.x, i);
+    f.that = f.p;
+    if constexpr (OF != kPlain) {
+        f.hat = (f.p - stats[0]) * stats[1];
+        f.p = BIAS ? __builtin_fmaf(f.hat, ch.pw[i], ch.pb[i]) : f.hat * ch.pw[i];
+        f.q = OF == kWithGate ? f.p * e.ga[i] : f.p;
+        f.that = __builtin_fmaf(ch.s[i], f.q, pick<T>(t.r, i));
+    }
+    f.that = (f.that - stats[2]) * stats[3];
+    f.dh = pick<T>(t.h, i);
+    f.c = f.dh * ch.w[i];
+    return f;
+}
+
+// Sums of eight channels over rows, of the norm and of the rest.
+template <int OF, bool BIAS>
+struct Sums {
+    static constexpr int N = OF == kPlain ? 2 : kNormSums;
+    static constexpr bool has(int k) { return k < N && (BIAS || (k != kSumBias && k != kSumPostBias)); }
+    float of[N][8];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) of[k][i] = 0.0f;
+    }
+    __device__ __forceinline__ void norm(int i, const Forward& f, bool dh) {
+        of[kSumWeight][i] = __builtin_fmaf(f.dh, dh ? f.that : 0.0f, of[kSumWeight][i]);
+        if constexpr (BIAS) of[kSumBias][i] += f.dh;
+    }
+    __device__ __forceinline__ void rest(int i, const Forward& f, float dt, float dp) {
+        of[kSumScale][i] = __builtin_fmaf(dt, f.q, of[kSumScale][i]);
+        of[kSumPostWeight][i] = __builtin_fmaf(dp, f.hat, of[kSumPostWeight][i]);
+        if constexpr (BIAS) of[kSumPostBias][i] += dp;
+    }
+};
+
+// dy' of a channel; `in`: of h's gradient too.
+template <int T, int OF>
+__device__ __forceinline__ float total(const Forward& f, const Raw& t, int i, const f4& stats, float c1, float c2,
+                                       bool in) {
+    const float dy = OF == kPlain ? 0.0f : pick<T>(t.y, i);
+    return in ? __builtin_fmaf(stats[3], f.c - f.that * c1 - c2, dy) : dy;
+}
+
 // Gradients.  With c = dh w, t^ = (y - mean) rstd,
 //   dy' = dy + rstd (c - t^ mean(c t^) - mean(c))       (the last for "layer"),
 //   dres = dy',  ds = sum of dy' q,  dgate = dy' s p ga'(g),  dp = dy' s ga(g),
 // and dx from dp as dy' from dh.  y and the norms are computed anew from the inputs
-// and the rows' saved means and factors, so nothing of y's rounding enters.  A
-// group goes through its rows with the channels' sums in registers; a workgroup
-// leaves one row of partial sums, which norm_sums_kernel adds in order.
-template <int T, int MODE, int V, bool SUMS>
-__global__ __launch_bounds__(MODE == kBlock ? 1024 : 256) void norm_bwd_kernel(NormGradArgs a) {
+// and the rows' saved means and factors, so nothing of y's rounding enters; and again
+// after each sum over the row, which costs less than registers for it.
+//
+// V = 1: a group goes through its rows with the parameters and (SUMS) the channels'
+// sums in registers, a row's inputs on their way while the row before is worked on,
+// and a workgroup leaves one row of partial sums, which norm_sums_kernel adds in
+// order.  Wider rows have no registers for that: they leave their rows' projections,
+// from which norm_channels_kernel sums the channels.
+template <int T, int MODE, int V, int OF, bool SUMS, bool BIAS>
+__global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bwd_kernel(NormGradArgs a) {
+    static_assert(!SUMS || V == 1, "sums of one eight a lane");
     Group<MODE> g;
     constexpr int R = MODE == kSub ? 16 : MODE == kWave ? 4 : 1;        // rows of a workgroup at a time
     const int sub = MODE == kSub ? threadIdx.x >> 4 : MODE == kWave ? threadIdx.x >> 6 : 0;
-    float sums[SUMS ? kNormSums : 1][V][8];
-    if constexpr (SUMS)
+    const int d = a.f.d, step = gridDim.x * R;
+    const float inv = 1.0f / (float)d;
+    struct Row {
+        Raw raw[V];
+        f4 stats;
+    };
+    auto load = [&](Row& t, int row) {
+        const size_t at = row < a.f.rows ? row : 0;
+        t.stats = *(const f4*)(a.f.stats + 4 * at);
 #pragma unroll
-        for (int k = 0; k < kNormSums; ++k)
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sums[k][v][i] = 0.0f;
-    const float inv = 1.0f / (float)a.f.d;
-    for (int base = blockIdx.x * R; base < a.f.rows; base += gridDim.x * R) {
+        for (int v = 0; v < V; ++v) load_raw<MODE, OF>(t.raw[v], a, at, (v * g.width + g.lane) * 8);
+    };
+    Sums<OF, BIAS> sums;
+    if constexpr (SUMS) sums.clear();
+    Channels kept;
+    Row next;
+    if constexpr (V == 1) {
+        load(next, blockIdx.x * R + sub);
+        load_channels<T, MODE, OF>(kept, a.f, g.lane * 8);
+    }
+    for (int base = blockIdx.x * R; base < a.f.rows; base += step) {
         const int row = base + sub;
         const bool in = row < a.f.rows;
         const size_t at = in ? row : 0;
-        const f4 stats = *(const f4*)(a.f.stats + 4 * at);
-        int n[V];
-        u4 wx[V], wr[V], wg[V], wy[V], wh[V];
-        const u4 zero = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int col = (v * g.width + g.lane) * 8;
-            n[v] = in ? a.f.d - col : 0;
-            wx[v] = load8(a.f.x + at * a.f.x_stride + col, n[v]);
-            wr[v] = a.f.res ? load8(a.f.res + at * a.f.res_stride + col, n[v]) : zero;
-            wg[v] = a.f.gate ? load8(a.f.gate + at * a.f.gate_stride + col, n[v]) : zero;
-            wy[v] = a.dy ? load8(a.dy + at * a.dy_stride + col, n[v]) : zero;
-            wh[v] = a.dh ? load8(a.dh + at * a.dh_stride + col, n[v]) : zero;
+        Row now;
+        if constexpr (V == 1) {
+            now = next;
+            if (base + step < a.f.rows) load(next, row + step);
+        } else {
+            load(now, row);
         }
-        float hat[V][8], that[V][8], p[V][8], q[V][8], dt[V][8], c[V][8];
+        Gate gate;                      // (of one eight kept for what follows the sum)
         float two[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int col = (v * g.width + g.lane) * 8;
-            float w[8], b[8], s[8];
-            unpack<T>(wx[v], hat[v]);
-            if (a.f.post) {
-                param8<T>(a.f.post_weight, col, n[v], 1.0f, w);
-                param8<T>(a.f.post_bias, col, n[v], 0.0f, b);
+            const int col = (v * g.width + g.lane) * 8, n = in ? d - col : 0;
+            raw_in_place<OF>(now.raw[v], n);
+            gates<T, OF>(gate, now.raw[v], a.f.gate_act);
+            Channels ch;
+            if constexpr (V == 1) ch = kept;
+            else load_channels<T, MODE, OF>(ch, a.f, col);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    hat[v][i] = i < n[v] ? (hat[v][i] - stats[0]) * stats[1] : 0.0f;
-                    p[v][i] = hat[v][i] * w[i] + b[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) p[v][i] = hat[v][i];
+            for (int i = 0; i < 8; ++i) {
+                const Forward f = again<T, OF, BIAS>(now.raw[v], i, gate, ch, now.stats);
+                two[0] = __builtin_fmaf(f.c, f.that, two[0]);
+                two[1] += f.c;
+                if constexpr (SUMS) sums.norm(i, f, a.dh);
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[v][i] = p[v][i];
-            if (a.f.gate) {
-                float e[8];
-                unpack<T>(wg[v], e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[v][i] *= gate_value(e[i], a.f.gate_act);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) that[v][i] = q[v][i];
-            if (a.f.res) {
-                float r[8];
-                unpack<T>(wr[v], r);
-                param8<T>(a.f.scale, col, n[v], a.f.scale_number, s);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) that[v][i] = r[i] + s[i] * q[v][i];
-            }
-            unpack<T>(wy[v], dt[v]);
-            if (a.dh) {
-                float dh[8];
-                unpack<T>(wh[v], dh);
-                param8<T>(a.f.weight, col, n[v], 1.0f, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    that[v][i] = i < n[v] ? (that[v][i] - stats[2]) * stats[3] : 0.0f;
-                    c[v][i] = dh[i] * w[i];
-                    two[0] = __builtin_fmaf(c[v][i], that[v][i], two[0]);
-                    two[1] += c[v][i];
-                    if constexpr (SUMS) {
-                        sums[kSumWeight][v][i] = __builtin_fmaf(dh[i], that[v][i], sums[kSumWeight][v][i]);
-                        sums[kSumBias][v][i] += dh[i];
-                    }
-                }
-            }
+            if (V > 1) __builtin_amdgcn_sched_barrier(0);       // (one eight's registers at a time)
         }
+        float c1 = 0.0f, c2 = 0.0f;
         if (a.dh) {
             g.sum(two);
-            const float c1 = two[0] * inv, c2 = a.f.kind == kNormLayer ? two[1] * inv : 0.0f;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dt[v][i] += stats[3] * (c[v][i] - that[v][i] * c1 - c2);
+            c1 = two[0] * inv;
+            if (a.f.kind == kNormLayer) c2 = two[1] * inv;
         }
+        if (V > 1 && a.means && threadIdx.x == 0) {
+            a.means[2 * at] = c1;
+            a.means[2 * at + 1] = c2;
+        }
+        float dp[V][8];
         two[0] = two[1] = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int col = (v * g.width + g.lane) * 8;
-            if (a.dres && n[v] > 0) store8<T>(a.dres + at * a.f.d + col, n[v], dt[v]);
-            if (a.f.res) {
-                float s[8];
-                param8<T>(a.f.scale, col, n[v], a.f.scale_number, s);
+            const int col = (v * g.width + g.lane) * 8, n = in ? d - col : 0, nh = a.dh ? n : 0;
+            forget<OF>(now.raw[v]);
+            Channels ch;
+            if constexpr (V == 1) ch = kept;
+            else load_channels<T, MODE, OF>(ch, a.f, col);
+            if (V > 1) gates<T, OF>(gate, now.raw[v], a.f.gate_act);
+            float dt[8], dg[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if constexpr (SUMS)
-                        sums[kSumScale][v][i] = __builtin_fmaf(i < n[v] ? dt[v][i] : 0.0f, q[v][i], sums[kSumScale][v][i]);
-                    dt[v][i] *= s[i];
+            for (int i = 0; i < 8; ++i) {
+                const Forward f = again<T, OF, BIAS>(now.raw[v], i, gate, ch, now.stats);
+                dt[i] = total<T, OF>(f, now.raw[v], i, now.stats, c1, c2, i < nh);
+                dp[v][i] = dt[i];
+                if constexpr (OF != kPlain) {
+                    const float ds = dt[i] * ch.s[i], to = OF == kWithGate ? ds * gate.ga[i] : ds;
+                    dg[i] = ds * f.p * gate.slope[i];
+                    if constexpr (SUMS) sums.rest(i, f, dt[i], to);
+                    dp[v][i] = to * ch.pw[i];
+                    two[0] = __builtin_fmaf(dp[v][i], f.hat, two[0]);
+                    two[1] += dp[v][i];
                 }
             }
-            if (a.f.gate) {
-                float e[8], o[8];
-                unpack<T>(wg[v], e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    o[i] = dt[v][i] * p[v][i] * gate_slope(e[i], a.f.gate_act);
-                    dt[v][i] *= gate_value(e[i], a.f.gate_act);
-                }
-                if (a.dgate && n[v] > 0) store8<T>(a.dgate + at * a.f.d + col, n[v], o);
-            }
-            if (a.f.post) {
-                float w[8];
-                param8<T>(a.f.post_weight, col, n[v], 1.0f, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float dp = i < n[v] ? dt[v][i] : 0.0f;
-                    c[v][i] = dp * w[i];
-                    two[0] = __builtin_fmaf(c[v][i], hat[v][i], two[0]);
-                    two[1] += c[v][i];
-                    if constexpr (SUMS) {
-                        sums[kSumPostWeight][v][i] = __builtin_fmaf(dp, hat[v][i], sums[kSumPostWeight][v][i]);
-                        sums[kSumPostBias][v][i] += dp;
-                    }
-                }
-            }
+            if constexpr (OF != kPlain)
+                if (a.dres && n > 0) store8<T>(a.dres + at * d + col, n, dt);
+            if constexpr (OF == kWithGate)
+                if (a.dgate && n > 0) store8<T>(a.dgate + at * d + col, n, dg);
+            if (V > 1) __builtin_amdgcn_sched_barrier(0);
         }
-        if (a.f.post) {
+        if (OF != kPlain && a.f.post) {
             g.sum(two);
-            const float c1 = two[0] * inv, c2 = a.f.post == kNormLayer ? two[1] * inv : 0.0f;
+            const float e1 = two[0] * inv, e2 = a.f.post == kNormLayer ? two[1] * inv : 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dt[v][i] = stats[1] * (c[v][i] - hat[v][i] * c1 - c2);
+                for (int i = 0; i < 8; ++i)
+                    dp[v][i] = now.stats[1] * (dp[v][i] - (pick<T>(now.raw[v].x, i) - now.stats[0]) * now.stats[1] * e1 - e2);
         }
         if (a.dx)
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (n[v] > 0) store8<T>(a.dx + at * a.f.d + (v * g.width + g.lane) * 8, n[v], dt[v]);
+            for (int v = 0; v < V; ++v) {
+                const int col = (v * g.width + g.lane) * 8, n = in ? d - col : 0;
+                if (n > 0) store8<T>(a.dx + at * d + col, n, dp[v]);
+            }
     }
     if constexpr (SUMS) {
         // [sum][workgroup][d]
         __shared__ float join[MODE == kBlock ? 1 : 256 * 8];
+        const int col = g.lane * 8;
 #pragma unroll
-        for (int k = 0; k < kNormSums; ++k) {
-            if (!a.dparam[k].p) continue;
-            float* out = a.part + ((size_t)a.place[k] * gridDim.x + blockIdx.x) * a.f.d;
+        for (int k = 0; k < Sums<OF, BIAS>::N; ++k) {
+            if (!Sums<OF, BIAS>::has(k) || !a.dparam[k].p) continue;
+            float* out = a.part + ((size_t)a.place[k] * gridDim.x + blockIdx.x) * d;
+            if constexpr (MODE != kBlock) {
+                __syncthreads();
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int col = (v * g.width + g.lane) * 8;
-                if constexpr (MODE != kBlock) {
-                    __syncthreads();
+                for (int i = 0; i < 8; ++i) join[i * 256 + threadIdx.x] = sums.of[k][i];
+                __syncthreads();
+                if (sub != 0) continue;
+                for (int o = 1; o < R; ++o)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) join[threadIdx.x * 8 + i] = sums[k][v][i];
-                    __syncthreads();
-                    if (sub == 0)
-                        for (int o = 1; o < R; ++o)
+                    for (int i = 0; i < 8; ++i) sums.of[k][i] += join[i * 256 + threadIdx.x + o * g.width];
+            }
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) sums[k][v][i] += join[(threadIdx.x + o * g.width) * 8 + i];
-                    if (sub != 0) continue;
-                }
+            for (int i = 0; i < 8; ++i)
+                if (col + i < d) out[col + i] = sums.of[k][i];
+        }
+    }
+}
+
+// The channels' sums of wide rows, from the inputs and the rows' projections: a
+// workgroup takes 2048 channels of every gridDim.y-th row.
+template <int T, int OF, bool BIAS>
+__global__ __launch_bounds__(256) void norm_channels_kernel(NormGradArgs a) {
+    const int d = a.f.d, col = (blockIdx.x * 256 + threadIdx.x) * 8, n = d - col;
+    if (n <= 0) return;
+    Channels ch;
+    load_channels<T, kBlock, OF>(ch, a.f, col);
+    Sums<OF, BIAS> sums;
+    sums.clear();
+    Raw next;
+    load_raw<kBlock, OF>(next, a, blockIdx.y, col);
+    for (int row = blockIdx.y; row < a.f.rows; row += gridDim.y) {
+        Raw now = next;
+        const f4 stats = *(const f4*)(a.f.stats + 4 * (size_t)row);
+        const float c1 = a.means[2 * (size_t)row], c2 = a.means[2 * (size_t)row + 1];
+        if (row + (int)gridDim.y < a.f.rows) load_raw<kBlock, OF>(next, a, row + gridDim.y, col);
+        raw_in_place<OF>(now, n);
+        Gate gate;
+        gates<T, OF>(gate, now, a.f.gate_act);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (col + i < a.f.d) out[col + i] = sums[k][v][i];
+        for (int i = 0; i < 8; ++i) {
+            const Forward f = again<T, OF, BIAS>(now, i, gate, ch, stats);
+            sums.norm(i, f, a.dh);
+            if constexpr (OF != kPlain) {
+                const float dt = total<T, OF>(f, now, i, stats, c1, c2, a.dh && i < n);
+                sums.rest(i, f, dt, dt * ch.s[i] * gate.ga[i]);
             }
         }
+    }
+#pragma unroll
+    for (int k = 0; k < Sums<OF, BIAS>::N; ++k) {
+        if (!Sums<OF, BIAS>::has(k) || !a.dparam[k].p) continue;
+        float* out = a.part + ((size_t)a.place[k] * gridDim.y + blockIdx.y) * d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) out[col + i] = sums.of[k][i];
     }
 }
 
@@ -455,48 +615,82 @@ struct Shape {
 Shape norm_shape(int d) {
     if (d <= 128) return {kSub, 1, 256, 16};
     if (d <= 512) return {kWave, 1, 256, 4};
-    if (d <= 1024) return {kWave, 2, 256, 4};
-    const int v = d <= 8192 ? 1 : d <= 16384 ? 2 : 4;
+    const int most = 512 * kRowWaves, v = d <= 4 * most ? (d + most - 1) / most : 6;
     return {kBlock, v, (d + 512 * v - 1) / (512 * v) * 64, 1};
 }
 
-template <int T, typename F>
+template <typename F>
 void with_shape(const Shape& s, F f) {
     using std::integral_constant;
     if (s.mode == kSub) f(integral_constant<int, kSub>(), integral_constant<int, 1>());
-    else if (s.mode == kWave && s.v == 1) f(integral_constant<int, kWave>(), integral_constant<int, 1>());
-    else if (s.mode == kWave) f(integral_constant<int, kWave>(), integral_constant<int, 2>());
+    else if (s.mode == kWave) f(integral_constant<int, kWave>(), integral_constant<int, 1>());
     else if (s.v == 1) f(integral_constant<int, kBlock>(), integral_constant<int, 1>());
     else if (s.v == 2) f(integral_constant<int, kBlock>(), integral_constant<int, 2>());
-    else f(integral_constant<int, kBlock>(), integral_constant<int, 4>());
+    else if (s.v == 3) f(integral_constant<int, kBlock>(), integral_constant<int, 3>());
+    else if (s.v == 4) f(integral_constant<int, kBlock>(), integral_constant<int, 4>());
+    else f(integral_constant<int, kBlock>(), integral_constant<int, 6>());
 }
 
 template <int T>
 void forward(const NormArgs& a, hipStream_t s) {
     const Shape sh = norm_shape(a.d);
     const dim3 grid((a.rows + sh.rows - 1) / sh.rows), block(sh.threads);
-    with_shape<T>(sh, [&](auto mode, auto v) {
+    with_shape(sh, [&](auto mode, auto v) {
         hipLaunchKernelGGL((norm_kernel<T, decltype(mode)::value, decltype(v)::value>), grid, block, 0, s, a);
     });
 }
 
-// Workgroups of a gradient, each of which leaves a part of the channels' sums.
-int norm_parts(int rows, int d) {
-    const int r = norm_shape(d).rows, all = (rows + r - 1) / r;
-    return all < 2 * kCUs ? all : 2 * kCUs;
+// A gradient's workgroups, and the parts of the channels' sums: as many of either as
+// are on the compute units at once, by their waves.
+struct NormPlan {
+    int groups, parts;
+    bool apart;                         // sums by norm_channels_kernel
+    size_t means, total;
+};
+
+NormPlan norm_plan(int rows, int d, int sums) {
+    const Shape sh = norm_shape(d);
+    NormPlan p;
+    const int all = (rows + sh.rows - 1) / sh.rows, most = kRowWaves / (sh.threads / 64) * kCUs;
+    p.groups = all < most ? all : most;
+    p.apart = sums && sh.v > 1;
+    p.parts = p.groups;
+    if (p.apart) {
+        const int fill = kRowWaves / 4 * kCUs / ((d + 2047) / 2048);
+        p.parts = rows < fill ? rows : fill;
+    }
+    p.means = ((size_t)sums * p.parts * d * 4 + 255) & ~(size_t)255;
+    p.total = p.apart ? p.means + (size_t)rows * 8 : (size_t)sums * p.parts * d * 4;
+    return p;
+}
+
+template <int T, int OF, bool BIAS>
+void backward_of(const NormGradArgs& a, const NormPlan& p, bool sums, hipStream_t s) {
+    const Shape sh = norm_shape(a.f.d);
+    with_shape(sh, [&](auto mode, auto v) {
+        constexpr int M = decltype(mode)::value, V = decltype(v)::value;
+        auto* kernel = norm_bwd_kernel<T, M, V, OF, false, BIAS>;
+        if constexpr (V == 1)
+            if (sums) kernel = norm_bwd_kernel<T, M, V, OF, true, BIAS>;
+        hipLaunchKernelGGL(kernel, dim3(p.groups), dim3(sh.threads), 0, s, a);
+    });
+    if (p.apart)
+        hipLaunchKernelGGL((norm_channels_kernel<T, OF, BIAS>), dim3((a.f.d + 2047) / 2048, p.parts), dim3(256), 0, s, a);
 }
 
 template <int T>
-void backward(const NormGradArgs& a, int sums, hipStream_t s) {
-    const Shape sh = norm_shape(a.f.d);
-    const int parts = norm_parts(a.f.rows, a.f.d);
-    with_shape<T>(sh, [&](auto mode, auto v) {
-        constexpr int M = decltype(mode)::value, V = decltype(v)::value;
-        if (sums) hipLaunchKernelGGL((norm_bwd_kernel<T, M, V, true>), dim3(parts), dim3(sh.threads), 0, s, a);
-        else hipLaunchKernelGGL((norm_bwd_kernel<T, M, V, false>), dim3(parts), dim3(sh.threads), 0, s, a);
-    });
+void backward(const NormGradArgs& a, const NormPlan& p, int sums, hipStream_t s) {
+    const bool bias = a.f.post_bias.p || a.dparam[kSumBias].p || a.dparam[kSumPostBias].p;
+    auto of = [&](auto what) {
+        constexpr int OF = decltype(what)::value;
+        if (bias) backward_of<T, OF, true>(a, p, sums > 0, s);
+        else backward_of<T, OF, false>(a, p, sums > 0, s);
+    };
+    if (!a.f.res) of(std::integral_constant<int, kPlain>());
+    else if (!a.f.gate) of(std::integral_constant<int, kResidual>());
+    else of(std::integral_constant<int, kWithGate>());
     if (sums)
-        hipLaunchKernelGGL(norm_sums_kernel, dim3((a.f.d + 63) / 64, sums), dim3(1024), 0, s, a, parts, T);
+        hipLaunchKernelGGL(norm_sums_kernel, dim3((a.f.d + 63) / 64, sums), dim3(1024), 0, s, a, p.parts, T);
 }
 
 }  // namespace
@@ -507,17 +701,17 @@ hipError_t launch_norm(const NormArgs& a, int type, hipStream_t s) {
     return hipGetLastError();
 }
 
-size_t norm_bwd_ws_bytes(int rows, int d, int sums) {
-    return rows ? (size_t)norm_parts(rows, d) * d * 4 * sums : 0;
-}
+size_t norm_bwd_ws_bytes(int rows, int d, int sums) { return rows ? norm_plan(rows, d, sums).total : 0; }
 
 hipError_t launch_norm_bwd(NormGradArgs a, int type, void* ws, hipStream_t s) {
-    a.part = (float*)ws;
     int sums = 0;
     for (int k = 0; k < kNormSums; ++k)
         if (a.dparam[k].p) a.place[k] = sums++;
-    if (type == kBf16) backward<kBf16>(a, sums, s);
-    else backward<kF16>(a, sums, s);
+    const NormPlan p = norm_plan(a.f.rows, a.f.d, sums);
+    a.part = (float*)ws;
+    a.means = p.apart ? (float*)((uint8_t*)ws + p.means) : nullptr;
+    if (type == kBf16) backward<kBf16>(a, p, sums, s);
+    else backward<kF16>(a, p, sums, s);
     return hipGetLastError();
 }
 

@@ -243,8 +243,9 @@ struct NormGradArgs {
     NormSum dparam[kNormSums];
     int place[kNormSums];               // of the sums in part
     float* part;                        // [place][workgroup][d]
+    float* means;                       // [rows][2] of the norm of y's projections, or NULL
 };
-constexpr int kNormMaxD = 32768;        // 16 waves of four eights a lane
+constexpr int kNormMaxD = 32768;        // within 12 waves of six eights a lane
 hipError_t launch_norm(const NormArgs& a, int type, hipStream_t s);
 size_t norm_bwd_ws_bytes(int rows, int d, int sums);
 hipError_t launch_norm_bwd(NormGradArgs a, int type, void* ws, hipStream_t s);

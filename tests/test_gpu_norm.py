@@ -128,6 +128,18 @@ def test_residual_norm(xt, kind, post, act, scale, m, d, dtype, pt):
         assert _off(h, wh) <= R.roundoff(dtype) + 2e-5
 
 
+def test_means_of_ragged_rows(xt):
+    """A centred norm after a centred norm with a bias: what lies past a row's end is none of its mean."""
+    for d in (9, 127, 130, 513, 1030, 2049, 6150, 13000):
+        x = (5.0 + _rows(3, d, torch.float32, d, spread=0.0)).to(torch.float16)
+        r = _rows(3, d, torch.float16, 2, spread=0.0)
+        pw, pb = _param(d, torch.float32, 3, 1.0), _param(d, torch.float32, 4, 2.0)
+        y, h = xt.residual_norm(x, r, kind="layer", post="layer", post_weight=pw, post_bias=pb)
+        wy = r.double() + _normed(x.double(), "layer", pw.double(), pb.double(), 1e-6)
+        assert _off(y, wy) <= R.roundoff(torch.float16) + 2e-5
+        assert _off(h, _normed(wy, "layer", None, None, 1e-6)) <= R.roundoff(torch.float16) + 2e-5
+
+
 def _gradients(v, douts, kind, post, act, number, eps, post_eps):
     """Gradients in 64 bits."""
     leaves = {n: t.detach().double().requires_grad_() for n, t in v.items()}
