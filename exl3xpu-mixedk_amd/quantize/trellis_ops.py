@@ -484,45 +484,67 @@ NORMS = {None: 0, "rms": 1, "layer": 2}
 GATES = {"none": 0, "sigmoid": 1, "silu": 2}
 _MAX_D = 32768
 _PARAMS = ("weight", "bias", "scale", "post_weight", "post_bias")
+_FIVE = ctypes.c_void_p * 5
+
+
+def _as(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised rows like t's.  (empty_like takes 1.1 us of the host, empty with
+    shape, type and device 2.2; but it keeps a transposed tensor's strides.)"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _norm_params(cfg, params):
+    """The C entries' structure, and the tensors that it points to."""
+    kind, post, gate_act, eps, post_eps, number = cfg
+    f32, bit, kept, at = 0, 1, [], []
+    for p in params:
+        if p is None:
+            at.append(None)
+        else:
+            p = p.contiguous()
+            kept.append(p)
+            at.append(p.data_ptr())
+            if p.dtype is torch.float32:
+                f32 |= bit
+        bit <<= 1
+    return _hb.NormParams(kind, post, gate_act, f32, eps, post_eps, number, *at), kept
 
 
 def _norm_rows(t, d):
-    """Address and stride of rows (None: none)."""
-    return (None, 0) if t is None else (t.data_ptr(), _stride(t))
+    """Rows, their address and stride (None: none)."""
+    if t is None:
+        return None, None, 0
+    t = _rows(t, d)
+    return t, t.data_ptr(), _stride(t)
 
 
-def _norm_struct(cfg, params):
-    kind, post, gate_act, eps, post_eps, number = cfg
-    return _hb.NormParams(kind, post, gate_act, _f32_bits(params), eps, post_eps, number,
-                          *(None if p is None else p.data_ptr() for p in params))
-
-
-def _norm_forward(x, res, gate, params, cfg, keep):
+def _residual_forward(x, res, gate, params, cfg, keep):
     d = x.shape[-1]
-    y = None if res is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if cfg[0] else None
-    rows = _rows(x, d)
+    y, h = _as(x), _as(x) if cfg[0] else None
+    rows, xp, xs = _norm_rows(x, d)
     m = rows.shape[0]
-    stats = torch.empty(m, 4, dtype=torch.float32, device=x.device) if keep else None
+    stats = torch.empty((m, 4), dtype=torch.float32, device=x.device) if keep else None
     if m == 0:
         return y, h, stats
-    res, gate = (None if t is None else _rows(t, d) for t in (res, gate))
-    params = [None if p is None else p.contiguous() for p in params]
-    with _on(x.device):
+    res, rp, rs = _norm_rows(res, d)
+    gate, gp, gs = _norm_rows(gate, d)
+    struct, params = _norm_params(cfg, params)
+    dev = x.device
+    with _on(dev):
         rc = _hb.lib().xtq_norm_dev(
-            ctypes.byref(_norm_struct(cfg, params)), _TYPES[x.dtype], m, d, *_norm_rows(rows, d),
-            *_norm_rows(res, d), *_norm_rows(gate, d), None if y is None else y.data_ptr(), d,
-            None if h is None else h.data_ptr(), d, None if stats is None else stats.data_ptr(),
-            _stream(x.device))
-    _hb._check("xtq_norm_dev", rc)
+            ctypes.byref(struct), _TYPES[x.dtype], m, d, xp, xs, rp, rs, gp, gs,
+            y.data_ptr(), d, None if h is None else h.data_ptr(), d,
+            None if stats is None else stats.data_ptr(), _stream(dev))
+    if rc:
+        _hb._check("xtq_norm_dev", rc)
     return y, h, stats
 
 
-class _Norm(torch.autograd.Function):
+class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, res, gate, weight, bias, scale, post_weight, post_bias, cfg):
         params = (weight, bias, scale, post_weight, post_bias)
-        y, h, stats = _norm_forward(x, res, gate, params, cfg, True)
+        y, h, stats = _residual_forward(x, res, gate, params, cfg, True)
         ctx.cfg = cfg
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, res, gate, *params, stats)
@@ -531,61 +553,108 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh):
-        x, res, gate, *params, stats = ctx.saved_tensors
+        inputs = ctx.saved_tensors
         _no_tangents("the norm's gradient", dy, dh)
-        want = ctx.needs_input_grad[:8]
+        x, res, gate = inputs[:3]
+        grads = [_as(t) if w else None for w, t in zip(ctx.needs_input_grad, inputs[:8])]
         d = x.shape[-1]
-        rows = _rows(x, d)
+        rows, xp, xs = _norm_rows(x, d)
         m = rows.shape[0]
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if w else None
-                 for w, t in zip(want, (x, res, gate, *params))]
         if m == 0:
             return (*(g if g is None else g.zero_() for g in grads), None)
-        res, gate, dy, dh = (None if t is None else _rows(t, d) for t in (res, gate, dy, dh))
-        params = [None if p is None else p.contiguous() for p in params]
-        L = _hb.lib()
+        res, rp, rs = _norm_rows(res, d)
+        gate, gp, gs = _norm_rows(gate, d)
+        dy, dyp, dys = _norm_rows(dy, d)
+        dh, dhp, dhs = _norm_rows(dh, d)
+        struct, params = _norm_params(ctx.cfg, inputs[3:8])
         out = [None if g is None else g.data_ptr() for g in grads]
-        with _on(x.device):
-            need = L.xtq_norm_bwd_ws_bytes(m, d, sum(p is not None for p in out[3:]))
-            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+        sums = sum(p is not None for p in out[3:])
+        L, dev, ws, need = _hb.lib(), x.device, None, 0
+        with _on(dev):
+            if sums:
+                need = L.xtq_norm_bwd_ws_bytes(m, d, sums)
+                ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
             rc = L.xtq_norm_bwd_dev(
-                ctypes.byref(_norm_struct(ctx.cfg, params)), _TYPES[x.dtype], m, d, *_norm_rows(rows, d),
-                *_norm_rows(res, d), *_norm_rows(gate, d), stats.data_ptr(), *_norm_rows(dy, d),
-                *_norm_rows(dh, d), *out[:3], (ctypes.c_void_p * 5)(*out[3:]), ws.data_ptr(), ws.numel(),
-                _stream(x.device))
-        _hb._check("xtq_norm_bwd_dev", rc)
+                ctypes.byref(struct), _TYPES[x.dtype], m, d, xp, xs, rp, rs, gp, gs, inputs[8].data_ptr(),
+                dyp, dys, dhp, dhs, *out[:3], _FIVE(*out[3:]), None if ws is None else ws.data_ptr(), need,
+                _stream(dev))
+        if rc:
+            _hb._check("xtq_norm_bwd_dev", rc)
         return (*grads, None)
 
 
-def _norm(name, x, res, gate, params, kind, post, gate_act, eps, post_eps, number):
+def _check_norm_rows(name, x):
     if x.dtype not in _TYPES:
         raise ValueError(f"{name}'s rows must be bfloat16 or float16, got {x.dtype}")
     if not x.is_cuda:
         raise ValueError(f"{name}'s rows must be a HIP device tensor, got {x.device}")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= _MAX_D:
         raise ValueError(f"{name}'s rows must be [.., 1 to {_MAX_D}], got {tuple(x.shape)}")
-    for t, what in ((res, "residual"), (gate, "gate")):
-        if t is not None:
-            _like(t, x, x.shape, what, (x.dtype,))
-    for t, what in zip(params, _PARAMS):
-        if t is not None:
-            _like(t, x, x.shape[-1:], what, (x.dtype, torch.float32))
-    for k in (kind, post):
-        if k not in NORMS:
-            raise ValueError(f"norm {k!r} not in {tuple(NORMS)}")
-    if gate_act not in GATES:
-        raise ValueError(f"gate_act {gate_act!r} not in {tuple(GATES)}")
-    if not (eps >= 0 and post_eps >= 0):
-        raise ValueError(f"eps must be at least 0, got {eps}, {post_eps}")
-    if (kind is None and any(t is not None for t in params[:2])) or \
-            (post is None and any(t is not None for t in params[3:])):
-        raise ValueError("weights and biases are of a norm that there is")
-    tensors = (x, res, gate, *params)
-    _no_tangents(name, *tensors)
-    cfg = (NORMS[kind], NORMS[post], GATES[gate_act], float(eps), float(post_eps), float(number))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _Norm.apply(*tensors, cfg)
-    return _norm_forward(x, res, gate, params, cfg, False)[:2]
+
+
+def _plain_struct(kind, eps, weight, bias):
+    return _hb.NormParams(
+        kind, 0, 0, (weight is not None and weight.dtype is torch.float32)
+        | (bias is not None and bias.dtype is torch.float32) << 1, eps, eps, 1.0,
+        None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+        None, None, None)
+
+
+def _plain_forward(x, weight, bias, kind, eps, keep):
+    """What _residual_forward does, for the norm alone, at less of the host's time."""
+    dev, d = x.device, x.shape[-1]
+    h = _as(x)
+    rows = _rows(x, d)
+    m = rows.shape[0]
+    stats = torch.empty((m, 4), dtype=torch.float32, device=dev) if keep else None
+    if m == 0:
+        return h, stats
+    weight, bias = None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
+    with _on(dev):
+        rc = _hb.lib().xtq_norm_dev(
+            ctypes.byref(_plain_struct(kind, eps, weight, bias)), _TYPES[x.dtype], m, d, rows.data_ptr(),
+            _stride(rows), None, 0, None, 0, None, 0, h.data_ptr(), d,
+            None if stats is None else stats.data_ptr(), _stream(dev))
+    if rc:
+        _hb._check("xtq_norm_dev", rc)
+    return h, stats
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, kind, eps):
+        h, stats = _plain_forward(x, weight, bias, kind, eps, True)
+        ctx.kind, ctx.eps = kind, eps
+        ctx.save_for_backward(x, weight, bias, stats)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, weight, bias, stats = ctx.saved_tensors
+        _no_tangents("norm's gradient", dh)
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dx, dw, db = _as(x) if want_x else None, _as(weight) if want_w else None, _as(bias) if want_b else None
+        dev, d = x.device, x.shape[-1]
+        rows, dh = _rows(x, d), _rows(dh, d)
+        m, sums, need, ws = rows.shape[0], want_w + want_b, 0, None
+        if m == 0:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
+        weight = None if weight is None else weight.contiguous()
+        L = _hb.lib()
+        with _on(dev):
+            if sums:
+                need = L.xtq_norm_bwd_ws_bytes(m, d, sums)
+                ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
+            rc = L.xtq_norm_bwd_dev(
+                ctypes.byref(_plain_struct(ctx.kind, ctx.eps, weight, bias)), _TYPES[x.dtype], m, d,
+                rows.data_ptr(), _stride(rows), None, 0, None, 0, stats.data_ptr(), None, 0, dh.data_ptr(),
+                _stride(dh), None if dx is None else dx.data_ptr(), None, None,
+                _FIVE(None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr()),
+                None if ws is None else ws.data_ptr(), need, _stream(dev))
+        if rc:
+            _hb._check("xtq_norm_bwd_dev", rc)
+        return dx, dw, db, None, None
 
 
 def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -595,9 +664,20 @@ def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor
     same without the mean for "rms".  weight and bias [d] have x's type or fp32 (None:
     1 and 0).  Differentiable in all three (once, in reverse mode).  A row's result is
     the same whatever rows are beside it."""
-    if kind is None:
-        raise ValueError("kind must be 'rms' or 'layer'")
-    return _norm("norm", x, None, None, (weight, bias, None, None, None), kind, None, "none", eps, eps, 1.0)[1]
+    _check_norm_rows("norm", x)
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _like(t, x, x.shape[-1:], what, (x.dtype, torch.float32))
+    number = NORMS.get(kind)
+    if not number:
+        raise ValueError(f"kind {kind!r} must be 'rms' or 'layer'")
+    if not eps >= 0:
+        raise ValueError(f"eps must be at least 0, got {eps}")
+    _no_tangents("norm", x, weight, bias)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _Norm.apply(x, weight, bias, number, float(eps))
+    return _plain_forward(x, weight, bias, number, float(eps), False)[0]
 
 
 def residual_norm(block: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
@@ -612,10 +692,33 @@ def residual_norm(block: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
     shape and type; gate_act: none (the gate itself), sigmoid or silu; scale is a number
     or [d]; scale, weights and biases [d] have the block's type or fp32.  h comes of y
     before y is rounded.  Differentiable in every tensor (once, in reverse mode)."""
-    number = 1.0
+    x, res, number = block, residual, 1.0
     if scale is not None and not isinstance(scale, torch.Tensor):
         number, scale = float(scale), None
-    if not isinstance(residual, torch.Tensor):
+    if not isinstance(res, torch.Tensor):
         raise ValueError("residual must be a tensor")
-    return _norm("residual_norm", block, residual, gate, (weight, bias, scale, post_weight, post_bias), kind,
-                 post, gate_act, eps, eps if post_eps is None else post_eps, number)
+    _check_norm_rows("residual_norm", x)
+    post_eps = eps if post_eps is None else post_eps
+    params = (weight, bias, scale, post_weight, post_bias)
+    _like(res, x, x.shape, "residual", (x.dtype,))
+    if gate is not None:
+        _like(gate, x, x.shape, "gate", (x.dtype,))
+    tensors, types = (x, res, gate, *params), (x.dtype, torch.float32)
+    for t, what in zip(params, _PARAMS):
+        if t is not None:
+            _like(t, x, x.shape[-1:], what, types)
+    for k in (kind, post):
+        if k not in NORMS:
+            raise ValueError(f"norm {k!r} not in {tuple(NORMS)}")
+    if gate_act not in GATES:
+        raise ValueError(f"gate_act {gate_act!r} not in {tuple(GATES)}")
+    if not (eps >= 0 and post_eps >= 0):
+        raise ValueError(f"eps must be at least 0, got {eps}, {post_eps}")
+    if (kind is None and any(t is not None for t in params[:2])) or \
+            (post is None and any(t is not None for t in params[3:])):
+        raise ValueError("weights and biases are of a norm that there is")
+    _no_tangents("residual_norm", *tensors)
+    cfg = (NORMS[kind], NORMS[post], GATES[gate_act], float(eps), float(post_eps), float(number))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return _ResidualNorm.apply(*tensors, cfg)
+    return _residual_forward(x, res, gate, params, cfg, False)[:2]
