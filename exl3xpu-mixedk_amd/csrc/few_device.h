@@ -286,9 +286,9 @@ constexpr int kFewMaxSlice = 8;
 // layout.
 template <int K, int CODE, int G, int W, bool FUSED, bool LO>
 __device__ __forceinline__ void few_sums(const FewSource& a, int s0, int s1, u4* lds, int32_t* shifts,
-                                         f4 (&total)[G][8 / W]) {
+                                         f4 (&total)[G][8 / W], int lane = threadIdx.x & 63) {
     constexpr int SL = few_slice(K, W, LO);
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Window win = lane_window<K>(lane);
     uint8_t* const buf = (uint8_t*)lds + wv * 2 * kPairBytes<K>;
     u4 *const frag = lds + W * 64 * K, *const frag_lo = frag + SL * 256;

@@ -23,15 +23,15 @@ constexpr int gated_lds() {
 
 template <int G, bool FUSED, bool LO>
 __device__ __forceinline__ void role_sums(int K, const FewSource& src, int s0, int s1, u4* lds, int32_t* shifts,
-                                          f4 (&total)[G][8 / few_waves(G)]) {
+                                          f4 (&total)[G][8 / few_waves(G)], int lane) {
     constexpr int W = few_waves(G);
     switch (K) {
-        case 2: return few_sums<2, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
-        case 3: return few_sums<3, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
-        case 4: return few_sums<4, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
-        case 5: return few_sums<5, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
-        case 6: return few_sums<6, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
-        default: return few_sums<7, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total);
+        case 2: return few_sums<2, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total, lane);
+        case 3: return few_sums<3, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total, lane);
+        case 4: return few_sums<4, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total, lane);
+        case 5: return few_sums<5, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total, lane);
+        case 6: return few_sums<6, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total, lane);
+        default: return few_sums<7, kCode, G, W, FUSED, LO>(src, s0, s1, lds, shifts, total, lane);
     }
 }
 
@@ -45,82 +45,140 @@ __device__ __forceinline__ Columns<2> role_columns(const GatedArgs& a, int role,
     return a.type == kBf16 ? load_columns<kBf16, 2>(ep, col) : load_columns<kF16, 2>(ep, col);
 }
 
-// A workgroup multiplies one weight's 128 columns over a run of the summed dimension
-// (few_sums).  The last one of the two weights' runs adds them in order, transforms
-// both and writes act(gate) * up: the values between stay in registers.
-template <int G, bool FUSED, bool LO>
+// The blocks are 128 columns of a weight, gate's and up's side by side (a gate's are
+// even), and a workgroup multiplies a run of the steps of all blocks one behind the
+// other.  EVEN: `each` steps and `more` times one more of every block's.  Else of all
+// steps, so that a run may go over blocks' ends.  Run i's part of block q has place
+// i + q: along the steps one of them or both grow.
+struct Runs {
+    int steps, each, more, per_block;
+    template <bool EVEN>
+    __device__ __forceinline__ int at(int i) const {
+        const int q = EVEN ? i / per_block : 0, j = i - q * per_block;
+        return q * steps + j * each + (j < more ? j : more);
+    }
+    // The run that holds a step (not EVEN).
+    __device__ __forceinline__ int of(int step) const {
+        const int big = more * (each + 1);
+        return step < big ? step / (each + 1) : more + (step - big) / each;
+    }
+};
+
+// The last run to arrive of two blocks' adds the parts in order, transforms both and
+// writes act(gate) * up: the values between stay in registers.
+//
+// EVEN where that fills the places, two workgroups a compute unit.  272 blocks of 17408
+// columns do not, and two compute units of three then wait for the third: 48 rows of
+// 5120 take 84.9 us in 272 runs and 72.3 in 512, one row 51.8 and 43.7.  (Going over a
+// block's end is a loop, which costs registers and 4 us where runs are short.)
+template <int G, bool FUSED, bool LO, bool EVEN>
 __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void gated_few_kernel(GatedArgs a, GatedFew f) {
     constexpr int W = few_waves(G), N = 8 / W;
     __shared__ __align__(16) u4 lds[gated_lds<G, FUSED, LO>() / 16];
     __shared__ int32_t shifts[FUSED ? kFewMaxSlice * 16 : 1];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nb = a.w[0].n / 128, blk = blockIdx.x >> 1, role = blockIdx.x & 1, split = blockIdx.y;
-    const Weight& w = a.w[role];
-    const int steps = w.k / 32, nk = w.k / 128;
-    const int s0 = (int)((long long)steps * split / f.splits), s1 = (int)((long long)steps * (split + 1) / f.splits);
-    const FewSource src{(const uint8_t*)w.trellis + (size_t)blk * 256 * w.K, (size_t)nb * 256 * w.K, a.rows, steps,
-                        a.x, a.x_stride, w.suh, a.type, 65536u / a.rows + 1,
-                        FUSED ? nullptr : f.frag + (size_t)role * f.groups * nk * 256,
-                        FUSED || !LO ? nullptr : f.frag_lo + (size_t)role * f.groups * nk * 256,
-                        FUSED ? nullptr : f.shift + (size_t)role * f.groups * nk * 16};
-    f4 total[G][N];
-    role_sums<G, FUSED, LO>(w.K, src, s0, s1, lds, shifts, total);
-    const size_t run = (size_t)a.rows * 128;
-    float* const part = f.part + (size_t)blk * 2 * f.splits * run;
-    float* const mine = part + (size_t)(role * f.splits + split) * run + 4 * (lane >> 4);
+    const int nb = a.w[0].n / 128, steps = a.w[0].k / 32, nk = a.w[0].k / 128, chunk = blockIdx.y;
+    const int row_base = chunk * kFewRows, rows = a.rows - row_base < 16 * G ? a.rows - row_base : 16 * G;
+    const Runs runs{steps, f.each, f.more, f.per_block};
+    // (EVEN: neighbours are blocks of the same steps, whose trellis lies side by side:
+    // 64 rows of 4096 by 6144 42.8 us, 50.1 with a block's runs as neighbours)
+    const int i = EVEN ? blockIdx.x % (2 * nb) * f.per_block + blockIdx.x / (2 * nb) : blockIdx.x;
+    const size_t run = (size_t)rows * 128;
+    float* const part = f.part + (size_t)chunk * (f.workers + 2 * nb) * 128 * kFewRows;
+    // Steps s0 .. s1 of block q.
+    auto multiply = [&](int q, int s0, int s1, int own) {
+        const int blk = q >> 1, role = q & 1;
+        const Weight& w = a.w[role];
+        const size_t group = (size_t)role * f.groups + (FUSED ? 0 : chunk * (kFewRows / 16));
+        const FewSource src{(const uint8_t*)w.trellis + (size_t)blk * 256 * w.K, (size_t)nb * 256 * w.K, rows, steps,
+                            a.x, a.x_stride, w.suh, a.type, 65536u / rows + 1,
+                            FUSED ? nullptr : f.frag + group * nk * 256,
+                            FUSED || !LO ? nullptr : f.frag_lo + group * nk * 256,
+                            FUSED ? nullptr : f.shift + group * nk * 16};
+        f4 total[G][N];
+        role_sums<G, FUSED, LO>(w.K, src, s0, s1, lds, shifts, total, own);
+        float* const mine = part + (size_t)(i + q) * run + 4 * (lane >> 4);
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        const int row = 16 * g + (lane & 15);
-        if (row < a.rows)
+        for (int g = 0; g < G; ++g) {
+            const int row = 16 * g + (lane & 15);
+            if (row < rows)
 #pragma unroll
-            for (int i = 0; i < N; ++i) store_shared(mine + row * 128 + 16 * (i * W + wv), total[g][i]);
-    }
-    // (on their way while the workgroups meet)
-    const int col = blk * 128 + 2 * lane;
-    const Columns<2> cg = role_columns(a, 0, col), cu = role_columns(a, 1, col);
-    if (!arrive(f.counters + blk, 2 * f.splits, threadIdx.x)) return;
-    constexpr int R = G == 1 ? 2 : 4, U = G == 1 ? 8 : 4;
-#pragma unroll 1
-    for (int r0 = wv; r0 < a.rows; r0 += R * W) {
-        float v[R][2], u[R][2];
-        sum_rows<U, R>(v, part, r0, W, a.rows, run, f.splits, lane);
-        sum_rows<U, R>(u, part + f.splits * run, r0, W, a.rows, run, f.splits, lane);
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            transform_row(v[i][0], v[i][1], lane);
-            transform_row(u[i][0], u[i][1], lane);
+                for (int n = 0; n < N; ++n) store_shared(mine + row * 128 + 16 * (n * W + wv), total[g][n]);
         }
+        // (on their way while the workgroups meet)
+        const int col = blk * 128 + 2 * lane;
+        const Columns<2> cg = role_columns(a, 0, col), cu = role_columns(a, 1, col);
+        // each role's first run and number of them
+        int first[2], parts[2];
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int row = r0 + i * W;
-            if (row >= a.rows) break;
+        for (int r = 0; r < 2; ++r) {
+            const int b = 2 * blk + r;
+            first[r] = EVEN ? b * f.per_block : runs.of(b * steps);
+            parts[r] = EVEN ? f.per_block : runs.of((b + 1) * steps - 1) - first[r] + 1;
+            first[r] += b;
+        }
+        if (!arrive(f.counters + chunk * nb + blk, parts[0] + parts[1], threadIdx.x)) return;
+        constexpr int R = G == 1 ? 2 : 4, U = G == 1 ? 8 : 4;
+#pragma unroll 1
+        for (int r0 = wv; r0 < rows; r0 += R * W) {
+            float v[R][2], u[R][2];
+            sum_rows<U, R>(v, part + first[0] * run, r0, W, rows, run, parts[0], lane);
+            sum_rows<U, R>(u, part + first[1] * run, r0, W, rows, run, parts[1], lane);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                v[i][c] = v[i][c] * cg.scale[c] + cg.bias[c];
-                u[i][c] = u[i][c] * cu.scale[c] + cu.bias[c];
+            for (int n = 0; n < R; ++n) {
+                transform_row(v[n][0], v[n][1], lane);
+                transform_row(u[n][0], u[n][1], lane);
             }
-            if (a.z) {
-                float* z = a.z + (size_t)row * a.w[0].n + col;
-                z[0] = v[i][0];
-                z[1] = v[i][1];
-                z += (size_t)a.rows * a.w[0].n;
-                z[0] = u[i][0];
-                z[1] = u[i][1];
+#pragma unroll
+            for (int n = 0; n < R; ++n) {
+                if (r0 + n * W >= rows) break;
+                const size_t row = row_base + r0 + n * W;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    v[n][c] = v[n][c] * cg.scale[c] + cg.bias[c];
+                    u[n][c] = u[n][c] * cu.scale[c] + cu.bias[c];
+                }
+                if (a.z) {
+                    float* z = a.z + row * a.w[0].n + col;
+                    z[0] = v[n][0];
+                    z[1] = v[n][1];
+                    z += (size_t)a.rows * a.w[0].n;
+                    z[0] = u[n][0];
+                    z[1] = u[n][1];
+                }
+                activate<2>(v[n], a.act);
+                v[n][0] *= u[n][0];
+                v[n][1] *= u[n][1];
+                uint16_t* y = a.y + row * a.y_stride + col;
+                if (a.type == kBf16) store16<kBf16, 2>(y, v[n]);
+                else store16<kF16, 2>(y, v[n]);
             }
-            activate<2>(v[i], a.act);
-            v[i][0] *= u[i][0];
-            v[i][1] *= u[i][1];
-            uint16_t* y = a.y + (size_t)row * a.y_stride + col;
-            if (a.type == kBf16) store16<kBf16, 2>(y, v[i]);
-            else store16<kF16, 2>(y, v[i]);
+        }
+    };
+    const int end = runs.at<EVEN>(i + 1);
+    int at = runs.at<EVEN>(i);
+    if constexpr (EVEN) {
+        const int q = i / f.per_block;
+        multiply(q, at - q * steps, end - q * steps, lane);
+    } else {
+#pragma unroll 1
+        while (at < end) {
+            const int q = at / steps, s0 = at - q * steps, s1 = end - at < steps - s0 ? s0 + end - at : steps;
+            // (unknown to the compiler, which would keep every width's windows in
+            // registers for the next block)
+            int own = lane;
+            asm volatile("" : "+v"(own));
+            multiply(q, s0, s1, own);
+            at += s1 - s0;
         }
     }
 }
 
 template <int G, bool FUSED, bool LO>
 hipError_t launch(const GatedArgs& a, const GatedFew& f, hipStream_t s) {
-    hipLaunchKernelGGL((gated_few_kernel<G, FUSED, LO>), dim3(2 * (a.w[0].n / 128), f.splits), dim3(64 * few_waves(G)),
-                       0, s, a, f);
+    const dim3 grid(f.workers, (a.rows + kFewRows - 1) / kFewRows), block(64 * few_waves(G));
+    if (f.per_block) hipLaunchKernelGGL((gated_few_kernel<G, FUSED, LO, true>), grid, block, 0, s, a, f);
+    else hipLaunchKernelGGL((gated_few_kernel<G, FUSED, LO, false>), grid, block, 0, s, a, f);
     return hipGetLastError();
 }
 
@@ -129,15 +187,17 @@ hipError_t launch(const GatedArgs& a, const GatedFew& f, hipStream_t s) {
 #define XTQ_CAT2(a, b) a##b
 #define XTQ_CAT(a, b) XTQ_CAT2(a, b)
 
-// (Rows and fragments are held against each other here: the kernels take them as
-// they come.)
+// (Rows, fragments and runs are held against each other here: the kernels take them
+// as they come.)
 hipError_t XTQ_CAT(launch_gated_few_code, XTQ_GATED_CODE)(const GatedArgs& a, const GatedFew& f, hipStream_t s) {
-    if (a.rows > (f.frag ? 16 * f.groups : kFusedRows) || (a.two && f.frag && !f.frag_lo)) return hipErrorInvalidValue;
+    const int groups = f.groups;
+    if (a.rows > (f.frag ? 16 * groups : kFusedRows) || (groups > 4 && groups % 4) ||
+        (a.two && f.frag && !f.frag_lo) || f.each < 1)
+        return hipErrorInvalidValue;
     if (!f.frag) return a.two ? launch<1, true, true>(a, f, s) : launch<1, true, false>(a, f, s);
-    if (f.groups == 1) return a.two ? launch<1, false, true>(a, f, s) : launch<1, false, false>(a, f, s);
-    if (f.groups == 2) return a.two ? launch<2, false, true>(a, f, s) : launch<2, false, false>(a, f, s);
-    if (f.groups == 4) return a.two ? launch<4, false, true>(a, f, s) : launch<4, false, false>(a, f, s);
-    return hipErrorInvalidValue;
+    if (groups == 1) return a.two ? launch<1, false, true>(a, f, s) : launch<1, false, false>(a, f, s);
+    if (groups == 2) return a.two ? launch<2, false, true>(a, f, s) : launch<2, false, false>(a, f, s);
+    return a.two ? launch<4, false, true>(a, f, s) : launch<4, false, false>(a, f, s);
 }
 
 }  // namespace xtq

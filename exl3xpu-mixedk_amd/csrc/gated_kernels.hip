@@ -72,13 +72,19 @@ __device__ __forceinline__ void store_gated(const f4* gate, const f4* up, const 
     }
 }
 
-// The product of fragments (gemm_kernel of linear_kernels.hip) with each wave's rows
-// those of its weight.
+// The product of fragments.  A workgroup's tile is 256 columns by 32 NB rows, 4 waves
+// of one weight's 128 columns by 16 NB rows, in steps of 32 of the summed dimension.
+// The columns' fragments are read by two waves each and come through three LDS
+// buffers, two steps ahead, as in gemm_kernel of linear_kernels.hip; a wave's rows are
+// its own weight's and its own half, so they come straight into its registers.
+// Two workgroups share a compute unit.  (The rows through LDS too: 32 KiB a step, two
+// buffers of which leave room for the second workgroup: 1508 us for 4096 rows of 5120
+// by 17408, and now 1308.)
 template <int T, int OUT, int NB, int TERMS>
 __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedArgs a) {
-    constexpr int kFrags = 16 + 4 * NB * TERMS, kOwn = 4 + NB * TERMS;
-    constexpr int kBuffers = kFrags > 24 ? 2 : 3;
-    __shared__ __align__(1024) uint8_t lds[kBuffers][kFrags * kFragBytes];
+    constexpr int kOwn = 4 + NB * TERMS;        // a wave's loads of a step
+    constexpr int kExchange = OUT == kGatedFinish ? 4 * (NB / 2) * 8192 : 0, kLoop = 3 * 16 * kFragBytes;
+    __shared__ __align__(1024) uint8_t lds[kLoop > kExchange ? kLoop : kExchange];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), role = wv & 1, wm = wv >> 1;
     const int tile = xcd_order(blockIdx.x, g.tiles);
@@ -89,52 +95,50 @@ __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedAr
     const int s0 = (int)((long long)g.steps * split / g.splits);
     const int s1 = (int)((long long)g.steps * (split + 1) / g.splits);
 
-    // this wave's fragments of a step: a quarter of A's 16 and of each B's 2 NB
-    const uint16_t* fa = g.A + (size_t)tn * g.steps * 8192 + wv * 2048 + lane * 8;
     const int gb0 = tm * 2 * NB;        // first group of rows
-    const size_t at_b = ((size_t)(gb0 >> 4) * g.steps * 16 + (gb0 & 15) + wv * (NB / 2)) * 512 + lane * 8;
-    auto load = [&](int s) {
-        uint8_t* l = lds[(s - s0) % kBuffers];
+    const uint16_t* fa = g.A + (size_t)tn * g.steps * 8192 + wv * 2048 + lane * 8;
+    const size_t at_b = ((size_t)(gb0 >> 4) * g.steps * 16 + (gb0 & 15) + wm * NB) * 512 + lane * 8;
+    const uint16_t* const fb[2] = {g.B[role] + at_b, TERMS == 2 ? g.B2[role] + at_b : nullptr};
+    // Stages of the rows' registers: a step's come two steps ahead, or one where four
+    // groups of two terms leave no room for more.
+    constexpr int kStages = NB * TERMS > 4 ? 2 : 3;
+    u4 b[kStages][TERMS][NB];
+    // (Past the end the last step comes once more, so that the waits can count.)
+    int to = 0;
+    auto load_a = [&](int s) {
+        const uint16_t* p = fa + (size_t)(s < s1 ? s : s1 - 1) * 8192;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            __builtin_amdgcn_global_load_lds((global_void*)(fa + (size_t)s * 8192 + i * 512),
-                                             (lds_void*)(l + (wv * 4 + i) * kFragBytes), 16, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-                for (int i = 0; i < NB / 2; ++i)
-                    __builtin_amdgcn_global_load_lds(
-                        (global_void*)((t ? g.B2[r] : g.B[r]) + at_b + (size_t)s * 8192 + i * 512),
-                        (lds_void*)(l + (16 + 2 * NB * (r * TERMS + t) + wv * (NB / 2) + i) * kFragBytes), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_void*)(p + i * 512),
+                                             (lds_void*)(lds + (to * 16 + wv * 4 + i) * kFragBytes), 16, 0, 0);
+        to = to == 2 ? 0 : to + 1;
     };
-    // All waves' pieces of the next step are in LDS, and all waves have read this
-    // one (their reads were waited for before they came here).
-    auto meet_up = [&](bool more) {
-        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kOwn) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+    auto load_b = [&](int s, auto stage) {
+        const size_t at = (size_t)(s < s1 ? s : s1 - 1) * 8192;
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) b[decltype(stage)::value][t][i] = *(const u4*)(fb[t] + at + i * 512);
     };
     f4 acc[8][NB];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[j][b] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int kAhead = kBuffers - 1;        // steps on their way beside the one that is multiplied
-    load(s0);
-    if (kAhead > 1 && s0 + 1 < s1) load(s0 + 1);
-    meet_up(kAhead > 1 && s0 + 1 < s1);
-    for (int s = s0; s < s1; ++s) {
-        if (s + kAhead < s1) load(s + kAhead);
-        u4 fr[8], b[TERMS][NB];
-        const uint8_t* l = lds[(s - s0) % kBuffers] + lane * 16;
-#pragma unroll
-        for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-                b[t][i] = *(const u4*)(l + (16 + 2 * NB * (role * TERMS + t) + wm * NB + i) * kFragBytes);
+        for (int i = 0; i < NB; ++i) acc[j][i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    // All waves' pieces of the next step are in LDS, and all waves have read this one
+    // (their reads were waited for before they came here).
+    auto meet_up = [&] {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kOwn) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    int from = 0;
+    auto step = [&](int s, auto stage) {
+        constexpr int I = decltype(stage)::value;
+        load_a(s + 2);
+        load_b(s + kStages - 1, std::integral_constant<int, (I + kStages - 1) % kStages>());
+        u4 fr[8];
+        const uint8_t* l = lds + from * 16 * kFragBytes + lane * 16;
 #pragma unroll
         for (int j = 0; j < 8; ++j) fr[j] = *(const u4*)(l + (role * 8 + j) * kFragBytes);
         __builtin_amdgcn_sched_barrier(0);      // all reads under way before the first product
@@ -143,10 +147,24 @@ __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedAr
 #pragma unroll
             for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-                for (int i = 0; i < NB; ++i) acc[j][i] = mfma<false>(fr[j], b[t][i], acc[j][i]);
+                for (int i = 0; i < NB; ++i) acc[j][i] = mfma<false>(fr[j], b[I][t][i], acc[j][i]);
         __builtin_amdgcn_sched_barrier(0);      // none after the others have met
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        meet_up(kAhead > 1 && s + kAhead < s1);
+        meet_up();
+        from = from == 2 ? 0 : from + 1;
+    };
+    const std::integral_constant<int, 0> c0;
+    const std::integral_constant<int, 1> c1;
+    load_a(s0);
+    load_b(s0, c0);
+    load_a(s0 + 1);
+    if constexpr (kStages == 3) load_b(s0 + 1, c1);
+    meet_up();
+    for (int s = s0; s < s1; s += kStages) {
+        step(s, c0);
+        if (s + 1 < s1) step(s + 1, c1);
+        if constexpr (kStages == 3)
+            if (s + 2 < s1) step(s + 2, std::integral_constant<int, 2>());
     }
     if constexpr (OUT == kGatedParts) {
 #pragma unroll
@@ -165,6 +183,8 @@ __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedAr
     // a tile's groups.)
     Columns<4> cols[8];
     role_columns<T>(cols, a, role, tn, lane);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // (the steps past the end lie where the factors go)
+    __syncthreads();
     f4* const give = (f4*)lds + (size_t)wv * (NB / 2) * 512 + lane;
     const f4* const take = (const f4*)lds + (size_t)(wv ^ 1) * (NB / 2) * 512 + lane;
 #pragma unroll
@@ -350,25 +370,73 @@ struct Taker {
 };
 
 struct FewPlan {
-    int groups, splits;
+    int groups, workers, per_block;
     bool apart;
     size_t part, frag, rest, shift, total;
 };
 
-bool takes_few(int rows, int n) { return rows <= kFewRows && n / 128 <= XTQ_OP_COUNTERS; }
+// Rows that go through the kernel of few rows, 64 at a time.
+constexpr int kGatedFew = 256;
+
+int few_chunks(int rows) { return (rows + kFewRows - 1) / kFewRows; }
+
+bool takes_few(int rows, int k, int n) {
+    return rows <= kGatedFew && few_chunks(rows) * (n / 128) <= XTQ_OP_COUNTERS &&
+           (long long)(n / 64) * (k / 32) < 1LL << 30;
+}
+
+// A chunk's workgroups: as few_splits cuts the blocks; evenly over all steps where
+// that leaves a fifth of the places empty and a run still has 32 steps.
+void few_workers(FewPlan& p, int rows, int k, int n, int waves) {
+    const int blocks = n / 64, chunks = few_chunks(rows), places = 2 * kCUs;
+    int s = few_splits(rows < kFewRows ? rows : kFewRows, k, 2 * n, waves);
+    while (s > 1 && blocks * s * chunks > places) --s;
+    const int all = blocks * s * chunks, rounds = (all + places - 1) / places;
+    p.per_block = s;
+    p.workers = blocks * s;
+    if (2 * all > places && 5LL * all < 4LL * rounds * places && (long long)blocks * (k / 32) * chunks / places >= 32) {
+        p.per_block = 0;
+        p.workers = places / chunks;
+    }
+}
 
 FewPlan few_plan(int rows, int k, int n, bool two) {
     FewPlan p;
-    p.groups = few_groups(rows);
-    p.splits = few_splits(rows, k, 2 * n, few_waves(p.groups));
-    p.apart = rows > kFusedRows || rows * (k / 128) > 16 * p.splits;
+    const int chunks = few_chunks(rows), blocks = n / 64;
+    p.groups = chunks > 1 ? 4 * chunks : few_groups(rows);
+    few_workers(p, rows, k, n, few_waves(chunks > 1 ? 4 : p.groups));
+    // (16: as few_plan of linear_kernels.hip, by the blocks of rows of a run)
+    p.apart = rows > kFusedRows || (long long)rows * blocks * (k / 128) > 16LL * p.workers;
     Taker take;
-    p.part = take((size_t)p.splits * 2 * n * rows * 4);
+    p.part = take((size_t)chunks * (p.workers + blocks) * 128 * (chunks > 1 ? kFewRows : rows) * 4);
     p.frag = take(p.apart ? (size_t)2 * p.groups * k * 32 : 0);
     p.rest = take(p.apart && two ? (size_t)2 * p.groups * k * 32 : 0);
     p.shift = take(p.apart ? (size_t)2 * p.groups * k / 2 : 0);
     p.total = take.at;
     return p;
+}
+
+// How the product of many rows is cut, as gemm_tiling of linear_kernels.hip does: by the
+// shortest estimate.  us of a workgroup's step alone on a compute unit, of two at once,
+// and of each where there are more, by terms and groups of rows.
+Tiling gated_tiling(int rows, int n, int steps, bool two) {
+    static const double cost[2][2][3] = {{{0.40, 0.55, 0.35}, {0.55, 0.80, 0.51}}, {{0.60, 0.90, 0.50}, {0.95, 1.45, 0.91}}};
+    Tiling best{};
+    double least = 0.0;
+    for (int nb = 4; nb >= 2; nb -= 2) {
+        const double* c = cost[two][nb == 4];
+        const int tiles = n / 128 * ((rows + 32 * nb - 1) / (32 * nb));
+        for (int s = 1; s == 1 || (s <= steps / 8 && (s - 1) * tiles < 2 * kCUs); ++s) {
+            const int each = (int)(((long long)tiles * s + kCUs - 1) / kCUs);
+            const double step = each == 1 ? c[0] : each == 2 ? c[1] : c[2] * (each % 2 ? each + 0.3 : each);
+            const double us = step * ((steps + s - 1) / s) + (s > 1 ? 3.0 + 4e-6 * s * rows * n : 0.0);
+            if (!best.nb || us < least) {
+                least = us;
+                best = Tiling{nb, tiles, s};
+            }
+        }
+    }
+    return best;
 }
 
 struct ManyPlan {
@@ -380,7 +448,7 @@ ManyPlan many_plan(int rows, int k, int n, bool two) {
     ManyPlan p;
     p.groups = (rows + 15) / 16;
     p.places = (p.groups + 15) / 16 * 256;      // whole tiles' rows
-    const Tiling t = gemm_tiling(rows, 2 * n, k / 32, two);
+    const Tiling t = gated_tiling(rows, n, k / 32, two);
     p.nb = t.nb;
     p.tiles = t.tiles;
     p.splits = t.splits;
@@ -424,11 +492,13 @@ hipError_t many(const GatedArgs& a, void* ws, hipStream_t s) {
     const dim3 grid(p.tiles, p.splits), block(256);
     auto gemm = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, g, a); };
     if (p.splits == 1) {
-        if (a.two) gemm(gated_gemm_kernel<T, kGatedFinish, 2, 2>);
+        if (a.two && p.nb == 4) gemm(gated_gemm_kernel<T, kGatedFinish, 4, 2>);
+        else if (a.two) gemm(gated_gemm_kernel<T, kGatedFinish, 2, 2>);
         else if (p.nb == 4) gemm(gated_gemm_kernel<T, kGatedFinish, 4, 1>);
         else gemm(gated_gemm_kernel<T, kGatedFinish, 2, 1>);
     } else {
-        if (a.two) gemm(gated_gemm_kernel<T, kGatedParts, 2, 2>);
+        if (a.two && p.nb == 4) gemm(gated_gemm_kernel<T, kGatedParts, 4, 2>);
+        else if (a.two) gemm(gated_gemm_kernel<T, kGatedParts, 2, 2>);
         else if (p.nb == 4) gemm(gated_gemm_kernel<T, kGatedParts, 4, 1>);
         else gemm(gated_gemm_kernel<T, kGatedParts, 2, 1>);
         hipLaunchKernelGGL((gated_join_kernel<T>), dim3(p.groups, n / 128), dim3(64), 0, s, g, a);
@@ -495,17 +565,19 @@ hipError_t gradient(const GatedGradArgs& a, void* ws, hipStream_t s) {
 }  // namespace
 
 size_t gated_ws_bytes(int rows, int k, int n, bool two) {
-    return takes_few(rows, n) ? few_plan(rows, k, n, two).total : many_plan(rows, k, n, two).total;
+    return takes_few(rows, k, n) ? few_plan(rows, k, n, two).total : many_plan(rows, k, n, two).total;
 }
 
 size_t gated_bwd_ws_bytes(int rows, int k, int n, bool two) { return grad_plan(rows, k, n, two).total; }
 
 hipError_t launch_gated(const GatedArgs& a, void* ws, uint32_t* counters, hipStream_t s) {
     const int k = a.w[0].k, n = a.w[0].n;
-    if (!takes_few(a.rows, n)) return a.type == kBf16 ? many<kBf16>(a, ws, s) : many<kF16>(a, ws, s);
+    if (!takes_few(a.rows, k, n)) return a.type == kBf16 ? many<kBf16>(a, ws, s) : many<kF16>(a, ws, s);
     const FewPlan p = few_plan(a.rows, k, n, a.two);
     uint8_t* base = (uint8_t*)ws;
-    GatedFew f{nullptr, nullptr, nullptr, p.groups, p.splits, (float*)(base + p.part), counters};
+    const int steps = p.per_block ? k / 32 : n / 64 * (k / 32), of = p.per_block ? p.per_block : p.workers;
+    GatedFew f{nullptr, nullptr, nullptr, p.groups, p.workers, p.per_block, steps / of, steps % of,
+               (float*)(base + p.part), counters};
     if (p.apart) {
         u4 *frag = (u4*)(base + p.frag), *rest = a.two ? (u4*)(base + p.rest) : nullptr;
         int32_t* shift = (int32_t*)(base + p.shift);

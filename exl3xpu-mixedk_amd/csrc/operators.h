@@ -194,13 +194,17 @@ hipError_t launch_gated(const GatedArgs& a, void* ws, uint32_t* counters, hipStr
 hipError_t launch_gated_bwd(const GatedGradArgs& a, void* ws, hipStream_t s);
 
 // Few rows, one function per codebook: frag [role][groups of 16 rows][k/32][64] and
-// shifts as in FewArgs, or NULL (one group: the kernel transforms x).
+// shifts as in FewArgs, or NULL (one group: the kernel transforms x).  1, 2 or 4
+// groups, or fours of them: chunks of 64 rows.  workers: workgroups of a chunk, each a
+// run of the steps of all blocks of 128 columns of both weights: per_block of every
+// block's steps, or (per_block 0) of all.
 struct GatedFew {
     const u4 *frag, *frag_lo;
     const int32_t* shift;
-    int groups, splits;
-    float* part;                        // [n/128][role][split][row][128]
-    uint32_t* counters;                 // [n/128]
+    int groups, workers, per_block;
+    int each, more;                     // steps of a run; runs with one more
+    float* part;                        // [chunk][worker + block][row][128], chunks 64 rows apart
+    uint32_t* counters;                 // [chunk][n/128]
 };
 #define XTQ_GATED(C) \
     hipError_t launch_gated_few_code##C(const GatedArgs& a, const GatedFew& f, hipStream_t s);

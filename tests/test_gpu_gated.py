@@ -47,7 +47,7 @@ def _ratio(got, want):
     return off and off / float((want.to(got.dtype).double() - want).norm())
 
 
-ROWS = (1, 2, 15, 16, 17, 33, 63, 64, 65, 130, 257)
+ROWS = (1, 2, 15, 16, 17, 33, 63, 64, 65, 128, 130, 192, 193, 256, 257)
 
 
 @pytest.mark.parametrize("m", ROWS)
@@ -65,7 +65,7 @@ def test_rows(xt, oracle_mod, m, k, n, K1, K2):
 
 @pytest.mark.parametrize("K", range(2, 8))
 @pytest.mark.parametrize("code", sorted(R.CODES))
-@pytest.mark.parametrize("m", (3, 12, 30, 50, 200))
+@pytest.mark.parametrize("m", (3, 12, 30, 50, 300))
 def test_codes(xt, oracle_mod, K, code, m):
     """Every width and codebook beside another width, every kernel of few rows, forward and gradient, with scales of
     the whole weights.  Float16: everything is rounded once."""
@@ -81,7 +81,8 @@ def test_codes(xt, oracle_mod, K, code, m):
     assert _ratio(dx, (dyd * zu * R.slope(zg, "gelu")) @ Wg.t() + (dyd * R.act(zg, "gelu")) @ Wu.t()) <= 1.02
 
 
-@pytest.mark.parametrize("m,k,n", [(9000, 128, 640), (3000, 2048, 256), (1815, 1024, 2176), (300, 4096, 384)])
+@pytest.mark.parametrize("m,k,n", [(9000, 128, 640), (3000, 2048, 256), (1815, 1024, 2176), (300, 4096, 384),
+                                   (150, 2048, 6144)])
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 def test_cuts(xt, oracle_mod, m, k, n, dtype):
     """Every way in which the products of many rows are cut: both heights of tile, whole and in parts."""
@@ -98,6 +99,28 @@ def test_cuts(xt, oracle_mod, m, k, n, dtype):
     want = (dyd * zu * sig * (1 + zg * (1 - sig))) @ Wg.t().contiguous() + (dyd * a) @ Wu.t().contiguous()
     assert float(R.row_errors(y, (a * zu).cpu()).max()) <= _tol(dtype)
     assert float(R.row_errors(dx, want.cpu()).max()) <= _tol(dtype)
+
+
+@pytest.fixture(scope="module")
+def wide(xt, oracle_mod):
+    """A pair of more blocks of 128 columns than there are compute units: few rows' runs go over their ends."""
+    ls, ws = _pair(xt, oracle_mod, 2048, 16640, 3, 5, seed=9)
+    return ls, [w.cuda() for w in ws]
+
+
+@pytest.mark.parametrize("m", (1, 7, 16, 30, 50, 64, 100, 130, 256))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_runs_over_blocks(xt, wide, m, dtype):
+    ls, (Wg, Wu) = wide
+    x = _x(m, 2048, dtype, m).requires_grad_()
+    zg, zu = x.detach().double() @ Wg, x.detach().double() @ Wu
+    want = (zg / (1 + torch.exp(-zg)) * zu).cpu()
+    y = xt.gated(x, *ls)
+    assert float(R.row_errors(y, want).max()) <= _tol(dtype)
+    if dtype == torch.float16:
+        assert _ratio(y, want) <= 1.02
+    with torch.no_grad():
+        assert all(torch.equal(xt.gated(x, *ls), y) for _ in range(5))
 
 
 @pytest.mark.parametrize("act", ("none", "relu", "silu", "gelu"))
@@ -142,7 +165,7 @@ def test_gradient(xt, oracle_mod, act, dtype, bias_dtypes, m):
         assert abs(mine - dif) <= 4 * (_tol(dtype) + 5e-4) * size + 1e-4
 
 
-@pytest.mark.parametrize("m", (1, 5, 16, 17, 40, 64, 65, 300))
+@pytest.mark.parametrize("m", (1, 5, 16, 17, 40, 64, 65, 200, 300))
 @pytest.mark.parametrize("act", ("none", "silu", "gelu"))
 def test_rounded_once(xt, oracle_mod, m, act):
     """Float16 results and gradients are off by their one rounding; bfloat16's by that and 11 bits of the rows (0.0003
@@ -174,7 +197,7 @@ def test_rounded_once(xt, oracle_mod, m, act):
 @pytest.mark.parametrize("fast", (False, True))
 def test_same_result_with_a_gradient(xt, oracle_mod, dtype, act, fast):
     ls, _ = _pair(xt, oracle_mod, 1280, 384, 4, 3)
-    for m in (1, 5, 16, 17, 40, 64, 65, 300):
+    for m in (1, 5, 16, 17, 40, 64, 65, 200, 300):
         x = _x(m, 1280, dtype, m)
         with torch.no_grad():
             want = xt.gated(x, *ls, act=act, fast=fast)
@@ -295,7 +318,7 @@ def test_far_rows(xt, oracle_mod, m, step):
     assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
 
 
-@pytest.mark.parametrize("m", (2, 20, 90))
+@pytest.mark.parametrize("m", (2, 20, 90, 300))
 def test_repeats_streams_and_graphs(xt, oracle_mod, m):
     """The same bits on every call, on another stream, and in a replayed graph with eager work in between."""
     ls, _ = _pair(xt, oracle_mod, 1024, 384, 4, 5)
