@@ -6,7 +6,7 @@
 // the norm of t being (t - mean) / sqrt(mean (t - mean)^2 + eps) w + b, without its
 // mean for "rms".  The plain norm is h of y = x.  h comes of y before it is rounded.
 //
-// A row's group of lanes (16, a wave or a workgroup, by the width alone, so that a
+// A row's group of lanes (16, 32, a wave or a workgroup, by the width alone, so that a
 // row's result does not depend on how many there are) holds the row in registers:
 // every input is read once, deviations are squared around the mean itself.
 #include "operators.h"
@@ -16,8 +16,11 @@
 namespace xtq {
 namespace {
 
-// Rows of 16 lanes (four a wave), of a wave, of a workgroup.
-enum Mode { kSub, kWave, kBlock };
+// Rows of 16 lanes (four a wave), of 32, of a wave, of a workgroup.
+enum Mode { kSub, kHalf, kWave, kBlock };
+constexpr int lanes_of(int mode) { return mode == kSub ? 16 : mode == kHalf ? 32 : 64; }
+// Rows that a workgroup has at a time.
+constexpr int rows_of(int mode) { return mode == kBlock ? 1 : 256 / lanes_of(mode); }
 
 // Waves that share a row at most: three a SIMD, whose 168 registers hold, of a
 // gradient, eight channels' parameters and sums and two rows' inputs.
@@ -108,7 +111,7 @@ __device__ __forceinline__ void gate_at(float g, int act, float& value, float& s
     slope = act == kGateSigmoid ? t : __builtin_fmaf(g, t, s);
 }
 
-// Sum over the lanes of 16, of the wave.
+// Sum over 16 lanes, over 32 and over the wave.
 __device__ __forceinline__ float sum16(float v) {
     v += lane_xor<1>(v);
     v += lane_xor<2>(v);
@@ -117,13 +120,15 @@ __device__ __forceinline__ float sum16(float v) {
     return v;
 }
 
+__device__ __forceinline__ float sum32(float v) {
+    const uint32_t b = __float_as_uint(sum16(v));
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 __device__ __forceinline__ float sum64(float v) {
-    v = sum16(v);
-    uint32_t b = __float_as_uint(v);
-    auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    b = __float_as_uint(v);
-    r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const uint32_t b = __float_as_uint(sum32(v));
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
@@ -134,18 +139,14 @@ template <int MODE>
 struct Group {
     int lane, width, turn = 0;          // the row's lane and lanes
     __device__ Group() {
-        lane = MODE == kSub ? threadIdx.x & 15 : MODE == kWave ? threadIdx.x & 63 : threadIdx.x;
-        width = MODE == kSub ? 16 : MODE == kWave ? 64 : blockDim.x;
+        lane = MODE == kBlock ? threadIdx.x : threadIdx.x & (lanes_of(MODE) - 1);
+        width = MODE == kBlock ? blockDim.x : lanes_of(MODE);
     }
     template <int N>
     __device__ __forceinline__ void sum(float (&v)[N]) {
-        if constexpr (MODE == kSub) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = sum16(v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = sum64(v[i]);
-        }
+        for (int i = 0; i < N; ++i)
+            v[i] = MODE == kSub ? sum16(v[i]) : MODE == kHalf ? sum32(v[i]) : sum64(v[i]);
         if constexpr (MODE == kBlock) {
             __shared__ float part[2][2][16];
             const int wv = threadIdx.x >> 6, waves = blockDim.x >> 6, l = threadIdx.x & 15;
@@ -192,8 +193,7 @@ __device__ __forceinline__ void row_stats(Group<MODE>& g, const float (&t)[V][8]
 template <int T, int MODE, int V>
 __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_kernel(NormArgs a) {
     Group<MODE> g;
-    const int row = MODE == kSub ? blockIdx.x * 16 + (threadIdx.x >> 4)
-                                 : MODE == kWave ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const int row = blockIdx.x * rows_of(MODE) + (MODE == kBlock ? 0 : threadIdx.x / lanes_of(MODE));
     const bool in = row < a.rows;
     const size_t at = in ? row : 0;
     int col[V], n[V];
@@ -411,8 +411,8 @@ template <int T, int MODE, int V, int OF, bool SUMS, bool BIAS>
 __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bwd_kernel(NormGradArgs a) {
     static_assert(!SUMS || V == 1, "sums of one eight a lane");
     Group<MODE> g;
-    constexpr int R = MODE == kSub ? 16 : MODE == kWave ? 4 : 1;        // rows of a workgroup at a time
-    const int sub = MODE == kSub ? threadIdx.x >> 4 : MODE == kWave ? threadIdx.x >> 6 : 0;
+    constexpr int R = rows_of(MODE);
+    const int sub = MODE == kBlock ? 0 : threadIdx.x / lanes_of(MODE);
     const int d = a.f.d, step = gridDim.x * R;
     const float inv = 1.0f / (float)d;
     struct Row {
@@ -607,22 +607,26 @@ __global__ __launch_bounds__(1024) void norm_sums_kernel(NormGradArgs a, int par
     else ((uint16_t*)o.p)[c] = (uint16_t)(type == kBf16 ? to16<kBf16>(s) : to16<kF16>(s));
 }
 
-// Lanes of a row and eights of a lane, by the width.
+// Lanes of a row and eights of a lane, by the width.  A workgroup's lanes have two
+// eights each forward, whose loads are then half as many workgroups' (8191 rows of 5120
+// with everything 94 us, 108 with one; one row 0.8 us more), and one for a gradient.
 struct Shape {
-    int mode, v, threads, rows;         // rows of a workgroup
+    int mode, v, threads;
 };
 
-Shape norm_shape(int d) {
-    if (d <= 128) return {kSub, 1, 256, 16};
-    if (d <= 512) return {kWave, 1, 256, 4};
-    const int most = 512 * kRowWaves, v = d <= 4 * most ? (d + most - 1) / most : 6;
-    return {kBlock, v, (d + 512 * v - 1) / (512 * v) * 64, 1};
+Shape norm_shape(int d, bool gradient) {
+    if (d <= 512) return {d <= 128 ? kSub : d <= 256 ? kHalf : kWave, 1, 256};
+    const int most = 512 * kRowWaves;
+    int v = d <= 4 * most ? (d + most - 1) / most : 6;
+    if (!gradient && v == 1) v = 2;
+    return {kBlock, v, (d + 512 * v - 1) / (512 * v) * 64};
 }
 
 template <typename F>
 void with_shape(const Shape& s, F f) {
     using std::integral_constant;
     if (s.mode == kSub) f(integral_constant<int, kSub>(), integral_constant<int, 1>());
+    else if (s.mode == kHalf) f(integral_constant<int, kHalf>(), integral_constant<int, 1>());
     else if (s.mode == kWave) f(integral_constant<int, kWave>(), integral_constant<int, 1>());
     else if (s.v == 1) f(integral_constant<int, kBlock>(), integral_constant<int, 1>());
     else if (s.v == 2) f(integral_constant<int, kBlock>(), integral_constant<int, 2>());
@@ -633,10 +637,11 @@ void with_shape(const Shape& s, F f) {
 
 template <int T>
 void forward(const NormArgs& a, hipStream_t s) {
-    const Shape sh = norm_shape(a.d);
-    const dim3 grid((a.rows + sh.rows - 1) / sh.rows), block(sh.threads);
+    const Shape sh = norm_shape(a.d, false);
+    const dim3 grid((a.rows + rows_of(sh.mode) - 1) / rows_of(sh.mode)), block(sh.threads);
     with_shape(sh, [&](auto mode, auto v) {
-        hipLaunchKernelGGL((norm_kernel<T, decltype(mode)::value, decltype(v)::value>), grid, block, 0, s, a);
+        constexpr int M = decltype(mode)::value, V = decltype(v)::value;
+        if constexpr (M != kBlock || V > 1) hipLaunchKernelGGL((norm_kernel<T, M, V>), grid, block, 0, s, a);
     });
 }
 
@@ -649,9 +654,9 @@ struct NormPlan {
 };
 
 NormPlan norm_plan(int rows, int d, int sums) {
-    const Shape sh = norm_shape(d);
+    const Shape sh = norm_shape(d, true);
     NormPlan p;
-    const int all = (rows + sh.rows - 1) / sh.rows, most = kRowWaves / (sh.threads / 64) * kCUs;
+    const int all = (rows + rows_of(sh.mode) - 1) / rows_of(sh.mode), most = kRowWaves / (sh.threads / 64) * kCUs;
     p.groups = all < most ? all : most;
     p.apart = sums && sh.v > 1;
     p.parts = p.groups;
@@ -666,7 +671,7 @@ NormPlan norm_plan(int rows, int d, int sums) {
 
 template <int T, int OF, bool BIAS>
 void backward_of(const NormGradArgs& a, const NormPlan& p, bool sums, hipStream_t s) {
-    const Shape sh = norm_shape(a.f.d);
+    const Shape sh = norm_shape(a.f.d, true);
     with_shape(sh, [&](auto mode, auto v) {
         constexpr int M = decltype(mode)::value, V = decltype(v)::value;
         auto* kernel = norm_bwd_kernel<T, M, V, OF, false, BIAS>;

@@ -67,7 +67,7 @@ def _off(got, want, terms=None):
     return float(torch.where(off > 0, off / norm.clamp(min=1e-300), off).max())
 
 
-WIDTHS = (1, 7, 16, 100, 127, 128, 129, 512, 513, 1000, 1024, 1025, 2047, 5120, 8192, 8193, 16385, 32768)
+WIDTHS = (1, 7, 8, 9, 16, 100, 127, 128, 129, 200, 256, 257, 512, 513, 1000, 1024, 1025, 2047, 5120, 8192, 8193, 16385, 32768)
 
 
 @pytest.mark.parametrize("d", WIDTHS)
@@ -148,7 +148,7 @@ def _gradients(v, douts, kind, post, act, number, eps, post_eps):
 
 
 @pytest.mark.parametrize("kind,post,act,scale", CASES)
-@pytest.mark.parametrize("m,d", [(1, 128), (5, 5120), (70, 100), (600, 96), (37, 700), (19, 1024), (530, 2049),
+@pytest.mark.parametrize("m,d", [(1, 128), (5, 5120), (70, 100), (600, 96), (300, 250), (37, 700), (19, 1024), (530, 2049),
                                  (3, 9000), (4, 17408)])
 def test_residual_norm_gradient(xt, kind, post, act, scale, m, d):
     """Every tensor's gradient."""
