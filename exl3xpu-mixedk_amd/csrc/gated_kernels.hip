@@ -250,12 +250,12 @@ __device__ __forceinline__ void gated_slopes(const GatedSource& s, size_t row, i
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const f4 a = *(const f4_a4*)(zg + 4 * h), b = *(const f4_a4*)(zu + 4 * h);
-        float v[4] = {a[0], a[1], a[2], a[3]};
-        activate<4>(v, s.act);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            dg[4 * h + i] = d[4 * h + i] * b[i] * act_slope(a[i], s.act);
-            du[4 * h + i] = d[4 * h + i] * v[i];
+            float value, slope;
+            act_and_slope(a[i], s.act, value, slope);
+            dg[4 * h + i] = d[4 * h + i] * b[i] * slope;
+            du[4 * h + i] = d[4 * h + i] * value;
         }
     }
 }

@@ -133,6 +133,22 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     return 1.0f;
 }
 
+// Both at once: the activation, as activate gives it, and its slope, as act_slope does.
+__device__ __forceinline__ void act_and_slope(float z, int act, float& value, float& slope) {
+    if (act == kActSilu) {
+        const float s = fast_rcp(1.0f + fast_exp(-z)), t = fabsf(z) > 100.0f ? 0.0f : z * (1.0f - s);
+        value = z * s;
+        slope = s * (1.0f + t);
+    } else if (act == kActGelu) {
+        const float c = normal_cdf(z), d = fabsf(z) > 20.0f ? 0.0f : z * fast_exp(-0.5f * z * z);
+        value = z * c;
+        slope = __builtin_fmaf(0.39894228f, d, c);
+    } else {
+        value = act == kActRelu && z < 0.0f ? 0.0f : z;
+        slope = act_slope(z, act);
+    }
+}
+
 // Data-parallel move inside a row of 16 lanes (4 of lane_xor is the mirror of 8
 // lanes and the mirror of 4).
 template <int CTRL>
