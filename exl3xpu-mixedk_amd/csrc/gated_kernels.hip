@@ -18,6 +18,140 @@
 namespace xtq {
 namespace {
 
+// ------------------------------------------------------------------ operands
+// Rows for both weights: x times each one's row signs, or (GRAD) dg and du, of dy and
+// z, times each one's column scales.
+struct PairRows {
+    const uint16_t* v;                  // x or dy
+    long long stride;
+    const float* z;                     // [2][rows][cols] (GRAD)
+    const uint16_t* scale[2];           // fp16 per column
+    int type, act, rows, cols;
+};
+
+// Eight values of a row for each weight, before the scales.
+template <bool GRAD>
+__device__ __forceinline__ void load_pair8(const PairRows& s, size_t row, int col, float* a, float* b) {
+    unpack8(*(const u4_a2*)(s.v + row * (size_t)s.stride + col), s.type, a);
+    if constexpr (GRAD) {
+        const float* zg = s.z + row * (size_t)s.cols + col;
+        const float* zu = zg + (size_t)s.rows * s.cols;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f4 g = *(const f4_a4*)(zg + 4 * h), u = *(const f4_a4*)(zu + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float value, slope;
+                act_and_slope(g[i], s.act, value, slope);
+                b[4 * h + i] = a[4 * h + i] * value;
+                a[4 * h + i] *= u[i] * slope;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = a[i];
+    }
+}
+
+__device__ __forceinline__ void scale_pair8(const uint16_t* scale, int col, float* v) {
+    float c[8];
+    unpack8(*(const u4_a2*)(scale + col), kF16, c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= c[i];
+}
+
+// As row_exponents of linear_kernels.hip, for both weights at once: to [weight][places].
+// (2048 rows of 17408 read 356 MB in 115 us; other orders of the columns, more loads in
+// flight and z in the matrix cores' layout took as long.)
+template <bool GRAD>
+__device__ __forceinline__ void pair_exponents(const PairRows& s, int row, int32_t* __restrict__ shift,
+                                               int32_t* __restrict__ rowexp, int places) {
+    __shared__ float part[2][4];
+    float top[2] = {0.0f, 0.0f};
+    for (int c = threadIdx.x * 8; c < s.cols; c += 2048) {
+        float v[2][8];
+        load_pair8<GRAD>(s, row, c, v[0], v[1]);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            scale_pair8(s.scale[n], c, v[n]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top[n] = fmaxf(top[n], fabsf(v[n][i]));
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        top[n] = wave_max(top[n]);
+        if ((threadIdx.x & 63) == 0) part[n][threadIdx.x >> 6] = top[n];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const float* p = part[threadIdx.x];
+        const int sh = shift_to(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), 7);
+        shift[threadIdx.x * places + row] = sh;
+        rowexp[threadIdx.x * places + row] = -sh - 7;
+    }
+}
+
+// Both weights to fragments, and their rows' exponents beside, in one launch.
+struct PairWeights {
+    const int16_t* trellis[2];
+    int K[2], tn, decoders;             // workgroups of either weight
+    uint16_t* frags;
+    FragPlace place[2];
+};
+
+template <int CODE, int GRAD>
+__global__ __launch_bounds__(256) void pair_prepare_kernel(PairWeights w, PairRows s, int32_t* __restrict__ shift,
+                                                           int32_t* __restrict__ rowexp, int places) {
+    __shared__ uint32_t words[256 * 7];
+    int block = blockIdx.x;
+    if (block >= 2 * w.decoders) return pair_exponents<GRAD>(s, block - 2 * w.decoders, shift, rowexp, places);
+    const int role = block >= w.decoders;
+    if (role) block -= w.decoders;
+    auto decode = [&](auto K) {
+        decode_tiles<decltype(K)::value, CODE, GRAD>(words, block, w.trellis[role], w.tn, w.frags, w.place[role]);
+    };
+    switch (w.K[role]) {
+        case 2: return decode(std::integral_constant<int, 2>());
+        case 3: return decode(std::integral_constant<int, 3>());
+        case 4: return decode(std::integral_constant<int, 4>());
+        case 5: return decode(std::integral_constant<int, 5>());
+        case 6: return decode(std::integral_constant<int, 6>());
+        default: return decode(std::integral_constant<int, 7>());
+    }
+}
+
+// Rows to fragments for both weights, a wave 16 rows of one 128-column block: apart, or
+// (GRAD) one weight's behind the other's in the summed dimension, with the sums of 16
+// rows for the biases' gradients.
+template <bool GRAD>
+__global__ __launch_bounds__(256) void pair_transform_kernel(PairRows s, const int32_t* __restrict__ shift, int places,
+                                                             uint16_t* __restrict__ f0, uint16_t* __restrict__ f1,
+                                                             uint16_t* __restrict__ r0, uint16_t* __restrict__ r1,
+                                                             float* __restrict__ colsum) {
+    const int lane = threadIdx.x & 63, nblk = s.cols / 128;
+    const int blk = blockIdx.x * 4 + (threadIdx.x >> 6), grp = blockIdx.y;
+    if (blk >= nblk) return;
+    const int q = lane >> 4, row = grp * 16 + (lane & 15);
+    float v[2][32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0.0f;
+    if (row < s.rows) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) load_pair8<GRAD>(s, row, 128 * blk + 32 * p + 8 * q, v[0] + 8 * p, v[1] + 8 * p);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        if (GRAD && colsum) rows_sum(v[n], lane, colsum + ((size_t)grp * 2 + n) * s.cols + 128 * blk);
+        if (GRAD && !f0) continue;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) scale_pair8(s.scale[n], 128 * blk + 32 * p + 8 * q, v[n] + 8 * p);
+        rows_to_frags(v[n], row < s.rows ? shift[n * places + row] : 0, lane, grp, 4 * (GRAD * n * nblk + blk),
+                      (GRAD ? 8 : 4) * nblk, n ? f1 : f0, n ? r1 : r0);
+    }
+}
+
+// ------------------------------------------------------------------- product
 // Fused epilogue or parts for gated_join_kernel.
 enum GatedOut { kGatedFinish, kGatedParts };
 
@@ -233,97 +367,6 @@ __global__ __launch_bounds__(64) void gated_join_kernel(GatedGemm g, GatedArgs a
 }
 
 // ------------------------------------------------------------------ gradient
-struct GatedSource {
-    const uint16_t* dy;
-    long long dy_stride;
-    const float* z;                     // [2][rows][n]
-    const uint16_t* svh[2];
-    int type, act, rows, n;
-};
-
-// Eight values of dg and du of a row.
-__device__ __forceinline__ void gated_slopes(const GatedSource& s, size_t row, int col, float* dg, float* du) {
-    float d[8];
-    unpack8(*(const u4_a2*)(s.dy + row * (size_t)s.dy_stride + col), s.type, d);
-    const float* zg = s.z + row * (size_t)s.n + col;
-    const float* zu = zg + (size_t)s.rows * s.n;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const f4 a = *(const f4_a4*)(zg + 4 * h), b = *(const f4_a4*)(zu + 4 * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float value, slope;
-            act_and_slope(a[i], s.act, value, slope);
-            dg[4 * h + i] = d[4 * h + i] * b[i] * slope;
-            du[4 * h + i] = d[4 * h + i] * value;
-        }
-    }
-}
-
-// As row_exponents of linear_kernels.hip, for both weights' rows at once.
-__global__ __launch_bounds__(256) void gated_exponents_kernel(GatedSource s, int32_t* __restrict__ shift,
-                                                              int32_t* __restrict__ rowexp, int places) {
-    __shared__ float part[2][4];
-    const int row = blockIdx.x;
-    float top[2] = {0.0f, 0.0f};
-    for (int c = threadIdx.x * 8; c < s.n; c += 2048) {
-        float v[2][8];
-        gated_slopes(s, row, c, v[0], v[1]);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float t[8];
-            unpack8(*(const u4_a2*)(s.svh[r] + c), kF16, t);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top[r] = fmaxf(top[r], fabsf(v[r][i] * t[i]));
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        top[r] = wave_max(top[r]);
-        if ((threadIdx.x & 63) == 0) part[r][threadIdx.x >> 6] = top[r];
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const float* p = part[threadIdx.x];
-        const int sh = shift_to(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), 7);
-        shift[threadIdx.x * places + row] = sh;
-        rowexp[threadIdx.x * places + row] = -sh - 7;
-    }
-}
-
-// dg's and du's rows to fragments, one behind the other in the summed dimension, a
-// wave 16 rows of one 128-column block of both; the biases' gradients' sums beside.
-__global__ __launch_bounds__(256) void gated_transform_kernel(GatedSource s, const int32_t* __restrict__ shift,
-                                                              int places, uint16_t* __restrict__ frags,
-                                                              uint16_t* __restrict__ rest,
-                                                              float* __restrict__ colsum) {
-    const int lane = threadIdx.x & 63, nblk = s.n / 128;
-    const int blk = blockIdx.x * 4 + (threadIdx.x >> 6), grp = blockIdx.y;
-    if (blk >= nblk) return;
-    const int q = lane >> 4, row = grp * 16 + (lane & 15);
-    float v[2][32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0.0f;
-    if (row < s.rows) {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) gated_slopes(s, row, 128 * blk + 32 * p + 8 * q, v[0] + 8 * p, v[1] + 8 * p);
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        if (colsum) rows_sum(v[r], lane, colsum + ((size_t)grp * 2 + r) * s.n + 128 * blk);
-        if (!frags) continue;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            float c[8];
-            unpack8(*(const u4_a2*)(s.svh[r] + 128 * blk + 32 * p + 8 * q), kF16, c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[r][8 * p + i] *= c[i];
-        }
-        rows_to_frags(v[r], row < s.rows ? shift[r * places + row] : 0, lane, grp, 4 * (r * nblk + blk), 8 * nblk, frags,
-                      rest);
-    }
-}
-
 __global__ __launch_bounds__(256) void gated_column_sums_kernel(ColSum a) {
     __shared__ float part[256];
     column_sums(a, blockIdx.x, part);
@@ -465,6 +508,19 @@ ManyPlan many_plan(int rows, int k, int n, bool two) {
     return p;
 }
 
+template <int GRAD>
+void pair_prepare(const Weight* w, uint16_t* frags, FragPlace p0, FragPlace p1, const PairRows& src, int32_t* shift,
+                  int32_t* rowexp, int places, hipStream_t s) {
+    const int decoders = (w[0].k / 16) * (w[0].n / 16) / 32;
+    const PairWeights pw{{w[0].trellis, w[1].trellis}, {w[0].K, w[1].K}, w[0].n / 16, decoders, frags, {p0, p1}};
+    auto launch = [&](auto* kernel) {
+        hipLaunchKernelGGL(kernel, dim3(2 * decoders + src.rows), dim3(256), 0, s, pw, src, shift, rowexp, places);
+    };
+    if (w[0].code == kCodeMul1) launch(pair_prepare_kernel<kCodeMul1, GRAD>);
+    else if (w[0].code == kCodeMcg) launch(pair_prepare_kernel<kCodeMcg, GRAD>);
+    else launch(pair_prepare_kernel<kCode3Inst, GRAD>);
+}
+
 template <int T>
 hipError_t many(const GatedArgs& a, void* ws, hipStream_t s) {
     const int k = a.w[0].k, n = a.w[0].n;
@@ -478,17 +534,18 @@ hipError_t many(const GatedArgs& a, void* ws, hipStream_t s) {
     g.tiles = p.tiles;
     g.splits = p.splits;
     g.part = (float*)(base + p.part);
+    int32_t *shift = (int32_t*)(base + p.shift), *rowexp = (int32_t*)(base + p.rowexp);
+    uint16_t *xf[2], *x2[2];
     for (int r = 0; r < 2; ++r) {
-        int32_t *shift = (int32_t*)(base + p.shift) + r * p.places, *rowexp = (int32_t*)(base + p.rowexp) + r * p.places;
-        uint16_t *xf = (uint16_t*)(base + p.xf[r]), *x2 = a.two ? (uint16_t*)(base + p.x2[r]) : nullptr;
-        const Source src{a.x, a.x_stride, nullptr, 0, a.w[r].suh, T, a.rows, k};
-        prepare(a.w[r], 0, Prepare{(uint16_t*)(base + p.wf), FragPlace{r, 0, k / 32}, (k / 16) * (n / 16) / 32, src, shift,
-                                   rowexp}, s);
-        transform_rows(src, shift, xf, x2, nullptr, s);
-        g.B[r] = xf;
-        g.B2[r] = x2;
-        g.rowexp[r] = rowexp;
+        g.B[r] = xf[r] = (uint16_t*)(base + p.xf[r]);
+        g.B2[r] = x2[r] = a.two ? (uint16_t*)(base + p.x2[r]) : nullptr;
+        g.rowexp[r] = rowexp + r * p.places;
     }
+    const PairRows src{a.x, a.x_stride, nullptr, {a.w[0].suh, a.w[1].suh}, T, 0, a.rows, k};
+    pair_prepare<0>(a.w, (uint16_t*)(base + p.wf), FragPlace{0, 0, k / 32}, FragPlace{1, 0, k / 32}, src, shift, rowexp,
+                    p.places, s);
+    hipLaunchKernelGGL(pair_transform_kernel<false>, dim3((k / 128 + 3) / 4, p.groups), dim3(256), 0, s, src,
+                       (const int32_t*)shift, p.places, xf[0], xf[1], x2[0], x2[1], (float*)nullptr);
     const dim3 grid(p.tiles, p.splits), block(256);
     auto gemm = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, g, a); };
     if (p.splits == 1) {
@@ -540,21 +597,20 @@ hipError_t gradient(const GatedGradArgs& a, void* ws, hipStream_t s) {
     uint16_t *wf = (uint16_t*)(base + p.wf), *zf = (uint16_t*)(base + p.zf), *z2 = a.two ? (uint16_t*)(base + p.z2) : nullptr;
     const bool sum = a.dbias[0] || a.dbias[1];
     float* colsum = sum ? (float*)(base + p.colsum) : nullptr;
-    const GatedSource src{a.dy, a.dy_stride, a.z, {a.w[0].svh, a.w[1].svh}, T, a.act, a.rows, n};
+    const PairRows src{a.dy, a.dy_stride, a.z, {a.w[0].svh, a.w[1].svh}, T, a.act, a.rows, n};
     const ColSum sums{colsum, p.groups, 2 * n, T, a.bias_f32[0], a.dbias[0], n, a.bias_f32[1], a.dbias[1]};
     const int adders = sum ? 2 * n / 64 : 0;
-    const dim3 rows_grid((n / 128 + 3) / 4, p.groups);
+    auto transform = [&](const int32_t* sh, uint16_t* f, uint16_t* rest) {
+        hipLaunchKernelGGL(pair_transform_kernel<true>, dim3((n / 128 + 3) / 4, p.groups), dim3(256), 0, s, src, sh,
+                           p.places, f, f, rest, rest, colsum);
+    };
     if (!a.dx) {
-        hipLaunchKernelGGL(gated_transform_kernel, rows_grid, dim3(256), 0, s, src, shift, p.places, (uint16_t*)nullptr,
-                           (uint16_t*)nullptr, colsum);
+        transform(nullptr, nullptr, nullptr);
         hipLaunchKernelGGL(gated_column_sums_kernel, dim3(adders), dim3(256), 0, s, sums);
         return hipGetLastError();
     }
-    for (int r = 0; r < 2; ++r)
-        prepare(a.w[r], 1, Prepare{wf, FragPlace{-1, r * (n / 32), n / 16}, (k / 16) * (n / 16) / 32, Source{}, nullptr,
-                                   nullptr}, s);
-    hipLaunchKernelGGL(gated_exponents_kernel, dim3(a.rows), dim3(256), 0, s, src, shift, rowexp, p.places);
-    hipLaunchKernelGGL(gated_transform_kernel, rows_grid, dim3(256), 0, s, src, (const int32_t*)shift, p.places, zf, z2, colsum);
+    pair_prepare<1>(a.w, wf, FragPlace{-1, 0, n / 16}, FragPlace{-1, n / 32, n / 16}, src, shift, rowexp, p.places, s);
+    transform(shift, zf, z2);
     const Gemm g{wf, zf, z2, k / 16, p.groups, n / 16, p.tiles, p.splits, (float*)(base + p.part), nullptr, nullptr, 0};
     const hipError_t e = launch_parts(g, T, p.nb, a.two, sums, adders, s);
     if (e != hipSuccess) return e;

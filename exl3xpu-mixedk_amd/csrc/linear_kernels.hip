@@ -24,6 +24,17 @@
 namespace xtq {
 namespace {
 
+// Input of a product: activations, or (z set) a gradient dy times the
+// activation's slope at the saved z.
+struct Source {
+    const uint16_t* x;
+    long long stride;
+    const uint16_t* z;          // [rows][cols] or NULL
+    int act;
+    const uint16_t* colscale;   // fp16 per column
+    int type, rows, cols;
+};
+
 // Eight consecutive values of a row before its column scales.
 __device__ __forceinline__ void load8(const Source& s, size_t row, int col, float* v) {
     unpack8(*(const u4_a2*)(s.x + row * (size_t)s.stride + col), s.type, v);
@@ -106,55 +117,17 @@ __device__ void row_exponents(const Source& s, int row, int32_t* __restrict__ sh
     }
 }
 
-// Trellis to fragments of the inner weight.  BWD = 0: fragment (ng, p) holds
-// columns 16 ng + r, summed rows 32 p + 8 q + j (operand of x Wi); BWD = 1:
-// rows 16 kg + r, summed columns (operand of dz Wi^T).  Element (r, c) of a tile
-// is symbol 32 (c % 8) + 8 ((r % 8) / 2) + 4 (c / 8) + 2 (r / 8) + r % 2, its state
-// the 16-bit circular window ending with the symbol's K bits.  A workgroup
-// takes 8 by 4 tiles (along the summed dimension by the other), the trellis
-// words staged in LDS.  Memory bounds it: 5120 by 17408 at K = 4 reads 45 MB and
-// writes 178 in 50 us, 4.5 TB/s (a copy moves 4.97).  The workgroups past `decoders` find the exponents of the
-// source's rows, which nothing here waits for.  place: where the fragments lie
-// among those of another weight.
+// Trellis to fragments (decode_tiles).  Memory bounds it: 5120 by 17408 at K = 4 reads
+// 45 MB and writes 178 in 50 us, 4.5 TB/s (a copy moves 4.97).  The workgroups past
+// `decoders` find the exponents of the source's rows, which nothing here waits for.
 template <int K, int CODE, int BWD>
 __global__ __launch_bounds__(256) void prepare_kernel(const int16_t* __restrict__ trellis, int tk, int tn,
-                                                      uint16_t* __restrict__ frags, FragPlace place, int decoders,
-                                                      Source src, int32_t* __restrict__ shift,
+                                                      uint16_t* __restrict__ frags, int decoders, Source src,
+                                                      int32_t* __restrict__ shift,
                                                       int32_t* __restrict__ rowexp) {
     if ((int)blockIdx.x >= decoders) return row_exponents(src, blockIdx.x - decoders, shift, rowexp);
-    constexpr int TW = 8 * K;                           // words of a tile
-    __shared__ uint32_t words[32 * TW];
-    constexpr int NJ = BWD ? 8 : 4;
-    const int nj = tn / NJ, bi = blockIdx.x / nj, i0 = bi * (32 / NJ), j0 = (blockIdx.x - bi * nj) * NJ;   // first tile
-    for (int t = threadIdx.x; t < 32 * TW; t += 256) {
-        const int tile = t / TW, w = t - tile * TW;
-        const int i = i0 + tile / NJ, j = j0 + tile % NJ;
-        words[t] = *(const u1_a2*)(trellis + ((size_t)i * tn + j) * 16 * K + 2 * w);
-    }
-    __syncthreads();
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        // tile of this lane's elements: summed-dimension tile 2 p + q / 2
-        const int tile = BWD ? wv * NJ + 2 * p + (q >> 1) : (2 * p + (q >> 1)) * NJ + wv;
-        const uint32_t* tw = words + tile * TW;
-        uint32_t st[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int row = BWD ? r : 8 * (q & 1) + j, col = BWD ? 8 * (q & 1) + j : r;
-            const int t = 32 * (col & 7) + 8 * ((row & 7) >> 1) + 4 * (col >> 3) + 2 * (row >> 3) +
-                          (row & 1);
-            const int e = t * K + K - 1, lo = e >> 5, hi = lo > 0 ? lo - 1 : TW - 1;
-            st[j] = __builtin_amdgcn_alignbit(tw[hi], tw[lo], 31 - (e & 31)) & 0xFFFFu;
-        }
-        u4 o;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = code_pair<CODE>(st[2 * j], st[2 * j + 1]);
-        size_t g = BWD ? i0 + wv : j0 + wv;
-        if (place.half >= 0) g = (g >> 3) * 16 + 8 * place.half + (g & 7);
-        const size_t f = place.step + (BWD ? j0 : i0) / 2 + p;
-        *(u4*)(frags + frag_at(g, f, place.steps) + lane * 8) = o;
-    }
+    __shared__ uint32_t words[256 * K];
+    decode_tiles<K, CODE, BWD>(words, blockIdx.x, trellis, tn, frags, FragPlace{-1, 0, (BWD ? tn : tk) / 2});
 }
 
 // -------------------------------------------------------------------- matrix
@@ -548,14 +521,21 @@ __global__ __launch_bounds__(64 * W, 4) void gram_few_kernel(const uint16_t* __r
     }
 }
 
+struct Prepare {
+    uint16_t* frags;
+    int decoders;
+    Source src;
+    int32_t *shift, *rowexp;
+};
+
 template <int K, int CODE>
 void prepare_kc(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     const int tk = w.k / 16, tn = w.n / 16;
     const dim3 grid(p.decoders + p.src.rows);
     if (bwd) hipLaunchKernelGGL((prepare_kernel<K, CODE, 1>), grid, dim3(256), 0, s, w.trellis, tk, tn, p.frags,
-                                p.place, p.decoders, p.src, p.shift, p.rowexp);
+                                p.decoders, p.src, p.shift, p.rowexp);
     else hipLaunchKernelGGL((prepare_kernel<K, CODE, 0>), grid, dim3(256), 0, s, w.trellis, tk, tn, p.frags,
-                            p.place, p.decoders, p.src, p.shift, p.rowexp);
+                            p.decoders, p.src, p.shift, p.rowexp);
 }
 
 template <int K>
@@ -564,8 +544,6 @@ void prepare_k(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     else if (w.code == kCodeMcg) prepare_kc<K, kCodeMcg>(w, bwd, p, s);
     else prepare_kc<K, kCode3Inst>(w, bwd, p, s);
 }
-
-}  // namespace
 
 void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
     switch (w.K) {
@@ -577,6 +555,8 @@ void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s) {
         default: return prepare_k<7>(w, bwd, p, s);
     }
 }
+
+}  // namespace
 
 // How a product of `steps` steps is cut: nb groups of 16 rows to a wave's tile,
 // splits of the summed dimension.  The choice is the shortest estimate, from what
@@ -645,12 +625,6 @@ void launch_parts_of(const Gemm& g, int nb, bool two, const ColSum& sums, int ad
 
 }  // namespace
 
-void transform_rows(const Source& src, const int32_t* shift, uint16_t* frags, uint16_t* rest, float* colsum,
-                    hipStream_t s) {
-    hipLaunchKernelGGL(transform_kernel, dim3((src.cols / 128 + 3) / 4, (src.rows + 15) / 16), dim3(256), 0, s, src,
-                       shift, frags, rest, colsum);
-}
-
 hipError_t launch_parts(const Gemm& g, int type, int nb, bool two, const ColSum& sums, int adders, hipStream_t s) {
     if (type == kBf16) launch_parts_of<kBf16>(g, nb, two, sums, adders, s);
     else launch_parts_of<kF16>(g, nb, two, sums, adders, s);
@@ -670,8 +644,9 @@ hipError_t many(const Weight& w, int bwd, const Source& src, Epilogue ep, void* 
     uint16_t *xf = (uint16_t*)(base + p.xf), *x2 = two ? (uint16_t*)(base + p.x2) : nullptr, *wf = (uint16_t*)(base + p.wf);
     float* colsum = dbias ? (float*)(base + p.colsum) : nullptr;
     const int decoders = ep.y ? (w.k / 16) * (w.n / 16) / 32 : 0;
-    prepare(w, bwd, Prepare{wf, FragPlace{-1, 0, k / 32}, decoders, src, shift, rowexp}, s);
-    transform_rows(src, shift, xf, x2, colsum, s);
+    prepare(w, bwd, Prepare{wf, decoders, src, shift, rowexp}, s);
+    hipLaunchKernelGGL(transform_kernel, dim3((k / 128 + 3) / 4, p.groups), dim3(256), 0, s, src,
+                       (const int32_t*)shift, xf, x2, colsum);
     const ColSum sums{colsum, p.groups, k, T, dbias_f32, dbias, k, 0, nullptr};
     const int adders = dbias ? (k + 63) / 64 : 0;
     if (!ep.y) {

@@ -57,37 +57,6 @@ inline bool two_terms(int type, int act, bool fast) { return !fast && (type == k
 // The same for a gradient's product: no slope is taken at what it gives.
 inline bool two_terms_gradient(int type, bool fast) { return !fast && type == kF16; }
 
-// Input of a product: activations, or (z set) a gradient dy times the
-// activation's slope at the saved z.
-struct Source {
-    const uint16_t* x;
-    long long stride;
-    const uint16_t* z;          // [rows][cols] or NULL
-    int act;
-    const uint16_t* colscale;   // fp16 per column
-    int type, rows, cols;
-};
-
-// What a weight's way to fragments takes: where they lie among another weight's
-// (half: of the groups of 128, its half of 256, or -1; step: its first of `steps`
-// of the summed dimension), workgroups that decode, and a source whose rows'
-// exponents are found beside.
-struct FragPlace {
-    int half, step, steps;
-};
-struct Prepare {
-    uint16_t* frags;
-    FragPlace place;
-    int decoders;
-    Source src;
-    int32_t *shift, *rowexp;
-};
-void prepare(const Weight& w, int bwd, const Prepare& p, hipStream_t s);
-// A source's rows to fragments (rest: and what the rounding left; colsum: and their
-// sums by 16 rows, each NULL for none).
-void transform_rows(const Source& src, const int32_t* shift, uint16_t* frags, uint16_t* rest, float* colsum,
-                    hipStream_t s);
-
 struct Tiling {
     int nb, tiles, splits;
 };

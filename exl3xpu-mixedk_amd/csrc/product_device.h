@@ -38,6 +38,56 @@ __device__ __forceinline__ void unpack8(u4 w, int type, float* v) {
     }
 }
 
+// Where a weight's fragments lie among another's: half: of groups of 128 columns, its
+// half of 256, or -1; step: its first of `steps` of the summed dimension.
+struct FragPlace {
+    int half, step, steps;
+};
+
+// Trellis to fragments of the inner weight.  BWD = 0: fragment (ng, p) holds
+// columns 16 ng + r, summed rows 32 p + 8 q + j (operand of x Wi); BWD = 1:
+// rows 16 kg + r, summed columns (operand of dz Wi^T).  Element (r, c) of a tile
+// is symbol 32 (c % 8) + 8 ((r % 8) / 2) + 4 (c / 8) + 2 (r / 8) + r % 2, its state
+// the 16-bit circular window ending with the symbol's K bits.  A workgroup
+// (`block`) takes 8 by 4 tiles (along the summed dimension by the other), the trellis
+// words staged in LDS, 256 K of them.
+template <int K, int CODE, int BWD>
+__device__ __forceinline__ void decode_tiles(uint32_t* words, int block, const int16_t* __restrict__ trellis, int tn,
+                                             uint16_t* __restrict__ frags, const FragPlace& place) {
+    constexpr int TW = 8 * K;                           // words of a tile
+    constexpr int NJ = BWD ? 8 : 4;
+    const int nj = tn / NJ, bi = block / nj, i0 = bi * (32 / NJ), j0 = (block - bi * nj) * NJ;   // first tile
+    for (int t = threadIdx.x; t < 32 * TW; t += 256) {
+        const int tile = t / TW, w = t - tile * TW;
+        const int i = i0 + tile / NJ, j = j0 + tile % NJ;
+        words[t] = *(const u1_a2*)(trellis + ((size_t)i * tn + j) * 16 * K + 2 * w);
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        // tile of this lane's elements: summed-dimension tile 2 p + q / 2
+        const int tile = BWD ? wv * NJ + 2 * p + (q >> 1) : (2 * p + (q >> 1)) * NJ + wv;
+        const uint32_t* tw = words + tile * TW;
+        uint32_t st[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int row = BWD ? r : 8 * (q & 1) + j, col = BWD ? 8 * (q & 1) + j : r;
+            const int t = 32 * (col & 7) + 8 * ((row & 7) >> 1) + 4 * (col >> 3) + 2 * (row >> 3) +
+                          (row & 1);
+            const int e = t * K + K - 1, lo = e >> 5, hi = lo > 0 ? lo - 1 : TW - 1;
+            st[j] = __builtin_amdgcn_alignbit(tw[hi], tw[lo], 31 - (e & 31)) & 0xFFFFu;
+        }
+        u4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = code_pair<CODE>(st[2 * j], st[2 * j + 1]);
+        size_t g = BWD ? i0 + wv : j0 + wv;
+        if (place.half >= 0) g = (g >> 3) * 16 + 8 * place.half + (g & 7);
+        const size_t f = place.step + (BWD ? j0 : i0) / 2 + p;
+        *(u4*)(frags + frag_at(g, f, place.steps) + lane * 8) = o;
+    }
+}
+
 // A wave's 16 rows of one 128-column block to fragments, `step` the block's first:
 // block-128 transform, times 2^shift, rounded to fp16.  Lane 16 q + r holds columns
 // 32 p + 8 q + j of row r in v[8 p + j], so five of the transform's seven stages are
