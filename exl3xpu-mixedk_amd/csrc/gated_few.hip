@@ -64,12 +64,68 @@ struct Runs {
     }
 };
 
-// The last run to arrive of two blocks' adds the parts in order, transforms both and
-// writes act(gate) * up: the values between stay in registers.
+// First part and number of parts of both weights' columns of block blk.
+template <bool EVEN>
+__device__ __forceinline__ void parts_of(const GatedFew& f, const Runs& runs, int blk, int (&first)[2], int (&parts)[2]) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int b = 2 * blk + r;
+        first[r] = EVEN ? b * f.per_block : runs.of(b * runs.steps);
+        parts[r] = EVEN ? f.per_block : runs.of((b + 1) * runs.steps - 1) - first[r] + 1;
+        first[r] += b;
+    }
+}
+
+// R rows of a chunk (row0 + n step) of 128 columns: both weights' parts added in order
+// and transformed, scales and biases, and act(gate) * up, with the values between in
+// registers.
+template <int U, int R>
+__device__ __forceinline__ void finish_rows_of(const GatedArgs& a, const Columns<2>& cg, const Columns<2>& cu,
+                                               const float* part, const int (&first)[2], const int (&parts)[2], int blk,
+                                               int row_base, int rows, int row0, int step, int lane) {
+    const size_t run = (size_t)rows * 128;
+    const int col = blk * 128 + 2 * lane;
+    float v[R][2], u[R][2];
+    sum_rows<U, R>(v, part + first[0] * run, row0, step, rows, run, parts[0], lane);
+    sum_rows<U, R>(u, part + first[1] * run, row0, step, rows, run, parts[1], lane);
+#pragma unroll
+    for (int n = 0; n < R; ++n) {
+        transform_row(v[n][0], v[n][1], lane);
+        transform_row(u[n][0], u[n][1], lane);
+    }
+#pragma unroll
+    for (int n = 0; n < R; ++n) {
+        if (row0 + n * step >= rows) break;
+        const size_t row = row_base + row0 + n * step;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            v[n][c] = v[n][c] * cg.scale[c] + cg.bias[c];
+            u[n][c] = u[n][c] * cu.scale[c] + cu.bias[c];
+        }
+        if (a.z) {
+            float* z = a.z + row * a.w[0].n + col;
+            z[0] = v[n][0];
+            z[1] = v[n][1];
+            z += (size_t)a.rows * a.w[0].n;
+            z[0] = u[n][0];
+            z[1] = u[n][1];
+        }
+        activate<2>(v[n], a.act);
+        v[n][0] *= u[n][0];
+        v[n][1] *= u[n][1];
+        uint16_t* y = a.y + row * a.y_stride + col;
+        if (a.type == kBf16) store16<kBf16, 2>(y, v[n]);
+        else store16<kF16, 2>(y, v[n]);
+    }
+}
+
+// Up to 16 rows the last run to arrive of two blocks' finishes them; more are left to
+// gated_few_join_kernel, since the last runs' rows would be all that still works: 64
+// rows of 4096 by 6144 38.0 us, XX with the other launch.
 //
 // EVEN where that fills the places, two workgroups a compute unit.  272 blocks of 17408
 // columns do not, and two compute units of three then wait for the third: 48 rows of
-// 5120 take 84.9 us in 272 runs and 72.3 in 512, one row 51.8 and 43.7.  (Going over a
+// 5120 take 84.9 us in 272 runs and 70.5 in 512, one row 51.8 and 40.4.  (Going over a
 // block's end is a loop, which costs registers and 4 us where runs are short.)
 template <int G, bool FUSED, bool LO, bool EVEN>
 __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void gated_few_kernel(GatedArgs a, GatedFew f) {
@@ -81,7 +137,7 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void gated_few_k
     const int row_base = chunk * kFewRows, rows = a.rows - row_base < 16 * G ? a.rows - row_base : 16 * G;
     const Runs runs{steps, f.each, f.more, f.per_block};
     // (EVEN: neighbours are blocks of the same steps, whose trellis lies side by side:
-    // 64 rows of 4096 by 6144 42.8 us, 50.1 with a block's runs as neighbours)
+    // 64 rows of 4096 by 6144 44.7 us, 50.1 with a block's runs as neighbours)
     const int i = EVEN ? blockIdx.x % (2 * nb) * f.per_block + blockIdx.x / (2 * nb) : blockIdx.x;
     const size_t run = (size_t)rows * 128;
     float* const part = f.part + (size_t)chunk * (f.workers + 2 * nb) * 128 * kFewRows;
@@ -103,56 +159,21 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void gated_few_k
             const int row = 16 * g + (lane & 15);
             if (row < rows)
 #pragma unroll
-                for (int n = 0; n < N; ++n) store_shared(mine + row * 128 + 16 * (n * W + wv), total[g][n]);
+                for (int n = 0; n < N; ++n) {
+                    float* const p = mine + row * 128 + 16 * (n * W + wv);
+                    if constexpr (G == 1) store_shared(p, total[g][n]);
+                    else *(f4*)p = total[g][n];
+                }
         }
-        // (on their way while the workgroups meet)
-        const int col = blk * 128 + 2 * lane;
-        const Columns<2> cg = role_columns(a, 0, col), cu = role_columns(a, 1, col);
-        // each role's first run and number of them
-        int first[2], parts[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int b = 2 * blk + r;
-            first[r] = EVEN ? b * f.per_block : runs.of(b * steps);
-            parts[r] = EVEN ? f.per_block : runs.of((b + 1) * steps - 1) - first[r] + 1;
-            first[r] += b;
-        }
-        if (!arrive(f.counters + chunk * nb + blk, parts[0] + parts[1], threadIdx.x)) return;
-        constexpr int R = G == 1 ? 2 : 4, U = G == 1 ? 8 : 4;
+        if constexpr (G == 1) {
+            // (on their way while the workgroups meet)
+            const Columns<2> cg = role_columns(a, 0, blk * 128 + 2 * lane), cu = role_columns(a, 1, blk * 128 + 2 * lane);
+            int first[2], parts[2];
+            parts_of<EVEN>(f, runs, blk, first, parts);
+            if (!arrive(f.counters + blk, parts[0] + parts[1], threadIdx.x)) return;
 #pragma unroll 1
-        for (int r0 = wv; r0 < rows; r0 += R * W) {
-            float v[R][2], u[R][2];
-            sum_rows<U, R>(v, part + first[0] * run, r0, W, rows, run, parts[0], lane);
-            sum_rows<U, R>(u, part + first[1] * run, r0, W, rows, run, parts[1], lane);
-#pragma unroll
-            for (int n = 0; n < R; ++n) {
-                transform_row(v[n][0], v[n][1], lane);
-                transform_row(u[n][0], u[n][1], lane);
-            }
-#pragma unroll
-            for (int n = 0; n < R; ++n) {
-                if (r0 + n * W >= rows) break;
-                const size_t row = row_base + r0 + n * W;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    v[n][c] = v[n][c] * cg.scale[c] + cg.bias[c];
-                    u[n][c] = u[n][c] * cu.scale[c] + cu.bias[c];
-                }
-                if (a.z) {
-                    float* z = a.z + row * a.w[0].n + col;
-                    z[0] = v[n][0];
-                    z[1] = v[n][1];
-                    z += (size_t)a.rows * a.w[0].n;
-                    z[0] = u[n][0];
-                    z[1] = u[n][1];
-                }
-                activate<2>(v[n], a.act);
-                v[n][0] *= u[n][0];
-                v[n][1] *= u[n][1];
-                uint16_t* y = a.y + row * a.y_stride + col;
-                if (a.type == kBf16) store16<kBf16, 2>(y, v[n]);
-                else store16<kF16, 2>(y, v[n]);
-            }
+            for (int r0 = wv; r0 < rows; r0 += 2 * W)
+                finish_rows_of<8, 2>(a, cg, cu, part, first, parts, blk, 0, rows, r0, W, lane);
         }
     };
     const int end = runs.at<EVEN>(i + 1);
@@ -174,11 +195,31 @@ __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void gated_few_k
     }
 }
 
+// Finishes 128 columns of eight rows, a wave two of them.
+template <bool EVEN>
+__global__ __launch_bounds__(256) void gated_few_join_kernel(GatedArgs a, GatedFew f) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, blk = blockIdx.x, nb = gridDim.x;
+    const int row = blockIdx.y * 8 + wv, chunk = row / kFewRows, row_base = chunk * kFewRows;
+    const int rows = a.rows - row_base < kFewRows ? a.rows - row_base : kFewRows;
+    if (row - row_base >= rows) return;
+    const Runs runs{a.w[0].k / 32, f.each, f.more, f.per_block};
+    int first[2], parts[2];
+    parts_of<EVEN>(f, runs, blk, first, parts);
+    const Columns<2> cg = role_columns(a, 0, blk * 128 + 2 * lane), cu = role_columns(a, 1, blk * 128 + 2 * lane);
+    finish_rows_of<4, 2>(a, cg, cu, f.part + (size_t)chunk * (f.workers + 2 * nb) * 128 * kFewRows, first, parts, blk,
+                         row_base, rows, row - row_base, 4, lane);
+}
+
 template <int G, bool FUSED, bool LO>
 hipError_t launch(const GatedArgs& a, const GatedFew& f, hipStream_t s) {
     const dim3 grid(f.workers, (a.rows + kFewRows - 1) / kFewRows), block(64 * few_waves(G));
     if (f.per_block) hipLaunchKernelGGL((gated_few_kernel<G, FUSED, LO, true>), grid, block, 0, s, a, f);
     else hipLaunchKernelGGL((gated_few_kernel<G, FUSED, LO, false>), grid, block, 0, s, a, f);
+    if (G > 1) {
+        const dim3 rest(a.w[0].n / 128, (a.rows + 7) / 8);
+        if (f.per_block) hipLaunchKernelGGL(gated_few_join_kernel<true>, rest, dim3(256), 0, s, a, f);
+        else hipLaunchKernelGGL(gated_few_join_kernel<false>, rest, dim3(256), 0, s, a, f);
+    }
     return hipGetLastError();
 }
 
