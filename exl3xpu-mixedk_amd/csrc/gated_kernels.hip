@@ -428,19 +428,22 @@ bool takes_few(int rows, int k, int n) {
            (long long)(n / 64) * (k / 32) < 1LL << 30;
 }
 
-// A chunk's workgroups: as few_splits cuts the blocks; evenly over all steps where
-// that leaves a fifth of the places empty and a run still has 32 steps.
+// A chunk's workgroups: as few_splits cuts the blocks, with 16 steps each at least where
+// there are several chunks (100 rows of 1024 by 4096 22.9 us, 27.8 with 8).  Where that
+// leaves a fifth of the places empty, blocks that come twice into them in four parts
+// each (172 of 4096: 1 row 28.2 us, 36.7 cut evenly over all steps, 64 rows 45.1, 48.4),
+// others evenly over all steps (272 of 5120: 45.5, 59.8 uncut; 66.2, 88) if a run still
+// has 32 of them.
 void few_workers(FewPlan& p, int rows, int k, int n, int waves) {
-    const int blocks = n / 64, chunks = few_chunks(rows), places = 2 * kCUs;
+    const int blocks = n / 64, chunks = few_chunks(rows), steps = k / 32, places = 2 * kCUs;
     int s = few_splits(rows < kFewRows ? rows : kFewRows, k, 2 * n, waves);
+    if (chunks > 1 && s > steps / 16) s = steps / 16 > 1 ? steps / 16 : 1;
     while (s > 1 && blocks * s * chunks > places) --s;
     const int all = blocks * s * chunks, rounds = (all + places - 1) / places;
     p.per_block = s;
-    p.workers = blocks * s;
-    if (2 * all > places && 5LL * all < 4LL * rounds * places && (long long)blocks * (k / 32) * chunks / places >= 32) {
-        p.per_block = 0;
-        p.workers = places / chunks;
-    }
+    if (2 * all > places && 5LL * all < 4LL * rounds * places && (long long)blocks * steps * chunks / places >= 32)
+        p.per_block = chunks == 1 && s == 2 && steps >= 4 * waves ? 4 : 0;
+    p.workers = p.per_block ? blocks * p.per_block : places / chunks;
 }
 
 FewPlan few_plan(int rows, int k, int n, bool two) {
