@@ -212,8 +212,10 @@ __device__ __forceinline__ void store_gated(const f4* gate, const f4* up, const 
 // buffers, two steps ahead, as in gemm_kernel of linear_kernels.hip; a wave's rows are
 // its own weight's and its own half, so they come straight into its registers.
 // Two workgroups share a compute unit.  (The rows through LDS too: 32 KiB a step, two
-// buffers of which leave room for the second workgroup: 1508 us for 4096 rows of 5120
-// by 17408, and now 1308.)
+// buffers of which leave room for the second workgroup: 1597 us in all for 4096 rows of
+// 5120 by 17408, 1542 so.)  Tiles go by XCD as gemm_kernel's, in bands of kRowBand.
+constexpr int kRowBand = 4;             // (4096 rows 1520 us in all; of 2, 3, 6, 8 and 16: 1584, 1648, 1638, 1579, 1624)
+
 template <int T, int OUT, int NB, int TERMS>
 __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedArgs a) {
     constexpr int kOwn = 4 + NB * TERMS;        // a wave's loads of a step
@@ -222,9 +224,9 @@ __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedAr
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), role = wv & 1, wm = wv >> 1;
     const int tile = xcd_order(blockIdx.x, g.tiles);
-    const int mt = (g.gb + 2 * NB - 1) / (2 * NB), band = tile / (g.nb * kBand);
-    const int high = mt - band * kBand < kBand ? mt - band * kBand : kBand, in = tile - band * g.nb * kBand;
-    const int tn = in / high, tm = band * kBand + in - tn * high;
+    const int mt = (g.gb + 2 * NB - 1) / (2 * NB), band = tile / (g.nb * kRowBand);
+    const int high = mt - band * kRowBand < kRowBand ? mt - band * kRowBand : kRowBand, in = tile - band * g.nb * kRowBand;
+    const int tn = in / high, tm = band * kRowBand + in - tn * high;
     const int split = blockIdx.y;
     const int s0 = (int)((long long)g.steps * split / g.splits);
     const int s1 = (int)((long long)g.steps * (split + 1) / g.splits);

@@ -703,22 +703,23 @@ def residual_norm(block: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
     _like(res, x, x.shape, "residual", (x.dtype,))
     if gate is not None:
         _like(gate, x, x.shape, "gate", (x.dtype,))
-    tensors, types = (x, res, gate, *params), (x.dtype, torch.float32)
+    tensors, types, width = (x, res, gate, *params), (x.dtype, torch.float32), x.shape[-1:]
+    grad = x.requires_grad or res.requires_grad or (gate is not None and gate.requires_grad)
     for t, what in zip(params, _PARAMS):
         if t is not None:
-            _like(t, x, x.shape[-1:], what, types)
-    for k in (kind, post):
-        if k not in NORMS:
-            raise ValueError(f"norm {k!r} not in {tuple(NORMS)}")
+            _like(t, x, width, what, types)
+            grad = grad or t.requires_grad
+    if kind not in NORMS or post not in NORMS:
+        raise ValueError(f"norm {kind!r}, {post!r} not in {tuple(NORMS)}")
     if gate_act not in GATES:
         raise ValueError(f"gate_act {gate_act!r} not in {tuple(GATES)}")
     if not (eps >= 0 and post_eps >= 0):
         raise ValueError(f"eps must be at least 0, got {eps}, {post_eps}")
-    if (kind is None and any(t is not None for t in params[:2])) or \
-            (post is None and any(t is not None for t in params[3:])):
+    if (kind is None and (weight is not None or bias is not None)) or \
+            (post is None and (post_weight is not None or post_bias is not None)):
         raise ValueError("weights and biases are of a norm that there is")
     _no_tangents("residual_norm", *tensors)
     cfg = (NORMS[kind], NORMS[post], GATES[gate_act], float(eps), float(post_eps), float(number))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if grad and torch.is_grad_enabled():
         return _ResidualNorm.apply(*tensors, cfg)
     return _residual_forward(x, res, gate, params, cfg, False)[:2]
