@@ -426,7 +426,7 @@ constexpr int kGatedFew = 256;
 int few_chunks(int rows) { return (rows + kFewRows - 1) / kFewRows; }
 
 bool takes_few(int rows, int k, int n) {
-    return rows <= kGatedFew && few_chunks(rows) * (n / 128) <= XTQ_OP_COUNTERS &&
+    return rows <= kGatedFew && n / 128 <= XTQ_OP_COUNTERS &&
            (long long)(n / 64) * (k / 32) < 1LL << 30;
 }
 

@@ -38,7 +38,8 @@ __device__ __forceinline__ void unpack(u4 w, float* v) {
 // Eight values of a row from column `col` on, on their way: every lane loads 16 bytes
 // inside the row, those at its end where its own reach past it, and in_place brings
 // them home once they are there.  (A load under a condition is waited for where the
-// branches meet: the gradient of 8191 rows of 5120 took 215 us so, and not 152.)
+// branches meet: a residual's norm of 8191 rows of 5120 and its gradient took 316 us so,
+// and 302 without.)
 template <int MODE>
 __device__ __forceinline__ u4 load8(const uint16_t* row, int col, int d) {
     if (MODE != kSub || d >= 8) return *(const u4_a2*)(row + (col < d - 8 ? col : d - 8));
@@ -75,7 +76,7 @@ __device__ __forceinline__ void store8(uint16_t* p, int n, const float* v) {
 }
 
 // Eight channels of a parameter (of the rows' type or fp32) from `col` on, `missing`
-// where there is none.  Those past the end are any finite numbers.
+// where there is none.  Those past the end are any numbers.
 template <int T, int MODE>
 __device__ __forceinline__ void param8(const NormParam& p, int col, int d, float missing, float* v) {
     if (!p.p) {
@@ -148,7 +149,7 @@ struct Group {
         for (int i = 0; i < N; ++i)
             v[i] = MODE == kSub ? sum16(v[i]) : MODE == kHalf ? sum32(v[i]) : sum64(v[i]);
         if constexpr (MODE == kBlock) {
-            __shared__ float part[2][2][16];
+            __shared__ float part[2][N][16];
             const int wv = threadIdx.x >> 6, waves = blockDim.x >> 6, l = threadIdx.x & 15;
             if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -282,6 +283,13 @@ __device__ __forceinline__ void load_channels(Channels& c, const NormArgs& a, in
         param8<T, MODE>(a.post_weight, col, a.d, 1.0f, c.pw);
         param8<T, MODE>(a.post_bias, col, a.d, 0.0f, c.pb);
     }
+    // (past the row's end zeros: an infinite one would make NaN of the zeros there)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (col + i < a.d) continue;
+        c.w[i] = 0.0f;
+        if constexpr (OF != kPlain) c.s[i] = c.pw[i] = c.pb[i] = 0.0f;
+    }
 }
 
 // Eight channels of a row's inputs.
@@ -399,69 +407,51 @@ __device__ __forceinline__ float total(const Forward& f, const Raw& t, int i, co
 //   dy' = dy + rstd (c - t^ mean(c t^) - mean(c))       (the last for "layer"),
 //   dres = dy',  ds = sum of dy' q,  dgate = dy' s p ga'(g),  dp = dy' s ga(g),
 // and dx from dp as dy' from dh.  y and the norms are computed anew from the inputs
-// and the rows' saved means and factors, so nothing of y's rounding enters; and again
-// after each sum over the row, which costs less than registers for it.
+// and the rows' saved means and factors, so nothing of y's rounding enters.
 //
-// V = 1: a group goes through its rows with the parameters and (SUMS) the channels'
-// sums in registers, a row's inputs on their way while the row before is worked on,
-// and a workgroup leaves one row of partial sums, which norm_sums_kernel adds in
-// order.  Wider rows have no registers for that: they leave their rows' projections,
-// from which norm_channels_kernel sums the channels.
-template <int T, int MODE, int V, int OF, bool SUMS, bool BIAS>
+// Rows of one eight a lane: a group goes through its rows with the parameters and
+// (SUMS) the channels' sums in registers, a row's inputs on their way while the row
+// before is worked on, and a workgroup leaves one row of partial sums, which
+// norm_sums_kernel adds in order.  What a sum over the row needs again after it is
+// computed anew, which costs less than registers for it.
+template <int T, int MODE, int OF, bool SUMS, bool BIAS>
 __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bwd_kernel(NormGradArgs a) {
-    static_assert(!SUMS || V == 1, "sums of one eight a lane");
     Group<MODE> g;
     constexpr int R = rows_of(MODE);
     const int sub = MODE == kBlock ? 0 : threadIdx.x / lanes_of(MODE);
-    const int d = a.f.d, step = gridDim.x * R;
+    const int d = a.f.d, step = gridDim.x * R, col = g.lane * 8;
     const float inv = 1.0f / (float)d;
     struct Row {
-        Raw raw[V];
+        Raw raw;
         f4 stats;
     };
     auto load = [&](Row& t, int row) {
         const size_t at = row < a.f.rows ? row : 0;
         t.stats = *(const f4*)(a.f.stats + 4 * at);
-#pragma unroll
-        for (int v = 0; v < V; ++v) load_raw<MODE, OF>(t.raw[v], a, at, (v * g.width + g.lane) * 8);
+        if (row >= a.f.rows) t.stats = (f4){0.0f, 0.0f, 0.0f, 0.0f};     // (the first row's may be infinite)
+        load_raw<MODE, OF>(t.raw, a, at, col);
     };
     Sums<OF, BIAS> sums;
     if constexpr (SUMS) sums.clear();
-    Channels kept;
+    Channels ch;
     Row next;
-    if constexpr (V == 1) {
-        load(next, blockIdx.x * R + sub);
-        load_channels<T, MODE, OF>(kept, a.f, g.lane * 8);
-    }
+    load(next, blockIdx.x * R + sub);
+    load_channels<T, MODE, OF>(ch, a.f, col);
     for (int base = blockIdx.x * R; base < a.f.rows; base += step) {
-        const int row = base + sub;
-        const bool in = row < a.f.rows;
-        const size_t at = in ? row : 0;
-        Row now;
-        if constexpr (V == 1) {
-            now = next;
-            if (base + step < a.f.rows) load(next, row + step);
-        } else {
-            load(now, row);
-        }
-        Gate gate;                      // (of one eight kept for what follows the sum)
+        const int row = base + sub, n = row < a.f.rows ? d - col : 0, nh = a.dh ? n : 0;
+        const size_t at = row < a.f.rows ? row : 0;
+        Row now = next;
+        if (base + step < a.f.rows) load(next, row + step);
+        Gate gate;
         float two[2] = {0.0f, 0.0f};
+        raw_in_place<OF>(now.raw, n);
+        gates<T, OF>(gate, now.raw, a.f.gate_act);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int col = (v * g.width + g.lane) * 8, n = in ? d - col : 0;
-            raw_in_place<OF>(now.raw[v], n);
-            gates<T, OF>(gate, now.raw[v], a.f.gate_act);
-            Channels ch;
-            if constexpr (V == 1) ch = kept;
-            else load_channels<T, MODE, OF>(ch, a.f, col);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const Forward f = again<T, OF, BIAS>(now.raw[v], i, gate, ch, now.stats);
-                two[0] = __builtin_fmaf(f.c, f.that, two[0]);
-                two[1] += f.c;
-                if constexpr (SUMS) sums.norm(i, f, a.dh);
-            }
-            if (V > 1) __builtin_amdgcn_sched_barrier(0);       // (one eight's registers at a time)
+        for (int i = 0; i < 8; ++i) {
+            const Forward f = again<T, OF, BIAS>(now.raw, i, gate, ch, now.stats);
+            two[0] = __builtin_fmaf(f.c, f.that, two[0]);
+            two[1] += f.c;
+            if constexpr (SUMS) sums.norm(i, f, a.dh);
         }
         float c1 = 0.0f, c2 = 0.0f;
         if (a.dh) {
@@ -469,61 +459,39 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
             c1 = two[0] * inv;
             if (a.f.kind == kNormLayer) c2 = two[1] * inv;
         }
-        if (V > 1 && a.means && threadIdx.x == 0) {
-            a.means[2 * at] = c1;
-            a.means[2 * at + 1] = c2;
-        }
-        float dp[V][8];
         two[0] = two[1] = 0.0f;
+        forget<OF>(now.raw);
+        float dt[8], dg[8], dp[8];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int col = (v * g.width + g.lane) * 8, n = in ? d - col : 0, nh = a.dh ? n : 0;
-            forget<OF>(now.raw[v]);
-            Channels ch;
-            if constexpr (V == 1) ch = kept;
-            else load_channels<T, MODE, OF>(ch, a.f, col);
-            if (V > 1) gates<T, OF>(gate, now.raw[v], a.f.gate_act);
-            float dt[8], dg[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const Forward f = again<T, OF, BIAS>(now.raw[v], i, gate, ch, now.stats);
-                dt[i] = total<T, OF>(f, now.raw[v], i, now.stats, c1, c2, i < nh);
-                dp[v][i] = dt[i];
-                if constexpr (OF != kPlain) {
-                    const float ds = dt[i] * ch.s[i], to = OF == kWithGate ? ds * gate.ga[i] : ds;
-                    dg[i] = ds * f.p * gate.slope[i];
-                    if constexpr (SUMS) sums.rest(i, f, dt[i], to);
-                    dp[v][i] = to * ch.pw[i];
-                    two[0] = __builtin_fmaf(dp[v][i], f.hat, two[0]);
-                    two[1] += dp[v][i];
-                }
+        for (int i = 0; i < 8; ++i) {
+            const Forward f = again<T, OF, BIAS>(now.raw, i, gate, ch, now.stats);
+            dt[i] = total<T, OF>(f, now.raw, i, now.stats, c1, c2, i < nh);
+            dp[i] = dt[i];
+            if constexpr (OF != kPlain) {
+                const float ds = dt[i] * ch.s[i], to = OF == kWithGate ? ds * gate.ga[i] : ds;
+                dg[i] = ds * f.p * gate.slope[i];
+                if constexpr (SUMS) sums.rest(i, f, dt[i], to);
+                dp[i] = to * ch.pw[i];
+                two[0] = __builtin_fmaf(dp[i], f.hat, two[0]);
+                two[1] += dp[i];
             }
-            if constexpr (OF != kPlain)
-                if (a.dres && n > 0) store8<T>(a.dres + at * d + col, n, dt);
-            if constexpr (OF == kWithGate)
-                if (a.dgate && n > 0) store8<T>(a.dgate + at * d + col, n, dg);
-            if (V > 1) __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (OF != kPlain)
+            if (a.dres && n > 0) store8<T>(a.dres + at * d + col, n, dt);
+        if constexpr (OF == kWithGate)
+            if (a.dgate && n > 0) store8<T>(a.dgate + at * d + col, n, dg);
         if (OF != kPlain && a.f.post) {
             g.sum(two);
             const float e1 = two[0] * inv, e2 = a.f.post == kNormLayer ? two[1] * inv : 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    dp[v][i] = now.stats[1] * (dp[v][i] - (pick<T>(now.raw[v].x, i) - now.stats[0]) * now.stats[1] * e1 - e2);
+            for (int i = 0; i < 8; ++i)
+                dp[i] = now.stats[1] * (dp[i] - (pick<T>(now.raw.x, i) - now.stats[0]) * now.stats[1] * e1 - e2);
         }
-        if (a.dx)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int col = (v * g.width + g.lane) * 8, n = in ? d - col : 0;
-                if (n > 0) store8<T>(a.dx + at * d + col, n, dp[v]);
-            }
+        if (a.dx && n > 0) store8<T>(a.dx + at * d + col, n, dp);
     }
     if constexpr (SUMS) {
         // [sum][workgroup][d]
         __shared__ float join[MODE == kBlock ? 1 : 256 * 8];
-        const int col = g.lane * 8;
 #pragma unroll
         for (int k = 0; k < Sums<OF, BIAS>::N; ++k) {
             if (!Sums<OF, BIAS>::has(k) || !a.dparam[k].p) continue;
@@ -545,10 +513,71 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
     }
 }
 
-// The channels' sums of wide rows, from the inputs and the rows' projections: a
-// workgroup takes 2048 channels of every gridDim.y-th row.
+// Wider rows do not stay in registers, and are read twice.  First all that a row's
+// gradients take of the whole row: with u = s ga(g) w' (w' the post norm's weight) and
+// x^ the post norm before it, dp = u dy', so that dx's sums over the row of u x^ dy' and
+// u dy' are, dy' being linear in them, combinations of sums that need no other first.
+// (2000 rows with everything, forward and back: of 17408 313 us, 483 with a lane's three
+// eights kept in registers, of 32768 685 and 1953; of 6144, a lane's one, 95.)
+constexpr int kWideWaves = 8;
+
 template <int T, int OF, bool BIAS>
-__global__ __launch_bounds__(256) void norm_channels_kernel(NormGradArgs a) {
+__global__ __launch_bounds__(64 * kWideWaves) void norm_rows_kernel(NormGradArgs a) {
+    constexpr int N = OF == kPlain ? 2 : 10;
+    Group<kBlock> g;
+    const int d = a.f.d;
+    const float inv = 1.0f / (float)d;
+    for (int row = blockIdx.x; row < a.f.rows; row += gridDim.x) {
+        const f4 stats = *(const f4*)(a.f.stats + 4 * (size_t)row);
+        float v[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = 0.0f;
+        Raw next;
+        load_raw<kBlock, OF>(next, a, row, g.lane * 8);
+        for (int col = g.lane * 8; col < d; col += 512 * kWideWaves) {
+            Raw now = next;
+            load_raw<kBlock, OF>(next, a, row, col + 512 * kWideWaves);
+            Channels ch;
+            load_channels<T, kBlock, OF>(ch, a.f, col);
+            raw_in_place<OF>(now, d - col);
+            Gate gate;
+            gates<T, OF>(gate, now, a.f.gate_act);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const Forward f = again<T, OF, BIAS>(now, i, gate, ch, stats);
+                v[0] = __builtin_fmaf(f.c, f.that, v[0]);
+                v[1] += f.c;
+                if constexpr (OF != kPlain) {
+                    const float dy = pick<T>(now.y, i), u = ch.s[i] * gate.ga[i] * ch.pw[i], uh = u * f.hat;
+                    v[2] = __builtin_fmaf(uh, dy, v[2]);
+                    v[3] = __builtin_fmaf(uh, f.c, v[3]);
+                    v[4] = __builtin_fmaf(uh, f.that, v[4]);
+                    v[5] += uh;
+                    v[6] = __builtin_fmaf(u, dy, v[6]);
+                    v[7] = __builtin_fmaf(u, f.c, v[7]);
+                    v[8] = __builtin_fmaf(u, f.that, v[8]);
+                    v[9] += u;
+                }
+            }
+        }
+        g.sum(v);
+        f4 m = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (a.dh) {
+            m[0] = v[0] * inv;
+            if (a.f.kind == kNormLayer) m[1] = v[1] * inv;
+        }
+        if constexpr (OF != kPlain) {
+            if (a.f.post) m[2] = (v[2] + (a.dh ? stats[3] * (v[3] - m[0] * v[4] - m[1] * v[5]) : 0.0f)) * inv;
+            if (a.f.post == kNormLayer) m[3] = (v[6] + (a.dh ? stats[3] * (v[7] - m[0] * v[8] - m[1] * v[9]) : 0.0f)) * inv;
+        }
+        if (threadIdx.x == 0) *(f4*)(a.means + 4 * (size_t)row) = m;
+    }
+}
+
+// Then the gradients, with the channels' sums beside: a workgroup takes 2048 channels
+// of every gridDim.y-th row and leaves a part of the sums.
+template <int T, int OF, bool BIAS>
+__global__ __launch_bounds__(256) void norm_wide_kernel(NormGradArgs a) {
     const int d = a.f.d, col = (blockIdx.x * 256 + threadIdx.x) * 8, n = d - col;
     if (n <= 0) return;
     Channels ch;
@@ -559,21 +588,32 @@ __global__ __launch_bounds__(256) void norm_channels_kernel(NormGradArgs a) {
     load_raw<kBlock, OF>(next, a, blockIdx.y, col);
     for (int row = blockIdx.y; row < a.f.rows; row += gridDim.y) {
         Raw now = next;
-        const f4 stats = *(const f4*)(a.f.stats + 4 * (size_t)row);
-        const float c1 = a.means[2 * (size_t)row], c2 = a.means[2 * (size_t)row + 1];
+        const f4 stats = *(const f4*)(a.f.stats + 4 * (size_t)row), m = *(const f4*)(a.means + 4 * (size_t)row);
         if (row + (int)gridDim.y < a.f.rows) load_raw<kBlock, OF>(next, a, row + gridDim.y, col);
         raw_in_place<OF>(now, n);
         Gate gate;
         gates<T, OF>(gate, now, a.f.gate_act);
+        float dt[8], dg[8], dp[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const Forward f = again<T, OF, BIAS>(now, i, gate, ch, stats);
             sums.norm(i, f, a.dh);
+            dt[i] = total<T, OF>(f, now, i, stats, m[0], m[1], a.dh && i < n);
+            dp[i] = dt[i];
             if constexpr (OF != kPlain) {
-                const float dt = total<T, OF>(f, now, i, stats, c1, c2, a.dh && i < n);
-                sums.rest(i, f, dt, dt * ch.s[i] * gate.ga[i]);
+                const float ds = dt[i] * ch.s[i], to = OF == kWithGate ? ds * gate.ga[i] : ds;
+                dg[i] = ds * f.p * gate.slope[i];
+                sums.rest(i, f, dt[i], to);
+                dp[i] = to * ch.pw[i];
+                if (a.f.post) dp[i] = stats[1] * (dp[i] - f.hat * m[2] - m[3]);
             }
         }
+        const size_t at = (size_t)row * d + col;
+        if constexpr (OF != kPlain)
+            if (a.dres) store8<T>(a.dres + at, n, dt);
+        if constexpr (OF == kWithGate)
+            if (a.dgate) store8<T>(a.dgate + at, n, dg);
+        if (a.dx) store8<T>(a.dx + at, n, dp);
     }
 #pragma unroll
     for (int k = 0; k < Sums<OF, BIAS>::N; ++k) {
@@ -614,10 +654,11 @@ struct Shape {
     int mode, v, threads;
 };
 
+constexpr int kWide = 512 * kRowWaves;          // rows wider than this have no one eight a lane
+
 Shape norm_shape(int d, bool gradient) {
     if (d <= 512) return {d <= 128 ? kSub : d <= 256 ? kHalf : kWave, 1, 256};
-    const int most = 512 * kRowWaves;
-    int v = d <= 4 * most ? (d + most - 1) / most : 6;
+    int v = d <= 4 * kWide ? (d + kWide - 1) / kWide : 6;
     if (!gradient && v == 1) v = 2;
     return {kBlock, v, (d + 512 * v - 1) / (512 * v) * 64};
 }
@@ -635,52 +676,69 @@ void with_shape(const Shape& s, F f) {
     else f(integral_constant<int, kBlock>(), integral_constant<int, 6>());
 }
 
+// A grid has less than 2^32 lanes: so many workgroups, of kRowWaves waves at most, a launch.
+constexpr int kMostGroups = 1 << 22;
+
 template <int T>
-void forward(const NormArgs& a, hipStream_t s) {
+void forward(NormArgs a, hipStream_t s) {
     const Shape sh = norm_shape(a.d, false);
-    const dim3 grid((a.rows + rows_of(sh.mode) - 1) / rows_of(sh.mode)), block(sh.threads);
-    with_shape(sh, [&](auto mode, auto v) {
-        constexpr int M = decltype(mode)::value, V = decltype(v)::value;
-        if constexpr (M != kBlock || V > 1) hipLaunchKernelGGL((norm_kernel<T, M, V>), grid, block, 0, s, a);
-    });
+    const int all = (a.rows + rows_of(sh.mode) - 1) / rows_of(sh.mode), rows = kMostGroups * rows_of(sh.mode);
+    for (int at = 0; at < all; at += kMostGroups) {
+        const dim3 grid(all - at < kMostGroups ? all - at : kMostGroups), block(sh.threads);
+        with_shape(sh, [&](auto mode, auto v) {
+            constexpr int M = decltype(mode)::value, V = decltype(v)::value;
+            if constexpr (M != kBlock || V > 1) hipLaunchKernelGGL((norm_kernel<T, M, V>), grid, block, 0, s, a);
+        });
+        a.rows -= rows;
+        a.x += rows * a.x_stride;
+        a.res += a.res ? rows * a.res_stride : 0;
+        a.gate += a.gate ? rows * a.gate_stride : 0;
+        a.y += a.y ? rows * a.y_stride : 0;
+        a.h += a.h ? rows * a.h_stride : 0;
+        a.stats += a.stats ? 4 * (size_t)rows : 0;
+    }
 }
 
 // A gradient's workgroups, and the parts of the channels' sums: as many of either as
 // are on the compute units at once, by their waves.
 struct NormPlan {
     int groups, parts;
-    bool apart;                         // sums by norm_channels_kernel
     size_t means, total;
 };
 
 NormPlan norm_plan(int rows, int d, int sums) {
     const Shape sh = norm_shape(d, true);
     NormPlan p;
-    const int all = (rows + rows_of(sh.mode) - 1) / rows_of(sh.mode), most = kRowWaves / (sh.threads / 64) * kCUs;
+    const int all = (rows + rows_of(sh.mode) - 1) / rows_of(sh.mode);
+    const int most = d > kWide ? kMostGroups : kRowWaves / (sh.threads / 64) * kCUs;
     p.groups = all < most ? all : most;
-    p.apart = sums && sh.v > 1;
     p.parts = p.groups;
-    if (p.apart) {
+    if (d > kWide) {
         const int fill = kRowWaves / 4 * kCUs / ((d + 2047) / 2048);
         p.parts = rows < fill ? rows : fill;
     }
     p.means = ((size_t)sums * p.parts * d * 4 + 255) & ~(size_t)255;
-    p.total = p.apart ? p.means + (size_t)rows * 8 : (size_t)sums * p.parts * d * 4;
+    p.total = p.means + (d > kWide ? (size_t)rows * 16 : 0);
     return p;
 }
 
 template <int T, int OF, bool BIAS>
 void backward_of(const NormGradArgs& a, const NormPlan& p, bool sums, hipStream_t s) {
     const Shape sh = norm_shape(a.f.d, true);
-    with_shape(sh, [&](auto mode, auto v) {
-        constexpr int M = decltype(mode)::value, V = decltype(v)::value;
-        auto* kernel = norm_bwd_kernel<T, M, V, OF, false, BIAS>;
-        if constexpr (V == 1)
-            if (sums) kernel = norm_bwd_kernel<T, M, V, OF, true, BIAS>;
+    if (a.f.d > kWide) {
+        hipLaunchKernelGGL((norm_rows_kernel<T, OF, BIAS>), dim3(p.groups), dim3(64 * kWideWaves), 0, s, a);
+        hipLaunchKernelGGL((norm_wide_kernel<T, OF, BIAS>), dim3((a.f.d + 2047) / 2048, p.parts), dim3(256), 0, s, a);
+        return;
+    }
+    auto launch = [&](auto mode) {
+        constexpr int M = decltype(mode)::value;
+        auto* kernel = sums ? norm_bwd_kernel<T, M, OF, true, BIAS> : norm_bwd_kernel<T, M, OF, false, BIAS>;
         hipLaunchKernelGGL(kernel, dim3(p.groups), dim3(sh.threads), 0, s, a);
-    });
-    if (p.apart)
-        hipLaunchKernelGGL((norm_channels_kernel<T, OF, BIAS>), dim3((a.f.d + 2047) / 2048, p.parts), dim3(256), 0, s, a);
+    };
+    if (sh.mode == kSub) launch(std::integral_constant<int, kSub>());
+    else if (sh.mode == kHalf) launch(std::integral_constant<int, kHalf>());
+    else if (sh.mode == kWave) launch(std::integral_constant<int, kWave>());
+    else launch(std::integral_constant<int, kBlock>());
 }
 
 template <int T>
@@ -714,7 +772,7 @@ hipError_t launch_norm_bwd(NormGradArgs a, int type, void* ws, hipStream_t s) {
         if (a.dparam[k].p) a.place[k] = sums++;
     const NormPlan p = norm_plan(a.f.rows, a.f.d, sums);
     a.part = (float*)ws;
-    a.means = p.apart ? (float*)((uint8_t*)ws + p.means) : nullptr;
+    a.means = (float*)((uint8_t*)ws + p.means);
     if (type == kBf16) backward<kBf16>(a, p, sums, s);
     else backward<kF16>(a, p, sums, s);
     return hipGetLastError();

@@ -216,7 +216,7 @@ struct NormGradArgs {
     NormSum dparam[kNormSums];
     int place[kNormSums];               // of the sums in part
     float* part;                        // [place][workgroup][d]
-    float* means;                       // [rows][2] of the norm of y's projections, or NULL
+    float* means;                       // [rows][4] what wide rows' gradients take of the whole row
 };
 constexpr int kNormMaxD = 32768;        // within 12 waves of six eights a lane
 hipError_t launch_norm(const NormArgs& a, int type, hipStream_t s);

@@ -1,7 +1,7 @@
 // operators_capi.hip -- C entries of the operators on trellis weights and of the
-// norms around them (declared in include/exl3_vit.h): arguments are checked on the host against everything
-// the kernels assume, then the kernels are enqueued.  No state is kept between
-// calls and nothing is locked.
+// norms around them (declared in include/exl3_vit.h): arguments are checked on the
+// host against everything the kernels assume, then the kernels are enqueued.  No
+// state is kept between calls and nothing is locked.
 #include <stdio.h>
 #include <string.h>
 

@@ -569,11 +569,11 @@ class _ResidualNorm(torch.autograd.Function):
         struct, params = _norm_params(ctx.cfg, inputs[3:8])
         out = [None if g is None else g.data_ptr() for g in grads]
         sums = sum(p is not None for p in out[3:])
-        L, dev, ws, need = _hb.lib(), x.device, None, 0
+        L, dev, ws = _hb.lib(), x.device, None
         with _on(dev):
-            if sums:
-                need = L.xtq_norm_bwd_ws_bytes(m, d, sums)
-                ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
+            need = L.xtq_norm_bwd_ws_bytes(m, d, sums)
+            if need > 0:
+                ws = torch.empty(need, dtype=torch.uint8, device=dev)
             rc = L.xtq_norm_bwd_dev(
                 ctypes.byref(struct), _TYPES[x.dtype], m, d, xp, xs, rp, rs, gp, gs, inputs[8].data_ptr(),
                 dyp, dys, dhp, dhs, *out[:3], _FIVE(*out[3:]), None if ws is None else ws.data_ptr(), need,
@@ -637,15 +637,15 @@ class _Norm(torch.autograd.Function):
         dx, dw, db = _as(x) if want_x else None, _as(weight) if want_w else None, _as(bias) if want_b else None
         dev, d = x.device, x.shape[-1]
         rows, dh = _rows(x, d), _rows(dh, d)
-        m, sums, need, ws = rows.shape[0], want_w + want_b, 0, None
+        m, sums, ws = rows.shape[0], want_w + want_b, None
         if m == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
         weight = None if weight is None else weight.contiguous()
         L = _hb.lib()
         with _on(dev):
-            if sums:
-                need = L.xtq_norm_bwd_ws_bytes(m, d, sums)
-                ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
+            need = L.xtq_norm_bwd_ws_bytes(m, d, sums)
+            if need > 0:
+                ws = torch.empty(need, dtype=torch.uint8, device=dev)
             rc = L.xtq_norm_bwd_dev(
                 ctypes.byref(_plain_struct(ctx.kind, ctx.eps, weight, bias)), _TYPES[x.dtype], m, d,
                 rows.data_ptr(), _stride(rows), None, 0, None, 0, stats.data_ptr(), None, 0, dh.data_ptr(),

@@ -389,3 +389,44 @@ def test_derivatives_refused(xt, name):
     g, = torch.autograd.grad((y, h), v[name], (torch.ones_like(y), torch.ones_like(h)), create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), v[name])
+
+
+def test_more_rows_than_a_grid_holds(xt):
+    """Each row has the bits it has alone, whatever rows there are: 2^28 of them are more lanes than one launch."""
+    m, d = (1 << 28) + 37, 8
+    x = torch.empty(m, d, dtype=torch.float16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(3))
+    x.requires_grad_()
+    w = torch.linspace(-1.0, 2.0, d, device="cuda")
+    h = xt.norm(x, w)
+    dx, = torch.autograd.grad(h, x, x.detach())
+    for at in (0, (1 << 26) - 50, (1 << 27) - 50, m - 100):
+        part = x.detach()[at:at + 100].clone().requires_grad_()
+        alone = xt.norm(part, w)
+        assert torch.equal(h[at:at + 100], alone)
+        assert torch.equal(dx[at:at + 100], torch.autograd.grad(alone, part, part.detach())[0])
+
+
+@pytest.mark.parametrize("d", (100, 120, 250, 7000, 7001))
+def test_an_infinite_scale_stays_infinite(xt, d):
+    """dp = dy s w' is infinite in the first channel alone, and so is its mean with x^, so that dx elsewhere is
+    infinite too, with the sign of -x^ dp x^[first]: nothing past the row's end makes NaN of it."""
+    g = torch.Generator("cuda").manual_seed(5)
+    x, dy, res = (torch.randn(5, d, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+    scale = torch.ones(d, device="cuda")
+    scale[0] = float("inf")
+    x.requires_grad_()
+    y, _ = xt.residual_norm(x, res, kind=None, post="rms", scale=scale)
+    dx, = torch.autograd.grad(y, x, dy)
+    want = -torch.sign(x.detach() * dy[:, :1] * x.detach()[:, :1])[:, 1:] * float("inf")
+    assert torch.equal(dx[:, 1:], want)
+
+
+@pytest.mark.parametrize("d", (100, 200, 400, 1000, 7000))
+def test_a_row_of_infinite_factor(xt, d):
+    """The squares of a first row of 1e-30 are zero and its factor infinite (eps 0): the weight's gradient is too,
+    and places of a workgroup without a row add no NaN to it."""
+    x = torch.ones(3, d, device="cuda", dtype=torch.bfloat16)
+    x[0] = 1e-30
+    w = torch.ones(d, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(xt.norm(x, w, eps=0.0), w, torch.ones_like(x))
+    assert torch.equal(dw, torch.full_like(dw, float("inf")))
