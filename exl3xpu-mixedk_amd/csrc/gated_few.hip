@@ -1,4 +1,4 @@
-// gated_few.hip -- the gated projection of few rows (up to 64): both weights are
+// gated_few.hip -- the gated projection of few rows, 64 at a time: both weights are
 // decoded on their way to the matrix cores, in one launch.
 //
 // Built once per codebook (XTQ_GATED_CODE); the weights' widths are chosen in the

@@ -206,33 +206,39 @@ __device__ __forceinline__ void store_gated(const f4* gate, const f4* up, const 
     }
 }
 
-// The product of fragments.  A workgroup's tile is 256 columns by 32 NB rows, 4 waves
-// of one weight's 128 columns by 16 NB rows, in steps of 32 of the summed dimension.
-// The columns' fragments are read by two waves each and come through three LDS
-// buffers, two steps ahead, as in gemm_kernel of linear_kernels.hip; a wave's rows are
-// its own weight's and its own half, so they come straight into its registers.
-// Two workgroups share a compute unit.  (The rows through LDS too: 32 KiB a step, two
-// buffers of which leave room for the second workgroup: 1597 us in all for 4096 rows of
-// 5120 by 17408, 1542 so.)  Tiles go by XCD as gemm_kernel's, in bands of kRowBand.
-constexpr int kRowBand = 4;             // (4096 rows 1520 us in all; of 2, 3, 6, 8 and 16: 1584, 1648, 1638, 1579, 1624)
+// The product of fragments.  A workgroup's tile is 256 columns by 8 W NB rows, a wave of
+// its W one weight's 128 columns by 16 NB rows, in steps of 32 of the summed dimension.
+// The columns' fragments are read by W / 2 waves each and come through three LDS buffers,
+// two steps ahead, as in gemm_kernel of linear_kernels.hip, but by buffer loads: behind
+// one of those, unlike behind a global load to LDS, the compiler counts what is still
+// under way, and waits for what it needs alone.  A wave's rows are its own weight's and
+// its own part, so they come straight into its registers.
+// Eight waves read 48 KiB for as many products as twice four waves 64, which is what the
+// compute unit's vector memory takes as long for as the matrix cores for the products:
+// 4096 rows of 5120 by 17408 1386 us in all, 1527 with four waves, whose two workgroups
+// share a compute unit.  (Rows through LDS too 1597; two terms 2395, 2365 with four.)
+// Tiles go by XCD as gemm_kernel's, in bands of kRowBand.
+constexpr int kRowBand = 4;             // (4096 rows 1386 us in all; of 2 and 8: 1391, 1394)
 
-template <int T, int OUT, int NB, int TERMS>
-__global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedArgs a) {
-    constexpr int kOwn = 4 + NB * TERMS;        // a wave's loads of a step
-    constexpr int kExchange = OUT == kGatedFinish ? 4 * (NB / 2) * 8192 : 0, kLoop = 3 * 16 * kFragBytes;
+template <int T, int OUT, int NB, int TERMS, int W>
+__global__ __launch_bounds__(64 * W, 2) void gated_gemm_kernel(GatedGemm g, GatedArgs a) {
+    constexpr int kGroups = NB * W / 2, kA = 16 / W;
+    constexpr int kOwn = kA + NB * TERMS;        // a wave's loads of a step
+    constexpr int kExchange = OUT == kGatedFinish ? W * (NB / 2) * 8192 : 0, kLoop = 3 * 16 * kFragBytes;
     __shared__ __align__(1024) uint8_t lds[kLoop > kExchange ? kLoop : kExchange];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), role = wv & 1, wm = wv >> 1;
     const int tile = xcd_order(blockIdx.x, g.tiles);
-    const int mt = (g.gb + 2 * NB - 1) / (2 * NB), band = tile / (g.nb * kRowBand);
+    const int mt = (g.gb + kGroups - 1) / kGroups, band = tile / (g.nb * kRowBand);
     const int high = mt - band * kRowBand < kRowBand ? mt - band * kRowBand : kRowBand, in = tile - band * g.nb * kRowBand;
     const int tn = in / high, tm = band * kRowBand + in - tn * high;
     const int split = blockIdx.y;
     const int s0 = (int)((long long)g.steps * split / g.splits);
     const int s1 = (int)((long long)g.steps * (split + 1) / g.splits);
 
-    const int gb0 = tm * 2 * NB;        // first group of rows
-    const uint16_t* fa = g.A + (size_t)tn * g.steps * 8192 + wv * 2048 + lane * 8;
+    const int gb0 = tm * kGroups;        // first group of rows
+    const auto fa = __builtin_amdgcn_make_buffer_rsrc((void*)(g.A + (size_t)tn * g.steps * 8192), 0, 0xFFFFFFFF, 0x00027000);
+    const int at_a = wv * kA * kFragBytes + lane * 16;
     const size_t at_b = ((size_t)(gb0 >> 4) * g.steps * 16 + (gb0 & 15) + wm * NB) * 512 + lane * 8;
     const uint16_t* const fb[2] = {g.B[role] + at_b, TERMS == 2 ? g.B2[role] + at_b : nullptr};
     // Stages of the rows' registers: a step's come two steps ahead, or one where four
@@ -242,11 +248,11 @@ __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedAr
     // (Past the end the last step comes once more, so that the waits can count.)
     int to = 0;
     auto load_a = [&](int s) {
-        const uint16_t* p = fa + (size_t)(s < s1 ? s : s1 - 1) * 8192;
+        const uint32_t at = (uint32_t)(s < s1 ? s : s1 - 1) * (16 * kFragBytes);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            __builtin_amdgcn_global_load_lds((global_void*)(p + i * 512),
-                                             (lds_void*)(lds + (to * 16 + wv * 4 + i) * kFragBytes), 16, 0, 0);
+        for (int i = 0; i < kA; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(fa, (lds_void*)(lds + (to * 16 + wv * kA + i) * kFragBytes), 16, at_a,
+                                                     at + i * kFragBytes, 0, 0);
         to = to == 2 ? 0 : to + 1;
     };
     auto load_b = [&](int s, auto stage) {
@@ -296,12 +302,17 @@ __global__ __launch_bounds__(256, 2) void gated_gemm_kernel(GatedGemm g, GatedAr
     load_a(s0 + 1);
     if constexpr (kStages == 3) load_b(s0 + 1, c1);
     meet_up();
-    for (int s = s0; s < s1; s += kStages) {
+    // (Whole turns of the stages, and the rest: were a turn cut short in the loop, the
+    // compiler would take a stage's loads for still under way where the next are issued.)
+    int s = s0;
+    for (; s + kStages <= s1; s += kStages) {
         step(s, c0);
-        if (s + 1 < s1) step(s + 1, c1);
-        if constexpr (kStages == 3)
-            if (s + 2 < s1) step(s + 2, std::integral_constant<int, 2>());
+        step(s + 1, c1);
+        if constexpr (kStages == 3) step(s + 2, std::integral_constant<int, 2>());
     }
+    if (s < s1) step(s, c0);
+    if constexpr (kStages == 3)
+        if (s + 1 < s1) step(s + 1, c1);
     if constexpr (OUT == kGatedParts) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -465,19 +476,22 @@ FewPlan few_plan(int rows, int k, int n, bool two) {
 }
 
 // How the product of many rows is cut, as gemm_tiling of linear_kernels.hip does: by the
-// shortest estimate.  us of a workgroup's step alone on a compute unit, of two at once,
-// and of each where there are more, by terms and groups of rows.
+// shortest estimate.  Tiles have 32 nb rows; nb 8, of one term, those of eight waves.  us
+// of a workgroup's step alone on a compute unit, of two at once, and of each where there
+// are more, by terms and rows, fitted to 90 sizes' times under every cut (257 to 4096
+// rows): the chosen one was 1.3% off the fastest in the mean when timed anew, 9% at most.
 Tiling gated_tiling(int rows, int n, int steps, bool two) {
-    static const double cost[2][2][3] = {{{0.40, 0.55, 0.35}, {0.55, 0.80, 0.51}}, {{0.60, 0.90, 0.50}, {0.95, 1.45, 0.91}}};
+    static const double cost[2][3][3] = {{{0.30, 0.51, 0.26}, {0.53, 0.59, 0.30}, {0.57, 1.00, 0.45}},
+                                         {{0.89, 0.93, 0.58}, {0.97, 1.40, 0.63}}};
     Tiling best{};
     double least = 0.0;
-    for (int nb = 4; nb >= 2; nb -= 2) {
-        const double* c = cost[two][nb == 4];
+    for (int nb = two ? 4 : 8; nb >= 2; nb /= 2) {
+        const double* c = cost[two][nb / 4];
         const int tiles = n / 128 * ((rows + 32 * nb - 1) / (32 * nb));
         for (int s = 1; s == 1 || (s <= steps / 8 && (s - 1) * tiles < 2 * kCUs); ++s) {
             const int each = (int)(((long long)tiles * s + kCUs - 1) / kCUs);
-            const double step = each == 1 ? c[0] : each == 2 ? c[1] : c[2] * (each % 2 ? each + 0.3 : each);
-            const double us = step * ((steps + s - 1) / s) + (s > 1 ? 3.0 + 4e-6 * s * rows * n : 0.0);
+            const double step = each == 1 ? c[0] : each == 2 ? c[1] : c[2] * (nb < 8 && each % 2 ? each + 0.2 : each);
+            const double us = step * ((steps + s - 1) / s) + (s > 1 ? 3.0 + 3.8e-6 * s * rows * n : 0.0);
             if (!best.nb || us < least) {
                 least = us;
                 best = Tiling{nb, tiles, s};
@@ -526,6 +540,18 @@ void pair_prepare(const Weight* w, uint16_t* frags, FragPlace p0, FragPlace p1, 
     else launch(pair_prepare_kernel<kCode3Inst, GRAD>);
 }
 
+template <int T, int OUT>
+void gemm(const GatedGemm& g, const GatedArgs& a, int nb, hipStream_t s) {
+    auto launch = [&](auto* kernel, int waves) {
+        hipLaunchKernelGGL(kernel, dim3(g.tiles, g.splits), dim3(64 * waves), 0, s, g, a);
+    };
+    if (a.two && nb == 4) launch(gated_gemm_kernel<T, OUT, 4, 2, 4>, 4);
+    else if (a.two) launch(gated_gemm_kernel<T, OUT, 2, 2, 4>, 4);
+    else if (nb == 8) launch(gated_gemm_kernel<T, OUT, 4, 1, 8>, 8);
+    else if (nb == 4) launch(gated_gemm_kernel<T, OUT, 4, 1, 4>, 4);
+    else launch(gated_gemm_kernel<T, OUT, 2, 1, 4>, 4);
+}
+
 template <int T>
 hipError_t many(const GatedArgs& a, void* ws, hipStream_t s) {
     const int k = a.w[0].k, n = a.w[0].n;
@@ -551,18 +577,10 @@ hipError_t many(const GatedArgs& a, void* ws, hipStream_t s) {
                     p.places, s);
     hipLaunchKernelGGL(pair_transform_kernel<false>, dim3((k / 128 + 3) / 4, p.groups), dim3(256), 0, s, src,
                        (const int32_t*)shift, p.places, xf[0], xf[1], x2[0], x2[1], (float*)nullptr);
-    const dim3 grid(p.tiles, p.splits), block(256);
-    auto gemm = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, g, a); };
     if (p.splits == 1) {
-        if (a.two && p.nb == 4) gemm(gated_gemm_kernel<T, kGatedFinish, 4, 2>);
-        else if (a.two) gemm(gated_gemm_kernel<T, kGatedFinish, 2, 2>);
-        else if (p.nb == 4) gemm(gated_gemm_kernel<T, kGatedFinish, 4, 1>);
-        else gemm(gated_gemm_kernel<T, kGatedFinish, 2, 1>);
+        gemm<T, kGatedFinish>(g, a, p.nb, s);
     } else {
-        if (a.two && p.nb == 4) gemm(gated_gemm_kernel<T, kGatedParts, 4, 2>);
-        else if (a.two) gemm(gated_gemm_kernel<T, kGatedParts, 2, 2>);
-        else if (p.nb == 4) gemm(gated_gemm_kernel<T, kGatedParts, 4, 1>);
-        else gemm(gated_gemm_kernel<T, kGatedParts, 2, 1>);
+        gemm<T, kGatedParts>(g, a, p.nb, s);
         hipLaunchKernelGGL((gated_join_kernel<T>), dim3(p.groups, n / 128), dim3(64), 0, s, g, a);
     }
     return hipGetLastError();

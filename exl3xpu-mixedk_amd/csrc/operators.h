@@ -131,7 +131,7 @@ constexpr int few_groups(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
 void transform_few(bool two, const void* x, long long x_stride, int type, int rows, int k, int groups,
                    const uint16_t* suh, const uint16_t* suh2, u4* frag, u4* rest, int32_t* shift, hipStream_t s);
 
-// The gated projection act(x Wg + bg) (x Wu + bu) (gated_kernels.hip; up to kFewRows rows
+// The gated projection act(x Wg + bg) (x Wu + bu) (gated_kernels.hip; of few rows
 // gated_few.hip).  Role 0 is the gate, 1 the up weight.
 struct GatedArgs {
     Weight w[2];                        // one k, n and code
@@ -173,7 +173,7 @@ struct GatedFew {
     int groups, workers, per_block;
     int each, more;                     // steps of a run; runs with one more
     float* part;                        // [chunk][worker + block][row][128], chunks 64 rows apart
-    uint32_t* counters;                 // [chunk][n/128]
+    uint32_t* counters;                 // [n/128], up to 16 rows
 };
 #define XTQ_GATED(C) \
     hipError_t launch_gated_few_code##C(const GatedArgs& a, const GatedFew& f, hipStream_t s);

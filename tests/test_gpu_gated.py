@@ -82,10 +82,10 @@ def test_codes(xt, oracle_mod, K, code, m):
 
 
 @pytest.mark.parametrize("m,k,n", [(9000, 128, 640), (3000, 2048, 256), (1815, 1024, 2176), (300, 4096, 384),
-                                   (150, 2048, 6144)])
+                                   (150, 2048, 6144), (5000, 128, 1664), (1815, 4096, 1408), (333, 4096, 2816)])
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 def test_cuts(xt, oracle_mod, m, k, n, dtype):
-    """Every way in which the products of many rows are cut: both heights of tile, whole and in parts."""
+    """Every way in which the products of many rows are cut: every height of tile, whole and in parts."""
     ls, ws = _pair(xt, oracle_mod, k, n, 4, 5)
     Wg, Wu = (w.cuda() for w in ws)
     x = _x(m, k, dtype, m).requires_grad_()
