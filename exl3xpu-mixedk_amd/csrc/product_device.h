@@ -179,7 +179,6 @@ __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
 
 // The sum over the splits from `first` to before `last` of a unit (128 columns by 16
 // rows), in order, U of them in flight for each register.
