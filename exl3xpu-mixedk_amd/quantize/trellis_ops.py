@@ -1,4 +1,5 @@
-"""trellis_ops.py -- products with weights in the EXL3 trellis format, on the GPU.
+"""trellis_ops.py -- products with weights in the EXL3 trellis format, and the norms
+between them, on the GPU.
 
 What quantize_linear returns is multiplied with as it is: the weight stays in
 its trellis, the kernels decode it on the way to the matrix cores.
@@ -8,6 +9,8 @@ its trellis, the kernels decode it on the way to the matrix cores.
     w = xt.TrellisLinear.from_result(r)
     y = xt.linear(x, w, bias=b, act="silu", residual=res)     # differentiable in x, bias, residual
     G = xt.input_gram(x)                                      # the H of the next quantize_linear
+    u = xt.gated(xt.norm(x, g), w_gate, w_up)                 # silu(t Wg) * (t Wu) of t = norm(x)
+    y, h = xt.residual_norm(xt.linear(u, w_down), x, g2)      # y = x + block, h = norm(y)
 
 Activations are bfloat16 or float16 and results have their type; sums are fp32
 and every result is rounded once.  Calls are ordered on the current stream,
@@ -662,8 +665,8 @@ def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor
     """The norm of each row of x [.., d] (bfloat16 or float16, d up to 32768), in x's
     type: (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias for "layer", the
     same without the mean for "rms".  weight and bias [d] have x's type or fp32 (None:
-    1 and 0).  Differentiable in all three (once, in reverse mode).  A row's result is
-    the same whatever rows are beside it."""
+    1 and 0).  Squares are fp32: values up to 2^63.  Differentiable in all three (once,
+    in reverse mode).  A row's result is the same whatever rows are beside it."""
     _check_norm_rows("norm", x)
     for t, what in ((weight, "weight"), (bias, "bias")):
         if t is not None:
