@@ -3,13 +3,13 @@ trellis weights.
 
     python exl3xpu-mixedk_amd/examples/trellis_block.py [--dim 512] [--hidden 1024] [--experts 8]
 
-A dense layer pair (up with silu, down with bias and residual) and a mixture of
-experts, random weights and activations:
+A dense layer pair (up with silu, down with bias and residual), a gated block
+between norms, and a mixture of experts, random weights and activations:
 
 1. calibrate  trellis_ops.input_gram sums the inputs' Gram over padded batches
 2. quantize   quantize.quantize_linear with that Gram, K by weight
-3. run        trellis_ops.linear and trellis_ops.moe on the trellis weights
-4. tune       the biases, by gradients through the frozen trellis weights
+3. run        trellis_ops.linear, norm, gated, residual_norm and moe on the trellis weights
+4. tune       the biases and the norms' weights, by gradients through the frozen trellis weights
 5. serve      one token at a time, from a captured HIP graph
 
 Prints what each step gives; main() returns it.
@@ -92,7 +92,24 @@ def main(argv=None) -> dict:
     def block(t):
         return xt.linear(xt.linear(t, q_up, bias=inner, act="silu"), q_down, bias=bias, residual=t)
 
+    norms = [torch.ones(d, device="cuda", requires_grad=True) for _ in range(2)]
+    q_gate, q_wide, q_back = layers[0]
+
+    def feed(t):
+        """The gated block of the first expert's weights: its result with the residual, and that one's norm."""
+        return xt.residual_norm(xt.linear(xt.gated(xt.norm(t, norms[0]), q_gate, q_wide), q_back), t, norms[1])
+
+    def rms(t):
+        return t * torch.rsqrt(t.square().mean(-1, keepdim=True) + 1e-6)
+
+    t = rms(rows.float())
+    wg, wu, wd = (w.cuda() for w in experts[0])
+    gated = (torch.nn.functional.silu(t @ wg.t()) * (t @ wu.t())) @ wd.t()
+
     with torch.no_grad():
+        y, h = feed(rows)
+        out["gated error"] = _error(y.float() - rows.float(), gated)
+        out["normed error"] = _error(h, rms(y.float()))
         out["dense error"] = _error(block(rows), dense)
         y, ids, weights = xt.moe(x.view(-1, d), router, mixture, 2, residual=x.view(-1, d).nan_to_num(),
                                  valid=valid.view(-1), return_routing=True)
@@ -118,13 +135,15 @@ def main(argv=None) -> dict:
             bias -= scale * g_bias
             inner -= scale * g_inner
     out["loss before, after"] = (losses[0], losses[-1])
+    loss = (feed(rows)[1].float() - rms(gated + rows.float())).square().mean()
+    out["norms' gradients"] = [float(g.norm()) for g in torch.autograd.grad(loss, norms)]
 
-    # 5. serve: one token through the dense layers and the mixture, captured once
+    # 5. serve: one token through the dense layers, the gated block and the mixture, captured once
     token = rows[:1].clone()
 
     def step():
-        t = block(token)
-        return xt.moe(t, router, mixture, 2, residual=t)
+        y, h = feed(block(token))
+        return xt.moe(h, router, mixture, 2, residual=y)
 
     with torch.no_grad():
         eager = step()
