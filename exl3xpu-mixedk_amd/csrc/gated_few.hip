@@ -125,8 +125,8 @@ __device__ __forceinline__ void finish_rows_of(const GatedArgs& a, const Columns
 //
 // EVEN where that fills the places, two workgroups a compute unit.  272 blocks of 17408
 // columns do not, and two compute units of three then wait for the third: 48 rows of
-// 5120 take 84.9 us in 272 runs and 70.5 in 512, one row 51.8 and 40.4.  (Going over a
-// block's end is a loop, which costs registers and 4 us where runs are short.)
+// 5120 take 80.4 us in 272 runs and 61.7 in 512, one row 57.5 and 47.0.  (Going over a
+// block's end is a loop, which costs registers: where runs are short, EVEN is faster.)
 template <int G, bool FUSED, bool LO, bool EVEN>
 __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void gated_few_kernel(GatedArgs a, GatedFew f) {
     constexpr int W = few_waves(G), N = 8 / W;

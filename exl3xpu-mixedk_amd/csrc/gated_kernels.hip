@@ -442,11 +442,11 @@ bool takes_few(int rows, int k, int n) {
 }
 
 // A chunk's workgroups: as few_splits cuts the blocks, with 16 steps each at least where
-// there are several chunks (100 rows of 1024 by 4096 22.9 us, 27.8 with 8).  Where that
+// there are several chunks (100 rows of 1024 by 4096 21.2 us, 26.1 with 8).  Where that
 // leaves a fifth of the places empty, blocks that come twice into them in four parts
-// each (172 of 4096: 1 row 28.2 us, 36.7 cut evenly over all steps, 64 rows 45.1, 48.4),
-// others evenly over all steps (272 of 5120: 45.5, 59.8 uncut; 66.2, 88) if a run still
-// has 32 of them.
+// each (172 of 4096: 1 row 25.8 us, 34.6 cut evenly over all steps, 64 rows 43.4, 46.3),
+// others evenly over all steps (272 of 5120: 1 row 47.0, 57.5 uncut; 64 rows 64.3, 81.4)
+// if a run still has 32 of them (1 row of 4096 by 6144 24.4 so, 18.7 in five parts each).
 void few_workers(FewPlan& p, int rows, int k, int n, int waves) {
     const int blocks = n / 64, chunks = few_chunks(rows), steps = k / 32, places = 2 * kCUs;
     int s = few_splits(rows < kFewRows ? rows : kFewRows, k, 2 * n, waves);
