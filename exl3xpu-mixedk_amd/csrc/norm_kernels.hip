@@ -350,33 +350,35 @@ __device__ __forceinline__ void gates(Gate& e, const Raw& t, int act) {
 }
 
 // What a row's i-th channel is forward: x^, p, q, t^, and c = dh w.  (A norm that is
-// not there has mean 0 and factor 1.)
+// not there has mean 0 and factor 1.)  FULL: with means and biases.  Without them, "rms"
+// alone, a gradient has a tenth less to work out (8191 rows of 5120, forward and back:
+// with gate, scale and two norms 287 us with them, 274 without; two norms 199 and 182).
 struct Forward {
     float hat, p, q, that, dh, c;
 };
 
-template <int T, int OF, bool BIAS>
+template <int T, int OF, bool FULL>
 __device__ __forceinline__ Forward again(const Raw& t, int i, const Gate& e, const Channels& ch, const f4& stats) {
     Forward f;
     f.p = pick<T>(t.x, i);
     f.that = f.p;
     if constexpr (OF != kPlain) {
-        f.hat = (f.p - stats[0]) * stats[1];
-        f.p = BIAS ? __builtin_fmaf(f.hat, ch.pw[i], ch.pb[i]) : f.hat * ch.pw[i];
+        f.hat = (FULL ? f.p - stats[0] : f.p) * stats[1];
+        f.p = FULL ? __builtin_fmaf(f.hat, ch.pw[i], ch.pb[i]) : f.hat * ch.pw[i];
         f.q = OF == kWithGate ? f.p * e.ga[i] : f.p;
         f.that = __builtin_fmaf(ch.s[i], f.q, pick<T>(t.r, i));
     }
-    f.that = (f.that - stats[2]) * stats[3];
+    f.that = (FULL ? f.that - stats[2] : f.that) * stats[3];
     f.dh = pick<T>(t.h, i);
     f.c = f.dh * ch.w[i];
     return f;
 }
 
 // Sums of eight channels over rows, of the norm and of the rest.
-template <int OF, bool BIAS>
+template <int OF, bool FULL>
 struct Sums {
     static constexpr int N = OF == kPlain ? 2 : kNormSums;
-    static constexpr bool has(int k) { return k < N && (BIAS || (k != kSumBias && k != kSumPostBias)); }
+    static constexpr bool has(int k) { return k < N && (FULL || (k != kSumBias && k != kSumPostBias)); }
     float of[N][8];
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -386,21 +388,21 @@ struct Sums {
     }
     __device__ __forceinline__ void norm(int i, const Forward& f, bool dh) {
         of[kSumWeight][i] = __builtin_fmaf(f.dh, dh ? f.that : 0.0f, of[kSumWeight][i]);
-        if constexpr (BIAS) of[kSumBias][i] += f.dh;
+        if constexpr (FULL) of[kSumBias][i] += f.dh;
     }
     __device__ __forceinline__ void rest(int i, const Forward& f, float dt, float dp) {
         of[kSumScale][i] = __builtin_fmaf(dt, f.q, of[kSumScale][i]);
         of[kSumPostWeight][i] = __builtin_fmaf(dp, f.hat, of[kSumPostWeight][i]);
-        if constexpr (BIAS) of[kSumPostBias][i] += dp;
+        if constexpr (FULL) of[kSumPostBias][i] += dp;
     }
 };
 
 // dy' of a channel; `in`: of h's gradient too.
-template <int T, int OF>
+template <int T, int OF, bool FULL>
 __device__ __forceinline__ float total(const Forward& f, const Raw& t, int i, const f4& stats, float c1, float c2,
                                        bool in) {
-    const float dy = OF == kPlain ? 0.0f : pick<T>(t.y, i);
-    return in ? __builtin_fmaf(stats[3], f.c - f.that * c1 - c2, dy) : dy;
+    const float dy = OF == kPlain ? 0.0f : pick<T>(t.y, i), part = __builtin_fmaf(-c1, f.that, f.c);
+    return in ? __builtin_fmaf(stats[3], FULL ? part - c2 : part, dy) : dy;
 }
 
 // Gradients.  With c = dh w, t^ = (y - mean) rstd,
@@ -414,7 +416,7 @@ __device__ __forceinline__ float total(const Forward& f, const Raw& t, int i, co
 // before is worked on, and a workgroup leaves one row of partial sums, which
 // norm_sums_kernel adds in order.  What a sum over the row needs again after it is
 // computed anew, which costs less than registers for it.
-template <int T, int MODE, int OF, bool SUMS, bool BIAS>
+template <int T, int MODE, int OF, bool SUMS, bool FULL>
 __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bwd_kernel(NormGradArgs a) {
     Group<MODE> g;
     constexpr int R = rows_of(MODE);
@@ -431,7 +433,7 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
         if (row >= a.f.rows) t.stats = (f4){0.0f, 0.0f, 0.0f, 0.0f};     // (the first row's may be infinite)
         load_raw<MODE, OF>(t.raw, a, at, col);
     };
-    Sums<OF, BIAS> sums;
+    Sums<OF, FULL> sums;
     if constexpr (SUMS) sums.clear();
     Channels ch;
     Row next;
@@ -448,9 +450,9 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
         gates<T, OF>(gate, now.raw, a.f.gate_act);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const Forward f = again<T, OF, BIAS>(now.raw, i, gate, ch, now.stats);
+            const Forward f = again<T, OF, FULL>(now.raw, i, gate, ch, now.stats);
             two[0] = __builtin_fmaf(f.c, f.that, two[0]);
-            two[1] += f.c;
+            if constexpr (FULL) two[1] += f.c;
             if constexpr (SUMS) sums.norm(i, f, a.dh);
         }
         float c1 = 0.0f, c2 = 0.0f;
@@ -464,8 +466,8 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
         float dt[8], dg[8], dp[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const Forward f = again<T, OF, BIAS>(now.raw, i, gate, ch, now.stats);
-            dt[i] = total<T, OF>(f, now.raw, i, now.stats, c1, c2, i < nh);
+            const Forward f = again<T, OF, FULL>(now.raw, i, gate, ch, now.stats);
+            dt[i] = total<T, OF, FULL>(f, now.raw, i, now.stats, c1, c2, i < nh);
             dp[i] = dt[i];
             if constexpr (OF != kPlain) {
                 const float ds = dt[i] * ch.s[i], to = OF == kWithGate ? ds * gate.ga[i] : ds;
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
                 if constexpr (SUMS) sums.rest(i, f, dt[i], to);
                 dp[i] = to * ch.pw[i];
                 two[0] = __builtin_fmaf(dp[i], f.hat, two[0]);
-                two[1] += dp[i];
+                if constexpr (FULL) two[1] += dp[i];
             }
         }
         if constexpr (OF != kPlain)
@@ -484,8 +486,11 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
             g.sum(two);
             const float e1 = two[0] * inv, e2 = a.f.post == kNormLayer ? two[1] * inv : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                dp[i] = now.stats[1] * (dp[i] - (pick<T>(now.raw.x, i) - now.stats[0]) * now.stats[1] * e1 - e2);
+            for (int i = 0; i < 8; ++i) {
+                const float x = pick<T>(now.raw.x, i), hat = (FULL ? x - now.stats[0] : x) * now.stats[1];
+                const float part = __builtin_fmaf(-e1, hat, dp[i]);
+                dp[i] = now.stats[1] * (FULL ? part - e2 : part);
+            }
         }
         if (a.dx && n > 0) store8<T>(a.dx + at * d + col, n, dp);
     }
@@ -493,8 +498,8 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
         // [sum][workgroup][d]
         __shared__ float join[MODE == kBlock ? 1 : 256 * 8];
 #pragma unroll
-        for (int k = 0; k < Sums<OF, BIAS>::N; ++k) {
-            if (!Sums<OF, BIAS>::has(k) || !a.dparam[k].p) continue;
+        for (int k = 0; k < Sums<OF, FULL>::N; ++k) {
+            if (!Sums<OF, FULL>::has(k) || !a.dparam[k].p) continue;
             float* out = a.part + ((size_t)a.place[k] * gridDim.x + blockIdx.x) * d;
             if constexpr (MODE != kBlock) {
                 __syncthreads();
@@ -521,7 +526,7 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
 // eights kept in registers, of 32768 685 and 1953; of 6144, a lane's one, 95.)
 constexpr int kWideWaves = 8;
 
-template <int T, int OF, bool BIAS>
+template <int T, int OF, bool FULL>
 __global__ __launch_bounds__(64 * kWideWaves) void norm_rows_kernel(NormGradArgs a) {
     constexpr int N = OF == kPlain ? 2 : 10;
     Group<kBlock> g;
@@ -544,19 +549,21 @@ __global__ __launch_bounds__(64 * kWideWaves) void norm_rows_kernel(NormGradArgs
             gates<T, OF>(gate, now, a.f.gate_act);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const Forward f = again<T, OF, BIAS>(now, i, gate, ch, stats);
+                const Forward f = again<T, OF, FULL>(now, i, gate, ch, stats);
                 v[0] = __builtin_fmaf(f.c, f.that, v[0]);
-                v[1] += f.c;
+                if constexpr (FULL) v[1] += f.c;
                 if constexpr (OF != kPlain) {
                     const float dy = pick<T>(now.y, i), u = ch.s[i] * gate.ga[i] * ch.pw[i], uh = u * f.hat;
                     v[2] = __builtin_fmaf(uh, dy, v[2]);
                     v[3] = __builtin_fmaf(uh, f.c, v[3]);
                     v[4] = __builtin_fmaf(uh, f.that, v[4]);
-                    v[5] += uh;
-                    v[6] = __builtin_fmaf(u, dy, v[6]);
-                    v[7] = __builtin_fmaf(u, f.c, v[7]);
-                    v[8] = __builtin_fmaf(u, f.that, v[8]);
-                    v[9] += u;
+                    if constexpr (FULL) {
+                        v[5] += uh;
+                        v[6] = __builtin_fmaf(u, dy, v[6]);
+                        v[7] = __builtin_fmaf(u, f.c, v[7]);
+                        v[8] = __builtin_fmaf(u, f.that, v[8]);
+                        v[9] += u;
+                    }
                 }
             }
         }
@@ -576,13 +583,13 @@ __global__ __launch_bounds__(64 * kWideWaves) void norm_rows_kernel(NormGradArgs
 
 // Then the gradients, with the channels' sums beside: a workgroup takes 2048 channels
 // of every gridDim.y-th row and leaves a part of the sums.
-template <int T, int OF, bool BIAS>
+template <int T, int OF, bool FULL>
 __global__ __launch_bounds__(256) void norm_wide_kernel(NormGradArgs a) {
     const int d = a.f.d, col = (blockIdx.x * 256 + threadIdx.x) * 8, n = d - col;
     if (n <= 0) return;
     Channels ch;
     load_channels<T, kBlock, OF>(ch, a.f, col);
-    Sums<OF, BIAS> sums;
+    Sums<OF, FULL> sums;
     sums.clear();
     Raw next;
     load_raw<kBlock, OF>(next, a, blockIdx.y, col);
@@ -596,9 +603,9 @@ __global__ __launch_bounds__(256) void norm_wide_kernel(NormGradArgs a) {
         float dt[8], dg[8], dp[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const Forward f = again<T, OF, BIAS>(now, i, gate, ch, stats);
+            const Forward f = again<T, OF, FULL>(now, i, gate, ch, stats);
             sums.norm(i, f, a.dh);
-            dt[i] = total<T, OF>(f, now, i, stats, m[0], m[1], a.dh && i < n);
+            dt[i] = total<T, OF, FULL>(f, now, i, stats, m[0], m[1], a.dh && i < n);
             dp[i] = dt[i];
             if constexpr (OF != kPlain) {
                 const float ds = dt[i] * ch.s[i], to = OF == kWithGate ? ds * gate.ga[i] : ds;
@@ -616,8 +623,8 @@ __global__ __launch_bounds__(256) void norm_wide_kernel(NormGradArgs a) {
         if (a.dx) store8<T>(a.dx + at, n, dp);
     }
 #pragma unroll
-    for (int k = 0; k < Sums<OF, BIAS>::N; ++k) {
-        if (!Sums<OF, BIAS>::has(k) || !a.dparam[k].p) continue;
+    for (int k = 0; k < Sums<OF, FULL>::N; ++k) {
+        if (!Sums<OF, FULL>::has(k) || !a.dparam[k].p) continue;
         float* out = a.part + ((size_t)a.place[k] * gridDim.y + blockIdx.y) * d;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -722,17 +729,17 @@ NormPlan norm_plan(int rows, int d, int sums) {
     return p;
 }
 
-template <int T, int OF, bool BIAS>
+template <int T, int OF, bool FULL>
 void backward_of(const NormGradArgs& a, const NormPlan& p, bool sums, hipStream_t s) {
     const Shape sh = norm_shape(a.f.d, true);
     if (a.f.d > kWide) {
-        hipLaunchKernelGGL((norm_rows_kernel<T, OF, BIAS>), dim3(p.groups), dim3(64 * kWideWaves), 0, s, a);
-        hipLaunchKernelGGL((norm_wide_kernel<T, OF, BIAS>), dim3((a.f.d + 2047) / 2048, p.parts), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((norm_rows_kernel<T, OF, FULL>), dim3(p.groups), dim3(64 * kWideWaves), 0, s, a);
+        hipLaunchKernelGGL((norm_wide_kernel<T, OF, FULL>), dim3((a.f.d + 2047) / 2048, p.parts), dim3(256), 0, s, a);
         return;
     }
     auto launch = [&](auto mode) {
         constexpr int M = decltype(mode)::value;
-        auto* kernel = sums ? norm_bwd_kernel<T, M, OF, true, BIAS> : norm_bwd_kernel<T, M, OF, false, BIAS>;
+        auto* kernel = sums ? norm_bwd_kernel<T, M, OF, true, FULL> : norm_bwd_kernel<T, M, OF, false, FULL>;
         hipLaunchKernelGGL(kernel, dim3(p.groups), dim3(sh.threads), 0, s, a);
     };
     if (sh.mode == kSub) launch(std::integral_constant<int, kSub>());
@@ -743,10 +750,11 @@ void backward_of(const NormGradArgs& a, const NormPlan& p, bool sums, hipStream_
 
 template <int T>
 void backward(const NormGradArgs& a, const NormPlan& p, int sums, hipStream_t s) {
-    const bool bias = a.f.post_bias.p || a.dparam[kSumBias].p || a.dparam[kSumPostBias].p;
+    const bool full = a.f.post_bias.p || a.dparam[kSumBias].p || a.dparam[kSumPostBias].p || a.f.kind == kNormLayer ||
+                      a.f.post == kNormLayer;
     auto of = [&](auto what) {
         constexpr int OF = decltype(what)::value;
-        if (bias) backward_of<T, OF, true>(a, p, sums > 0, s);
+        if (full) backward_of<T, OF, true>(a, p, sums > 0, s);
         else backward_of<T, OF, false>(a, p, sums > 0, s);
     };
     if (!a.f.res) of(std::integral_constant<int, kPlain>());
