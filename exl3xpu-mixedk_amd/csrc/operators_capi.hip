@@ -87,6 +87,9 @@ int check_norm(const xtq_norm* p, int type, int rows, int d, const void* x, int6
         *q.to = xtq::NormParam{q.p, (p->f32 & q.bit) != 0};
         if (!aligned(q.p, q.to->f32 ? 4 : 2)) return 12;
     }
+    // (of a norm that is not there neither direction reads any)
+    if (!p->kind) a.weight.p = a.bias.p = nullptr;
+    if (!p->post) a.post_weight.p = a.post_bias.p = nullptr;
     int rc;
     if (rows && (rc = check_rows(x, x_stride, d))) return rc;
     if (rows && res && (rc = check_rows(res, res_stride, d))) return rc;

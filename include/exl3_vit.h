@@ -472,7 +472,8 @@ XTQ_API int xtq_gated_bwd_dev(const xtq_weight* gate, const xtq_weight* up, int 
  *   gate         or NULL (factor 1); gate_act: XTQ_GATE_NONE (the gate itself),
  *                XTQ_GATE_SIGMOID or XTQ_GATE_SILU of it
  *   scale        [d], or NULL: scale_number for all channels
- *   weight, bias, post_weight, post_bias   [d] or NULL (1 and 0)
+ *   weight, bias, post_weight, post_bias   [d] or NULL (1 and 0); those of a norm
+ *                that is not there (kind, post XTQ_NORM_NONE) are not read
  *   f32          bits XTQ_NORM_*_F32: that parameter is fp32, else of the rows' type
  *   stats        [rows][4] fp32 (out), 16-byte aligned, for xtq_norm_bwd_dev; or NULL
  * Stream-ordered, as the operators above are, with their types and strides; no
