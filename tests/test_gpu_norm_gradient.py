@@ -1,6 +1,6 @@
 """Gradients of norms and residual sums in every form that is launched apart: plain norms, with and without means and
-biases, every number of lanes a row has, rows wider than the registers; against the definitions in 64 bits, differentiated there
-by torch.
+biases, every number of lanes a row has, more rows than the lanes have at a time, rows wider than the registers; against
+the definitions in 64 bits, differentiated there by torch.
 
 Tolerances.  A result is rounded once, by u = roundoff(type) of itself at most.  Before that everything is fp32, with
 sums of up to 32768 values of a row, whose chain of additions is off by 2^-24 times the root of their number (1.1e-5),
@@ -72,12 +72,15 @@ def _check_param(got, want, terms, dtype, name):
 # 16, 32 and 64 lanes a row, workgroups of one to twelve waves, two passes
 SHAPES = [(1, 1), (3, 7), (40, 8), (37, 100), (18, 128), (21, 129), (9, 200), (7, 300), (5, 512), (11, 513), (6, 1000),
           (5, 2049), (3, 6144), (4, 6145), (5, 7001), (3, 17408), (2, 32768)]
+# rows that a group of lanes comes back for, and a remainder: 16 rows in each of 768 workgroups, 8, 4; workgroups of
+# two waves and of twelve; two passes' workgroups, of which 153 and 85 take rows
+TURNS = [(12300, 128), (12345, 40), (6200, 200), (3100, 400), (1600, 1000), (300, 6144), (200, 9000), (100, 17408)]
 FORMS = [("rms", False, False), ("rms", True, False), ("rms", True, True), ("layer", False, False),
          ("layer", True, False), ("layer", True, True)]
 
 
 @pytest.mark.parametrize("kind,weight,bias", FORMS)
-@pytest.mark.parametrize("m,d", SHAPES)
+@pytest.mark.parametrize("m,d", SHAPES + TURNS)
 @pytest.mark.parametrize("dtype,pt", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
 def test_norm(xt, m, d, kind, weight, bias, dtype, pt):
     """dx, dweight and dbias of the plain norm."""
@@ -128,7 +131,7 @@ CASES = [("rms", "rms", "sigmoid", "tensor"), ("rms", "rms", None, "tensor"), ("
 
 
 @pytest.mark.parametrize("kind,post,act,scale", CASES)
-@pytest.mark.parametrize("m,d", [(37, 100), (9, 200), (7, 300), (5, 1000), (4, 2049), (3, 6144), (5, 7001)])
+@pytest.mark.parametrize("m,d", [(37, 100), (9, 200), (7, 300), (5, 1000), (4, 2049), (3, 6144), (5, 7001)] + TURNS)
 @pytest.mark.parametrize("bias", (False, True))
 def test_residual_norm(xt, m, d, kind, post, act, scale, bias):
     """Every tensor's gradient, with biases and without: "rms" alone has kernels of its own."""
