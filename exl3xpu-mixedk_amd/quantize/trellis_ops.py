@@ -665,8 +665,10 @@ def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor
     """The norm of each row of x [.., d] (bfloat16 or float16, d up to 32768), in x's
     type: (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias for "layer", the
     same without the mean for "rms".  weight and bias [d] have x's type or fp32 (None:
-    1 and 0).  Squares are fp32: values up to 2^63.  Differentiable in all three (once,
-    in reverse mode).  A row's result is the same whatever rows are beside it."""
+    1 and 0).  The squares' sum is fp32: a row's 2-norm ("layer": its deviations') is
+    below 2^64, or its result is 0 before the bias, and with eps 0 its rms at least
+    2^-63.  Differentiable in all three (once, in reverse mode).  A row's result is the
+    same whatever rows are beside it."""
     _check_norm_rows("norm", x)
     for t, what in ((weight, "weight"), (bias, "bias")):
         if t is not None:

@@ -479,8 +479,10 @@ XTQ_API int xtq_gated_bwd_dev(const xtq_weight* gate, const xtq_weight* up, int 
  * Stream-ordered, as the operators above are, with their types and strides; no
  * scratch, no counters.  Sums are fp32 and in an order that d alone fixes, so a row's
  * results do not depend on the other rows; h comes of y before y is rounded.  Squares
- * are fp32: rows are taken up to 2^63.  Results overlap no input and one another
- * nowhere.  d up to 32,768, at most 2^30 rows; zero rows: nothing is enqueued.
+ * and their sum are fp32: a normed row (XTQ_NORM_LAYER: its deviations from the mean)
+ * has a 2-norm below 2^64, which 32,768 values reach at an rms of 2^56.5; past it the
+ * factor is 0, and so is the row.  With eps 0 its rms is at least 2^-63.  Results
+ * overlap no input and one another nowhere.  d up to 32,768, at most 2^30 rows; zero rows: nothing is enqueued.
  */
 enum { XTQ_NORM_NONE = 0, XTQ_NORM_RMS = 1, XTQ_NORM_LAYER = 2 };
 enum { XTQ_GATE_NONE = 0, XTQ_GATE_SIGMOID = 1, XTQ_GATE_SILU = 2 };
