@@ -76,7 +76,7 @@ int check_norm(const xtq_norm* p, int type, int rows, int d, const void* x, int6
     for (int k : {p->kind, p->post})
         if (k < XTQ_NORM_NONE || k > XTQ_NORM_LAYER) return 15;
     if (p->gate_act < XTQ_GATE_NONE || p->gate_act > XTQ_GATE_SILU) return 15;
-    if (!res && (!p->kind || p->post || gate || p->scale)) return 15;       // nothing that they would be of
+    if (rows && !res && (!p->kind || p->post || gate || p->scale)) return 15;       // nothing that they would be of
     if (d <= 0 || d > xtq::kNormMaxD || rows < 0 || rows > (1 << 30)) return 6;
     xtq::NormArgs a{};
     struct { const void* p; int bit; xtq::NormParam* to; } params[] = {
