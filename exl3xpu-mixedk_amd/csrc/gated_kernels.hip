@@ -297,7 +297,11 @@ __global__ __launch_bounds__(64 * W, 2) void gated_gemm_kernel(GatedGemm g, Gate
     };
     const std::integral_constant<int, 0> c0;
     const std::integral_constant<int, 1> c1;
+    // (The first step's pieces before all else: the wait below leaves under way the last
+    // loads to be issued, and these may not be among them.  Loads to registers could
+    // otherwise be moved ahead of loads to LDS.)
     load_a(s0);
+    asm volatile("" ::: "memory");
     load_b(s0, c0);
     load_a(s0 + 1);
     if constexpr (kStages == 3) load_b(s0 + 1, c1);
