@@ -121,12 +121,20 @@ __device__ __forceinline__ void finish_rows_of(const GatedArgs& a, const Columns
 
 // Up to 16 rows the last run to arrive of two blocks' finishes them; more are left to
 // gated_few_join_kernel, since the last runs' rows would be all that still works: 64
-// rows of 4096 by 6144 45.9 us in all, and 34.7 with the other launch.
+// rows of 4096 by 6144 45.9 us in all, and 34.7 with the other launch (31.8 since).
 //
 // EVEN where that fills the places, two workgroups a compute unit.  272 blocks of 17408
 // columns do not, and two compute units of three then wait for the third: 48 rows of
-// 5120 take 80.4 us in 272 runs and 61.7 in 512, one row 57.5 and 47.0.  (Going over a
-// block's end is a loop, which costs registers: where runs are short, EVEN is faster.)
+// 5120 take 82.3 us in 272 runs and 62.8 in 512, one row 53.3 and 43 (calls one behind
+// the other, bf16; few_workers has more).  (Going over a block's end is a loop, which
+// costs registers: where runs are short, EVEN is faster.)
+//
+// One kernel holds all six widths, and the widest of them says how many registers it
+// keeps in scratch: of four groups and two terms (33 rows of float16 and more) 43 to 70
+// by the codebook, 109 to 126 over blocks' ends, some of them read again in the steps
+// (48 rows of 5120 by 17408, K = 4: 78 us, 63 with one term), and of one term over
+// blocks' ends 2 to 4; of one group 12 to 31 over blocks' ends, and 3 in one block where
+// the rows are transformed here for two terms.
 template <int G, bool FUSED, bool LO, bool EVEN>
 __global__ __launch_bounds__(64 * few_waves(G), G == 1 ? 4 : 2) void gated_few_kernel(GatedArgs a, GatedFew f) {
     constexpr int W = few_waves(G), N = 8 / W;

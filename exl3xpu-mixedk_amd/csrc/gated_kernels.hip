@@ -446,11 +446,23 @@ bool takes_few(int rows, int k, int n) {
 }
 
 // A chunk's workgroups: as few_splits cuts the blocks, with 16 steps each at least where
-// there are several chunks (100 rows of 1024 by 4096 21.2 us, 26.1 with 8).  Where that
+// there are several chunks (100 rows of 1024 by 4096 21 us, 24 with 8).  Where that
 // leaves a fifth of the places empty, blocks that come twice into them in four parts
-// each (172 of 4096: 1 row 25.8 us, 34.6 cut evenly over all steps, 64 rows 43.4, 46.3),
-// others evenly over all steps (272 of 5120: 1 row 47.0, 57.5 uncut; 64 rows 64.3, 81.4)
-// if a run still has 32 of them (1 row of 4096 by 6144 24.4 so, 18.7 in five parts each).
+// each, others evenly over all steps if a run still has 32 of them.
+//
+// us a call, called one behind the other, bf16, K = 4, weights that no cache holds:
+//   blocks, steps       rows   whole   in 2   in 3   in 4   in 5   over all   taken
+//   172 of 4096            1    28.9   29.1   31.8   25.1   28.8       33.0   4
+//                         64    51.7   45.4   50.8   44.4   49.1       46.4
+//   172 of 2048            1    20.1   18.1   20.6   18.3   20.9       23.6   2
+//   272 of 5120            1    53.3   43.1   47.2   45.0   42.5       42.9   over all
+//                         64    84.2   74.7   71.4   72.3   74.7       65.6
+//   96 of 4096             1    28.5   20.5   23.1   18.2   17.6       22.7   5
+//   144 of 16384          24   132.5  103.6   76.7   77.0   67.0       71.6   3
+// In 268 cases (19 sizes of 1024 to 17408 by 4096 to 17408, 1 to 200 rows, one term and
+// two) what is taken is 1.4% slower in the mean than the fastest of these, 6 and 8 parts.
+// It is furthest off in the table's last row (14%) and at one row of two terms of 8192 by
+// 11008 (52.7 in four parts, 46.7 over all) and 2048 by 11008 (20.7 in two, 18.2 in four).
 void few_workers(FewPlan& p, int rows, int k, int n, int waves) {
     const int blocks = n / 64, chunks = few_chunks(rows), steps = k / 32, places = 2 * kCUs;
     int s = few_splits(rows < kFewRows ? rows : kFewRows, k, 2 * n, waves);

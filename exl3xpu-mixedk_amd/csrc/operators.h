@@ -43,8 +43,11 @@ struct Epilogue {
 // Whether a forward product's rows enter with 22 bits, as two fp16 terms, and not with
 // the 11 of one.  fp16: one rounding of the rows is as large as the result's own
 // (together 1.4 times the error of that alone), so only the result's is left.
-// bf16 results are rounded to 8 bits, beside which the rows' 11 do not show
-// (0.0017 of a result's norm with one term and with two); but relu's slope jumps
+// bf16 results are rounded to 8 bits, beside which the rows' 11 add little: 0.8% to
+// the error of the rounded exact result in a linear layer, 1.4 to 1.6% in a gated
+// projection, which takes two factors', and 1.8% in its gradient (48 and 500 rows of
+// 5120 by 1280 and the other way round, 0.00166 of the norm); a second term would take
+// that away for up to twice the matrix work.  But relu's slope jumps
 // at zero: results that near to it take the wrong side, e of them for an error
 // e, and the gradient is off by the root of that, so relu's rows have 22 bits in
 // either type.  It does not go by whether z is kept: a call's results are the

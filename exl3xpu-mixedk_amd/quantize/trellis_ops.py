@@ -315,7 +315,8 @@ def gated(x: torch.Tensor, gate: TrellisLinear, up: TrellisLinear, gate_bias: to
     Biases [n] have x's type or fp32.  Differentiable in x and the biases (once, in
     reverse mode; the weights are frozen), which keeps both factors in fp32; the same
     result with a gradient and without.  x enters the products, and the gradient its
-    own, with as many bits as linear's; fast as there."""
+    own, with as many bits as linear's (bfloat16 with 11, which makes the error 1.6% and
+    the gradient's 1.8% larger than the result's own rounding); fast as there."""
     if x.dtype not in _TYPES:
         raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
     if (up.k, up.n) != (gate.k, gate.n) or up.device != gate.device or \
