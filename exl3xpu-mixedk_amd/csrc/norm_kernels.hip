@@ -472,11 +472,14 @@ __global__ __launch_bounds__(MODE == kBlock ? 64 * kRowWaves : 256) void norm_bw
         float dt[8], dg[8], dp[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const Forward f = again<T, OF, FULL>(now.raw, i, gate, ch, now.stats);
+            Forward f = again<T, OF, FULL>(now.raw, i, gate, ch, now.stats);
             dt[i] = total<T, OF, FULL>(f, now.raw, i, now.stats, c1, c2, i < nh);
             dp[i] = dt[i];
             if constexpr (OF != kPlain) {
-                const float ds = dt[i] * ch.s[i], to = OF == kWithGate ? ds * gate.ga[i] : ds;
+                const float ds = dt[i] * ch.s[i];
+                float to = OF == kWithGate ? ds * gate.ga[i] : ds;
+                // (where there is no row an infinite parameter makes NaN of its zeros)
+                if (MODE != kBlock && row >= a.f.rows) f.q = to = 0.0f;
                 dg[i] = ds * f.p * gate.slope[i];
                 if constexpr (SUMS) sums.rest(i, f, dt[i], to);
                 dp[i] = to * ch.pw[i];
