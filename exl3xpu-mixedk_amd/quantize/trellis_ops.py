@@ -14,7 +14,10 @@ its trellis, the kernels decode it on the way to the matrix cores.
 
 Activations are bfloat16 or float16 and results have their type; sums are fp32
 and every result is rounded once.  Calls are ordered on the current stream,
-never wait for the GPU, and can be captured in a HIP graph.  There is no
+never wait for the GPU, and can be captured in a HIP graph.  (A backward pass only
+while no eager graph of the same leaves is alive: torch's nodes of these keep the
+stream that they were made on, a capture on another cannot wait for it, and the
+process ends.  Delete the eager results first, or make the leaves anew.)  There is no
 fallback: tensors that are not on a HIP device raise.
 
 The reference multiplies with its weights in a serving stack of its own
